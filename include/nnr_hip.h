@@ -36,7 +36,7 @@ enum {
     NNRH_ERR_HIP = 3,          /* a HIP runtime call failed                */
     NNRH_ERR_NOMEM = 4
 };
-enum { NNRH_U8 = 0, NNRH_S8 = 1, NNRH_I32 = 2, NNRH_F32 = 3, NNRH_F16 = 4 };
+enum { NNRH_U8 = 0, NNRH_S8 = 1, NNRH_I32 = 2, NNRH_F32 = 3, NNRH_F16 = 4, NNRH_BF16 = 5 };
 
 /* Message of the last failing call on this thread (never NULL). */
 const char* nnrh_last_error(void);
@@ -571,6 +571,108 @@ int nnrh_transpose_f32(const float* x_dev, float* y_dev, int ndim, const int* di
                        const int* perm_host, void* stream);
 /* Clip / Relu (src/backend/cpu/Clip.cpp, Relu.cpp): y = min(max(x, lo), hi) */
 int nnrh_clip_f32(const float* x_dev, float* y_dev, size_t n, float lo, float hi, void* stream);
+
+/* ---- a decoder's serving step ---------------------------------------------
+ * No counterparts in the reference, which has neither 4-bit weights nor a
+ * key/value cache. Activations, scales, biases and outputs of one call are of
+ * one type, NNRH_F32, NNRH_F16 or NNRH_BF16; sums are fp32, rounded once.   */
+
+/* com.microsoft MatMulNBits with a constant B, bits = 4:
+ *   y[m][n] = sum_k a[m][k] (q[n][k] - zp[n][k / block]) scale[n][k / block] + bias[n]
+ * block_size: a power of two >= 32; K need not be a multiple of it. Column n's
+ * ceil(k / block_size) blocks lie one after another, block_size / 2 bytes
+ * each, the lower nibble first; zero points likewise, two a byte, a column's
+ * rounded up to a whole byte (NULL: 8). run takes a of m x k and writes y of
+ * m x n, both row-major and dense, any m >= 0, and uses no workspace: calls
+ * on several streams may share a handle. y must not overlap a. a and y are
+ * aligned to their element; rows of 16-byte multiples at 16-byte aligned
+ * addresses are faster.                                                     */
+typedef struct nnrh_matmul_nbits_desc {
+    int n, k;
+    int bits;                     /* 4                                       */
+    int block_size;
+    int dtype;                    /* of a, the scales, the bias and y        */
+    const uint8_t* b_host;        /* [n][blocks][block_size / 2]             */
+    const void* scales_host;      /* [n][blocks]                             */
+    const uint8_t* zero_points_host;   /* [n][(blocks + 1) / 2], or NULL      */
+    const void* bias_host;        /* [n], or NULL                            */
+} nnrh_matmul_nbits_desc;
+typedef struct nnrh_matmul_nbits* nnrh_matmul_nbits_t;
+int nnrh_matmul_nbits_create(nnrh_matmul_nbits_t* h, const nnrh_matmul_nbits_desc* d);
+int nnrh_matmul_nbits_run(nnrh_matmul_nbits_t h, const void* a_dev, void* y_dev, int m, void* stream);
+int nnrh_matmul_nbits_destroy(nnrh_matmul_nbits_t h);
+
+/* A paged key/value cache that is quantized as it is written. A group (8 bits:
+ * a token's head; 4 bits: 32 elements of it) is held as
+ *   scale = bf16(max |x| / L), code = clamp(rint(x / scale), -L, L), L = 127 or 7
+ * and stands for code * scale. Elements that are not finite do not enter the
+ * maximum; a NaN is held as 0, an infinity as its sign's last code. A scale
+ * that is no normal float is 0.
+ * The cache is one device buffer of nnrh_kv_cache_bytes, 16-byte aligned, of
+ * the caller; its layout is the library's. Zero it before its first use.
+ * A sequence's tokens lie in the pages that its row of page_table names, in
+ * order: position i in page page_table[b][i / page_size]. An entry outside 0
+ * .. num_pages - 1 is a page that does not exist: nothing is written to it
+ * and it holds no tokens. seq_lens[b] counts sequence b's tokens up to and
+ * with the newest. Both are int32 in device memory, read when the kernels run.
+ *
+ * write: token s of `seq` new tokens of sequence b goes to position
+ *   seq_lens[b] - seq + s. Tokens at negative positions (a batch padded at the
+ *   front) and behind the last page are skipped. The pages that one call
+ *   writes to must belong to one sequence each.
+ * read: the same positions back, code * scale rounded to dtype; those that
+ *   hold no token as zeros.
+ * k and v are [batch][seq][kv_heads][head_dim] with batch and token strides in
+ * elements (shared by k and v; heads are dense, tokens of an output do not
+ * overlap); addresses and strides in bytes are multiples of 16.            */
+typedef struct nnrh_kv_cache_desc {
+    int num_pages;
+    int page_size;                /* tokens: a power of two, 32 .. 4096      */
+    int kv_heads;
+    int head_dim;                 /* 64, 96, 128 or 256                      */
+    int bits;                     /* 8 or 4                                  */
+} nnrh_kv_cache_desc;
+typedef struct nnrh_kv_tokens {
+    int dtype;
+    int batch, seq;
+    long long batch_stride, token_stride;
+    const int32_t* page_table_dev;   /* [batch][max_pages]                   */
+    int max_pages;
+    const int32_t* seq_lens_dev;     /* [batch]                              */
+} nnrh_kv_tokens;
+int nnrh_kv_cache_bytes(const nnrh_kv_cache_desc* c, size_t* bytes);
+int nnrh_kv_cache_write(const nnrh_kv_cache_desc* c, void* cache_dev, const nnrh_kv_tokens* t,
+                        const void* k_dev, const void* v_dev, void* stream);
+int nnrh_kv_cache_read(const nnrh_kv_cache_desc* c, const void* cache_dev, const nnrh_kv_tokens* t,
+                       void* k_dev, void* v_dev, void* stream);
+
+/* Attention over the cache. Query (b, s, h) of `seq` newest tokens, whose own
+ * keys are already written, sees
+ *   the first prefix_len tokens of the pages of prefix_table, which all of the
+ *   batch shares (each read once for the whole batch), and
+ *   positions 0 .. seq_lens[b] - seq + s of its own sequence,
+ * with key/value head h / (q_heads / kv_heads):
+ *   y = sum_j softmax_j(scale q k_j) v_j.   A query that sees no key gives 0.
+ * q: [batch][seq][q_heads][head_dim], strides as above; y dense, 16-byte
+ * aligned; y may be q itself where q is dense, and must not overlap it
+ * otherwise. Zero, one or several tokens a sequence, in any mixture of
+ * lengths. workspace: nnrh_kv_attention_workspace bytes (a function of the
+ * shapes, not of the lengths), 256-byte aligned, NULL where that is 0; calls
+ * that may overlap need one each.                                          */
+typedef struct nnrh_kv_attention_desc {
+    int dtype;
+    int batch, seq, q_heads;
+    long long q_batch_stride, q_token_stride;
+    float scale;
+    const int32_t* page_table_dev;   /* [batch][max_pages]                   */
+    int max_pages;
+    const int32_t* seq_lens_dev;     /* [batch]                              */
+    const int32_t* prefix_table_dev; /* [ceil(prefix_len / page_size)]       */
+    int prefix_len;                  /* 0: no prefix                         */
+} nnrh_kv_attention_desc;
+int nnrh_kv_attention_workspace(const nnrh_kv_cache_desc* c, const nnrh_kv_attention_desc* a, size_t* bytes);
+int nnrh_kv_attention(const nnrh_kv_cache_desc* c, const void* cache_dev, const nnrh_kv_attention_desc* a,
+                      const void* q_dev, void* y_dev, void* workspace_dev, void* stream);
 
 #ifdef __cplusplus
 }

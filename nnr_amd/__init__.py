@@ -14,12 +14,12 @@ import ctypes as ct
 import numpy as np
 
 from ._lib import (BRANCH_NAMES, F16, F32, I32, NNRH_ERR_UNSUPPORTED, S8, U8, NnrHipError,  # noqa: F401
-                   QConvDesc,
+                   KvAttentionDesc, KvCacheDesc, KvTokens, MatMulNBitsDesc, QConvDesc,
                    QMatMulDesc, check, cur_stream, lib, ptr)
 
 __all__ = ["QLinearConv", "QLinearMatMul", "MatMulIntegerScaled", "MatMulInteger", "quantize_linear",
            "dequantize_linear", "dynamic_quantize_linear", "qlinear_add", "maxpool_u8_nhwc",
-           "conv_dispatch", "NnrHipError", "lib"]
+           "conv_dispatch", "MatMulNBits", "KVCache", "NnrHipError", "lib"]
 
 
 def _dt(np_dtype) -> int:
@@ -545,3 +545,201 @@ def maxpool_u8_nhwc(x, kH, kW, sH, sW, pH, pW, oH, oW):
     check(lib().nnrh_maxpool_u8_nhwc(ptr(x), ptr(y), N, C, H, W, oH, oW, kH, kW, sH, sW, pH, pW,
                                      cur_stream()))
     return y
+
+
+# ---------------------------------------------------------------------------
+# a decoder's serving step
+
+def _float_dt(dtype) -> int:
+    import torch
+    from ._lib import BF16
+    dt = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}.get(dtype)
+    if dt is None:
+        raise TypeError(f"{dtype}: float32, float16 or bfloat16")
+    return dt
+
+
+def _launch(device, stream, call):
+    """call(stream) with the tensors' device current, on their current stream unless one is given."""
+    import torch
+    if device.index == torch.cuda.current_device():
+        check(call(torch.cuda.current_stream().cuda_stream if stream is None else stream))
+        return
+    with torch.cuda.device(device):
+        check(call(torch.cuda.current_stream().cuda_stream if stream is None else stream))
+
+
+def _on_device(device, **tensors):
+    for name, t in tensors.items():
+        if t.device != device:
+            raise ValueError(f"{name} is on {t.device}, not on {device}")
+
+
+class MatMulNBits:
+    """y = a W^T + bias with 4-bit weights, W[n][k] = (q - zp) * scale of block
+    k // block_size (com.microsoft MatMulNBits with a constant B).
+
+    b: uint8 [n][blocks][block_size / 2] (or that many bytes in any shape of n
+    rows), low nibble first. scales: torch tensor [n][blocks], float32, float16
+    or bfloat16: the type of a, bias and y too. zero_points: uint8
+    [n][(blocks + 1) // 2], two a byte, or None (8). bias: [n] or None.
+    Laid out on the current device at construction, or on `device`."""
+
+    def __init__(self, b, scales, k, block_size, zero_points=None, bias=None, bits=4, device=None):
+        import torch
+        host = lambda t, dt: None if t is None else torch.as_tensor(t).to("cpu", dt).contiguous()
+        if scales.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+            raise TypeError(f"scales of {scales.dtype}: float32, float16 or bfloat16")
+        n, nb = int(b.shape[0]), -(-int(k) // int(block_size))
+        keep = [host(b, torch.uint8), host(scales, scales.dtype), host(zero_points, torch.uint8),
+                host(bias, scales.dtype)]
+        for t, count, name in zip(keep, (n * nb * (block_size // 2), n * nb, n * ((nb + 1) // 2), n),
+                                  ("b", "scales", "zero_points", "bias")):
+            if t is not None and t.numel() != count:
+                raise ValueError(f"{name} has {t.numel()} elements, {count} expected")
+        self.n, self.k, self.block_size, self.dtype = n, int(k), int(block_size), scales.dtype
+        self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+        if self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        desc = MatMulNBitsDesc(n, self.k, bits, self.block_size, _float_dt(self.dtype), *[ptr(t) for t in keep])
+        h = ct.c_void_p()
+        with torch.cuda.device(self.device):
+            check(lib().nnrh_matmul_nbits_create(ct.byref(h), ct.byref(desc)))
+        self.h = h
+
+    def __call__(self, a, y=None, stream=None):
+        """a [..., k] -> y [..., n]"""
+        import torch
+        if a.dtype != self.dtype or a.shape[-1] != self.k:
+            raise ValueError(f"a must be {self.dtype} [..., {self.k}]")
+        _on_device(self.device, a=a)
+        a = a.contiguous()
+        shape = (*a.shape[:-1], self.n)
+        if y is None:
+            y = torch.empty(shape, dtype=self.dtype, device=a.device)
+        elif y.shape != shape or y.dtype != self.dtype or y.device != a.device or not y.is_contiguous():
+            raise ValueError(f"y must be contiguous {self.dtype} of shape {shape} on {a.device}")
+        m = a.numel() // self.k
+        run = lib().nnrh_matmul_nbits_run
+        _launch(self.device, stream, lambda s: run(self.h, a.data_ptr(), y.data_ptr(), m, s))
+        return y
+
+    def __del__(self):
+        try:
+            if getattr(self, "h", None):
+                lib().nnrh_matmul_nbits_destroy(self.h)
+                self.h = None
+        except Exception:
+            pass
+
+
+class KVCache:
+    """Paged key/value cache of 8- or 4-bit codes, quantized as it is written
+    (nnr_hip.h says how), and the attention that reads it.
+
+    Tables are int32 tensors on the cache's device: page_table [batch][pages]
+    names a sequence's pages in order, seq_lens [batch] counts its tokens up to
+    and with the newest. k, v and q are [batch, seq, heads, head_dim] in
+    float32, float16 or bfloat16; the last two axes are dense, the others may
+    be strided (a slice of a fused projection's output)."""
+
+    def __init__(self, num_pages, kv_heads, head_dim, page_size=64, bits=8, device=None):
+        import torch
+        self.desc = KvCacheDesc(int(num_pages), int(page_size), int(kv_heads), int(head_dim), int(bits))
+        n = ct.c_size_t()
+        check(lib().nnrh_kv_cache_bytes(ct.byref(self.desc), ct.byref(n)))
+        self.data = torch.zeros(n.value, dtype=torch.uint8, device="cuda" if device is None else device)
+        self.device = self.data.device
+        self.num_pages, self.page_size, self.kv_heads = int(num_pages), int(page_size), int(kv_heads)
+        self.head_dim, self.bits = int(head_dim), int(bits)
+
+    def _tables(self, batch, page_table, seq_lens):
+        import torch
+        if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != batch:
+            raise ValueError(f"page_table must be int32 [{batch}][pages]")
+        if seq_lens.dtype != torch.int32 or tuple(seq_lens.shape) != (batch,):
+            raise ValueError(f"seq_lens must be int32 [{batch}]")
+        _on_device(self.device, page_table=page_table, seq_lens=seq_lens)
+        return page_table.contiguous(), seq_lens.contiguous()
+
+    def _rows(self, name, t, heads):
+        """t with dense heads and 16-byte steps: itself, or a copy."""
+        if t.dim() != 4 or t.shape[2] != heads or t.shape[3] != self.head_dim:
+            raise ValueError(f"{name} must be [batch, seq, {heads}, {self.head_dim}]")
+        _on_device(self.device, **{name: t})
+        st, es = t.stride(), t.element_size()
+        if (st[3] != 1 or (heads > 1 and st[2] != self.head_dim) or t.data_ptr() % 16 or st[0] * es % 16 or
+                st[1] * es % 16):
+            t = t.contiguous()
+            if t.data_ptr() % 16:
+                t = t.clone()
+        return t
+
+    def _tokens(self, k, page_table, seq_lens):
+        B, S = k.shape[:2]
+        return KvTokens(_float_dt(k.dtype), B, S, k.stride(0), k.stride(1), page_table.data_ptr(),
+                        page_table.shape[1], seq_lens.data_ptr())
+
+    def write(self, k, v, page_table, seq_lens, stream=None):
+        """Token s of sequence b to position seq_lens[b] - seq + s; tokens at
+        negative positions are skipped."""
+        k, v = self._rows("k", k, self.kv_heads), self._rows("v", v, self.kv_heads)
+        if k.shape != v.shape or k.dtype != v.dtype:
+            raise ValueError("k and v must agree in shape and type")
+        if k.stride() != v.stride():
+            k, v = k.contiguous(), v.contiguous()
+        page_table, seq_lens = self._tables(k.shape[0], page_table, seq_lens)
+        t, run = self._tokens(k, page_table, seq_lens), lib().nnrh_kv_cache_write
+        _launch(self.device, stream, lambda s: run(self.desc, self.data.data_ptr(), t, k.data_ptr(), v.data_ptr(), s))
+
+    def read(self, seq, page_table, seq_lens, dtype, stream=None):
+        """(k, v) of positions seq_lens[b] - seq .. seq_lens[b] - 1 as `dtype`; zeros
+        where there is no token."""
+        import torch
+        B = page_table.shape[0]
+        page_table, seq_lens = self._tables(B, page_table, seq_lens)
+        k, v = (torch.empty((B, seq, self.kv_heads, self.head_dim), dtype=dtype, device=self.device) for _ in "kv")
+        t, run = self._tokens(k, page_table, seq_lens), lib().nnrh_kv_cache_read
+        _launch(self.device, stream, lambda s: run(self.desc, self.data.data_ptr(), t, k.data_ptr(), v.data_ptr(), s))
+        return k, v
+
+    def attention(self, q, page_table, seq_lens, scale=None, prefix_table=None, prefix_len=0, y=None, workspace=None,
+                  stream=None):
+        """softmax(scale q K^T) V, scale 1 / sqrt(head_dim) unless given. Query
+        (b, s) sees the first prefix_len tokens of the pages in prefix_table
+        (int32 [pages], shared by the batch) and positions up to seq_lens[b] -
+        seq + s of its own. workspace: a uint8 tensor of attention_workspace's
+        size, made by the call unless given (a call on a stream that is not
+        current should bring it)."""
+        import torch
+        if q.dim() != 4:
+            raise ValueError("q must be [batch, seq, heads, head_dim]")
+        Hq = q.shape[2]
+        q = self._rows("q", q, Hq)
+        B, S = q.shape[:2]
+        page_table, seq_lens = self._tables(B, page_table, seq_lens)
+        if y is None:
+            y = torch.empty((B, S, Hq, self.head_dim), dtype=q.dtype, device=self.device)
+        elif y.shape != q.shape or y.dtype != q.dtype or y.device != self.device or not y.is_contiguous():
+            raise ValueError("y must be contiguous, of q's shape, type and device")
+        pt = None
+        if prefix_len:
+            if prefix_table is None or prefix_table.dtype != torch.int32 or prefix_table.dim() != 1 or \
+                    prefix_table.numel() * self.page_size < prefix_len:
+                raise ValueError(f"prefix_table must be int32 and name the pages of {prefix_len} tokens")
+            _on_device(self.device, prefix_table=prefix_table)
+            prefix_table = prefix_table.contiguous()
+            pt = prefix_table.data_ptr()
+        d = KvAttentionDesc(_float_dt(q.dtype), B, S, Hq, q.stride(0), q.stride(1),
+                            self.head_dim ** -0.5 if scale is None else float(scale), page_table.data_ptr(),
+                            page_table.shape[1], seq_lens.data_ptr(), pt, int(prefix_len))
+        n = ct.c_size_t()
+        check(lib().nnrh_kv_attention_workspace(self.desc, d, n))
+        if workspace is None:
+            workspace = torch.empty(n.value, dtype=torch.uint8, device=self.device) if n.value else None
+        elif workspace.dtype != torch.uint8 or workspace.numel() < n.value or workspace.device != self.device:
+            raise ValueError(f"workspace must be uint8 of at least {n.value} elements on {self.device}")
+        run = lib().nnrh_kv_attention
+        _launch(self.device, stream, lambda s: run(self.desc, self.data.data_ptr(), d, q.data_ptr(), y.data_ptr(),
+                                                   ptr(workspace), s))
+        return y

@@ -13,7 +13,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libnnr_hip.so")
 
 NNRH_OK, NNRH_ERR_INVALID, NNRH_ERR_UNSUPPORTED, NNRH_ERR_HIP, NNRH_ERR_NOMEM = range(5)
-U8, S8, I32, F32, F16 = range(5)
+U8, S8, I32, F32, F16, BF16 = range(6)
 BRANCH_NAMES = {1: "DW", 2: "FIRST", 3: "DIRECT", 4: "PACKED", 5: "NR16",
                 6: "IM2COL_S1", 7: "IM2COL", 8: "FLOAT", 9: "TYPED"}
 
@@ -47,6 +47,9 @@ EXPORTS = [
     "nnrh_nchw_to_nhwc_u8", "nnrh_global_avgpool_f32", "nnrh_gemm_f32", "nnrh_clip_f32",
     "nnrh_gemm_f32_batched", "nnrh_binary_f32", "nnrh_softmax_f32", "nnrh_layernorm_f32",
     "nnrh_gelu_f32", "nnrh_hardswish_f32", "nnrh_transpose_f32",
+    "nnrh_matmul_nbits_create", "nnrh_matmul_nbits_run", "nnrh_matmul_nbits_destroy",
+    "nnrh_kv_cache_bytes", "nnrh_kv_cache_write", "nnrh_kv_cache_read",
+    "nnrh_kv_attention_workspace", "nnrh_kv_attention",
 ]
 
 
@@ -91,6 +94,28 @@ class MmiScaledDesc(C.Structure):
 
 class DqCodes(C.Structure):
     _fields_ = [("codes_dev", C.c_void_p), ("zp", C.c_int), ("scale", C.c_float), ("bias_dev", C.c_void_p)]
+
+
+class MatMulNBitsDesc(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("n", "k", "bits", "block_size", "dtype")] + [
+        (n, C.c_void_p) for n in ("b_host", "scales_host", "zero_points_host", "bias_host")]
+
+
+class KvCacheDesc(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("num_pages", "page_size", "kv_heads", "head_dim", "bits")]
+
+
+class KvTokens(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("dtype", "batch", "seq")] + [
+        ("batch_stride", C.c_longlong), ("token_stride", C.c_longlong), ("page_table_dev", C.c_void_p),
+        ("max_pages", C.c_int), ("seq_lens_dev", C.c_void_p)]
+
+
+class KvAttentionDesc(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("dtype", "batch", "seq", "q_heads")] + [
+        ("q_batch_stride", C.c_longlong), ("q_token_stride", C.c_longlong), ("scale", C.c_float),
+        ("page_table_dev", C.c_void_p), ("max_pages", C.c_int), ("seq_lens_dev", C.c_void_p),
+        ("prefix_table_dev", C.c_void_p), ("prefix_len", C.c_int)]
 
 
 _lib = None
@@ -200,6 +225,14 @@ def lib():
         "nnrh_gelu_f32": (i, [vp, vp, sz, vp]),
         "nnrh_hardswish_f32": (i, [vp, vp, sz, i, vp]),
         "nnrh_transpose_f32": (i, [vp, vp, i, P(i), P(i), vp]),
+        "nnrh_matmul_nbits_create": (i, [P(vp), P(MatMulNBitsDesc)]),
+        "nnrh_matmul_nbits_run": (i, [vp, vp, vp, i, vp]),
+        "nnrh_matmul_nbits_destroy": (i, [vp]),
+        "nnrh_kv_cache_bytes": (i, [P(KvCacheDesc), P(sz)]),
+        "nnrh_kv_cache_write": (i, [P(KvCacheDesc), vp, P(KvTokens), vp, vp, vp]),
+        "nnrh_kv_cache_read": (i, [P(KvCacheDesc), vp, P(KvTokens), vp, vp, vp]),
+        "nnrh_kv_attention_workspace": (i, [P(KvCacheDesc), P(KvAttentionDesc), P(sz)]),
+        "nnrh_kv_attention": (i, [P(KvCacheDesc), vp, P(KvAttentionDesc), vp, vp, vp, vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)

@@ -18,6 +18,7 @@
 #include <vector>
 
 #include "nnr_hip.h"
+#include "nnrh_decode.h"
 #include "nnrh_elem.h"
 #include "nnrh_f32.h"
 #include "nnrh_internal.h"
@@ -2234,5 +2235,301 @@ extern "C" int nnrh_clip_f32(const float* x, float* y, size_t n, float lo, float
     if (n && (!x || !y)) return set_err(NNRH_ERR_INVALID, "clip_f32: NULL");
     ProfScope ps("clip_f32", S(stream));
     HIP_TRY(launch_clip_f32(x, y, (long long)n, lo, hi, S(stream)), "clip_f32");
+    return NNRH_OK;
+}
+
+// ===========================================================================
+// A decoder's serving step: 4-bit weights, quantized key/value cache
+
+namespace {
+
+int float_type(int dtype) {
+    return dtype == NNRH_F32 ? FT_F32 : dtype == NNRH_F16 ? FT_F16 : dtype == NNRH_BF16 ? FT_BF16 : -1;
+}
+bool overlap(const void* a, size_t na, const void* b, size_t nb) {
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+    return na && nb && x < y + nb && y < x + na;
+}
+
+}  // namespace
+
+struct nnrh_matmul_nbits {
+    NbitsArgs a{};
+    uint32_t* w = nullptr;
+    void* scales = nullptr;
+    uint16_t* zp = nullptr;
+    void* bias = nullptr;
+    ~nnrh_matmul_nbits() {
+        dfree(w);
+        dfree(scales);
+        dfree(zp);
+        dfree(bias);
+    }
+};
+
+namespace {
+
+// device memory of a create call, freed when it ends
+struct Upload {
+    uint8_t* p = nullptr;
+    ~Upload() { dfree(p); }
+};
+
+int nbits_build(nnrh_matmul_nbits* h, const nnrh_matmul_nbits_desc* d) {
+    const size_t nb = ((size_t)d->k + d->block_size - 1) / d->block_size, es = float_type_size(h->a.type);
+    Upload raw, raw_scales, raw_zp;
+    int rc;
+    if ((rc = upload(&raw.p, d->b_host, (size_t)d->n * nb * (d->block_size / 2))) ||
+        (rc = upload(&raw_scales.p, (const uint8_t*)d->scales_host, (size_t)d->n * nb * es)))
+        return rc;
+    if (d->zero_points_host && (rc = upload(&raw_zp.p, d->zero_points_host, (size_t)d->n * ((nb + 1) / 2)))) return rc;
+    if (d->bias_host) {
+        uint8_t* b = nullptr;
+        if ((rc = upload(&b, (const uint8_t*)d->bias_host, (size_t)d->n * es))) return rc;
+        h->bias = b;
+    }
+    const size_t pieces = (size_t)(nbits_cols(d->n) / 16) * h->a.P;
+    if ((rc = nnrh_malloc((void**)&h->w, pieces * 1024)) ||
+        (rc = nnrh_malloc(&h->scales, pieces * 16 * h->a.nspp * es)) ||
+        (d->zero_points_host && (rc = nnrh_malloc((void**)&h->zp, pieces * 32))))
+        return rc;
+    HIP_TRY(launch_nbits_pack(raw.p, raw_scales.p, raw_zp.p, d->n, d->k, d->block_size, h->a.type, h->w, h->scales,
+                              h->zp, nullptr),
+            "matmul_nbits: pack");
+    // what was uploaded goes away with this call, and runs may come on any stream
+    HIP_TRY(hipStreamSynchronize(nullptr), "matmul_nbits: pack");
+    h->a.w = h->w;
+    h->a.scales = h->scales;
+    h->a.zp = h->zp;
+    h->a.bias = h->bias;
+    return NNRH_OK;
+}
+
+}  // namespace
+
+extern "C" int nnrh_matmul_nbits_create(nnrh_matmul_nbits_t* out, const nnrh_matmul_nbits_desc* d) {
+    if (!out) return set_err(NNRH_ERR_INVALID, "matmul_nbits: handle NULL");
+    *out = nullptr;
+    if (!d || !d->b_host || !d->scales_host) return set_err(NNRH_ERR_INVALID, "matmul_nbits: NULL argument");
+    if (d->n <= 0 || d->k <= 0) return set_err(NNRH_ERR_INVALID, "matmul_nbits: n %d, k %d", d->n, d->k);
+    if (d->block_size <= 0 || (d->block_size & (d->block_size - 1)))
+        return set_err(NNRH_ERR_INVALID, "matmul_nbits: block size %d is no power of two", d->block_size);
+    if (d->bits != 4 || d->block_size < 32 || float_type(d->dtype) < 0)
+        return set_err(NNRH_ERR_UNSUPPORTED, "matmul_nbits: bits %d, block size %d, type %d (4 bits, blocks of 32 and "
+                                             "more, fp32 / fp16 / bf16)", d->bits, d->block_size, d->dtype);
+    // K of the last block, and columns of the last tile, in an int
+    if (d->k > (1 << 30) || d->n > (1 << 30) || d->block_size > (1 << 30))
+        return set_err(NNRH_ERR_UNSUPPORTED, "matmul_nbits: n %d, k %d, block size %d", d->n, d->k, d->block_size);
+    nnrh_matmul_nbits* h = new (std::nothrow) nnrh_matmul_nbits();
+    if (!h) return set_err(NNRH_ERR_NOMEM, "matmul_nbits: host allocation");
+    h->a.N = d->n;
+    h->a.K = d->k;
+    h->a.P = nbits_pieces(d->k);
+    h->a.nspp = nbits_nspp(d->block_size);
+    h->a.type = float_type(d->dtype);
+    const int rc = nbits_build(h, d);
+    if (rc != NNRH_OK) {
+        delete h;
+        return rc;
+    }
+    *out = h;
+    return NNRH_OK;
+}
+
+extern "C" int nnrh_matmul_nbits_run(nnrh_matmul_nbits_t h, const void* a, void* y, int m, void* stream) {
+    if (!h || m < 0 || (m && (!a || !y))) return set_err(NNRH_ERR_INVALID, "matmul_nbits_run: bad argument");
+    if (m > (1 << 22)) return set_err(NNRH_ERR_UNSUPPORTED, "matmul_nbits_run: %d rows (at most %d)", m, 1 << 22);
+    const size_t es = float_type_size(h->a.type);
+    if (((uintptr_t)a | (uintptr_t)y) & (es - 1)) return set_err(NNRH_ERR_INVALID, "matmul_nbits_run: alignment");
+    if (overlap(a, (size_t)m * h->a.K * es, y, (size_t)m * h->a.N * es))
+        return set_err(NNRH_ERR_INVALID, "matmul_nbits_run: y lies over a");
+    NbitsArgs g = h->a;
+    g.a = a;
+    g.y = y;
+    g.M = m;
+    ProfScope ps("matmul_nbits", S(stream));
+    HIP_TRY(launch_nbits(g, S(stream)), "matmul_nbits");
+    return NNRH_OK;
+}
+
+extern "C" int nnrh_matmul_nbits_destroy(nnrh_matmul_nbits_t h) {
+    delete h;
+    return NNRH_OK;
+}
+
+namespace {
+
+// the cache's description; data may be NULL
+int kv_cache(const nnrh_kv_cache_desc* c, const void* data, KvCache* out) {
+    if (!c) return set_err(NNRH_ERR_INVALID, "kv_cache: NULL description");
+    if (c->num_pages < 0 || c->kv_heads <= 0 || c->head_dim <= 0 || c->page_size <= 0)
+        return set_err(NNRH_ERR_INVALID, "kv_cache: %d pages of %d tokens, %d heads of %d", c->num_pages, c->page_size,
+                       c->kv_heads, c->head_dim);
+    if (c->page_size < 32 || c->page_size > 4096 || (c->page_size & (c->page_size - 1)))
+        return set_err(NNRH_ERR_UNSUPPORTED, "kv_cache: page size %d (a power of two, 32 .. 4096)", c->page_size);
+    if (c->head_dim != 64 && c->head_dim != 96 && c->head_dim != 128 && c->head_dim != 256)
+        return set_err(NNRH_ERR_UNSUPPORTED, "kv_cache: head size %d (64, 96, 128 or 256)", c->head_dim);
+    if (c->bits != 8 && c->bits != 4) return set_err(NNRH_ERR_UNSUPPORTED, "kv_cache: %d bits (8 or 4)", c->bits);
+    if (c->kv_heads > 32767) return set_err(NNRH_ERR_UNSUPPORTED, "kv_cache: %d heads", c->kv_heads);
+    if ((uintptr_t)data & 15) return set_err(NNRH_ERR_INVALID, "kv_cache: the cache must be 16-byte aligned");
+    out->data = (uint8_t*)data;
+    out->num_pages = c->num_pages;
+    out->page_size = c->page_size;
+    out->heads = c->kv_heads;
+    out->hd = c->head_dim;
+    out->bits = c->bits;
+    return NNRH_OK;
+}
+long long kv_page_bytes(const KvCache& c) { return c.heads * kv_head_bytes(c.page_size, c.hd, c.bits); }
+
+// what write, read and attention ask of a batch's tables
+int kv_batch(const char* what, int batch, int seq, int max_pages, int page_size, const int32_t* table,
+             const int32_t* lens) {
+    if (batch < 0 || seq < 0 || max_pages < 0)
+        return set_err(NNRH_ERR_INVALID, "%s: batch %d, seq %d, pages %d", what, batch, seq, max_pages);
+    if (batch > 65535 || seq > (1 << 30) || (long long)max_pages * page_size > (1 << 30))
+        return set_err(NNRH_ERR_UNSUPPORTED, "%s: batch %d (at most 65535), seq %d, %d pages of %d tokens (at most 2^30)",
+                       what, batch, seq, max_pages, page_size);
+    if (!batch || !seq) return NNRH_OK;
+    if (!lens || (max_pages && !table)) return set_err(NNRH_ERR_INVALID, "%s: NULL table or lengths", what);
+    if (((uintptr_t)table | (uintptr_t)lens) & 3) return set_err(NNRH_ERR_INVALID, "%s: table alignment", what);
+    return NNRH_OK;
+}
+// rows of `width` dense elements at strides; out: rows must not overlap
+int kv_strides(const char* what, int type, int batch, int seq, long long width, long long bs, long long ts, bool out) {
+    const long long per16 = 16 / float_type_size(type);
+    if (bs < 0 || ts < 0 || (batch > 1 && bs % per16) || (seq > 1 && ts % per16))
+        return set_err(NNRH_ERR_INVALID, "%s: strides %lld, %lld (multiples of 16 bytes)", what, bs, ts);
+    if (bs > (1LL << 40) || ts > (1LL << 40)) return set_err(NNRH_ERR_UNSUPPORTED, "%s: strides %lld, %lld", what, bs, ts);
+    // one of the two orders, each row or sequence behind the one before
+    const bool rows = seq <= 1 || ts >= width, seqs = batch <= 1 || bs >= (seq - 1) * ts + width;
+    const bool inner = batch <= 1 || bs >= width, outer = seq <= 1 || ts >= (batch - 1) * bs + width;
+    if (out && !(rows && seqs) && !(inner && outer))
+        return set_err(NNRH_ERR_INVALID, "%s: rows at strides %lld, %lld overlap", what, bs, ts);
+    return NNRH_OK;
+}
+
+int kv_tokens(const char* what, const KvCache& c, const nnrh_kv_tokens* t, const void* k, const void* v, bool out,
+              KvTokens* r) {
+    if (!t) return set_err(NNRH_ERR_INVALID, "%s: NULL description", what);
+    const int type = float_type(t->dtype);
+    if (type < 0) return set_err(NNRH_ERR_UNSUPPORTED, "%s: type %d (fp32, fp16 or bf16)", what, t->dtype);
+    int rc = kv_batch(what, t->batch, t->seq, t->max_pages, c.page_size, t->page_table_dev, t->seq_lens_dev);
+    if (rc != NNRH_OK) return rc;
+    *r = KvTokens{const_cast<void*>(k), const_cast<void*>(v), type, t->batch_stride, t->token_stride, t->batch, t->seq,
+                  t->page_table_dev, t->max_pages, t->seq_lens_dev};
+    if (!t->batch || !t->seq) return NNRH_OK;
+    if (!k || !v || (!c.data && c.num_pages)) return set_err(NNRH_ERR_INVALID, "%s: NULL argument", what);
+    if (((uintptr_t)k | (uintptr_t)v) & 15) return set_err(NNRH_ERR_INVALID, "%s: k and v must be 16-byte aligned", what);
+    const long long width = (long long)c.heads * c.hd;
+    if ((rc = kv_strides(what, type, t->batch, t->seq, width, t->batch_stride, t->token_stride, out)) != NNRH_OK) return rc;
+    const size_t extent = ((t->batch - 1) * t->batch_stride + (t->seq - 1) * t->token_stride + width) * float_type_size(type);
+    const size_t all = (size_t)c.num_pages * kv_page_bytes(c);
+    if (overlap(k, extent, c.data, all) || overlap(v, extent, c.data, all))
+        return set_err(NNRH_ERR_INVALID, "%s: k or v lies over the cache", what);
+    // k and v may alternate in one tensor; the same rows are two results in one place
+    if (out && k == v) return set_err(NNRH_ERR_INVALID, "%s: k and v are one tensor", what);
+    return NNRH_OK;
+}
+
+}  // namespace
+
+extern "C" int nnrh_kv_cache_bytes(const nnrh_kv_cache_desc* d, size_t* bytes) {
+    KvCache c;
+    if (!bytes) return set_err(NNRH_ERR_INVALID, "kv_cache_bytes: NULL");
+    const int rc = kv_cache(d, nullptr, &c);
+    if (rc == NNRH_OK) *bytes = (size_t)c.num_pages * kv_page_bytes(c);
+    return rc;
+}
+
+extern "C" int nnrh_kv_cache_write(const nnrh_kv_cache_desc* d, void* cache, const nnrh_kv_tokens* t, const void* k,
+                                   const void* v, void* stream) {
+    KvCache c;
+    KvTokens a;
+    int rc;
+    if ((rc = kv_cache(d, cache, &c)) || (rc = kv_tokens("kv_cache_write", c, t, k, v, false, &a))) return rc;
+    ProfScope ps("kv_cache_write", S(stream));
+    HIP_TRY(launch_kv_write(c, a, S(stream)), "kv_cache_write");
+    return NNRH_OK;
+}
+
+extern "C" int nnrh_kv_cache_read(const nnrh_kv_cache_desc* d, const void* cache, const nnrh_kv_tokens* t, void* k,
+                                  void* v, void* stream) {
+    KvCache c;
+    KvTokens a;
+    int rc;
+    if ((rc = kv_cache(d, cache, &c)) || (rc = kv_tokens("kv_cache_read", c, t, k, v, true, &a))) return rc;
+    ProfScope ps("kv_cache_read", S(stream));
+    HIP_TRY(launch_kv_read(c, a, S(stream)), "kv_cache_read");
+    return NNRH_OK;
+}
+
+namespace {
+
+int kv_attention_args(const nnrh_kv_cache_desc* d, const void* cache, const nnrh_kv_attention_desc* a, KvCache* c,
+                      KvAttention* r) {
+    int rc = kv_cache(d, cache, c);
+    if (rc != NNRH_OK) return rc;
+    if (!a) return set_err(NNRH_ERR_INVALID, "kv_attention: NULL description");
+    const int type = float_type(a->dtype);
+    if (type < 0) return set_err(NNRH_ERR_UNSUPPORTED, "kv_attention: type %d (fp32, fp16 or bf16)", a->dtype);
+    if (a->q_heads <= 0 || a->q_heads % c->heads)
+        return set_err(NNRH_ERR_INVALID, "kv_attention: %d query heads over %d", a->q_heads, c->heads);
+    if (a->prefix_len < 0 || a->batch < 0 || a->seq < 0)
+        return set_err(NNRH_ERR_INVALID, "kv_attention: batch %d, seq %d, prefix of %d", a->batch, a->seq, a->prefix_len);
+    // rows, and blocks of rows times splits, in an int
+    if (a->prefix_len > (1 << 30) || (double)a->batch * a->seq * a->q_heads * c->hd > 17179869184.0)
+        return set_err(NNRH_ERR_UNSUPPORTED, "kv_attention: batch %d, seq %d, %d heads, prefix of %d", a->batch, a->seq,
+                       a->q_heads, a->prefix_len);
+    *r = KvAttention{nullptr, nullptr, type, a->q_batch_stride, a->q_token_stride, a->batch, a->seq, a->q_heads,
+                     a->scale, a->page_table_dev, a->max_pages, a->seq_lens_dev, a->prefix_table_dev, a->prefix_len};
+    return NNRH_OK;
+}
+
+}  // namespace
+
+extern "C" int nnrh_kv_attention_workspace(const nnrh_kv_cache_desc* d, const nnrh_kv_attention_desc* a, size_t* bytes) {
+    KvCache c;
+    KvAttention r;
+    if (!bytes) return set_err(NNRH_ERR_INVALID, "kv_attention_workspace: NULL");
+    const int rc = kv_attention_args(d, nullptr, a, &c, &r);
+    if (rc != NNRH_OK) return rc;
+    if (a->max_pages < 0 || (long long)a->max_pages * c.page_size > (1 << 30))
+        return set_err(NNRH_ERR_INVALID, "kv_attention_workspace: %d pages", a->max_pages);
+    *bytes = r.batch && r.seq ? kv_attention_workspace(c, r) : 0;
+    return NNRH_OK;
+}
+
+extern "C" int nnrh_kv_attention(const nnrh_kv_cache_desc* d, const void* cache, const nnrh_kv_attention_desc* a,
+                                 const void* q, void* y, void* workspace, void* stream) {
+    KvCache c;
+    KvAttention r;
+    int rc = kv_attention_args(d, cache, a, &c, &r);
+    if (rc != NNRH_OK) return rc;
+    if ((rc = kv_batch("kv_attention", a->batch, a->seq, a->max_pages, c.page_size, a->page_table_dev,
+                       a->seq_lens_dev)) != NNRH_OK)
+        return rc;
+    if (!a->batch || !a->seq) return NNRH_OK;
+    if (!q || !y || (!c.data && c.num_pages) || (a->prefix_len && !a->prefix_table_dev))
+        return set_err(NNRH_ERR_INVALID, "kv_attention: NULL argument");
+    if (((uintptr_t)q | (uintptr_t)y) & 15) return set_err(NNRH_ERR_INVALID, "kv_attention: q and y must be 16-byte aligned");
+    if ((uintptr_t)a->prefix_table_dev & 3) return set_err(NNRH_ERR_INVALID, "kv_attention: table alignment");
+    const long long width = (long long)a->q_heads * c.hd, ts = a->q_token_stride, bs = a->q_batch_stride;
+    if ((rc = kv_strides("kv_attention", r.type, a->batch, a->seq, width, bs, ts, false)) != NNRH_OK) return rc;
+    const size_t es = float_type_size(r.type), ysize = (size_t)a->batch * a->seq * width * es;
+    const size_t qsize = ((a->batch - 1) * bs + (a->seq - 1) * ts + width) * es;
+    const bool dense = (a->seq == 1 || ts == width) && (a->batch == 1 || bs == a->seq * width);
+    if (overlap(q, qsize, y, ysize) && !(q == y && dense)) return set_err(NNRH_ERR_INVALID, "kv_attention: y lies over q");
+    if (overlap(y, ysize, c.data, (size_t)c.num_pages * kv_page_bytes(c)))
+        return set_err(NNRH_ERR_INVALID, "kv_attention: y lies over the cache");
+    const size_t need = kv_attention_workspace(c, r);
+    if (need && !workspace) return set_err(NNRH_ERR_INVALID, "kv_attention: this shape needs a workspace of %zu bytes", need);
+    if ((uintptr_t)workspace & 255) return set_err(NNRH_ERR_INVALID, "kv_attention: the workspace must be 256-byte aligned");
+    if (overlap(workspace, need, q, qsize) || overlap(workspace, need, y, ysize))
+        return set_err(NNRH_ERR_INVALID, "kv_attention: the workspace lies over q or y");
+    r.q = q;
+    r.y = y;
+    ProfScope ps("kv_attention", S(stream));
+    HIP_TRY(launch_kv_attention(c, r, workspace, S(stream)), "kv_attention");
     return NNRH_OK;
 }

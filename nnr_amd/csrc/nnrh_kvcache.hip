@@ -1,0 +1,359 @@
+// nnrh_kvcache.hip -- writing tokens into the quantized key/value cache and
+// reading them back. A group x of a token's elements (a head's at 8 bits, 32
+// at 4 bits) is held as
+//   scale = bf16(max |x| / L), code = clamp(rint(x / scale), -L, L), L = 127 or 7.
+// The scale is rounded to bf16 before the codes are formed, so rounding it
+// costs no accuracy beyond a step 2^-9 wider; both quotients are correctly
+// rounded fp32 divisions, which decide every border between two codes (or two
+// scales) as the exact quotient would: a border times the divisor has 16 bits,
+// and an fp32 dividend beside it is at least 2^-24 of itself away.
+// Elements that are not finite do not enter the maximum; a NaN is held as 0
+// and an infinity as +-L. A scale below the normal floats is 0, and so are its
+// codes.
+#include "nnrh_decode.h"
+
+namespace nnrh {
+namespace {
+
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+
+constexpr int kLdsRow = 40;   // bytes of an element's 32 tokens, padded
+
+template <int TY>
+__device__ __forceinline__ void load8(const void* p, long long i, float* v) {
+    if constexpr (TY == FT_F32) {
+        const f4 a = *(const f4*)((const float*)p + i), b = *(const f4*)((const float*)p + i + 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { v[j] = a[j]; v[4 + j] = b[j]; }
+    } else {
+        const u4 a = *(const u4*)((const uint16_t*)p + i);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t h = (a[j >> 1] >> (16 * (j & 1))) & 0xffffu;
+            v[j] = TY == FT_F16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)h) : __builtin_bit_cast(float, h << 16);
+        }
+    }
+}
+template <int TY>
+__device__ __forceinline__ void store8(void* p, long long i, const float* v) {
+    if constexpr (TY == FT_F32) {
+        *(f4*)((float*)p + i) = f4{v[0], v[1], v[2], v[3]};
+        *(f4*)((float*)p + i + 4) = f4{v[4], v[5], v[6], v[7]};
+    } else {
+        u4 a;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint32_t lo, hi;
+            if constexpr (TY == FT_F16) {
+                lo = __builtin_bit_cast(uint16_t, (_Float16)v[2 * j]);
+                hi = __builtin_bit_cast(uint16_t, (_Float16)v[2 * j + 1]);
+            } else {
+                lo = __builtin_bit_cast(uint16_t, (__bf16)v[2 * j]);
+                hi = __builtin_bit_cast(uint16_t, (__bf16)v[2 * j + 1]);
+            }
+            a[j] = lo | (hi << 16);
+        }
+        *(u4*)((uint16_t*)p + i) = a;
+    }
+}
+
+// Which tokens a wave handles: tile `x` of the positions of sequence b's newest
+// seq tokens, position lens[b] - seq + token. False: no memory behind the tile.
+struct TileAt {
+    long long pos;      // of the tile's first token
+    long long p0;       // of token 0
+    long long end;      // positions from here on hold nothing
+    uint8_t* part;      // the head's part of the page; NULL: none
+    int in_page;        // tile within the page
+};
+__device__ __forceinline__ TileAt tile_at(const KvCache& c, const KvTokens& t, int b, int head, int x) {
+    TileAt r;
+    const long long len = t.lens[b], cap = (long long)t.max_pages * c.page_size;
+    r.p0 = len - t.seq;
+    r.pos = ((r.p0 >> 5) + x) * 32;
+    r.end = len < cap ? len : cap;
+    r.part = nullptr;
+    r.in_page = 0;
+    if (r.pos >= 0 && r.pos < r.end) {
+        const int pi = (int)(r.pos / c.page_size);
+        const int id = t.table[(long long)b * t.max_pages + pi];
+        if (id >= 0 && id < c.num_pages) {
+            r.part = c.data + ((long long)id * c.heads + head) * kv_head_bytes(c.page_size, c.hd, c.bits);
+            r.in_page = (int)(r.pos - (long long)pi * c.page_size) / 32;
+        }
+    }
+    return r;
+}
+// tokens of a tile that hold something and are among the call's seq
+__device__ __forceinline__ bool token_in(const TileAt& w, int seq, int t) {
+    const long long p = w.pos + t;
+    return w.part && p >= 0 && p >= w.p0 && p < w.end && p < w.p0 + seq;
+}
+
+__device__ __forceinline__ float finite_abs(float v) {
+    const float a = fabsf(v);
+    return a < __builtin_inff() ? a : 0.0f;
+}
+__device__ __forceinline__ float across_groups_max(float m) {   // lanes of one token
+    m = fmaxf(m, __shfl_xor(m, 16));
+    return fmaxf(m, __shfl_xor(m, 32));
+}
+__device__ __forceinline__ float scale_of(float top, float limit) {
+    const float s = (float)(__bf16)(top / limit);
+    return s >= 1.17549435e-38f ? s : 0.0f;
+}
+__device__ __forceinline__ int code_of(float v, float s, float limit) {
+    if (s == 0.0f || !(v == v)) return 0;
+    return (int)fminf(fmaxf(rintf(v / s), -limit), limit);
+}
+// nibbles in the order of a word (j even: j / 2, j odd: 4 + j / 2)
+__device__ __forceinline__ uint32_t pack_nibbles(const uint32_t* q) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w |= q[j] << (4 * ((j >> 1) + 4 * (j & 1)));
+    return w;
+}
+__device__ __forceinline__ uint32_t nibble(uint32_t w, int j) { return (w >> (4 * ((j >> 1) + 4 * (j & 1)))) & 15u; }
+
+// One wave a (tile of 32 positions, head, sequence, keys or values). Lanes read
+// 8 neighbouring elements of a token, form scales and codes, and store keys as
+// they are; values pass through LDS, where an element's tokens come together.
+// A tile whose tokens are not all written is merged with what it holds: no
+// other wave of the launch has this tile.
+template <int TY, int BITS, int HD>
+__global__ __launch_bounds__(64) void kv_write_kernel(KvCache c, KvTokens t) {
+    constexpr int NC = HD / 32;
+    constexpr float limit = BITS == 8 ? 127.0f : 7.0f;
+    constexpr int zero = BITS == 8 ? 128 : 8;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[HD * kLdsRow];
+    const int lane = threadIdx.x, g = lane >> 4;
+    const int values = blockIdx.y & 1, head = blockIdx.y >> 1, b = blockIdx.z;
+    const TileAt w = tile_at(c, t, b, head, blockIdx.x);
+    if (!w.part) return;
+    const void* src = values ? t.v : t.k;
+    bool in[2];
+    float x[2][NC][8], sc[2][NC];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int tok = (lane & 15) + 16 * h;
+        in[h] = token_in(w, t.seq, tok);
+        const long long at = (long long)b * t.bstride + (w.pos + tok - w.p0) * t.tstride + (long long)head * HD + 8 * g;
+#pragma unroll
+        for (int k = 0; k < NC; ++k) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[h][k][j] = 0.0f;
+            if (in[h]) load8<TY>(src, at + 32 * k, x[h][k]);
+        }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        float all = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NC; ++k) {
+            float m = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) m = fmaxf(m, finite_abs(x[h][k][j]));
+            if (BITS == 8) all = fmaxf(all, m);
+            else sc[h][k] = scale_of(across_groups_max(m), limit);
+        }
+        if (BITS == 8) {
+            all = scale_of(across_groups_max(all), limit);
+#pragma unroll
+            for (int k = 0; k < NC; ++k) sc[h][k] = all;
+        }
+    }
+    const long long cb = kv_codes_bytes(c.page_size, HD, BITS);
+    uint8_t* codes = w.part + (values ? cb : 0);
+    __bf16* scales = (__bf16*)(w.part + 2 * cb) + (values ? (long long)c.page_size * kv_groups(HD, BITS) : 0);
+    if (g == 0) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            if (in[h])
+#pragma unroll
+                for (int k = 0; k < (BITS == 8 ? 1 : NC); ++k)
+                    scales[(long long)k * c.page_size + w.in_page * 32 + kv_slot((lane & 15) + 16 * h)] = (__bf16)sc[h][k];
+    }
+    constexpr int BB = BITS == 8 ? 1024 : 512;   // bytes of a block
+    uint8_t* blocks = codes + (long long)w.in_page * NC * BB;
+    if (!values) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (!in[h]) continue;
+#pragma unroll
+            for (int k = 0; k < NC; ++k) {
+                uint32_t q[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) q[j] = (uint32_t)(code_of(x[h][k][j], sc[h][k], limit) + zero);
+                if constexpr (BITS == 8)
+                    *(u2*)(blocks + k * BB + lane * 16 + h * 8) =
+                        u2{q[0] | q[1] << 8 | q[2] << 16 | q[3] << 24, q[4] | q[5] << 8 | q[6] << 16 | q[7] << 24};
+                else
+                    *(uint32_t*)(blocks + k * BB + lane * 8 + h * 4) = pack_nibbles(q);
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int k = 0; k < NC; ++k)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                lds[(32 * k + 8 * g + j) * kLdsRow + kv_slot((lane & 15) + 16 * h)] =
+                    (uint8_t)(code_of(x[h][k][j], sc[h][k], limit) + zero);
+    __syncthreads();
+    // this lane's 8 tokens: slots 8 g .. 8 g + 7
+    uint32_t keep = 0;   // bit j: slot 8 g + j is not written
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        if (!token_in(w, t.seq, 4 * g + (j & 3) + 16 * (j >> 2))) keep |= 1u << j;
+    if (keep == 0xff) return;
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+        u2 e[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) e[h] = *(const u2*)(lds + (32 * k + (lane & 15) + 16 * h) * kLdsRow + 8 * g);
+        if constexpr (BITS == 8) {
+            u4 out = {e[0][0], e[0][1], e[1][0], e[1][1]};
+            u4* to = (u4*)(blocks + k * BB + lane * 16);
+            if (keep) {
+                const u4 old = *to;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t m = 0;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (keep >> (4 * (i & 1) + j) & 1) m |= 0xffu << (8 * j);
+                    out[i] = (out[i] & ~m) | (old[i] & m);
+                }
+            }
+            *to = out;
+        } else {
+            u2 out;
+            u2* to = (u2*)(blocks + k * BB + lane * 8);
+            uint32_t m = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (keep >> j & 1) m |= 15u << (4 * ((j >> 1) + 4 * (j & 1)));
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint32_t q[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) q[j] = (e[h][j >> 2] >> (8 * (j & 3))) & 0xff;
+                out[h] = pack_nibbles(q);
+            }
+            if (keep) {
+                const u2 old = *to;
+                out = (out & ~m) | (old & m);
+            }
+            *to = out;
+        }
+    }
+}
+
+// The same wave the other way; a position that holds no token reads as zeros.
+template <int TY, int BITS, int HD>
+__global__ __launch_bounds__(64) void kv_read_kernel(KvCache c, KvTokens t) {
+    constexpr int NC = HD / 32;
+    constexpr int zero = BITS == 8 ? 128 : 8;
+    constexpr int BB = BITS == 8 ? 1024 : 512;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[HD * kLdsRow];
+    const int lane = threadIdx.x, g = lane >> 4;
+    const int values = blockIdx.y & 1, head = blockIdx.y >> 1, b = blockIdx.z;
+    const TileAt w = tile_at(c, t, b, head, blockIdx.x);
+    const long long cb = kv_codes_bytes(c.page_size, HD, BITS);
+    if (w.part && values) {
+        const uint8_t* blocks = w.part + cb + (long long)w.in_page * NC * BB;
+#pragma unroll
+        for (int k = 0; k < NC; ++k) {
+            u2 e[2];
+            if constexpr (BITS == 8) {
+                const u4 v = *(const u4*)(blocks + k * BB + lane * 16);
+                e[0] = u2{v[0], v[1]};
+                e[1] = u2{v[2], v[3]};
+            } else {
+                const u2 v = *(const u2*)(blocks + k * BB + lane * 8);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    e[h] = u2{0, 0};
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) e[h][j >> 2] |= nibble(v[h], j) << (8 * (j & 3));
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) *(u2*)(lds + (32 * k + (lane & 15) + 16 * h) * kLdsRow + 8 * g) = e[h];
+        }
+    }
+    __syncthreads();
+    void* dst = values ? t.v : t.k;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int tok = (lane & 15) + 16 * h;
+        const long long s = w.pos + tok - w.p0;
+        if (s < 0 || s >= t.seq) continue;
+        const bool in = token_in(w, t.seq, tok);
+        const long long at = (long long)b * t.bstride + s * t.tstride + (long long)head * HD + 8 * g;
+        const uint8_t* blocks = w.part + (long long)w.in_page * NC * BB;
+        const __bf16* scales = (const __bf16*)(w.part + 2 * cb) + (values ? (long long)c.page_size * kv_groups(HD, BITS) : 0);
+#pragma unroll
+        for (int k = 0; k < NC; ++k) {
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = 0.0f;
+            if (in) {
+                const float sc = (float)scales[(long long)(BITS == 8 ? 0 : k) * c.page_size + w.in_page * 32 + kv_slot(tok)];
+                u2 q = {0, 0};
+                uint32_t n = 0;
+                if (!values) {
+                    if constexpr (BITS == 8) q = *(const u2*)(blocks + k * BB + lane * 16 + h * 8);
+                    else n = *(const uint32_t*)(blocks + k * BB + lane * 8 + h * 4);
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    int code;
+                    if (values) code = lds[(32 * k + 8 * g + j) * kLdsRow + kv_slot(tok)];
+                    else if constexpr (BITS == 8) code = (q[j >> 2] >> (8 * (j & 3))) & 0xff;
+                    else code = nibble(n, j);
+                    x[j] = (float)(code - zero) * sc;
+                }
+            }
+            store8<TY>(dst, at + 32 * k, x);
+        }
+    }
+}
+
+template <int TY, int BITS, int HD>
+hipError_t go(bool write, const KvCache& c, const KvTokens& t, hipStream_t s) {
+    // seq positions from anywhere in a tile on
+    const dim3 grid((unsigned)(((long long)t.seq + 62) / 32), (unsigned)(2 * c.heads), (unsigned)t.batch);
+    if (write) kv_write_kernel<TY, BITS, HD><<<grid, 64, 0, s>>>(c, t);
+    else kv_read_kernel<TY, BITS, HD><<<grid, 64, 0, s>>>(c, t);
+    return hipGetLastError();
+}
+template <int TY, int BITS>
+hipError_t by_hd(bool write, const KvCache& c, const KvTokens& t, hipStream_t s) {
+    switch (c.hd) {
+    case 64: return go<TY, BITS, 64>(write, c, t, s);
+    case 96: return go<TY, BITS, 96>(write, c, t, s);
+    case 128: return go<TY, BITS, 128>(write, c, t, s);
+    case 256: return go<TY, BITS, 256>(write, c, t, s);
+    }
+    return hipErrorInvalidValue;
+}
+hipError_t by_type(bool write, const KvCache& c, const KvTokens& t, hipStream_t s) {
+    if (t.batch == 0 || t.seq == 0) return hipSuccess;
+    if (c.bits == 8)
+        return t.type == FT_F32 ? by_hd<FT_F32, 8>(write, c, t, s)
+             : t.type == FT_F16 ? by_hd<FT_F16, 8>(write, c, t, s) : by_hd<FT_BF16, 8>(write, c, t, s);
+    return t.type == FT_F32 ? by_hd<FT_F32, 4>(write, c, t, s)
+         : t.type == FT_F16 ? by_hd<FT_F16, 4>(write, c, t, s) : by_hd<FT_BF16, 4>(write, c, t, s);
+}
+
+}  // namespace
+
+hipError_t launch_kv_write(const KvCache& c, const KvTokens& t, hipStream_t s) { return by_type(true, c, t, s); }
+hipError_t launch_kv_read(const KvCache& c, const KvTokens& t, hipStream_t s) { return by_type(false, c, t, s); }
+
+}  // namespace nnrh
