@@ -13,7 +13,7 @@ import ctypes as ct
 
 import numpy as np
 
-from ._lib import (BRANCH_NAMES, F16, F32, I32, NNRH_ERR_UNSUPPORTED, S8, U8, NnrHipError,  # noqa: F401
+from ._lib import (BF16, BRANCH_NAMES, F16, F32, I32, NNRH_ERR_UNSUPPORTED, S8, U8, NnrHipError,  # noqa: F401
                    KvAttentionDesc, KvCacheDesc, KvTokens, MatMulNBitsDesc, QConvDesc,
                    QMatMulDesc, check, cur_stream, lib, ptr)
 
@@ -552,21 +552,27 @@ def maxpool_u8_nhwc(x, kH, kW, sH, sW, pH, pW, oH, oW):
 
 def _float_dt(dtype) -> int:
     import torch
-    from ._lib import BF16
-    dt = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}.get(dtype)
-    if dt is None:
-        raise TypeError(f"{dtype}: float32, float16 or bfloat16")
-    return dt
+    if dtype is torch.float16:
+        return F16
+    if dtype is torch.bfloat16:
+        return BF16
+    if dtype is torch.float32:
+        return F32
+    raise TypeError(f"{dtype}: float32, float16 or bfloat16")
 
 
-def _launch(device, stream, call):
-    """call(stream) with the tensors' device current, on their current stream unless one is given."""
-    import torch
-    if device.index == torch.cuda.current_device():
-        check(call(torch.cuda.current_stream().cuda_stream if stream is None else stream))
-        return
-    with torch.cuda.device(device):
-        check(call(torch.cuda.current_stream().cuda_stream if stream is None else stream))
+def _launch(index, stream, fn, *args):
+    """fn(*args, stream) with device `index` current, on its current stream
+    unless one is given."""
+    from torch import _C
+    if _C._cuda_getDevice() == index:
+        rc = fn(*args, _C._cuda_getCurrentRawStream(index) if stream is None else stream)
+    else:
+        import torch
+        with torch.cuda.device(index):
+            rc = fn(*args, _C._cuda_getCurrentRawStream(index) if stream is None else stream)
+    if rc:
+        check(rc)
 
 
 def _on_device(device, **tensors):
@@ -609,19 +615,20 @@ class MatMulNBits:
 
     def __call__(self, a, y=None, stream=None):
         """a [..., k] -> y [..., n]"""
-        import torch
-        if a.dtype != self.dtype or a.shape[-1] != self.k:
+        shape = a.shape
+        if a.dtype != self.dtype or shape[-1] != self.k:
             raise ValueError(f"a must be {self.dtype} [..., {self.k}]")
-        _on_device(self.device, a=a)
-        a = a.contiguous()
-        shape = (*a.shape[:-1], self.n)
+        if a.device != self.device:
+            _on_device(self.device, a=a)
+        if not a.is_contiguous():
+            a = a.contiguous()
+        shape = (*shape[:-1], self.n)
         if y is None:
-            y = torch.empty(shape, dtype=self.dtype, device=a.device)
-        elif y.shape != shape or y.dtype != self.dtype or y.device != a.device or not y.is_contiguous():
-            raise ValueError(f"y must be contiguous {self.dtype} of shape {shape} on {a.device}")
-        m = a.numel() // self.k
-        run = lib().nnrh_matmul_nbits_run
-        _launch(self.device, stream, lambda s: run(self.h, a.data_ptr(), y.data_ptr(), m, s))
+            y = a.new_empty(shape)
+        elif y.shape != shape or y.dtype != self.dtype or y.device != self.device or not y.is_contiguous():
+            raise ValueError(f"y must be contiguous {self.dtype} of shape {shape} on {self.device}")
+        _launch(self.device.index, stream, lib().nnrh_matmul_nbits_run, self.h, a.data_ptr(), y.data_ptr(),
+                a.numel() // self.k)
         return y
 
     def __del__(self):
@@ -654,19 +661,23 @@ class KVCache:
         self.head_dim, self.bits = int(head_dim), int(bits)
 
     def _tables(self, batch, page_table, seq_lens):
-        import torch
-        if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != batch:
+        from torch import int32
+        if page_table.dtype != int32 or page_table.dim() != 2 or page_table.shape[0] != batch:
             raise ValueError(f"page_table must be int32 [{batch}][pages]")
-        if seq_lens.dtype != torch.int32 or tuple(seq_lens.shape) != (batch,):
+        if seq_lens.dtype != int32 or seq_lens.shape != (batch,):
             raise ValueError(f"seq_lens must be int32 [{batch}]")
-        _on_device(self.device, page_table=page_table, seq_lens=seq_lens)
-        return page_table.contiguous(), seq_lens.contiguous()
+        if page_table.device != self.device or seq_lens.device != self.device:
+            _on_device(self.device, page_table=page_table, seq_lens=seq_lens)
+        if not page_table.is_contiguous():
+            page_table = page_table.contiguous()
+        return page_table, seq_lens.contiguous()
 
     def _rows(self, name, t, heads):
         """t with dense heads and 16-byte steps: itself, or a copy."""
         if t.dim() != 4 or t.shape[2] != heads or t.shape[3] != self.head_dim:
             raise ValueError(f"{name} must be [batch, seq, {heads}, {self.head_dim}]")
-        _on_device(self.device, **{name: t})
+        if t.device != self.device:
+            _on_device(self.device, **{name: t})
         st, es = t.stride(), t.element_size()
         if (st[3] != 1 or (heads > 1 and st[2] != self.head_dim) or t.data_ptr() % 16 or st[0] * es % 16 or
                 st[1] * es % 16):
@@ -677,8 +688,9 @@ class KVCache:
 
     def _tokens(self, k, page_table, seq_lens):
         B, S = k.shape[:2]
-        return KvTokens(_float_dt(k.dtype), B, S, k.stride(0), k.stride(1), page_table.data_ptr(),
-                        page_table.shape[1], seq_lens.data_ptr())
+        st = k.stride()
+        return KvTokens(_float_dt(k.dtype), B, S, st[0], st[1], page_table.data_ptr(), page_table.shape[1],
+                        seq_lens.data_ptr())
 
     def write(self, k, v, page_table, seq_lens, stream=None):
         """Token s of sequence b to position seq_lens[b] - seq + s; tokens at
@@ -689,8 +701,8 @@ class KVCache:
         if k.stride() != v.stride():
             k, v = k.contiguous(), v.contiguous()
         page_table, seq_lens = self._tables(k.shape[0], page_table, seq_lens)
-        t, run = self._tokens(k, page_table, seq_lens), lib().nnrh_kv_cache_write
-        _launch(self.device, stream, lambda s: run(self.desc, self.data.data_ptr(), t, k.data_ptr(), v.data_ptr(), s))
+        _launch(self.device.index, stream, lib().nnrh_kv_cache_write, self.desc, self.data.data_ptr(),
+                self._tokens(k, page_table, seq_lens), k.data_ptr(), v.data_ptr())
 
     def read(self, seq, page_table, seq_lens, dtype, stream=None):
         """(k, v) of positions seq_lens[b] - seq .. seq_lens[b] - 1 as `dtype`; zeros
@@ -698,10 +710,17 @@ class KVCache:
         import torch
         B = page_table.shape[0]
         page_table, seq_lens = self._tables(B, page_table, seq_lens)
-        k, v = (torch.empty((B, seq, self.kv_heads, self.head_dim), dtype=dtype, device=self.device) for _ in "kv")
-        t, run = self._tokens(k, page_table, seq_lens), lib().nnrh_kv_cache_read
-        _launch(self.device, stream, lambda s: run(self.desc, self.data.data_ptr(), t, k.data_ptr(), v.data_ptr(), s))
+        k, v = torch.empty((2, B, seq, self.kv_heads, self.head_dim), dtype=dtype, device=self.device).unbind(0)
+        _launch(self.device.index, stream, lib().nnrh_kv_cache_read, self.desc, self.data.data_ptr(),
+                self._tokens(k, page_table, seq_lens), k.data_ptr(), v.data_ptr())
         return k, v
+
+    def attention_workspace(self, batch, seq, q_heads, max_pages, prefix_len=0):
+        """Bytes of workspace that such an attention takes, whatever the lengths."""
+        d = KvAttentionDesc(F32, batch, seq, q_heads, 0, 0, 1.0, None, max_pages, None, None, int(prefix_len))
+        n = ct.c_size_t()
+        check(lib().nnrh_kv_attention_workspace(self.desc, d, n))
+        return n.value
 
     def attention(self, q, page_table, seq_lens, scale=None, prefix_table=None, prefix_len=0, y=None, workspace=None,
                   stream=None):
@@ -709,14 +728,13 @@ class KVCache:
         (b, s) sees the first prefix_len tokens of the pages in prefix_table
         (int32 [pages], shared by the batch) and positions up to seq_lens[b] -
         seq + s of its own. workspace: a uint8 tensor of attention_workspace's
-        size, made by the call unless given (a call on a stream that is not
-        current should bring it)."""
+        size, 256-byte aligned, made by the call unless given (a call on a
+        stream that is not current should bring it)."""
         import torch
         if q.dim() != 4:
             raise ValueError("q must be [batch, seq, heads, head_dim]")
-        Hq = q.shape[2]
+        B, S, Hq, _ = q.shape
         q = self._rows("q", q, Hq)
-        B, S = q.shape[:2]
         page_table, seq_lens = self._tables(B, page_table, seq_lens)
         if y is None:
             y = torch.empty((B, S, Hq, self.head_dim), dtype=q.dtype, device=self.device)
@@ -730,16 +748,22 @@ class KVCache:
             _on_device(self.device, prefix_table=prefix_table)
             prefix_table = prefix_table.contiguous()
             pt = prefix_table.data_ptr()
-        d = KvAttentionDesc(_float_dt(q.dtype), B, S, Hq, q.stride(0), q.stride(1),
+        st = q.stride()
+        d = KvAttentionDesc(_float_dt(q.dtype), B, S, Hq, st[0], st[1],
                             self.head_dim ** -0.5 if scale is None else float(scale), page_table.data_ptr(),
                             page_table.shape[1], seq_lens.data_ptr(), pt, int(prefix_len))
         n = ct.c_size_t()
-        check(lib().nnrh_kv_attention_workspace(self.desc, d, n))
-        if workspace is None:
-            workspace = torch.empty(n.value, dtype=torch.uint8, device=self.device) if n.value else None
-        elif workspace.dtype != torch.uint8 or workspace.numel() < n.value or workspace.device != self.device:
-            raise ValueError(f"workspace must be uint8 of at least {n.value} elements on {self.device}")
-        run = lib().nnrh_kv_attention
-        _launch(self.device, stream, lambda s: run(self.desc, self.data.data_ptr(), d, q.data_ptr(), y.data_ptr(),
-                                                   ptr(workspace), s))
+        rc = lib().nnrh_kv_attention_workspace(self.desc, d, n)
+        if rc:
+            check(rc)
+        ws = None
+        if n.value:
+            if workspace is None:
+                workspace = torch.empty(n.value, dtype=torch.uint8, device=self.device)
+            elif workspace.dtype != torch.uint8 or workspace.numel() < n.value or workspace.device != self.device or \
+                    not workspace.is_contiguous():
+                raise ValueError(f"workspace must be contiguous uint8 of at least {n.value} elements on {self.device}")
+            ws = workspace.data_ptr()
+        _launch(self.device.index, stream, lib().nnrh_kv_attention, self.desc, self.data.data_ptr(), d, q.data_ptr(),
+                y.data_ptr(), ws)
         return y

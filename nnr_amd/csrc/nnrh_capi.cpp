@@ -2291,7 +2291,7 @@ int nbits_build(nnrh_matmul_nbits* h, const nnrh_matmul_nbits_desc* d) {
     const size_t pieces = (size_t)(nbits_cols(d->n) / 16) * h->a.P;
     if ((rc = nnrh_malloc((void**)&h->w, pieces * 1024)) ||
         (rc = nnrh_malloc(&h->scales, pieces * 16 * h->a.nspp * es)) ||
-        (d->zero_points_host && (rc = nnrh_malloc((void**)&h->zp, pieces * 32))))
+        (rc = nnrh_malloc((void**)&h->zp, (d->zero_points_host ? pieces : 1) * 32)))
         return rc;
     HIP_TRY(launch_nbits_pack(raw.p, raw_scales.p, raw_zp.p, d->n, d->k, d->block_size, h->a.type, h->w, h->scales,
                               h->zp, nullptr),
@@ -2301,6 +2301,7 @@ int nbits_build(nnrh_matmul_nbits* h, const nnrh_matmul_nbits_desc* d) {
     h->a.w = h->w;
     h->a.scales = h->scales;
     h->a.zp = h->zp;
+    h->a.zp_mask = d->zero_points_host ? -1 : 0;
     h->a.bias = h->bias;
     return NNRH_OK;
 }

@@ -24,7 +24,8 @@ struct NbitsArgs {
     const void* a;
     const uint32_t* w;                     // [Np / 16][P] pieces
     const void* scales;                    // [Np / 16][P][16][nspp], activations' type
-    const uint16_t* zp;                    // [Np / 16][P][16], nibble s for word s; NULL: 8
+    const uint16_t* zp;                    // [Np / 16][P][16], nibble s for word s; without
+    long long zp_mask;                     // zero points one piece's 8s for all: 0, else -1
     const void* bias;                      // [N] or NULL, activations' type
     void* y;
     int M, N, K, P;

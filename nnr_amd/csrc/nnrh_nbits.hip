@@ -66,37 +66,50 @@ __device__ __forceinline__ AFrag<FT_F32> split3(const float* x) {
     return f;
 }
 
-// k .. k+7 of a row; elements from K on are 0. vec: 16-byte loads are aligned
-// and no 16 bytes straddle K.
-template <int TY>
-__device__ __forceinline__ AFrag<TY> load_a(const void* row, int k, int K, bool vec) {
-    if constexpr (TY == FT_F32) {
-        float x[8];
-        if (vec) {
-            f4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
-            if (k < K) lo = *(const f4*)((const float*)row + k);
-            if (k + 4 < K) hi = *(const f4*)((const float*)row + k + 4);
+// How a block reads activations: 16 bytes at a time where addresses allow it
+// (whole pieces of K, or with the last one cut short), else element by element
+enum AMode : int { A_WHOLE = 0, A_EDGE = 1, A_ANY = 2 };
+
+// k .. k + 7 of a row, as they lie; elements from K on are 0
+template <int TY> struct ARaw {
+    u4 v[TY == FT_F32 ? 2 : 1];
+    template <int AM>
+    __device__ __forceinline__ void load(const void* row, int k, int K) {
+        constexpr int N = TY == FT_F32 ? 4 : 8;   // elements of 16 bytes
+        constexpr int ES = TY == FT_F32 ? 4 : 2;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) { x[j] = lo[j]; x[4 + j] = hi[j]; }
-        } else {
+        for (int i = 0; i < (TY == FT_F32 ? 2 : 1); ++i, k += N) {
+            if constexpr (AM == A_WHOLE) {
+                v[i] = *(const u4*)((const char*)row + (long long)k * ES);
+            } else if constexpr (AM == A_EDGE) {   // no branch: loads stay in flight past it
+                const bool in = k < K;
+                const u4 x = *(const u4*)((const char*)row + (long long)(in ? k : 0) * ES);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = k + j < K ? ((const float*)row)[k + j] : 0.0f;
+                for (int j = 0; j < 4; ++j) v[i][j] = in ? x[j] : 0u;
+            } else {
+                v[i] = u4{0, 0, 0, 0};
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+                    if (k + j < K) {
+                        if constexpr (TY == FT_F32) v[i][j] = ((const uint32_t*)row)[k + j];
+                        else v[i][j >> 1] |= (uint32_t)((const uint16_t*)row)[k + j] << (16 * (j & 1));
+                    }
+            }
         }
-        return split3(x);
-    } else {
-        AFrag<TY> f;
-        u4 v = {0, 0, 0, 0};
-        if (vec) {
-            if (k < K) v = *(const u4*)((const uint16_t*)row + k);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (k + j < K) v[j >> 1] |= (uint32_t)((const uint16_t*)row)[k + j] << (16 * (j & 1));
-        }
-        f.p[0] = v;
-        return f;
     }
-}
+    __device__ __forceinline__ AFrag<TY> frag() const {
+        if constexpr (TY == FT_F32) {
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = __builtin_bit_cast(float, (uint32_t)v[j >> 2][j & 3]);
+            return split3(x);
+        } else {
+            AFrag<TY> f;
+            f.p[0] = v[0];
+            return f;
+        }
+    }
+};
 
 // q - zp of a word's 8 nibbles as an MFMA operand
 __device__ __forceinline__ h8 weights_f16(uint32_t w, h2 off) {
@@ -110,17 +123,16 @@ __device__ __forceinline__ h8 weights_f16(uint32_t w, h2 off) {
     }
     return r;
 }
+// A byte 0 .. 15 read as e4m3 is q * 2^-9, below 8 as a subnormal: one
+// instruction turns two of them into floats, and a multiply-add gives q - zp.
 __device__ __forceinline__ b8 weights_bf16(uint32_t w, float zp) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
     const uint32_t lo = w & 0x0f0f0f0fu, hi = (w >> 4) & 0x0f0f0f0fu;   // elements 0 4 1 5 and 2 6 3 7
-    float v[8];
-    v[0] = (float)(lo & 0xff) - zp;
-    v[4] = (float)((lo >> 8) & 0xff) - zp;
-    v[1] = (float)((lo >> 16) & 0xff) - zp;
-    v[5] = (float)(lo >> 24) - zp;
-    v[2] = (float)(hi & 0xff) - zp;
-    v[6] = (float)((hi >> 8) & 0xff) - zp;
-    v[3] = (float)((hi >> 16) & 0xff) - zp;
-    v[7] = (float)(hi >> 24) - zp;
+    const f2 v04 = __builtin_amdgcn_cvt_pk_f32_fp8(lo, false), v15 = __builtin_amdgcn_cvt_pk_f32_fp8(lo, true);
+    const f2 v26 = __builtin_amdgcn_cvt_pk_f32_fp8(hi, false), v37 = __builtin_amdgcn_cvt_pk_f32_fp8(hi, true);
+    float v[8] = {v04[0], v15[0], v26[0], v37[0], v04[1], v15[1], v26[1], v37[1]};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __builtin_fmaf(v[i], 512.0f, -zp);
     u4 r;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -130,14 +142,47 @@ __device__ __forceinline__ b8 weights_bf16(uint32_t w, float zp) {
 
 constexpr int NB_WAVES = 8;
 
+// scales of a piece and column, as they lie
+template <int TY, int NSPP> struct Scales {
+    static constexpr int W = TY == FT_F32 ? NSPP : (NSPP + 1) / 2;   // words
+    uint32_t w[W];
+    __device__ __forceinline__ void load(const void* p, long long at) {   // at: piece x 16 + column
+        if constexpr (TY != FT_F32 && NSPP == 1) {
+            w[0] = ((const uint16_t*)p)[at];
+        } else {
+            typedef uint32_t vec __attribute__((ext_vector_type(W)));
+            const vec v = ((const vec*)p)[at];
+            if constexpr (W == 1) w[0] = __builtin_bit_cast(uint32_t, v);
+            else
+#pragma unroll
+                for (int i = 0; i < W; ++i) w[i] = v[i];
+        }
+    }
+    __device__ __forceinline__ float get(int s) const {
+        if constexpr (TY == FT_F32) return __builtin_bit_cast(float, w[s]);
+        const uint32_t v = w[s / 2] >> (16 * (s & 1)) & 0xffffu;
+        return TY == FT_F16 ? f16_f32((uint16_t)v) : bf16_f32(v);
+    }
+};
+
+// The weights of one piece of K, loaded well before they are used
+template <int TY, int NSPP, int NT> struct Stage {
+    u4 w[NT];
+    Scales<TY, NSPP> sc[NT];
+    uint32_t zp[NT];
+};
+
 // One block: MT x 16 rows, NT x 16 columns, all of K. Its waves take pieces of
-// K in turn, straight from memory into registers, and their sums meet in LDS.
-template <int TY, int NSPP, int MT, int NT>
-__global__ __launch_bounds__(NB_WAVES * 64) void nbits_kernel(NbitsArgs p, int vec) {
+// K in turn, straight from memory into registers, in rounds of D pieces each:
+// a round's weights are loaded before the one before is multiplied, a piece's
+// activations as those of the piece before are used up. The waves' sums meet
+// in LDS.
+template <int TY, int NSPP, int AM, int MT, int NT, int D>
+__global__ __launch_bounds__(NB_WAVES * 64) void nbits_kernel(NbitsArgs p) {
     __shared__ f4 red[NB_WAVES][MT * NT][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
-    const long long tile0 = (long long)blockIdx.x * NT;
+    const int tile0 = blockIdx.x * NT;
     const int m0 = blockIdx.y * (16 * MT);
     constexpr int ES = TY == FT_F32 ? 4 : 2;
     const char* row[MT];
@@ -152,56 +197,82 @@ __global__ __launch_bounds__(NB_WAVES * 64) void nbits_kernel(NbitsArgs p, int v
 #pragma unroll
         for (int u = 0; u < NT; ++u) acc[t][u] = f4{0, 0, 0, 0};
 
-    for (int piece = wave; piece < p.P; piece += NB_WAVES) {
-        u4 w[NT];
-        float sc[NT][NSPP];
-        uint32_t zp[NT];
+    const int last = p.P - 1;
+    ARaw<TY> a[4][MT];
+    auto load_w = [&](Stage<TY, NSPP, NT>* x, int piece) {
 #pragma unroll
-        for (int u = 0; u < NT; ++u) {
-            const long long pc = (tile0 + u) * p.P + piece;
-            w[u] = *(const u4*)(p.w + pc * 256 + lane * 4);
+        for (int d = 0; d < D; ++d) {
+            const int at = min(piece + d * NB_WAVES, last);
 #pragma unroll
-            for (int s = 0; s < NSPP; ++s) sc[u][s] = load_f32<TY>(p.scales, (pc * 16 + col) * NSPP + s);
-            zp[u] = p.zp ? p.zp[pc * 16 + col] : 0x8888u;
+            for (int u = 0; u < NT; ++u) {
+                const long long pc = (long long)(tile0 + u) * p.P + at;
+                x[d].w[u] = *(const u4*)(p.w + pc * 256 + lane * 4);
+                x[d].sc[u].load(p.scales, pc * 16 + col);
+                x[d].zp[u] = p.zp[(pc & p.zp_mask) * 16 + col];
+            }
         }
+    };
+    auto load_a = [&](int s, int piece) {
+#pragma unroll
+        for (int t = 0; t < MT; ++t) a[s][t].template load<AM>(row[t], piece * NB_PK + 32 * s + 8 * g, p.K);
+    };
+    auto multiply = [&](const Stage<TY, NSPP, NT>& x, int next) {
         f4 part[MT][NT];
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-            AFrag<TY> a[MT];
+            AFrag<TY> f[MT];
 #pragma unroll
-            for (int t = 0; t < MT; ++t) a[t] = load_a<TY>(row[t], piece * NB_PK + 32 * s + 8 * g, p.K, vec);
+            for (int t = 0; t < MT; ++t) f[t] = a[s][t].frag();
+            load_a(s, next);
             constexpr int SPS = 4 / NSPP;   // MFMA steps a scale
 #pragma unroll
             for (int u = 0; u < NT; ++u) {
-                const uint32_t z = (zp[u] >> (4 * s)) & 15;
+                const uint32_t z = (x.zp[u] >> (4 * s)) & 15;
                 if constexpr (TY == FT_F16) {
-                    const _Float16 o = (_Float16)(float)(1024 + z);
-                    const h8 b = weights_f16(w[u][s], h2{o, o});
+                    const uint32_t o = (0x6400u + z) * 0x10001u;   // 1024 + zp, twice
+                    const h8 b = weights_f16(x.w[u][s], __builtin_bit_cast(h2, o));
 #pragma unroll
                     for (int t = 0; t < MT; ++t)
                         part[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                            __builtin_bit_cast(h8, a[t].p[0]), b, s % SPS ? part[t][u] : f4{0, 0, 0, 0}, 0, 0, 0);
+                            __builtin_bit_cast(h8, f[t].p[0]), b, s % SPS ? part[t][u] : f4{0, 0, 0, 0}, 0, 0, 0);
                 } else {
-                    const b8 b = weights_bf16(w[u][s], (float)z);
+                    const b8 b = weights_bf16(x.w[u][s], (float)z);
 #pragma unroll
                     for (int t = 0; t < MT; ++t) {
                         if (s % SPS == 0) part[t][u] = f4{0, 0, 0, 0};
 #pragma unroll
                         for (int q = 0; q < kPieces<TY>; ++q)
                             part[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                                __builtin_bit_cast(b8, a[t].p[q]), b, part[t][u], 0, 0, 0);
+                                __builtin_bit_cast(b8, f[t].p[q]), b, part[t][u], 0, 0, 0);
                     }
                 }
                 if (s % SPS == SPS - 1) {
+                    const float sc = x.sc[u].get(s / SPS);
 #pragma unroll
                     for (int t = 0; t < MT; ++t)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            acc[t][u][i] = __builtin_fmaf(part[t][u][i], sc[u][s / SPS], acc[t][u][i]);
+                        for (int i = 0; i < 4; ++i) acc[t][u][i] = __builtin_fmaf(part[t][u][i], sc, acc[t][u][i]);
                 }
             }
+            if (NSPP == 4 && MT == 4) __builtin_amdgcn_sched_barrier(0);   // one step's block sums at a time, or registers spill
         }
+    };
+    Stage<TY, NSPP, NT> cur[D];
+    load_w(cur, wave);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) load_a(s, min(wave, last));
+    int piece = wave;
+    for (; piece + D * NB_WAVES < p.P; piece += D * NB_WAVES) {
+        Stage<TY, NSPP, NT> nxt[D];
+        load_w(nxt, piece + D * NB_WAVES);
+#pragma unroll
+        for (int d = 0; d < D; ++d) multiply(cur[d], min(piece + (d + 1) * NB_WAVES, last));
+#pragma unroll
+        for (int d = 0; d < D; ++d) cur[d] = nxt[d];
     }
+#pragma unroll
+    for (int d = 0; d < D; ++d)
+        if (piece + d * NB_WAVES < p.P) multiply(cur[d], min(piece + (d + 1) * NB_WAVES, last));
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
@@ -211,7 +282,7 @@ __global__ __launch_bounds__(NB_WAVES * 64) void nbits_kernel(NbitsArgs p, int v
     const int rows = p.M - m0 < 16 * MT ? p.M - m0 : 16 * MT;
     for (int o = threadIdx.x; o < rows * (16 * NT); o += NB_WAVES * 64) {
         const int r = o / (16 * NT), c = o % (16 * NT);
-        const long long n = tile0 * 16 + c;
+        const int n = tile0 * 16 + c;
         if (n >= p.N) continue;
         const int t = (r >> 4) * NT + (c >> 4), l = (c & 15) + 16 * ((r & 15) >> 2);
         float v = 0.0f;
@@ -250,7 +321,7 @@ __global__ __launch_bounds__(256) void nbits_pack_kernel(const uint8_t* raw, con
         w[i * 4 + s] = word;
     }
     if (lane >= 16) return;
-    if (zp) zp[pc * 16 + lane] = (uint16_t)zps;
+    if (raw_zp || pc == 0) zp[pc * 16 + lane] = (uint16_t)zps;   // without zero points one piece's serve all
     for (int s = 0; s < nspp; ++s) {
         const int k0 = piece * NB_PK + s * (NB_PK / nspp);
         const bool in = n < N && k0 < K;
@@ -260,31 +331,41 @@ __global__ __launch_bounds__(256) void nbits_pack_kernel(const uint8_t* raw, con
     }
 }
 
-template <int TY, int NSPP, int MT, int NT>
-hipError_t go(const NbitsArgs& a, int vec, hipStream_t s) {
+template <int TY, int NSPP, int AM, int MT, int NT, int D>
+hipError_t go(const NbitsArgs& a, hipStream_t s) {
     const dim3 grid((unsigned)(nbits_cols(a.N) / 16 / NT), (unsigned)((a.M + 16 * MT - 1) / (16 * MT)));
-    nbits_kernel<TY, NSPP, MT, NT><<<grid, NB_WAVES * 64, 0, s>>>(a, vec);
+    nbits_kernel<TY, NSPP, AM, MT, NT, D><<<grid, NB_WAVES * 64, 0, s>>>(a);
     return hipGetLastError();
 }
+template <int TY, int NSPP, int AM>
+hipError_t by_size(const NbitsArgs& a, hipStream_t s) {
+    if constexpr (AM == A_ANY) {
+        return a.M <= 16 ? go<TY, NSPP, AM, 1, 1, 2>(a, s) : go<TY, NSPP, AM, 2, 2, 1>(a, s);
+    } else {
+        const int tiles = nbits_cols(a.N) / 16;
+        if (a.M <= 16) return tiles >= 1024 ? go<TY, NSPP, AM, 1, 2, 2>(a, s) : go<TY, NSPP, AM, 1, 1, 4>(a, s);
+        if constexpr (TY != FT_F32)   // (fp32 activations take twice the registers)
+            if (a.M > 32) return go<TY, NSPP, AM, 4, 2, 1>(a, s);
+        return go<TY, NSPP, AM, 2, 2, 2>(a, s);
+    }
+}
 template <int TY, int NSPP>
-hipError_t by_size(const NbitsArgs& a, int vec, hipStream_t s) {
-    const int tiles = nbits_cols(a.N) / 16;
-    if (a.M <= 16) return tiles >= 1024 ? go<TY, NSPP, 1, 2>(a, vec, s) : go<TY, NSPP, 1, 1>(a, vec, s);
-    if (a.M <= 32) return go<TY, NSPP, 2, 2>(a, vec, s);
-    return go<TY, NSPP, 4, 2>(a, vec, s);
+hipError_t by_loads(const NbitsArgs& a, hipStream_t s) {
+    const int es = float_type_size(a.type);
+    if ((long long)a.K * es % 16 || ((uintptr_t)a.a & 15)) return by_size<TY, NSPP, A_ANY>(a, s);
+    return a.K % NB_PK ? by_size<TY, NSPP, A_EDGE>(a, s) : by_size<TY, NSPP, A_WHOLE>(a, s);
 }
 template <int TY>
-hipError_t by_scales(const NbitsArgs& a, int vec, hipStream_t s) {
-    return a.nspp == 4 ? by_size<TY, 4>(a, vec, s) : a.nspp == 2 ? by_size<TY, 2>(a, vec, s) : by_size<TY, 1>(a, vec, s);
+hipError_t by_scales(const NbitsArgs& a, hipStream_t s) {
+    return a.nspp == 4 ? by_loads<TY, 4>(a, s) : a.nspp == 2 ? by_loads<TY, 2>(a, s) : by_loads<TY, 1>(a, s);
 }
 
 }  // namespace
 
 hipError_t launch_nbits(const NbitsArgs& a, hipStream_t s) {
     if (a.M == 0) return hipSuccess;
-    const int vec = (long long)a.K * float_type_size(a.type) % 16 == 0 && ((uintptr_t)a.a & 15) == 0;
-    return a.type == FT_F32 ? by_scales<FT_F32>(a, vec, s)
-         : a.type == FT_F16 ? by_scales<FT_F16>(a, vec, s) : by_scales<FT_BF16>(a, vec, s);
+    return a.type == FT_F32 ? by_scales<FT_F32>(a, s)
+         : a.type == FT_F16 ? by_scales<FT_F16>(a, s) : by_scales<FT_BF16>(a, s);
 }
 
 hipError_t launch_nbits_pack(const uint8_t* raw, const void* raw_scales, const uint8_t* raw_zp, int N, int K,
