@@ -52,7 +52,8 @@ hipError_t launch_nbits_pack(const uint8_t* raw, const void* raw_scales, const u
 // so attention loads operands of either product with no shuffle. 8-bit codes
 // are stored as code + 128, 4-bit ones as code + 8, j even in nibble j / 2 and
 // j odd in nibble 4 + j / 2 of a word of eight.
-// Scales are bf16, [group][page_size], a tile's 32 in the order of kv_slot.
+// Scales are bf16, [group][page_size], a tile's 32 in the order of kv_slot; the
+// keys' at 4 bits, which belong to an operand's rows, in the order of kv_pair.
 struct KvCache {
     uint8_t* data;
     int num_pages, page_size, heads, hd, bits;
@@ -67,6 +68,8 @@ __host__ __device__ inline long long kv_head_bytes(int page, int hd, int bits) {
 // the order in which the two 16-token tiles of a score product leave a lane
 // its four rows each
 __host__ __device__ inline int kv_slot(int t) { return 8 * ((t >> 2) & 3) + 4 * (t >> 4) + (t & 3); }
+// tokens t and t + 16 side by side
+__host__ __device__ inline int kv_pair(int t) { return 2 * (t & 15) + (t >> 4); }
 
 struct KvTokens {           // write: const sources; read: destinations
     void* k;

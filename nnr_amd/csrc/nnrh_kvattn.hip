@@ -35,6 +35,12 @@ typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr int AW = 4;              // waves of a block
+// Weights are kept as 2^15 p where p <= 1. With one fp16 piece a weight, the
+// maximum may lag behind by 2^4, and weights are 2^11 p where p <= 2^4: rescaling
+// the sums of 32 rows is then rare instead of usual.
+constexpr float kTop = 15.0f, kSlack = 4.0f;
+constexpr int kNoUnit = -126;      // the least unit of scales (they are 0 or normal)
+constexpr float kLeast = 1e-37f;   // a factor of 0 would make NaN of a masked score, -inf
 constexpr float kNegInf = -__builtin_inff();
 
 struct AttnArgs {
@@ -50,6 +56,12 @@ struct AttnArgs {
     float2* part_ml;               // [rows][slots]
 };
 
+// Tables and lengths are read through the scalar cache: a wait for a vector
+// load would wait for every code that was asked for before it.
+typedef const __attribute__((address_space(4))) int32_t* scalar_ints;
+__device__ __forceinline__ int scalar_load(const int32_t* p, long long i) {
+    return ((scalar_ints)(uintptr_t)p)[i];
+}
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 // maximum and sum over the lanes that differ in bits 4 and 5 (the four lane
 // groups of a row), without a trip through LDS
@@ -71,10 +83,27 @@ __device__ __forceinline__ float max_16(float m) {
 }
 __device__ __forceinline__ float bf16_lo(uint32_t w) { return __builtin_bit_cast(float, w << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t w) { return __builtin_bit_cast(float, w & 0xffff0000u); }
-// exponent e of the least 2^e >= x > 0 (x a normal float)
-__device__ __forceinline__ int ceil_exp(float x) {
-    return (int)((__builtin_bit_cast(uint32_t, x) + 0x7fffffu) >> 23) - 127;
+// the same on whole numbers (bf16 scales, which are not negative, compare as such)
+__device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
+__device__ __forceinline__ uint32_t swap_umax(uint32_t u, bool wide) {
+    const auto r = wide ? __builtin_amdgcn_permlane32_swap(u, u, false, false)
+                        : __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    return umax((uint32_t)r[0], (uint32_t)r[1]);
 }
+__device__ __forceinline__ uint32_t umax16_32(uint32_t u) { return swap_umax(swap_umax(u, false), true); }
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_umax(uint32_t u) {
+    return umax(u, (uint32_t)__builtin_amdgcn_update_dpp((int)u, (int)u, CTRL, 0xf, 0xf, false));
+}
+__device__ __forceinline__ uint32_t umax_16(uint32_t u) {
+    return dpp_umax<0x140>(dpp_umax<0x141>(dpp_umax<0x4e>(dpp_umax<0xb1>(u))));
+}
+// exponent e of the least 2^e >= the bf16 number of these bits; none for 0
+__device__ __forceinline__ int ceil_exp(uint32_t bf16, int none) {
+    return bf16 ? (int)((bf16 + 0x7fu) >> 7) - 127 : none;
+}
+// keeps the compiler from computing both sides of a branch that a tile hardly ever takes
+__device__ __forceinline__ void stay_a_branch() { asm volatile(""); }
 
 // eight 8-bit codes (code + 128) as fp16
 __device__ __forceinline__ h8 codes8(uint32_t lo, uint32_t hi) {
@@ -129,10 +158,15 @@ __device__ __forceinline__ void store_y4(const KvAttention& a, long long at, f4 
 template <int HD, int NP, int NR> struct Rows {
     static constexpr int NC = HD / 32, ND = HD / 16;
     h8 q[NP][NR][NC];
-    float rf[NR];       // a row's score is rf times its raw score (codes times scaled query), rf > 0
-    float m[NR];        // largest raw score
-    float l[NR];        // this lane's part of the total of 2^15 p
-    f4 o[NR][ND];       // sums of 2^15 p v in units of 2^eu
+    // A raw score is a product of operands (times the key's scale at 8 bits);
+    // the score, in powers of two, is rf 2^ek times as much. rf > 0.
+    float rf[NR], rk[NR];   // rk: rf 2^ek
+    int ek;             // unit of the keys' operands (4 bits)
+    float m[NR];        // raw score that weights refer to: the largest, or less by no more than kSlack (in scores)
+    // the total of kTop p: this lane's part (8 bits), or, summed by an MFMA whose
+    // other operand is all ones, the whole in every element (4 bits)
+    f4 l[NR];
+    f4 o[NR][ND];       // sums of kTop p v in units of 2^eu
     int eu;
     int lim[NR];        // keys that the row sees
     int at[NR];         // its place among all rows
@@ -164,7 +198,7 @@ __device__ __forceinline__ void set_rows(const AttnArgs& p, const Job& job, int 
         w.at[t] = (job.pre ? tok : job.b * a.seq + tok) * a.q_heads + hq;
         long long l = job.len;
         if (!job.pre) {
-            const long long last = (long long)a.lens[job.b] - a.seq + tok + 1;
+            const long long last = (long long)scalar_load(a.lens, job.b) - a.seq + tok + 1;
             l = last < l ? last : l;
         }
         w.lim[t] = l > 0 ? (int)l : 0;
@@ -180,7 +214,7 @@ __device__ __forceinline__ void set_rows(const AttnArgs& p, const Job& job, int 
     w.hi = __builtin_amdgcn_readfirstlane(w.hi);
 }
 
-template <int HD, int NP, int NR>
+template <int BITS, int HD, int NP, int NR>
 __device__ __forceinline__ void load_rows(const AttnArgs& p, Rows<HD, NP, NR>& w) {
     constexpr int NC = HD / 32;
     const KvAttention& a = p.a;
@@ -201,8 +235,8 @@ __device__ __forceinline__ void load_rows(const AttnArgs& p, Rows<HD, NP, NR>& w
         top = max16_32(top);
         int e = 0;
         if (top > 0.0f && top < __builtin_inff()) e = 15 - __builtin_amdgcn_frexp_expf(top);
-        // (0 would make 0 * -inf of a masked score)
-        w.rf[t] = fmaxf(ldexpf(fabsf(a.scale) * 1.44269504088896341f, -e), 1e-37f);
+        w.rf[t] = ldexpf(fabsf(a.scale) * 1.44269504088896341f, -e);
+        w.rk[t] = fmaxf(w.rf[t], kLeast);
 #pragma unroll
         for (int k = 0; k < NC; ++k)
 #pragma unroll
@@ -213,113 +247,183 @@ __device__ __forceinline__ void load_rows(const AttnArgs& p, Rows<HD, NP, NR>& w
                 if constexpr (NP == 2) w.q[1][t][k][j] = (_Float16)(s - (float)h);
             }
         w.m[t] = kNegInf;
-        w.l[t] = 0.0f;
+        w.l[t] = f4{0, 0, 0, 0};
 #pragma unroll
         for (int d = 0; d < HD / 16; ++d) w.o[t][d] = f4{0, 0, 0, 0};
     }
-    w.eu = -126;
+    w.eu = kNoUnit;
+    w.ek = BITS == 8 ? 0 : kNoUnit;
 }
 
-// A tile against a wave's rows. key(c, i): elements 32 c .. of keys 16 i .. as
-// an operand, value(c, i): elements 32 c + 16 i .. of the tile's keys. ks, vs:
-// scales of this lane's 8 keys (8 bits; at 4 bits they are in the operands,
-// keys over 2^ek, values over 2^en). en: the values' unit from here on.
-template <int HD, int BITS, int NP, int NR, class Key, class Value>
-__device__ __forceinline__ void tile_step(Rows<HD, NP, NR>& w, int tile, const float* ks, const float* vs, int ek, int en,
-                                          Key key, Value value) {
+// element j of 8 bf16 numbers
+__device__ __forceinline__ float bf16_at(u4 w, int j) { return j & 1 ? bf16_hi(w[j >> 1]) : bf16_lo(w[j >> 1]); }
+
+// KT tiles from key `key0` on against a wave's rows. keys(z, f): tile z's keys as
+// operands, f[2 c + i] elements 32 c .. of keys 16 i ..; values(z, f): f[2 c + i]
+// elements 32 c + 16 i .. of its keys. They are asked for well before they are
+// used. ks, vs: scales of this lane's 8 keys (8 bits; vs are 0 where there is no
+// token; at 4 bits scales are in the operands, keys' over 2^ek, values' over
+// 2^en). ek, en: the units from here on. held: tokens in each tile; some: not all
+// have 32. between: what can be done while the first keys are on their way.
+template <int HD, int BITS, int NP, int NR, int KT, class Keys, class Values, class Between>
+__device__ __forceinline__ void tile_step(Rows<HD, NP, NR>& w, int key0, const int* held, bool some, const u4* ks,
+                                          const u4* vs, int ek, int en, Keys keys, Values values, Between between) {
     constexpr int NC = HD / 32, ND = HD / 16;
+    constexpr float slack = NP == 1 ? kSlack : 0.0f, top = NP == 1 ? kTop - kSlack : kTop;
     const int g = (threadIdx.x & 63) >> 4;
-    f4 acc[NR][2];
-#pragma unroll
-    for (int t = 0; t < NR; ++t) acc[t][0] = acc[t][1] = f4{0, 0, 0, 0};
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const h8 kf = key(c, i);
-#pragma unroll
-            for (int t = 0; t < NR; ++t)
-#pragma unroll
-                for (int q = 0; q < NP; ++q)
-                    acc[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, w.q[q][t][c], acc[t][i], 0, 0, 0);
-        }
-    // raw scores of 2 x 4 keys a row: key 16 i + 4 g + r in element 4 i + r
-    float s[NR][8];
-    const float kunit = BITS == 8 ? 1.0f : ldexpf(1.0f, ek);
+    h8 kf[2 * NC];
+    keys(0, kf);
+    between();
+    f4 acc[NR][KT][2];
 #pragma unroll
     for (int t = 0; t < NR; ++t)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s[t][j] = acc[t][j >> 2][j & 3] * (BITS == 8 ? ks[j] : kunit);
-    if (tile * 32 + 32 > w.lo) {
+        for (int z = 0; z < KT; ++z) acc[t][z][0] = acc[t][z][1] = f4{0, 0, 0, 0};
+#pragma unroll
+    for (int z = 0; z < KT; ++z) {
+        h8 kn[2 * NC];
+        if (z + 1 < KT) keys(z + 1, kn);
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int t = 0; t < NR; ++t)
+#pragma unroll
+                    for (int q = 0; q < NP; ++q)
+                        acc[t][z][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[2 * c + i], w.q[q][t][c], acc[t][z][i], 0, 0, 0);
+        if (z + 1 < KT)
+#pragma unroll
+            for (int j = 0; j < 2 * NC; ++j) kf[j] = kn[j];
+    }
+    h8 vf[2 * NC];
+    values(0, vf);
+    if (BITS == 4 && ek != w.ek) {
+        stay_a_branch();
+#pragma unroll
+        for (int t = 0; t < NR; ++t) {
+            w.m[t] = ldexpf(w.m[t], w.ek - ek);
+            w.rk[t] = fmaxf(ldexpf(w.rf[t], ek), kLeast);
+        }
+        w.ek = ek;
+    }
+    // raw scores of 2 x 4 keys a tile and row: key 16 i + 4 g + r in element 4 i + r
+    float s[NR][KT][8];
+#pragma unroll
+    for (int t = 0; t < NR; ++t)
+#pragma unroll
+        for (int z = 0; z < KT; ++z)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s[t][z][j] = BITS == 8 ? acc[t][z][j >> 2][j & 3] * bf16_at(ks[z], j) : acc[t][z][j >> 2][j & 3];
+    if (key0 + 32 * KT > w.lo || some) {
+        stay_a_branch();
 #pragma unroll
         for (int t = 0; t < NR; ++t)
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (tile * 32 + 16 * (j >> 2) + 4 * g + (j & 3) >= w.lim[t]) s[t][j] = kNegInf;
+            for (int z = 0; z < KT; ++z) {
+                const int end = min(w.lim[t] - key0 - 32 * z, held[z]) - 4 * g;
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (16 * (j >> 2) + (j & 3) >= end) s[t][z][j] = kNegInf;
+            }
     }
-    // running maximum; weights 2^15 p
-    bool moved = en != w.eu;
-    float al[NR];
+    // running maximum: moved on only where a score outgrows it by more than the slack
+    float mx[NR];
+    bool moved = false;
 #pragma unroll
     for (int t = 0; t < NR; ++t) {
-        float mx = w.m[t];
+        mx[t] = s[t][0][0];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) mx = fmaxf(mx, s[t][j]);
-        mx = max16_32(mx);
-        const float base = mx == kNegInf ? 0.0f : mx * w.rf[t];
-        al[t] = exp2_(__builtin_fmaf(w.m[t], w.rf[t], -base));
-        moved |= mx != w.m[t];
-        w.m[t] = mx;
-        float sum = 0.0f;
+        for (int z = 0; z < KT; ++z)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            s[t][j] = exp2_(__builtin_fmaf(s[t][j], w.rf[t], 15.0f - base));
-            sum += s[t][j];
-        }
-        w.l[t] = __builtin_fmaf(w.l[t], al[t], sum);
+            for (int j = 0; j < 8; ++j) mx[t] = fmaxf(mx[t], s[t][z][j]);
+        mx[t] = max16_32(mx[t]);
+        moved |= slack == 0.0f ? mx[t] > w.m[t] : mx[t] * w.rk[t] > __builtin_fmaf(w.m[t], w.rk[t], slack);
     }
-    if (__any(moved)) {
+    if (__any(moved) || en != w.eu) {
+        stay_a_branch();
 #pragma unroll
         for (int t = 0; t < NR; ++t) {
-            const float f = ldexpf(al[t], w.eu - en);
+            const float m = fmaxf(w.m[t], mx[t]);
+            const float al = m == w.m[t] ? 1.0f : exp2_((w.m[t] - m) * w.rk[t]);
+            w.m[t] = m;
+            w.l[t] *= al;
+            const float f = ldexpf(al, w.eu - en);
 #pragma unroll
             for (int d = 0; d < ND; ++d) w.o[t][d] *= f;
         }
+        w.eu = en;
     }
-    w.eu = en;
-    h8 pf[NP][NR];
-    float vu[8];
-    if constexpr (BITS == 8) {
+    // weights kTop p
+    const float fv = ldexpf(1.0f, -en);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) vu[j] = ldexpf(vs[j], -en);
+    for (int t = 0; t < NR; ++t) {
+        const float base = w.m[t] == kNegInf ? 0.0f : w.m[t] * w.rk[t];
+        const float off = top - base;
+#pragma unroll
+        for (int z = 0; z < KT; ++z)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s[t][z][j] = exp2_(__builtin_fmaf(s[t][z][j], w.rk[t], off));
+        if constexpr (BITS == 8) {
+            float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int z = 0; z < KT; ++z)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sum[j & 1] += s[t][z][j];
+            w.l[t][0] += sum[0] + sum[1];
+        }
     }
 #pragma unroll
-    for (int t = 0; t < NR; ++t)
+    for (int z = 0; z < KT; ++z) {
+        h8 pf[NP][NR];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float x = BITS == 8 ? s[t][j] * vu[j] : s[t][j];
-            const _Float16 h = (_Float16)x;
-            pf[0][t][j] = h;
-            if constexpr (NP == 2) pf[1][t][j] = (_Float16)(x - (float)h);
+            const float vu = BITS == 8 ? bf16_at(vs[z], j) * fv : 1.0f;
+#pragma unroll
+            for (int t = 0; t < NR; ++t) {
+                const float x = BITS == 8 ? s[t][z][j] * vu : s[t][z][j];
+                const _Float16 h = (_Float16)x;
+                pf[0][t][j] = h;
+                if constexpr (NP == 2) pf[1][t][j] = (_Float16)(x - (float)h);
+            }
         }
+        if constexpr (BITS == 4) {
+            h8 ones;
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const h8 v = value(c, i);
+            for (int j = 0; j < 8; ++j) ones[j] = (_Float16)1.0f;
 #pragma unroll
             for (int t = 0; t < NR; ++t)
 #pragma unroll
                 for (int q = 0; q < NP; ++q)
-                    w.o[t][2 * c + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pf[q][t], w.o[t][2 * c + i], 0, 0, 0);
+                    w.l[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pf[q][t], w.l[t], 0, 0, 0);
         }
+        h8 vn[2 * NC];
+        if (z + 1 < KT) values(z + 1, vn);
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int t = 0; t < NR; ++t)
+#pragma unroll
+                for (int q = 0; q < NP; ++q)
+                    w.o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[d], pf[q][t], w.o[t][d], 0, 0, 0);
+        if (z + 1 < KT)
+#pragma unroll
+            for (int d = 0; d < ND; ++d) vf[d] = vn[d];
+    }
+}
+
+template <int BITS>
+__device__ __forceinline__ float row_total(f4 l) {
+    if (BITS == 4) return l[0];
+    float x = l[0] + __shfl_xor(l[0], 16);
+    return x + __shfl_xor(x, 32);
 }
 
 // ---- a tile in memory ---------------------------------------------------------
 struct TilePtr {
     const uint8_t* codes;        // keys' blocks; values' vcodes further
     const uint16_t* scales;      // keys'; values' vscales further
-    bool ok;                     // the page exists
+    bool ok;                     // the page exists (else this is page 0, of which no token counts)
 };
 template <int HD, int BITS>
 __device__ __forceinline__ TilePtr tile_ptr(const AttnArgs& p, int head, int id, int tile) {
@@ -333,22 +437,50 @@ __device__ __forceinline__ TilePtr tile_ptr(const AttnArgs& p, int head, int id,
     r.scales = (const uint16_t*)(base + 2 * kv_codes_bytes(c.page_size, HD, BITS)) + in_page * 32;
     return r;
 }
-// 8 scales of a lane's keys; those past `held` are 0
-__device__ __forceinline__ void scales8(u4 w, int held, float* s) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) s[j] = j & 1 ? bf16_hi(w[j >> 1]) : bf16_lo(w[j >> 1]);
+// 8 scales of a lane's keys; those past `held` become 0
+__device__ __forceinline__ u4 held_scales(u4 w, int held) {
     if (held < 32) {
-        const int g = (threadIdx.x & 63) >> 4;
+        stay_a_branch();
+        const int end = held - 4 * (int)((threadIdx.x & 63) >> 4);
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            if (16 * (j >> 2) + 4 * g + (j & 3) >= held) s[j] = 0.0f;
+            if (16 * (j >> 2) + (j & 3) >= end) w[j >> 1] &= j & 1 ? 0xffffu : 0xffff0000u;
+    }
+    return w;
+}
+// the largest of a lane's 8 scales, as bits of bf16
+__device__ __forceinline__ uint32_t top8(u4 w) {
+    typedef uint16_t us2 __attribute__((ext_vector_type(2)));
+    const auto m = [](uint32_t a, uint32_t b) {
+        return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(us2, a), __builtin_bit_cast(us2, b)));
+    };
+    const uint32_t x = m(m(w[0], w[1]), m(w[2], w[3]));
+    return umax(x & 0xffffu, x >> 16);
+}
+// scales of keys col and col + 16 (4 bits), as floats' bits; 0 past `held`
+__device__ __forceinline__ void held_pair(uint32_t w, int held, uint32_t* s) {
+    s[0] = w << 16;
+    s[1] = w & 0xffff0000u;
+    if (held < 32) {
+        stay_a_branch();
+        const int col = threadIdx.x & 15;
+        if (col >= held) s[0] = 0;
+        if (col + 16 >= held) s[1] = 0;
     }
 }
-__device__ __forceinline__ h2 scale_pair(float a, float b) { return h2{(_Float16)a, (_Float16)b}; }
-__device__ __forceinline__ int unit_of(float top, int none) { return top > 0.0f ? ceil_exp(top) : none; }
+__device__ __forceinline__ h8 key4(uint32_t codes, uint32_t scale, float unit) {
+    const _Float16 x = (_Float16)(__builtin_bit_cast(float, scale) * unit);
+    const h2 s = {x, x};
+    const h2 s4[4] = {s, s, s, s};
+    return codes4(codes, s4);
+}
+__device__ __forceinline__ void value_scales(u4 w, float unit, h2* s) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[j] = h2{(_Float16)(bf16_lo(w[j]) * unit), (_Float16)(bf16_hi(w[j]) * unit)};
+}
 
 __device__ __forceinline__ int page_id(const Job& job, const AttnArgs& p, int tile) {
-    return __builtin_amdgcn_readfirstlane(job.table[tile >> p.page_shift]);
+    return scalar_load(job.table, tile >> p.page_shift);
 }
 
 // ---- few rows: the block's waves split its keys -------------------------------
@@ -359,14 +491,13 @@ template <int HD, int BITS> struct RawTile {
     vec k[NC], v[NC];
     u4 vs[BITS == 8 ? 1 : NC];
     u4 ks;                        // 8 bits
-    uint16_t ks4[NC][2];          // 4 bits
+    uint32_t ks4[NC];             // 4 bits
     bool ok;
     __device__ __forceinline__ void load(const AttnArgs& p, const Job& job, int tile) {
         constexpr int BB = BITS == 8 ? 1024 : 512;
         const int lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
         const TilePtr t = tile_ptr<HD, BITS>(p, job.head, page_id(job, p, tile), tile);
         ok = t.ok;
-        if (!ok) return;
         const uint8_t* vc = t.codes + kv_codes_bytes(p.c.page_size, HD, BITS);
         const uint16_t* vsp = t.scales + (long long)p.c.page_size * kv_groups(HD, BITS);
 #pragma unroll
@@ -374,9 +505,7 @@ template <int HD, int BITS> struct RawTile {
         if constexpr (BITS == 8) ks = *(const u4*)(t.scales + 8 * g);
         else
 #pragma unroll
-            for (int c = 0; c < NC; ++c)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) ks4[c][i] = t.scales[c * p.c.page_size + kv_slot(col + 16 * i)];
+            for (int c = 0; c < NC; ++c) ks4[c] = *(const uint32_t*)(t.scales + c * p.c.page_size + 2 * col);
 #pragma unroll
         for (int c = 0; c < (BITS == 8 ? 1 : NC); ++c) vs[c] = *(const u4*)(vsp + c * p.c.page_size + 8 * g);
 #pragma unroll
@@ -388,47 +517,52 @@ template <int HD, int BITS, int NP>
 __device__ __forceinline__ void few_tile(Rows<HD, NP, 1>& w, const RawTile<HD, BITS>& r, int tile, int held) {
     constexpr int NC = HD / 32;
     const int col = threadIdx.x & 15;
-    float vtop = 0.0f;
-    float vs[BITS == 8 ? 1 : NC][8];
+    u4 vs[BITS == 8 ? 1 : NC];
+    uint32_t vtop = 0;
 #pragma unroll
     for (int c = 0; c < (BITS == 8 ? 1 : NC); ++c) {
-        scales8(r.vs[c], held, vs[c]);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) vtop = fmaxf(vtop, vs[c][j]);
+        vs[c] = held_scales(r.vs[c], held);
+        vtop = umax(vtop, top8(vs[c]));
     }
-    vtop = max16_32(vtop);
-    const int en = max(w.eu, unit_of(vtop, w.eu));
+    const int en = max(w.eu, ceil_exp(__builtin_amdgcn_readfirstlane(umax16_32(vtop)), kNoUnit));
+    const auto nothing = [] {};
     if constexpr (BITS == 8) {
-        float ks[8];
-        scales8(r.ks, held, ks);
-        tile_step<HD, 8, NP, 1>(
-            w, tile, ks, vs[0], 0, en, [&](int c, int i) { return codes8(r.k[c][2 * i], r.k[c][2 * i + 1]); },
-            [&](int c, int i) { return codes8(r.v[c][2 * i], r.v[c][2 * i + 1]); });
-    } else {
-        float ks[NC][2], top = 0.0f;
+        tile_step<HD, 8, NP, 1, 1>(
+            w, tile * 32, &held, held < 32, &r.ks, vs, 0, en,
+            [&](int, h8* f) {
 #pragma unroll
-        for (int c = 0; c < NC; ++c)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                ks[c][i] = col + 16 * i < held ? bf16_lo(r.ks4[c][i]) : 0.0f;
-                top = fmaxf(top, ks[c][i]);
-            }
-        top = max_16(top);
-        const int ek = unit_of(top, 0);
-        const float fk = ldexpf(1.0f, -ek), fv = ldexpf(1.0f, -en);   // (-126 only where all scales are 0)
-        tile_step<HD, 4, NP, 1>(
-            w, tile, nullptr, nullptr, ek, en,
-            [&](int c, int i) {
-                const h2 f = scale_pair(ks[c][i] * fk, ks[c][i] * fk);
-                const h2 f4_[4] = {f, f, f, f};
-                return codes4(r.k[c][i], f4_);
+                for (int j = 0; j < 2 * NC; ++j) f[j] = codes8(r.k[j >> 1][2 * (j & 1)], r.k[j >> 1][2 * (j & 1) + 1]);
             },
-            [&](int c, int i) {
-                h2 f[4];
+            [&](int, h8* f) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) f[j] = scale_pair(vs[c][2 * j] * fv, vs[c][2 * j + 1] * fv);
-                return codes4(r.v[c][i], f);
-            });
+                for (int j = 0; j < 2 * NC; ++j) f[j] = codes8(r.v[j >> 1][2 * (j & 1)], r.v[j >> 1][2 * (j & 1) + 1]);
+            },
+            nothing);
+    } else {
+        uint32_t kb[NC][2], top = 0;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            held_pair(r.ks4[c], held, kb[c]);
+            top = umax(top, umax(kb[c][0], kb[c][1]));
+        }
+        const int ek = max(w.ek, ceil_exp(__builtin_amdgcn_readfirstlane(umax_16(top) >> 16), kNoUnit));
+        const float fk = ldexpf(1.0f, -ek), fv = ldexpf(1.0f, -en);
+        tile_step<HD, 4, NP, 1, 1>(
+            w, tile * 32, &held, held < 32, nullptr, nullptr, ek, en,
+            [&](int, h8* f) {
+#pragma unroll
+                for (int j = 0; j < 2 * NC; ++j) f[j] = key4(r.k[j >> 1][j & 1], kb[j >> 1][j & 1], fk);
+            },
+            [&](int, h8* f) {
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    h2 s[4];
+                    value_scales(vs[c], fv, s);
+                    f[2 * c] = codes4(r.v[c][0], s);
+                    f[2 * c + 1] = codes4(r.v[c][1], s);
+                }
+            },
+            nothing);
     }
 }
 
@@ -464,24 +598,23 @@ __device__ __forceinline__ void few(const AttnArgs& p, Job& job, char* lds) {
     set_rows(p, job, job.row0, w);
     job.t1 = min(job.t1, (w.hi + 31) / 32);
     int tile = job.t0 + wave;
-    RawTile<HD, BITS> cur, nxt;
+    RawTile<HD, BITS> cur{}, nxt{};
     if (tile < job.t1) cur.load(p, job, tile);
-    load_rows(p, w);
+    load_rows<BITS>(p, w);
     for (; tile < job.t1; tile += AW) {
         if (tile + AW < job.t1) nxt.load(p, job, tile + AW);
-        if (cur.ok) few_tile<HD, BITS, NP>(w, cur, tile, (int)min(job.len - (long long)tile * 32, 32ll));
+        few_tile<HD, BITS, NP>(w, cur, tile, cur.ok ? (int)min(job.len - (long long)tile * 32, 32ll) : 0);
         cur = nxt;
     }
     // join the waves: first everyone's maximum, then sums in the units of it
     f4(*buf)[ND][64] = (f4(*)[ND][64])lds;                       // [2]
     float(*sm)[16] = (float(*)[16])(lds + 2 * sizeof(*buf));     // [AW]
     float(*sl)[16] = sm + AW;
-    w.l[0] += __shfl_xor(w.l[0], 16);
-    w.l[0] += __shfl_xor(w.l[0], 32);
-    const float top = w.m[0] == kNegInf ? kNegInf : w.m[0] * w.rf[0];
+    const float lw = row_total<BITS>(w.l[0]);
+    const float top = w.m[0] == kNegInf ? kNegInf : w.m[0] * w.rk[0];
     if (g == 0) {
         sm[wave][col] = top;
-        sl[wave][col] = w.l[0];
+        sl[wave][col] = lw;
     }
     __syncthreads();
     float mall = kNegInf, lall = 0.0f;
@@ -516,14 +649,20 @@ __device__ __forceinline__ void few(const AttnArgs& p, Job& job, char* lds) {
 template <int HD> constexpr int kFewLds = 2 * (HD / 16) * 1024 + 2 * AW * 64;
 
 // ---- many rows: the block's waves split its rows ------------------------------
+constexpr int kManyTiles = 2;   // tiles between two barriers
+
 // A tile is turned into operands once, a part by each wave, and lies in LDS
 // for all of them; the next tile is written beside it meanwhile, and the codes
 // of the one after are on their way.
 template <int HD, int BITS> struct Parts {
     static constexpr int NC = HD / 32, NU = (2 * NC + AW - 1) / AW;   // a wave's blocks (NC of keys, then NC of values)
     typedef uint32_t vec __attribute__((ext_vector_type(BITS == 8 ? 4 : 2)));
+    // block of round u; is it one of keys (known at compile time where the waves divide them)
+    __device__ __forceinline__ static int block(int u, int wave) { return wave + u * AW; }
+    __device__ __forceinline__ static bool keys(int u, int b) { return NC % AW == 0 ? u < NC / AW : b < NC; }
+    __device__ __forceinline__ static bool none(int b) { return 2 * NC % AW != 0 && b >= 2 * NC; }
     vec code[NU];
-    u4 sc[NU];                    // 4 bits: a value block's scales; a key block's two in the first word
+    u4 sc[NU];                    // 4 bits: a value block's scales; a key block's pair in the first word
     u4 ks, vs;                    // 8 bits
     u2 all_k, all_v;              // 4 bits: the tile's scales, 4 a lane, for its units
     bool ok;
@@ -532,19 +671,19 @@ template <int HD, int BITS> struct Parts {
         const int lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
         const TilePtr t = tile_ptr<HD, BITS>(p, head, id, tile);
         ok = t.ok;
-        if (!ok) return;
         const uint8_t* vc = t.codes + kv_codes_bytes(p.c.page_size, HD, BITS);
         const uint16_t* vsp = t.scales + (long long)p.c.page_size * kv_groups(HD, BITS);
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
-            const int b = wave + u * AW;
-            if (b >= 2 * NC) break;
-            const int c = b < NC ? b : b - NC;
-            code[u] = *(const vec*)((b < NC ? t.codes : vc) + c * BB + lane * sizeof(vec));
+            const int b = block(u, wave);
+            if (none(b)) break;
+            const bool is_key = keys(u, b);
+            const int c = is_key ? b : b - NC;
+            code[u] = *(const vec*)((is_key ? t.codes : vc) + c * BB + lane * sizeof(vec));
             if constexpr (BITS == 4) {
-                if (b < NC) {
+                if (is_key) {
                     const uint16_t* s = t.scales + c * p.c.page_size;
-                    sc[u][0] = s[kv_slot(col)] | (uint32_t)s[kv_slot(col + 16)] << 16;
+                    sc[u][0] = *(const uint32_t*)(s + 2 * col);
                 } else {
                     sc[u] = *(const u4*)(vsp + c * p.c.page_size + 8 * g);
                 }
@@ -559,27 +698,29 @@ template <int HD, int BITS> struct Parts {
             all_v = *(const u2*)(vsp + grp * p.c.page_size + (lane & 7) * 4);
         }
     }
-    // largest scale of a tile, from all_k or all_v
-    __device__ __forceinline__ static float top(u2 w, int held) {
+    // largest scale of a tile's tokens, from all_k or all_v, as bits of bf16
+    __device__ __forceinline__ static uint32_t top(u2 w, int held, bool key) {
         const int lane = threadIdx.x & 63;
-        float m = 0.0f;
+        uint32_t f[4] = {w[0] & 0xffffu, w[0] >> 16, w[1] & 0xffffu, w[1] >> 16};
+        if (held < 32) {
+            stay_a_branch();
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int slot = (lane & 7) * 4 + q, tok = 16 * ((slot >> 2) & 1) + 4 * (slot >> 3) + (slot & 3);
-            const float f = q & 1 ? bf16_hi(w[q >> 1]) : bf16_lo(w[q >> 1]);
-            m = fmaxf(m, tok < held ? f : 0.0f);
+            for (int q = 0; q < 4; ++q) {
+                const int slot = (lane & 7) * 4 + q;
+                const int tok = key ? (slot >> 1) + 16 * (slot & 1) : 16 * ((slot >> 2) & 1) + 4 * (slot >> 3) + (slot & 3);
+                if (tok >= held) f[q] = 0;
+            }
         }
-        m = max16_32(max_16(m));
-        return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, m)));
+        return umax(umax(f[0], f[1]), umax(f[2], f[3]));
     }
 };
 
 template <int HD, int BITS, int NP, int NR>
 __device__ __forceinline__ void many(const AttnArgs& p, Job& job, char* lds) {
-    constexpr int NC = HD / 32, NU = Parts<HD, BITS>::NU;
+    constexpr int NC = HD / 32, NU = Parts<HD, BITS>::NU, KT = kManyTiles;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int col = lane & 15, g = lane >> 4;
-    h8(*frag)[4 * NC][64] = (h8(*)[4 * NC][64])lds;   // [2]: keys (c, i) then values (c, i)
+    const int col = lane & 15;
+    h8(*frag)[KT][4 * NC][64] = (h8(*)[KT][4 * NC][64])lds;   // [2]: a tile's keys (c, i), then its values (c, i)
     Rows<HD, NP, NR> w;
     const int row0 = job.row0 + wave * 16 * NR;
     // the block's tiles: the last of its rows sees most
@@ -587,118 +728,141 @@ __device__ __forceinline__ void many(const AttnArgs& p, Job& job, char* lds) {
         const int last = min(job.row0 + AW * 16 * NR, job.nrows) - 1;
         long long hi = job.len;
         if (!job.pre) {
-            const long long seen = (long long)p.a.lens[job.b] - p.a.seq + last / p.G + 1;
+            const long long seen = (long long)scalar_load(p.a.lens, job.b) - p.a.seq + last / p.G + 1;
             hi = seen < hi ? seen : hi;
         }
         job.t1 = min(job.t1, hi > 0 ? (int)((hi + 31) / 32) : 0);
     }
-    const bool rows = row0 < job.nrows;   // this wave has some
-    set_rows(p, job, row0, w);
+    set_rows(p, job, row0, w);   // (a wave past the rows repeats the last one)
 
-    Parts<HD, BITS> raw;
-    int id = 0, ek = 0, ek_next = 0, en = -126, en_next = -126;
-    float ks[8], vs[8];
-    bool ok = false;
-    u4 ks_raw = {0, 0, 0, 0}, vs_raw = {0, 0, 0, 0};
-    if (job.t0 < job.t1) raw.load(p, job.head, page_id(job, p, job.t0), job.t0, wave);
-    if (job.t0 + 1 < job.t1) id = page_id(job, p, job.t0 + 1);
-    load_rows(p, w);
-
-    // raw tile -> operands in frag[at]
+    Parts<HD, BITS> raw[KT] = {};
+    int id[KT], held[KT], held_next[KT], ek = kNoUnit, ek_next = kNoUnit, en = kNoUnit, en_next = kNoUnit;
+    u4 ks_next[KT], vs_next[KT];   // 8 bits
+    auto ids = [&](int tile) {
+#pragma unroll
+        for (int z = 0; z < KT; ++z) id[z] = tile + z < job.t1 ? page_id(job, p, tile + z) : -1;
+    };
+    auto load = [&](int tile) {
+#pragma unroll
+        for (int z = 0; z < KT; ++z) raw[z].load(p, job.head, id[z], tile + z, wave);
+    };
+    // raw tiles -> operands in frag[at]; tokens past the source's end have scale 0
     auto convert = [&](int tile, int at) {
-        const int held = (int)min(job.len - (long long)tile * 32, 32ll);
         float fk = 1.0f, fv = 1.0f;
+#pragma unroll
+        for (int z = 0; z < KT; ++z) {
+            held_next[z] = raw[z].ok ? (int)min(job.len - (long long)(tile + z) * 32, 32ll) : 0;
+            ks_next[z] = raw[z].ks;
+            vs_next[z] = raw[z].vs;
+        }
         if constexpr (BITS == 4) {
-            ek_next = unit_of(raw.top(raw.all_k, held), 0);
-            en_next = max(en_next, unit_of(raw.top(raw.all_v, held), -126));
+            uint32_t tk = 0, tv = 0;
+#pragma unroll
+            for (int z = 0; z < KT; ++z) {
+                tk = umax(tk, raw[z].top(raw[z].all_k, held_next[z], true));
+                tv = umax(tv, raw[z].top(raw[z].all_v, held_next[z], false));
+            }
+            tk = __builtin_amdgcn_readfirstlane(umax16_32(umax_16(tk)));
+            tv = __builtin_amdgcn_readfirstlane(umax16_32(umax_16(tv)));
+            ek_next = max(ek_next, ceil_exp(tk, kNoUnit));
+            en_next = max(en_next, ceil_exp(tv, kNoUnit));
             fk = ldexpf(1.0f, -ek_next);
             fv = ldexpf(1.0f, -en_next);
         }
 #pragma unroll
-        for (int u = 0; u < NU; ++u) {
-            const int b = wave + u * AW;
-            if (b >= 2 * NC) break;
+        for (int z = 0; z < KT; ++z)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                h8 x;
+            for (int u = 0; u < NU; ++u) {
+                const int b = Parts<HD, BITS>::block(u, wave);
+                if (Parts<HD, BITS>::none(b)) break;
+                h8* to = &frag[at][z][2 * b][lane];
                 if constexpr (BITS == 8) {
-                    x = codes8(raw.code[u][2 * i], raw.code[u][2 * i + 1]);
-                } else if (b < NC) {
-                    float s = i ? bf16_hi(raw.sc[u][0]) : bf16_lo(raw.sc[u][0]);
-                    s = col + 16 * i < held ? s * fk : 0.0f;
-                    const h2 f = scale_pair(s, s);
-                    const h2 f4_[4] = {f, f, f, f};
-                    x = codes4(raw.code[u][i], f4_);
-                } else {
-                    float s[8];
-                    scales8(raw.sc[u], held, s);
-                    h2 f[4];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) f[j] = scale_pair(s[2 * j] * fv, s[2 * j + 1] * fv);
-                    x = codes4(raw.code[u][i], f);
+                    for (int i = 0; i < 2; ++i) to[64 * i] = codes8(raw[z].code[u][2 * i], raw[z].code[u][2 * i + 1]);
+                } else if (Parts<HD, BITS>::keys(u, b)) {
+                    uint32_t s[2];
+                    held_pair(raw[z].sc[u][0], held_next[z], s);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) to[64 * i] = key4(raw[z].code[u][i], s[i], fk);
+                } else {
+                    h2 s[4];
+                    value_scales(held_scales(raw[z].sc[u], held_next[z]), fv, s);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) to[64 * i] = codes4(raw[z].code[u][i], s);
                 }
-                frag[at][2 * b + i][lane] = x;
             }
-        }
     };
     if (job.t0 < job.t1) {
-        ok = raw.ok;
-        if (ok) convert(job.t0, 0);
-        ks_raw = raw.ks;
-        vs_raw = raw.vs;
-        ek = ek_next;
-        en = en_next;
-        if (job.t0 + 1 < job.t1) raw.load(p, job.head, id, job.t0 + 1, wave);
-        if (job.t0 + 2 < job.t1) id = page_id(job, p, job.t0 + 2);
+        ids(job.t0);
+        load(job.t0);
+        ids(job.t0 + KT);
+    }
+    load_rows<BITS>(p, w);
+    if (job.t0 < job.t1) {
+        convert(job.t0, 0);
+        load(job.t0 + KT);
+        ids(job.t0 + 2 * KT);
     }
     __syncthreads();
     int at = 0;
-    for (int tile = job.t0; tile < job.t1; ++tile, at ^= 1) {
-        const u4 ks_cur = ks_raw, vs_cur = vs_raw;
-        const int ek_cur = ek, en_cur = en;
-        const bool ok_cur = ok;
-        if (tile + 1 < job.t1) {
-            ok = raw.ok;
-            if (ok) convert(tile + 1, at ^ 1);
-            ks_raw = raw.ks;
-            vs_raw = raw.vs;
-            ek = ek_next;
-            en = en_next;
-            if (tile + 2 < job.t1) raw.load(p, job.head, id, tile + 2, wave);
-            if (tile + 3 < job.t1) id = page_id(job, p, tile + 3);
-        }
-        if (rows && ok_cur) {
-            int unit = en_cur;
-            if constexpr (BITS == 8) {
-                const int held = (int)min(job.len - (long long)tile * 32, 32ll);
-                scales8(ks_cur, held, ks);
-                scales8(vs_cur, held, vs);
-                float vtop = 0.0f;
+    for (int tile = job.t0; tile < job.t1; tile += KT, at ^= 1) {
+        u4 ks_raw[KT], vs_raw[KT];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) vtop = fmaxf(vtop, vs[j]);
-                unit = max(w.eu, unit_of(max16_32(vtop), w.eu));
-            }
-            const h8(*f)[64] = frag[at];
-            tile_step<HD, BITS, NP, NR>(
-                w, tile, ks, vs, ek_cur, unit, [&](int c, int i) { return f[2 * c + i][lane]; },
-                [&](int c, int i) { return f[2 * NC + 2 * c + i][lane]; });
+        for (int z = 0; z < KT; ++z) {
+            held[z] = held_next[z];
+            ks_raw[z] = ks_next[z];
+            vs_raw[z] = vs_next[z];
         }
+        ek = ek_next;
+        en = en_next;
+        bool some = false;
+#pragma unroll
+        for (int z = 0; z < KT; ++z) some |= held[z] < 32;
+        if constexpr (BITS == 8) {
+            uint32_t vtop = 0;
+#pragma unroll
+            for (int z = 0; z < KT; ++z) {
+                vs_raw[z] = held_scales(vs_raw[z], held[z]);
+                vtop = umax(vtop, top8(vs_raw[z]));
+            }
+            ek = 0;
+            en = max(w.eu, ceil_exp(__builtin_amdgcn_readfirstlane(umax16_32(vtop)), kNoUnit));
+        }
+        const h8(*f)[4 * NC][64] = frag[at];
+        tile_step<HD, BITS, NP, NR, KT>(
+            w, tile * 32, held, some, ks_raw, vs_raw, ek, en,
+            [&](int z, h8* x) {
+#pragma unroll
+                for (int j = 0; j < 2 * NC; ++j) x[j] = f[z][j][lane];
+                __builtin_amdgcn_sched_barrier(0);
+            },
+            [&](int z, h8* x) {
+#pragma unroll
+                for (int j = 0; j < 2 * NC; ++j) x[j] = f[z][2 * NC + j][lane];
+                __builtin_amdgcn_sched_barrier(0);
+            },
+            [&] {   // past the last tile for nothing: without a branch
+                convert(tile + KT, at ^ 1);
+                __builtin_amdgcn_sched_barrier(0);
+                load(tile + 2 * KT);
+                ids(tile + 3 * KT);
+                __builtin_amdgcn_sched_barrier(0);
+            });
         __syncthreads();
     }
-    if (!rows) return;
+    if (row0 >= job.nrows) return;
     float m[NR], l[NR];
 #pragma unroll
     for (int t = 0; t < NR; ++t) {
-        l[t] = w.l[t] + __shfl_xor(w.l[t], 16);
-        l[t] += __shfl_xor(l[t], 32);
-        m[t] = w.m[t] == kNegInf ? kNegInf : w.m[t] * w.rf[t];
+        l[t] = row_total<BITS>(w.l[t]);
+        m[t] = w.m[t] == kNegInf ? kNegInf : w.m[t] * w.rk[t];
         const float f = ldexpf(1.0f, w.eu);
 #pragma unroll
         for (int d = 0; d < HD / 16; ++d) w.o[t][d] *= f;
     }
     put_rows(p, job, row0, w, m, l);
 }
-template <int HD> constexpr int kManyLds = 2 * 4 * (HD / 32) * 1024;
+template <int HD> constexpr int kManyLds = 2 * kManyTiles * 4 * (HD / 32) * 1024;
 
 // row tiles of a wave with many rows: two where they fit beside the rest
 template <int HD, int NP> constexpr int kManyRows = HD <= 128 && NP == 1 ? 2 : 1;
@@ -733,7 +897,7 @@ __global__ __launch_bounds__(AW * 64, HD <= 128 ? 2 : 1) void kv_attn_kernel(Att
     job.table = job.pre ? a.prefix_table : a.table + (long long)job.b * a.max_pages;
     job.len = a.prefix_len;
     if (!job.pre) {
-        const long long cap = (long long)a.max_pages * p.c.page_size, len = a.lens[job.b];
+        const long long cap = (long long)a.max_pages * p.c.page_size, len = scalar_load(a.lens, job.b);
         job.len = len < cap ? len : cap;
     }
     const int chunk = job.pre ? p.pre_chunk : p.own_chunk;
@@ -809,11 +973,14 @@ Plan plan(const KvCache& c, const KvAttention& a) {
     p.pre_groups = a.prefix_len ? ceil_div(pre_rows, p.pre_many ? many : 16) : 0;
     const long long pre_items = (long long)p.pre_groups * c.heads, own_items = (long long)p.own_groups * c.heads * a.batch;
     const long long pre_tiles = (a.prefix_len + 31) / 32, own_tiles = (long long)a.max_pages * c.page_size / 32;
-    const long long total = pre_items * pre_tiles + own_items * own_tiles;
-    long long chunk = (total + 2047) / 2048;
-    chunk = chunk < 8 ? 8 : chunk;
-    p.pre_slots = p.pre_groups ? ceil_div(pre_tiles, chunk) : 0;
-    p.own_slots = own_tiles ? ceil_div(own_tiles, chunk) : 1;
+    // prefix blocks, and others with many rows: as many as run at once
+    const auto chunk = [](long long items, long long tiles, bool many) {
+        const long long blocks = many ? 512 : 2048, least = 8;
+        const long long c = (items * tiles + blocks - 1) / blocks;
+        return c < least ? least : c;
+    };
+    p.pre_slots = p.pre_groups ? ceil_div(pre_tiles, chunk(pre_items, pre_tiles, p.pre_many)) : 0;
+    p.own_slots = own_tiles ? ceil_div(own_tiles, chunk(own_items, own_tiles, p.own_many)) : 1;
     p.pre_chunk = p.pre_slots ? ceil_div(pre_tiles, p.pre_slots) : 0;
     p.own_chunk = ceil_div(own_tiles, p.own_slots);
     return p;
@@ -852,6 +1019,10 @@ hipError_t launch_kv_attention(const KvCache& c, const KvAttention& a, void* wor
     AttnArgs p;
     p.c = c;
     p.a = a;
+    if (c.num_pages == 0) {   // no keys, and no page 0 to read in place of one that does not exist
+        p.a.prefix_len = 0;
+        p.a.max_pages = 0;
+    }
     p.G = a.q_heads / c.heads;
     p.rows = a.batch * a.seq * a.q_heads;
     p.pre_slots = pl.pre_slots;

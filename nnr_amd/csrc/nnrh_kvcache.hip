@@ -117,6 +117,9 @@ __device__ __forceinline__ uint32_t pack_nibbles(const uint32_t* q) {
 }
 __device__ __forceinline__ uint32_t nibble(uint32_t w, int j) { return (w >> (4 * ((j >> 1) + 4 * (j & 1)))) & 15u; }
 
+template <int BITS>
+__device__ __forceinline__ int scale_slot(int values, int t) { return BITS == 4 && !values ? kv_pair(t) : kv_slot(t); }
+
 // One wave a (tile of 32 positions, head, sequence, keys or values). Lanes read
 // 8 neighbouring elements of a token, form scales and codes, and store keys as
 // they are; values pass through LDS, where an element's tokens come together.
@@ -173,7 +176,7 @@ __global__ __launch_bounds__(64) void kv_write_kernel(KvCache c, KvTokens t) {
             if (in[h])
 #pragma unroll
                 for (int k = 0; k < (BITS == 8 ? 1 : NC); ++k)
-                    scales[(long long)k * c.page_size + w.in_page * 32 + kv_slot((lane & 15) + 16 * h)] = (__bf16)sc[h][k];
+                    scales[(long long)k * c.page_size + w.in_page * 32 + scale_slot<BITS>(values, (lane & 15) + 16 * h)] = (__bf16)sc[h][k];
     }
     constexpr int BB = BITS == 8 ? 1024 : 512;   // bytes of a block
     uint8_t* blocks = codes + (long long)w.in_page * NC * BB;
@@ -303,7 +306,7 @@ __global__ __launch_bounds__(64) void kv_read_kernel(KvCache c, KvTokens t) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[j] = 0.0f;
             if (in) {
-                const float sc = (float)scales[(long long)(BITS == 8 ? 0 : k) * c.page_size + w.in_page * 32 + kv_slot(tok)];
+                const float sc = (float)scales[(long long)(BITS == 8 ? 0 : k) * c.page_size + w.in_page * 32 + scale_slot<BITS>(values, tok)];
                 u2 q = {0, 0};
                 uint32_t n = 0;
                 if (!values) {

@@ -62,6 +62,7 @@ def attention(q, keys, vals, scale, visible):
     """One sequence and key/value head, float64. q [S, G, hd], keys / vals
     [n, hd], visible [S] counts of keys seen. Returns (y, tolerance terms)."""
     S, G, hd = q.shape
+    floor = 2.0 ** -39 if q.dtype == torch.float32 else 2.0 ** -35
     q = q.double()
     y, tol = torch.zeros(S, G, hd, dtype=torch.float64), torch.zeros(S, G, hd, dtype=torch.float64)
     for s in range(S):
@@ -74,11 +75,12 @@ def attention(q, keys, vals, scale, visible):
         size = (q[s].abs() @ keys[:n].abs().T * abs(scale)).amax(-1, keepdim=True)
         # fp16 has no steps below 2^-24. A query's elements are rounded to such
         # a half step of a row scaled to 2^14 and more: 2^-25 / 2^14 of the
-        # largest. A weight times 2^15 (times its value's scale over the unit u,
-        # a power of two at most twice the largest scale) is rounded so too:
-        # 2^-40 u a code, so 2^-39 of the largest value a key.
+        # largest. A weight p times 2^15 (2^11 for fp16 and bf16 tensors; times
+        # its value's scale over the unit u, a power of two at most twice the
+        # largest scale) is rounded so too: 2^-40 u (2^-36 u) a code, so twice
+        # that of the largest value a key.
         low = 2.0 ** -39 * q[s].abs().amax() * keys[:n].abs().sum(-1).amax() * abs(scale)
-        tol[s] = mag * (2 * size * (hd + 16) * U + 2 * low + (64 + n / 8) * U) + n * 2.0 ** -39 * vals[:n].abs().amax()
+        tol[s] = mag * (2 * size * (hd + 16) * U + 2 * low + (64 + n / 8) * U) + n * floor * vals[:n].abs().amax()
     return y, tol
 
 
