@@ -50,8 +50,9 @@ hipError_t launch_nbits_pack(const uint8_t* raw, const void* raw_scales, const u
 //   keys    lane (t & 15) + 16 (e >> 3): elements 8 (e >> 3) + j of token t, then of t + 16
 //   values  lane (e & 15) + 16 g:        tokens kv_slot^-1(8 g + j) of element e, then of e + 16
 // so attention loads operands of either product with no shuffle. 8-bit codes
-// are stored as code + 128, 4-bit ones as code + 8, j even in nibble j / 2 and
-// j odd in nibble 4 + j / 2 of a word of eight.
+// are stored as code + 128. Of 4-bit ones eight make a word, code + 8 each:
+// j even in nibble j / 2, j odd in nibble 4 + j / 2, and the word turned left
+// by two bits (a shift and a mask then leave a pair in its fp16 places).
 // Scales are bf16, [group][page_size], a tile's 32 in the order of kv_slot; the
 // keys' at 4 bits, which belong to an operand's rows, in the order of kv_pair.
 struct KvCache {
@@ -68,6 +69,8 @@ __host__ __device__ inline long long kv_head_bytes(int page, int hd, int bits) {
 // the order in which the two 16-token tiles of a score product leave a lane
 // its four rows each
 __host__ __device__ inline int kv_slot(int t) { return 8 * ((t >> 2) & 3) + 4 * (t >> 4) + (t & 3); }
+__host__ __device__ inline uint32_t kv_turn(uint32_t w) { return w << 2 | w >> 30; }
+__host__ __device__ inline uint32_t kv_unturn(uint32_t w) { return w >> 2 | w << 30; }
 // tokens t and t + 16 side by side
 __host__ __device__ inline int kv_pair(int t) { return 2 * (t & 15) + (t >> 4); }
 

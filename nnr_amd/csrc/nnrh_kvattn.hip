@@ -24,6 +24,8 @@
 // writes the result itself.
 #include "nnrh_decode.h"
 
+#include <algorithm>
+
 namespace nnrh {
 namespace {
 
@@ -117,16 +119,26 @@ __device__ __forceinline__ h8 codes8(uint32_t lo, uint32_t hi) {
     for (int i = 0; i < 4; ++i) r[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, (uint32_t)r[i]) - off);
     return __builtin_bit_cast(h8, r);
 }
-// eight 4-bit codes (code + 8) times scales s[0..3], a pair each
-__device__ __forceinline__ h8 codes4(uint32_t w, const h2* s) {
-    const h2 off = {(_Float16)1032.0f, (_Float16)1032.0f};
-    u4 r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const h2 v = __builtin_bit_cast(h2, ((w >> (4 * i)) & 0x000f000fu) | 0x64006400u) - off;
-        r[i] = __builtin_bit_cast(uint32_t, v * s[i]);
+// Eight 4-bit codes (code + 8) times scales s[0..3], a pair each: a nibble q
+// under the exponent of 16 is 16 + q, and (16 + q) s - 24 s = code s, where 24 s
+// has 10 bits and the result 11.
+struct Scale4 {
+    h2 s, s24;
+    __device__ __forceinline__ void set(_Float16 a, _Float16 b) {
+        s = h2{a, b};
+        s24 = s * h2{(_Float16)-24.0f, (_Float16)-24.0f};
     }
-    return __builtin_bit_cast(h8, r);
+};
+__device__ __forceinline__ h2 pair4(uint32_t w, uint32_t magic, const Scale4& s) {
+    return __builtin_elementwise_fma(__builtin_bit_cast(h2, (w & 0x03c003c0u) | magic), s.s, s.s24);
+}
+__device__ __forceinline__ h8 codes4(uint32_t w, const Scale4& a, const Scale4& b, const Scale4& c, const Scale4& d) {
+    // (in a vector register: mask, or and word are then one instruction)
+    uint32_t magic;
+    asm("v_mov_b32 %0, 0x4c004c00" : "=v"(magic));
+    const h2 r[4] = {pair4(w << 4, magic, a), pair4(w, magic, b), pair4(w >> 4, magic, c),
+                     pair4(__builtin_amdgcn_alignbit(w, w, 8), magic, d)};
+    return h8{r[0][0], r[0][1], r[1][0], r[1][1], r[2][0], r[2][1], r[3][0], r[3][1]};
 }
 
 __device__ __forceinline__ void load_q8(const KvAttention& a, long long at, float* v) {
@@ -215,6 +227,18 @@ __device__ __forceinline__ void set_rows(const AttnArgs& p, const Job& job, int 
 }
 
 template <int BITS, int HD, int NP, int NR>
+__device__ __forceinline__ void clear_rows(Rows<HD, NP, NR>& w) {
+#pragma unroll
+    for (int t = 0; t < NR; ++t) {
+        w.m[t] = kNegInf;
+        w.l[t] = f4{0, 0, 0, 0};
+#pragma unroll
+        for (int d = 0; d < HD / 16; ++d) w.o[t][d] = f4{0, 0, 0, 0};
+    }
+    w.eu = kNoUnit;
+    w.ek = BITS == 8 ? 0 : kNoUnit;
+}
+template <int BITS, int HD, int NP, int NR>
 __device__ __forceinline__ void load_rows(const AttnArgs& p, Rows<HD, NP, NR>& w) {
     constexpr int NC = HD / 32;
     const KvAttention& a = p.a;
@@ -246,58 +270,55 @@ __device__ __forceinline__ void load_rows(const AttnArgs& p, Rows<HD, NP, NR>& w
                 w.q[0][t][k][j] = h;
                 if constexpr (NP == 2) w.q[1][t][k][j] = (_Float16)(s - (float)h);
             }
-        w.m[t] = kNegInf;
-        w.l[t] = f4{0, 0, 0, 0};
-#pragma unroll
-        for (int d = 0; d < HD / 16; ++d) w.o[t][d] = f4{0, 0, 0, 0};
     }
-    w.eu = kNoUnit;
-    w.ek = BITS == 8 ? 0 : kNoUnit;
+    clear_rows<BITS>(w);
 }
 
 // element j of 8 bf16 numbers
 __device__ __forceinline__ float bf16_at(u4 w, int j) { return j & 1 ? bf16_hi(w[j >> 1]) : bf16_lo(w[j >> 1]); }
 
-// KT tiles from key `key0` on against a wave's rows. keys(z, f): tile z's keys as
-// operands, f[2 c + i] elements 32 c .. of keys 16 i ..; values(z, f): f[2 c + i]
-// elements 32 c + 16 i .. of its keys. They are asked for well before they are
-// used. ks, vs: scales of this lane's 8 keys (8 bits; vs are 0 where there is no
-// token; at 4 bits scales are in the operands, keys' over 2^ek, values' over
-// 2^en). ek, en: the units from here on. held: tokens in each tile; some: not all
-// have 32. between: what can be done while the first keys are on their way.
-template <int HD, int BITS, int NP, int NR, int KT, class Keys, class Values, class Between>
+// KT tiles from key `key0` on against a wave's rows. key(z, 2 c + i): elements
+// 32 c .. of keys 16 i .. of tile z as an operand; value(z, 2 c + i): elements
+// 32 c + 16 i .. of its keys. They are asked for a tile before they are used.
+// ks, vs: scales of this lane's 8 keys (8 bits; vs are 0 where there is no token;
+// at 4 bits scales are in the operands, keys' over 2^ek, values' over 2^en). ek,
+// en: the units from here on. held: tokens in each tile; some: not all have 32.
+// after_keys, after_values: what can be done while the first are on their way.
+template <int HD, int BITS, int NP, int NR, int KT, class Key, class Value, class AfterKeys, class AfterValues>
 __device__ __forceinline__ void tile_step(Rows<HD, NP, NR>& w, int key0, const int* held, bool some, const u4* ks,
-                                          const u4* vs, int ek, int en, Keys keys, Values values, Between between) {
+                                          const u4* vs, int ek, int en, Key key, Value value, AfterKeys after_keys,
+                                          AfterValues after_values) {
     constexpr int NC = HD / 32, ND = HD / 16;
     constexpr float slack = NP == 1 ? kSlack : 0.0f, top = NP == 1 ? kTop - kSlack : kTop;
     const int g = (threadIdx.x & 63) >> 4;
     h8 kf[2 * NC];
-    keys(0, kf);
-    between();
+#pragma unroll
+    for (int j = 0; j < 2 * NC; ++j) kf[j] = key(0, j);
+    __builtin_amdgcn_sched_barrier(0);
+    after_keys();
     f4 acc[NR][KT][2];
 #pragma unroll
     for (int t = 0; t < NR; ++t)
 #pragma unroll
         for (int z = 0; z < KT; ++z) acc[t][z][0] = acc[t][z][1] = f4{0, 0, 0, 0};
 #pragma unroll
-    for (int z = 0; z < KT; ++z) {
-        h8 kn[2 * NC];
-        if (z + 1 < KT) keys(z + 1, kn);
+    for (int z = 0; z < KT; ++z)
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < 2; ++i) {
 #pragma unroll
                 for (int t = 0; t < NR; ++t)
 #pragma unroll
                     for (int q = 0; q < NP; ++q)
                         acc[t][z][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[2 * c + i], w.q[q][t][c], acc[t][z][i], 0, 0, 0);
-        if (z + 1 < KT)
-#pragma unroll
-            for (int j = 0; j < 2 * NC; ++j) kf[j] = kn[j];
-    }
+                if (z + 1 < KT) kf[2 * c + i] = key(z + 1, 2 * c + i);
+            }
     h8 vf[2 * NC];
-    values(0, vf);
+#pragma unroll
+    for (int j = 0; j < 2 * NC; ++j) vf[j] = value(0, j);
+    __builtin_amdgcn_sched_barrier(0);
+    after_values();
     if (BITS == 4 && ek != w.ek) {
         stay_a_branch();
 #pragma unroll
@@ -397,18 +418,15 @@ __device__ __forceinline__ void tile_step(Rows<HD, NP, NR>& w, int key0, const i
                 for (int q = 0; q < NP; ++q)
                     w.l[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pf[q][t], w.l[t], 0, 0, 0);
         }
-        h8 vn[2 * NC];
-        if (z + 1 < KT) values(z + 1, vn);
 #pragma unroll
-        for (int d = 0; d < ND; ++d)
+        for (int d = 0; d < ND; ++d) {
 #pragma unroll
             for (int t = 0; t < NR; ++t)
 #pragma unroll
                 for (int q = 0; q < NP; ++q)
                     w.o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[d], pf[q][t], w.o[t][d], 0, 0, 0);
-        if (z + 1 < KT)
-#pragma unroll
-            for (int d = 0; d < ND; ++d) vf[d] = vn[d];
+            if (z + 1 < KT) vf[d] = value(z + 1, d);
+        }
     }
 }
 
@@ -470,13 +488,13 @@ __device__ __forceinline__ void held_pair(uint32_t w, int held, uint32_t* s) {
 }
 __device__ __forceinline__ h8 key4(uint32_t codes, uint32_t scale, float unit) {
     const _Float16 x = (_Float16)(__builtin_bit_cast(float, scale) * unit);
-    const h2 s = {x, x};
-    const h2 s4[4] = {s, s, s, s};
-    return codes4(codes, s4);
+    Scale4 s;
+    s.set(x, x);
+    return codes4(codes, s, s, s, s);
 }
-__device__ __forceinline__ void value_scales(u4 w, float unit, h2* s) {
+__device__ __forceinline__ void value_scales(u4 w, float unit, Scale4* s) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) s[j] = h2{(_Float16)(bf16_lo(w[j]) * unit), (_Float16)(bf16_hi(w[j]) * unit)};
+    for (int j = 0; j < 4; ++j) s[j].set((_Float16)(bf16_lo(w[j]) * unit), (_Float16)(bf16_hi(w[j]) * unit));
 }
 
 __device__ __forceinline__ int page_id(const Job& job, const AttnArgs& p, int tile) {
@@ -484,7 +502,8 @@ __device__ __forceinline__ int page_id(const Job& job, const AttnArgs& p, int ti
 }
 
 // ---- few rows: the block's waves split its keys -------------------------------
-// Each wave loads a tile's codes into registers one tile ahead.
+// A wave has the codes of one tile on their way: as soon as its keys are turned
+// into operands, the next tile's are asked for, and so the values.
 template <int HD, int BITS> struct RawTile {
     static constexpr int NC = HD / 32;
     typedef uint32_t vec __attribute__((ext_vector_type(BITS == 8 ? 4 : 2)));
@@ -492,20 +511,21 @@ template <int HD, int BITS> struct RawTile {
     u4 vs[BITS == 8 ? 1 : NC];
     u4 ks;                        // 8 bits
     uint32_t ks4[NC];             // 4 bits
-    bool ok;
-    __device__ __forceinline__ void load(const AttnArgs& p, const Job& job, int tile) {
+    __device__ __forceinline__ void load_keys(const AttnArgs& p, const TilePtr& t) {
         constexpr int BB = BITS == 8 ? 1024 : 512;
         const int lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
-        const TilePtr t = tile_ptr<HD, BITS>(p, job.head, page_id(job, p, tile), tile);
-        ok = t.ok;
-        const uint8_t* vc = t.codes + kv_codes_bytes(p.c.page_size, HD, BITS);
-        const uint16_t* vsp = t.scales + (long long)p.c.page_size * kv_groups(HD, BITS);
-#pragma unroll
-        for (int c = 0; c < NC; ++c) k[c] = *(const vec*)(t.codes + c * BB + lane * sizeof(vec));
         if constexpr (BITS == 8) ks = *(const u4*)(t.scales + 8 * g);
         else
 #pragma unroll
             for (int c = 0; c < NC; ++c) ks4[c] = *(const uint32_t*)(t.scales + c * p.c.page_size + 2 * col);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) k[c] = *(const vec*)(t.codes + c * BB + lane * sizeof(vec));
+    }
+    __device__ __forceinline__ void load_values(const AttnArgs& p, const TilePtr& t) {
+        constexpr int BB = BITS == 8 ? 1024 : 512;
+        const int lane = threadIdx.x & 63, g = lane >> 4;
+        const uint8_t* vc = t.codes + kv_codes_bytes(p.c.page_size, HD, BITS);
+        const uint16_t* vsp = t.scales + (long long)p.c.page_size * kv_groups(HD, BITS);
 #pragma unroll
         for (int c = 0; c < (BITS == 8 ? 1 : NC); ++c) vs[c] = *(const u4*)(vsp + c * p.c.page_size + 8 * g);
 #pragma unroll
@@ -513,10 +533,11 @@ template <int HD, int BITS> struct RawTile {
     }
 };
 
+// next: the tile to load meanwhile
 template <int HD, int BITS, int NP>
-__device__ __forceinline__ void few_tile(Rows<HD, NP, 1>& w, const RawTile<HD, BITS>& r, int tile, int held) {
+__device__ __forceinline__ void few_tile(const AttnArgs& p, Rows<HD, NP, 1>& w, RawTile<HD, BITS>& r, int tile, int held,
+                                         const TilePtr& next) {
     constexpr int NC = HD / 32;
-    const int col = threadIdx.x & 15;
     u4 vs[BITS == 8 ? 1 : NC];
     uint32_t vtop = 0;
 #pragma unroll
@@ -525,45 +546,42 @@ __device__ __forceinline__ void few_tile(Rows<HD, NP, 1>& w, const RawTile<HD, B
         vtop = umax(vtop, top8(vs[c]));
     }
     const int en = max(w.eu, ceil_exp(__builtin_amdgcn_readfirstlane(umax16_32(vtop)), kNoUnit));
-    const auto nothing = [] {};
-    if constexpr (BITS == 8) {
-        tile_step<HD, 8, NP, 1, 1>(
-            w, tile * 32, &held, held < 32, &r.ks, vs, 0, en,
-            [&](int, h8* f) {
-#pragma unroll
-                for (int j = 0; j < 2 * NC; ++j) f[j] = codes8(r.k[j >> 1][2 * (j & 1)], r.k[j >> 1][2 * (j & 1) + 1]);
-            },
-            [&](int, h8* f) {
-#pragma unroll
-                for (int j = 0; j < 2 * NC; ++j) f[j] = codes8(r.v[j >> 1][2 * (j & 1)], r.v[j >> 1][2 * (j & 1) + 1]);
-            },
-            nothing);
-    } else {
-        uint32_t kb[NC][2], top = 0;
+    int ek = 0;
+    const u4 ks = r.ks;
+    uint32_t kb[NC][2];
+    if constexpr (BITS == 4) {
+        uint32_t top = 0;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             held_pair(r.ks4[c], held, kb[c]);
             top = umax(top, umax(kb[c][0], kb[c][1]));
         }
-        const int ek = max(w.ek, ceil_exp(__builtin_amdgcn_readfirstlane(umax_16(top) >> 16), kNoUnit));
-        const float fk = ldexpf(1.0f, -ek), fv = ldexpf(1.0f, -en);
-        tile_step<HD, 4, NP, 1, 1>(
-            w, tile * 32, &held, held < 32, nullptr, nullptr, ek, en,
-            [&](int, h8* f) {
-#pragma unroll
-                for (int j = 0; j < 2 * NC; ++j) f[j] = key4(r.k[j >> 1][j & 1], kb[j >> 1][j & 1], fk);
-            },
-            [&](int, h8* f) {
-#pragma unroll
-                for (int c = 0; c < NC; ++c) {
-                    h2 s[4];
-                    value_scales(vs[c], fv, s);
-                    f[2 * c] = codes4(r.v[c][0], s);
-                    f[2 * c + 1] = codes4(r.v[c][1], s);
-                }
-            },
-            nothing);
+        ek = max(w.ek, ceil_exp(__builtin_amdgcn_readfirstlane(umax_16(top) >> 16), kNoUnit));
     }
+    const float fk = ldexpf(1.0f, -ek), fv = ldexpf(1.0f, -en);
+    tile_step<HD, BITS, NP, 1, 1>(
+        w, tile * 32, &held, held < 32, &ks, vs, ek, en,
+        [&](int, int j) {
+            if constexpr (BITS == 8) return codes8(r.k[j >> 1][2 * (j & 1)], r.k[j >> 1][2 * (j & 1) + 1]);
+            else return key4(r.k[j >> 1][j & 1], kb[j >> 1][j & 1], fk);
+        },
+        [&](int, int j) {
+            if constexpr (BITS == 8) {
+                return codes8(r.v[j >> 1][2 * (j & 1)], r.v[j >> 1][2 * (j & 1) + 1]);
+            } else {
+                Scale4 s[4];
+                value_scales(vs[j >> 1], fv, s);
+                return codes4(r.v[j >> 1][j & 1], s[0], s[1], s[2], s[3]);
+            }
+        },
+        [&] {
+            r.load_keys(p, next);
+            __builtin_amdgcn_sched_barrier(0);
+        },
+        [&] {
+            r.load_values(p, next);
+            __builtin_amdgcn_sched_barrier(0);
+        });
 }
 
 // the results of a wave's rows: into the call's result, or among the parts
@@ -598,20 +616,32 @@ __device__ __forceinline__ void few(const AttnArgs& p, Job& job, char* lds) {
     set_rows(p, job, job.row0, w);
     job.t1 = min(job.t1, (w.hi + 31) / 32);
     int tile = job.t0 + wave;
-    RawTile<HD, BITS> cur{}, nxt{};
-    if (tile < job.t1) cur.load(p, job, tile);
-    load_rows<BITS>(p, w);
-    for (; tile < job.t1; tile += AW) {
-        if (tile + AW < job.t1) nxt.load(p, job, tile + AW);
-        few_tile<HD, BITS, NP>(w, cur, tile, cur.ok ? (int)min(job.len - (long long)tile * 32, 32ll) : 0);
-        cur = nxt;
+    RawTile<HD, BITS> raw;
+    // (past the last tile its own are loaded again, for nothing)
+    const auto at = [&](int x) {
+        const int y = min(x, job.t1 - 1);
+        return tile_ptr<HD, BITS>(p, job.head, page_id(job, p, y), y);
+    };
+    if (tile < job.t1) {
+        TilePtr cur = at(tile), next = at(tile + AW);
+        raw.load_keys(p, cur);
+        raw.load_values(p, cur);
+        load_rows<BITS>(p, w);
+        for (; tile < job.t1; tile += AW) {
+            const TilePtr after = at(tile + 2 * AW);
+            few_tile<HD, BITS, NP>(p, w, raw, tile, cur.ok ? (int)min(job.len - (long long)tile * 32, 32ll) : 0, next);
+            cur = next;
+            next = after;
+        }
+    } else {
+        clear_rows<BITS>(w);
     }
     // join the waves: first everyone's maximum, then sums in the units of it
     f4(*buf)[ND][64] = (f4(*)[ND][64])lds;                       // [2]
     float(*sm)[16] = (float(*)[16])(lds + 2 * sizeof(*buf));     // [AW]
     float(*sl)[16] = sm + AW;
     const float lw = row_total<BITS>(w.l[0]);
-    const float top = w.m[0] == kNegInf ? kNegInf : w.m[0] * w.rk[0];
+    const float top = w.m[0] == kNegInf ? kNegInf : w.m[0] * w.rk[0];   // (rk is not set where there was no tile)
     if (g == 0) {
         sm[wave][col] = top;
         sl[wave][col] = lw;
@@ -785,10 +815,10 @@ __device__ __forceinline__ void many(const AttnArgs& p, Job& job, char* lds) {
 #pragma unroll
                     for (int i = 0; i < 2; ++i) to[64 * i] = key4(raw[z].code[u][i], s[i], fk);
                 } else {
-                    h2 s[4];
+                    Scale4 s[4];
                     value_scales(held_scales(raw[z].sc[u], held_next[z]), fv, s);
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) to[64 * i] = codes4(raw[z].code[u][i], s);
+                    for (int i = 0; i < 2; ++i) to[64 * i] = codes4(raw[z].code[u][i], s[0], s[1], s[2], s[3]);
                 }
             }
     };
@@ -831,23 +861,15 @@ __device__ __forceinline__ void many(const AttnArgs& p, Job& job, char* lds) {
         const h8(*f)[4 * NC][64] = frag[at];
         tile_step<HD, BITS, NP, NR, KT>(
             w, tile * 32, held, some, ks_raw, vs_raw, ek, en,
-            [&](int z, h8* x) {
-#pragma unroll
-                for (int j = 0; j < 2 * NC; ++j) x[j] = f[z][j][lane];
-                __builtin_amdgcn_sched_barrier(0);
-            },
-            [&](int z, h8* x) {
-#pragma unroll
-                for (int j = 0; j < 2 * NC; ++j) x[j] = f[z][2 * NC + j][lane];
-                __builtin_amdgcn_sched_barrier(0);
-            },
+            [&](int z, int j) { return f[z][j][lane]; }, [&](int z, int j) { return f[z][2 * NC + j][lane]; },
             [&] {   // past the last tile for nothing: without a branch
                 convert(tile + KT, at ^ 1);
                 __builtin_amdgcn_sched_barrier(0);
                 load(tile + 2 * KT);
                 ids(tile + 3 * KT);
                 __builtin_amdgcn_sched_barrier(0);
-            });
+            },
+            [] {});
         __syncthreads();
     }
     if (row0 >= job.nrows) return;
@@ -882,15 +904,24 @@ __global__ __launch_bounds__(AW * 64, HD <= 128 ? 2 : 1) void kv_attn_kernel(Att
     job.pre = (int)blockIdx.x < npre;
     int x = job.pre ? blockIdx.x : blockIdx.x - npre;
     const int ns = job.pre ? p.pre_slots : p.slots - p.pre_slots;
-    job.split = x % ns;
-    x /= ns;
-    job.head = x % H;
-    x /= H;
+    // Blocks go to the 8 XCDs in turn. The prefix's: splits first, then heads, so
+    // that row groups which read the same keys are a multiple of 8 apart where
+    // heads times splits is one. The sequences': heads first and splits last, as
+    // late splits of short sequences are empty and would leave an XCD idle.
     job.b = 0;
-    int group = x;
-    if (!job.pre) {
-        job.b = x / p.own_groups;
-        group = x - job.b * p.own_groups;
+    int group;
+    if (job.pre) {
+        job.split = x % ns;
+        x /= ns;
+        job.head = x % H;
+        group = x / H;
+    } else {
+        job.head = x % H;
+        x /= H;
+        group = x % p.own_groups;
+        x /= p.own_groups;
+        job.b = x % a.batch;
+        job.split = x / a.batch;
     }
     job.slot = job.pre ? job.split : p.pre_slots + job.split;
     job.nrows = (job.pre ? a.batch : 1) * a.seq * p.G;
@@ -973,14 +1004,25 @@ Plan plan(const KvCache& c, const KvAttention& a) {
     p.pre_groups = a.prefix_len ? ceil_div(pre_rows, p.pre_many ? many : 16) : 0;
     const long long pre_items = (long long)p.pre_groups * c.heads, own_items = (long long)p.own_groups * c.heads * a.batch;
     const long long pre_tiles = (a.prefix_len + 31) / 32, own_tiles = (long long)a.max_pages * c.page_size / 32;
-    // prefix blocks, and others with many rows: as many as run at once
-    const auto chunk = [](long long items, long long tiles, bool many) {
-        const long long blocks = many ? 512 : 2048, least = 8;
-        const long long c = (items * tiles + blocks - 1) / blocks;
-        return c < least ? least : c;
+    // Blocks with many rows: no more than run at once, of 8 tiles or more. (128
+    // sequences after a prefix of 32768: 512 blocks 139 us, 384 147, 768 154.)
+    const long long at_once = c.hd <= 128 ? 512 : 256;
+    long long chunk = 8;
+    for (;; chunk += 2) {
+        const long long pre = p.pre_many ? pre_items * ceil_div(pre_tiles, chunk) : 0;
+        const long long own = p.own_many ? own_items * ceil_div(own_tiles, chunk) : 0;
+        if (pre + own <= at_once || chunk >= std::max(pre_tiles, own_tiles)) break;
+        chunk += chunk / 16 * 2;
+    }
+    // Those with few: 32 tiles or more, and short ones whole. (A split of 8 tiles a
+    // block, and its join: 48 sequences of 8192 87 us instead of 85, 16 of 1000
+    // 14 instead of 12.7, 4 of 8192 20 instead of 16, one of 700 13.7 instead of 10.)
+    const auto few = [](long long items, long long tiles) {
+        return tiles <= 32 ? std::max(tiles, 1ll) : std::max(items * tiles / 1024, 32ll);
     };
-    p.pre_slots = p.pre_groups ? ceil_div(pre_tiles, chunk(pre_items, pre_tiles, p.pre_many)) : 0;
-    p.own_slots = own_tiles ? ceil_div(own_tiles, chunk(own_items, own_tiles, p.own_many)) : 1;
+    const long long pre_c = p.pre_many ? chunk : few(pre_items, pre_tiles), own_c = p.own_many ? chunk : few(own_items, own_tiles);
+    p.pre_slots = p.pre_groups ? ceil_div(pre_tiles, pre_c) : 0;
+    p.own_slots = own_tiles ? ceil_div(own_tiles, own_c) : 1;
     p.pre_chunk = p.pre_slots ? ceil_div(pre_tiles, p.pre_slots) : 0;
     p.own_chunk = ceil_div(own_tiles, p.own_slots);
     return p;

@@ -108,12 +108,12 @@ __device__ __forceinline__ int code_of(float v, float s, float limit) {
     if (s == 0.0f || !(v == v)) return 0;
     return (int)fminf(fmaxf(rintf(v / s), -limit), limit);
 }
-// nibbles in the order of a word (j even: j / 2, j odd: 4 + j / 2)
+// eight codes as a word (j even: nibble j / 2, j odd: 4 + j / 2; turned)
 __device__ __forceinline__ uint32_t pack_nibbles(const uint32_t* q) {
     uint32_t w = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) w |= q[j] << (4 * ((j >> 1) + 4 * (j & 1)));
-    return w;
+    return kv_turn(w);
 }
 __device__ __forceinline__ uint32_t nibble(uint32_t w, int j) { return (w >> (4 * ((j >> 1) + 4 * (j & 1)))) & 15u; }
 
@@ -240,6 +240,7 @@ __global__ __launch_bounds__(64) void kv_write_kernel(KvCache c, KvTokens t) {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
                 if (keep >> j & 1) m |= 15u << (4 * ((j >> 1) + 4 * (j & 1)));
+            m = kv_turn(m);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 uint32_t q[8];
@@ -282,7 +283,7 @@ __global__ __launch_bounds__(64) void kv_read_kernel(KvCache c, KvTokens t) {
                 for (int h = 0; h < 2; ++h) {
                     e[h] = u2{0, 0};
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) e[h][j >> 2] |= nibble(v[h], j) << (8 * (j & 3));
+                    for (int j = 0; j < 8; ++j) e[h][j >> 2] |= nibble(kv_unturn(v[h]), j) << (8 * (j & 3));
                 }
             }
 #pragma unroll
@@ -311,7 +312,7 @@ __global__ __launch_bounds__(64) void kv_read_kernel(KvCache c, KvTokens t) {
                 uint32_t n = 0;
                 if (!values) {
                     if constexpr (BITS == 8) q = *(const u2*)(blocks + k * BB + lane * 16 + h * 8);
-                    else n = *(const uint32_t*)(blocks + k * BB + lane * 8 + h * 4);
+                    else n = kv_unturn(*(const uint32_t*)(blocks + k * BB + lane * 8 + h * 4));
                 }
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
