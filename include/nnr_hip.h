@@ -579,7 +579,7 @@ int nnrh_clip_f32(const float* x_dev, float* y_dev, size_t n, float lo, float hi
 
 /* com.microsoft MatMulNBits with a constant B, bits = 4:
  *   y[m][n] = sum_k a[m][k] (q[n][k] - zp[n][k / block]) scale[n][k / block] + bias[n]
- * block_size: a power of two >= 32; K need not be a multiple of it. Column n's
+ * block_size: a power of two >= 32; K (at most 2^22) need not be a multiple of it. Column n's
  * ceil(k / block_size) blocks lie one after another, block_size / 2 bytes
  * each, the lower nibble first; zero points likewise, two a byte, a column's
  * rounded up to a whole byte (NULL: 8). run takes a of m x k and writes y of

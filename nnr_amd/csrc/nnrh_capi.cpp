@@ -2318,8 +2318,8 @@ extern "C" int nnrh_matmul_nbits_create(nnrh_matmul_nbits_t* out, const nnrh_mat
     if (d->bits != 4 || d->block_size < 32 || float_type(d->dtype) < 0)
         return set_err(NNRH_ERR_UNSUPPORTED, "matmul_nbits: bits %d, block size %d, type %d (4 bits, blocks of 32 and "
                                              "more, fp32 / fp16 / bf16)", d->bits, d->block_size, d->dtype);
-    // K of the last block, and columns of the last tile, in an int
-    if (d->k > (1 << 30) || d->n > (1 << 30) || d->block_size > (1 << 30))
+    // bytes of a block's rows (64 fp32 ones) and columns of the last tile in an int
+    if (d->k > (1 << 22) || d->n > (1 << 30) || d->block_size > (1 << 22))
         return set_err(NNRH_ERR_UNSUPPORTED, "matmul_nbits: n %d, k %d, block size %d", d->n, d->k, d->block_size);
     nnrh_matmul_nbits* h = new (std::nothrow) nnrh_matmul_nbits();
     if (!h) return set_err(NNRH_ERR_NOMEM, "matmul_nbits: host allocation");

@@ -33,7 +33,7 @@ struct NbitsArgs {
     int type;                              // FloatType
 };
 inline int nbits_pieces(int K) { return (K + NB_PK - 1) / NB_PK; }
-inline int nbits_cols(int N) { return (N + 63) / 64 * 64; }
+inline int nbits_cols(int N) { return (N + 127) / 128 * 128; }   // columns held: whole blocks of them
 inline int nbits_nspp(int block) { return block >= NB_PK ? 1 : NB_PK / block; }
 hipError_t launch_nbits(const NbitsArgs& a, hipStream_t s);
 // raw: [N][nb][block / 2] codes, low nibble first; raw_scales [N][nb] of `type`;

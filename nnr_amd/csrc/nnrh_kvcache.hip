@@ -108,15 +108,41 @@ __device__ __forceinline__ int code_of(float v, float s, float limit) {
     if (s == 0.0f || !(v == v)) return 0;
     return (int)fminf(fmaxf(rintf(v / s), -limit), limit);
 }
-// eight codes as a word (j even: nibble j / 2, j odd: 4 + j / 2; turned)
-__device__ __forceinline__ uint32_t pack_nibbles(const uint32_t* q) {
-    uint32_t w = 0;
+// Codes + zero of 8 elements, a byte each: the quotient by way of the scale's
+// reciprocal, which is off by 2e-5 at most (127 x 2^-23 x 1.5), decides all that
+// lie further than that from a border; the rest, and what is not finite, take
+// the division. (A finite element's code needs no clamp: top / scale is below
+// L + 1/2, as scale is top / L within 2^-9.)
+template <int BITS>
+__device__ __forceinline__ u2 codes_of(const float* v, float s, float inv) {
+    constexpr float limit = BITS == 8 ? 127.0f : 7.0f, zero = BITS == 8 ? 128.0f : 8.0f;
+    float c[8];
+    bool near = false;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) w |= q[j] << (4 * ((j >> 1) + 4 * (j & 1)));
-    return kv_turn(w);
+    for (int j = 0; j < 8; ++j) {
+        const float t = v[j] * inv;
+        c[j] = rintf(t);
+        near |= !(fabsf(t - c[j]) < 0.4999f);
+    }
+    if (__any(near)) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) c[j] = (float)code_of(v[j], s, limit);
+    }
+    uint32_t lo = 0, hi = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        lo = __builtin_amdgcn_cvt_pk_u8_f32(c[j] + zero, j, lo);
+        hi = __builtin_amdgcn_cvt_pk_u8_f32(c[4 + j] + zero, j, hi);
+    }
+    return u2{lo, hi};
 }
 __device__ __forceinline__ uint32_t nibble(uint32_t w, int j) { return (w >> (4 * ((j >> 1) + 4 * (j & 1)))) & 15u; }
-
+// eight codes, a byte each, as a word of nibbles (j even: nibble j / 2, j odd: 4 + j / 2; turned)
+__device__ __forceinline__ uint32_t pack_nibbles(u2 q) {
+    // bytes 0 4 1 5 below bytes 2 6 3 7
+    const uint32_t x = __builtin_amdgcn_perm(q[1], q[0], 0x05010400u), y = __builtin_amdgcn_perm(q[1], q[0], 0x07030602u);
+    return kv_turn(x | y << 4);
+}
 template <int BITS>
 __device__ __forceinline__ int scale_slot(int values, int t) { return BITS == 4 && !values ? kv_pair(t) : kv_slot(t); }
 
@@ -129,19 +155,23 @@ template <int TY, int BITS, int HD>
 __global__ __launch_bounds__(64) void kv_write_kernel(KvCache c, KvTokens t) {
     constexpr int NC = HD / 32;
     constexpr float limit = BITS == 8 ? 127.0f : 7.0f;
-    constexpr int zero = BITS == 8 ? 128 : 8;
+    constexpr int BB = BITS == 8 ? 1024 : 512;   // bytes of a block
+    typedef uint32_t vec __attribute__((ext_vector_type(BITS == 8 ? 4 : 2)));   // a lane's bytes of it
     __shared__ __attribute__((aligned(16))) uint8_t lds[HD * kLdsRow];
     const int lane = threadIdx.x, g = lane >> 4;
     const int values = blockIdx.y & 1, head = blockIdx.y >> 1, b = blockIdx.z;
     const TileAt w = tile_at(c, t, b, head, blockIdx.x);
     if (!w.part) return;
     const void* src = values ? t.v : t.k;
-    bool in[2];
-    float x[2][NC][8], sc[2][NC];
+    const long long cb = kv_codes_bytes(c.page_size, HD, BITS);
+    uint8_t* blocks = w.part + (values ? cb : 0) + (long long)w.in_page * NC * BB;
+    bool in[2], half[2];   // this lane's tokens; has the wave any
+    float x[2][NC][8];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const int tok = (lane & 15) + 16 * h;
         in[h] = token_in(w, t.seq, tok);
+        half[h] = __any(in[h]);
         const long long at = (long long)b * t.bstride + (w.pos + tok - w.p0) * t.tstride + (long long)head * HD + 8 * g;
 #pragma unroll
         for (int k = 0; k < NC; ++k) {
@@ -150,110 +180,84 @@ __global__ __launch_bounds__(64) void kv_write_kernel(KvCache c, KvTokens t) {
             if (in[h]) load8<TY>(src, at + 32 * k, x[h][k]);
         }
     }
+    // values: what this lane's bytes hold beside the new tokens (slots 8 g .. 8 g + 7)
+    uint32_t keep = 0;   // bit j: slot 8 g + j is not written
+    vec old[NC];
+    if (values) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (!token_in(w, t.seq, 4 * g + (j & 3) + 16 * (j >> 2))) keep |= 1u << j;
+        if (keep != 0 && keep != 0xff)
+#pragma unroll
+            for (int k = 0; k < NC; ++k) old[k] = *(const vec*)(blocks + k * BB + lane * sizeof(vec));
+    }
+    __bf16* scales = (__bf16*)(w.part + 2 * cb) + (values ? (long long)c.page_size * kv_groups(HD, BITS) : 0);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        float all = 0.0f;
+        if (!half[h]) continue;
+        const int tok = (lane & 15) + 16 * h;
+        float sc[NC], inv[NC], all = 0.0f;
 #pragma unroll
         for (int k = 0; k < NC; ++k) {
             float m = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) m = fmaxf(m, finite_abs(x[h][k][j]));
             if (BITS == 8) all = fmaxf(all, m);
-            else sc[h][k] = scale_of(across_groups_max(m), limit);
+            else sc[k] = scale_of(across_groups_max(m), limit);
         }
         if (BITS == 8) {
             all = scale_of(across_groups_max(all), limit);
 #pragma unroll
-            for (int k = 0; k < NC; ++k) sc[h][k] = all;
+            for (int k = 0; k < NC; ++k) sc[k] = all;
         }
-    }
-    const long long cb = kv_codes_bytes(c.page_size, HD, BITS);
-    uint8_t* codes = w.part + (values ? cb : 0);
-    __bf16* scales = (__bf16*)(w.part + 2 * cb) + (values ? (long long)c.page_size * kv_groups(HD, BITS) : 0);
-    if (g == 0) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-            if (in[h])
+        for (int k = 0; k < NC; ++k) inv[k] = BITS == 8 && k ? inv[0] : sc[k] > 0.0f ? 1.0f / sc[k] : 0.0f;
+        if (g == 0 && in[h])
 #pragma unroll
-                for (int k = 0; k < (BITS == 8 ? 1 : NC); ++k)
-                    scales[(long long)k * c.page_size + w.in_page * 32 + scale_slot<BITS>(values, (lane & 15) + 16 * h)] = (__bf16)sc[h][k];
-    }
-    constexpr int BB = BITS == 8 ? 1024 : 512;   // bytes of a block
-    uint8_t* blocks = codes + (long long)w.in_page * NC * BB;
-    if (!values) {
+            for (int k = 0; k < (BITS == 8 ? 1 : NC); ++k)
+                scales[(long long)k * c.page_size + w.in_page * 32 + scale_slot<BITS>(values, tok)] = (__bf16)sc[k];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            if (!in[h]) continue;
+        for (int k = 0; k < NC; ++k) {
+            const u2 q = codes_of<BITS>(x[h][k], sc[k], inv[k]);
+            if (values) {
+                uint8_t* to = lds + (32 * k + 8 * g) * kLdsRow + kv_slot(tok);
 #pragma unroll
-            for (int k = 0; k < NC; ++k) {
-                uint32_t q[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) q[j] = (uint32_t)(code_of(x[h][k][j], sc[h][k], limit) + zero);
-                if constexpr (BITS == 8)
-                    *(u2*)(blocks + k * BB + lane * 16 + h * 8) =
-                        u2{q[0] | q[1] << 8 | q[2] << 16 | q[3] << 24, q[4] | q[5] << 8 | q[6] << 16 | q[7] << 24};
-                else
-                    *(uint32_t*)(blocks + k * BB + lane * 8 + h * 4) = pack_nibbles(q);
+                for (int j = 0; j < 8; ++j) to[j * kLdsRow] = (uint8_t)(q[j >> 2] >> (8 * (j & 3)));
+            } else if (in[h]) {
+                if constexpr (BITS == 8) *(u2*)(blocks + k * BB + lane * 16 + h * 8) = q;
+                else *(uint32_t*)(blocks + k * BB + lane * 8 + h * 4) = pack_nibbles(q);
             }
         }
-        return;
     }
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int k = 0; k < NC; ++k)
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                lds[(32 * k + 8 * g + j) * kLdsRow + kv_slot((lane & 15) + 16 * h)] =
-                    (uint8_t)(code_of(x[h][k][j], sc[h][k], limit) + zero);
+    if (!values) return;
     __syncthreads();
-    // this lane's 8 tokens: slots 8 g .. 8 g + 7
-    uint32_t keep = 0;   // bit j: slot 8 g + j is not written
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-        if (!token_in(w, t.seq, 4 * g + (j & 3) + 16 * (j >> 2))) keep |= 1u << j;
     if (keep == 0xff) return;
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
         u2 e[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) e[h] = *(const u2*)(lds + (32 * k + (lane & 15) + 16 * h) * kLdsRow + 8 * g);
+        vec out, m;
         if constexpr (BITS == 8) {
-            u4 out = {e[0][0], e[0][1], e[1][0], e[1][1]};
-            u4* to = (u4*)(blocks + k * BB + lane * 16);
-            if (keep) {
-                const u4 old = *to;
+            out = vec{e[0][0], e[0][1], e[1][0], e[1][1]};
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint32_t m = 0;
+            for (int i = 0; i < 4; ++i) {
+                m[i] = 0;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (keep >> (4 * (i & 1) + j) & 1) m |= 0xffu << (8 * j);
-                    out[i] = (out[i] & ~m) | (old[i] & m);
-                }
+                for (int j = 0; j < 4; ++j)
+                    if (keep >> (4 * (i & 1) + j) & 1) m[i] |= 0xffu << (8 * j);
             }
-            *to = out;
         } else {
-            u2 out;
-            u2* to = (u2*)(blocks + k * BB + lane * 8);
-            uint32_t m = 0;
+            uint32_t mm = 0;
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                if (keep >> j & 1) m |= 15u << (4 * ((j >> 1) + 4 * (j & 1)));
-            m = kv_turn(m);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                uint32_t q[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) q[j] = (e[h][j >> 2] >> (8 * (j & 3))) & 0xff;
-                out[h] = pack_nibbles(q);
-            }
-            if (keep) {
-                const u2 old = *to;
-                out = (out & ~m) | (old & m);
-            }
-            *to = out;
+                if (keep >> j & 1) mm |= 15u << (4 * ((j >> 1) + 4 * (j & 1)));
+            // (LDS holds anything where the wave has no token)
+            out = vec{pack_nibbles(e[0] & 0x0f0f0f0fu), pack_nibbles(e[1] & 0x0f0f0f0fu)};
+            m = vec{kv_turn(mm), kv_turn(mm)};
         }
+        if (keep) out = (out & ~m) | (old[k] & m);
+        *(vec*)(blocks + k * BB + lane * sizeof(vec)) = out;
     }
 }
 

@@ -17,6 +17,7 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef u4 __attribute__((aligned(2))) u4_any;
 
 __device__ __forceinline__ float f16_f32(uint16_t v) { return (float)__builtin_bit_cast(_Float16, v); }
 __device__ __forceinline__ float bf16_f32(uint32_t v) { return __builtin_bit_cast(float, v << 16); }
@@ -66,46 +67,88 @@ __device__ __forceinline__ AFrag<FT_F32> split3(const float* x) {
     return f;
 }
 
-// How a block reads activations: 16 bytes at a time where addresses allow it
-// (whole pieces of K, or with the last one cut short), else element by element
+// How activations are read, 16 bytes at a time: whole pieces of K at aligned
+// addresses, with the last one cut short, or at any address with the last chunk
+// element by element
 enum AMode : int { A_WHOLE = 0, A_EDGE = 1, A_ANY = 2 };
 
-// k .. k + 7 of a row, as they lie; elements from K on are 0
-template <int TY> struct ARaw {
-    u4 v[TY == FT_F32 ? 2 : 1];
+// Activations of MT row tiles, 64 K at a time (a chunk, two MFMA steps). An MFMA
+// wants neighbouring lanes to hold neighbouring rows, and loads that are
+// addressed so cost the L1 an access a lane: 64 rows x 8192 x 8192 columns took
+// 34 us with them, all of it accesses. So lanes load rows 16 bytes after 16
+// bytes, and operands come out of the wave's own stretch of LDS, in which the
+// 16-byte cells of a row are turned by its number (eight rows a read then lie
+// in different banks).
+template <int TY, int MT> struct Activations {
+    static constexpr int ES = TY == FT_F32 ? 4 : 2;
+    static constexpr int CELLS = 64 * ES / 16;              // cells of a row
+    static constexpr int NL = MT * 16 * CELLS / 64;         // cells a lane
+    static constexpr int BYTES = MT * 16 * 64 * ES;         // of a wave's stretch
+    u4 v[NL];
+    __device__ __forceinline__ static int row_of(int i) { return (i * 64 + (int)(threadIdx.x & 63)) / CELLS; }
+    __device__ __forceinline__ static int cell_of() { return (threadIdx.x & 63) % CELLS; }
+    // base: row m0 (uniform over the block); rows: that many from there on exist
+    // (the last one is repeated). K k0 .. k0 + 63 (uniform); elements from K on
+    // are 0. Offsets from uniform addresses fit 32 bits.
     template <int AM>
-    __device__ __forceinline__ void load(const void* row, int k, int K) {
-        constexpr int N = TY == FT_F32 ? 4 : 8;   // elements of 16 bytes
-        constexpr int ES = TY == FT_F32 ? 4 : 2;
+    __device__ __forceinline__ void load(const char* base, int rows, int k0, int K) {
+        constexpr int N = 16 / ES;
+        const int c = cell_of() * N;
 #pragma unroll
-        for (int i = 0; i < (TY == FT_F32 ? 2 : 1); ++i, k += N) {
+        for (int i = 0; i < NL; ++i) {
+            const uint32_t row = (uint32_t)min(row_of(i), rows - 1) * (uint32_t)(K * ES);
             if constexpr (AM == A_WHOLE) {
-                v[i] = *(const u4*)((const char*)row + (long long)k * ES);
+                v[i] = *(const u4*)(base + (long long)k0 * ES + (row + (uint32_t)(c * ES)));
             } else if constexpr (AM == A_EDGE) {   // no branch: loads stay in flight past it
-                const bool in = k < K;
-                const u4 x = *(const u4*)((const char*)row + (long long)(in ? k : 0) * ES);
+                const bool in = k0 + c < K;
+                const u4 x = *(const u4*)(base + (row + (uint32_t)(in ? (k0 + c) * ES : 0)));
 #pragma unroll
                 for (int j = 0; j < 4; ++j) v[i][j] = in ? x[j] : 0u;
+            } else if (k0 + 64 <= K) {   // (16 bytes from any address: a load like others)
+                v[i] = *(const u4_any*)(base + (long long)k0 * ES + (row + (uint32_t)(c * ES)));
             } else {
-                v[i] = u4{0, 0, 0, 0};
+                u4 x = {0, 0, 0, 0};
 #pragma unroll
-                for (int j = 0; j < N; ++j)
-                    if (k + j < K) {
-                        if constexpr (TY == FT_F32) v[i][j] = ((const uint32_t*)row)[k + j];
-                        else v[i][j >> 1] |= (uint32_t)((const uint16_t*)row)[k + j] << (16 * (j & 1));
-                    }
+                for (int j = 0; j < N; ++j) {
+                    const bool in = k0 + c + j < K;
+                    const uint32_t at = row + (uint32_t)(in ? (k0 + c + j) * ES : 0);
+                    if constexpr (TY == FT_F32) x[j] = in ? *(const uint32_t*)(base + at) : 0u;
+                    else x[j >> 1] |= (in ? (uint32_t)*(const uint16_t*)(base + at) : 0u) << (16 * (j & 1));
+                }
+                v[i] = x;
             }
         }
     }
-    __device__ __forceinline__ AFrag<TY> frag() const {
+    __device__ __forceinline__ void store(char* lds) const {
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+            const int r = row_of(i);
+            *(u4*)(lds + (r * CELLS + (cell_of() ^ (r & (CELLS - 1)))) * 16) = v[i];
+        }
+    }
+    // operand of step s (0, 1) and row tile t, as it lies
+    struct Raw { u4 v[TY == FT_F32 ? 2 : 1]; };
+    __device__ __forceinline__ static Raw read(const char* lds, int s, int t) {
+        const int r = 16 * t + (int)(threadIdx.x & 15), g = (threadIdx.x & 63) >> 4;
+        const auto cell = [&](int c) { return *(const u4*)(lds + (r * CELLS + (c ^ (r & (CELLS - 1)))) * 16); };
+        Raw x;
+        if constexpr (TY == FT_F32) {
+            x.v[0] = cell(8 * s + 2 * g);
+            x.v[1] = cell(8 * s + 2 * g + 1);
+        } else {
+            x.v[0] = cell(4 * s + g);
+        }
+        return x;
+    }
+    __device__ __forceinline__ static AFrag<TY> operand(const Raw& r) {
         if constexpr (TY == FT_F32) {
             float x[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = __builtin_bit_cast(float, (uint32_t)v[j >> 2][j & 3]);
+            for (int j = 0; j < 8; ++j) x[j] = __builtin_bit_cast(float, (uint32_t)r.v[j >> 2][j & 3]);
             return split3(x);
         } else {
             AFrag<TY> f;
-            f.p[0] = v[0];
+            f.p[0] = r.v[0];
             return f;
         }
     }
@@ -113,11 +156,14 @@ template <int TY> struct ARaw {
 
 // q - zp of a word's 8 nibbles as an MFMA operand
 __device__ __forceinline__ h8 weights_f16(uint32_t w, h2 off) {
-    // 0x6400 | q is 1024 + q; off = 1024 + zp
+    // 0x6400 | q is 1024 + q; off = 1024 + zp. (In a vector register: mask, or
+    // and word are then one instruction.)
+    uint32_t magic;
+    asm("v_mov_b32 %0, 0x64006400" : "=v"(magic));
     h8 r;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const h2 v = __builtin_bit_cast(h2, ((w >> (4 * i)) & 0x000f000fu) | 0x64006400u) - off;
+        const h2 v = __builtin_bit_cast(h2, ((w >> (4 * i)) & 0x000f000fu) | magic) - off;
         r[2 * i] = v[0];
         r[2 * i + 1] = v[1];
     }
@@ -146,12 +192,12 @@ constexpr int NB_WAVES = 8;
 template <int TY, int NSPP> struct Scales {
     static constexpr int W = TY == FT_F32 ? NSPP : (NSPP + 1) / 2;   // words
     uint32_t w[W];
-    __device__ __forceinline__ void load(const void* p, long long at) {   // at: piece x 16 + column
+    __device__ __forceinline__ void load(const char* p, uint32_t col) {   // p: the piece's
         if constexpr (TY != FT_F32 && NSPP == 1) {
-            w[0] = ((const uint16_t*)p)[at];
+            w[0] = *(const uint16_t*)(p + col * 2);
         } else {
             typedef uint32_t vec __attribute__((ext_vector_type(W)));
-            const vec v = ((const vec*)p)[at];
+            const vec v = *(const vec*)(p + col * (uint32_t)sizeof(vec));
             if constexpr (W == 1) w[0] = __builtin_bit_cast(uint32_t, v);
             else
 #pragma unroll
@@ -173,24 +219,22 @@ template <int TY, int NSPP, int NT> struct Stage {
 };
 
 // One block: MT x 16 rows, NT x 16 columns, all of K. Its waves take pieces of
-// K in turn, straight from memory into registers, in rounds of D pieces each:
-// a round's weights are loaded before the one before is multiplied, a piece's
-// activations as those of the piece before are used up. The waves' sums meet
+// K in turn, weights straight from memory into registers, asked for D pieces
+// ahead, activations through LDS, asked for a chunk ahead. The waves' sums meet
 // in LDS.
 template <int TY, int NSPP, int AM, int MT, int NT, int D>
 __global__ __launch_bounds__(NB_WAVES * 64) void nbits_kernel(NbitsArgs p) {
-    __shared__ f4 red[NB_WAVES][MT * NT][64];
+    typedef Activations<TY, MT> Act;
+    constexpr int sums = NB_WAVES * MT * NT * 1024, acts = NB_WAVES * Act::BYTES;
+    __shared__ __attribute__((aligned(16))) char lds[sums > acts ? sums : acts];
+    f4(*red)[MT * NT][64] = (f4(*)[MT * NT][64])lds;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int col = lane & 15, g = lane >> 4;
+    const int col = lane & 15;
     const int tile0 = blockIdx.x * NT;
     const int m0 = blockIdx.y * (16 * MT);
-    constexpr int ES = TY == FT_F32 ? 4 : 2;
-    const char* row[MT];
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-        const int m = m0 + 16 * t + col;
-        row[t] = (const char*)p.a + (long long)(m < p.M ? m : p.M - 1) * p.K * ES;
-    }
+    char* const mine = lds + wave * Act::BYTES;
+    const char* const base = (const char*)p.a + (long long)m0 * p.K * Act::ES;
+    const int rows = p.M - m0;
     f4 acc[MT][NT];
 #pragma unroll
     for (int t = 0; t < MT; ++t)
@@ -198,53 +242,226 @@ __global__ __launch_bounds__(NB_WAVES * 64) void nbits_kernel(NbitsArgs p) {
         for (int u = 0; u < NT; ++u) acc[t][u] = f4{0, 0, 0, 0};
 
     const int last = p.P - 1;
-    ARaw<TY> a[4][MT];
-    auto load_w = [&](Stage<TY, NSPP, NT>* x, int piece) {
+    Stage<TY, NSPP, NT> st[D];
+    Act act[2];
+    auto load_w = [&](int d, int piece) {
+        Stage<TY, NSPP, NT>& x = st[d];
 #pragma unroll
-        for (int d = 0; d < D; ++d) {
-            const int at = min(piece + d * NB_WAVES, last);
+        for (int u = 0; u < NT; ++u) {
+            const long long pc = (long long)(tile0 + u) * p.P + piece;
+            x.w[u] = *(const u4*)((const char*)p.w + pc * 1024 + (uint32_t)(lane * 16));
+            x.sc[u].load((const char*)p.scales + pc * (16 * NSPP * Act::ES), (uint32_t)col);
+            x.zp[u] = *(const uint16_t*)((const char*)p.zp + (pc & p.zp_mask) * 32 + (uint32_t)(col * 2));
+        }
+    };
+    // Operands of the chunk at hand are in registers when its turn comes; the next
+    // one's go through LDS meanwhile, and the two after are on their way.
+    typename Act::Raw f[2][2][MT];
+    auto pass = [&](int to, int k) {   // act[to] -> f[to]; act[to] <- the chunk at k
+        act[to].store(mine);
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_sched_barrier(0);   // loads stay where they are asked for
+        act[to].template load<AM>(base, rows, k, p.K);
 #pragma unroll
-            for (int u = 0; u < NT; ++u) {
-                const long long pc = (long long)(tile0 + u) * p.P + at;
-                x[d].w[u] = *(const u4*)(p.w + pc * 256 + lane * 4);
-                x[d].sc[u].load(p.scales, pc * 16 + col);
-                x[d].zp[u] = p.zp[(pc & p.zp_mask) * 16 + col];
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) f[to][s][t] = Act::read(mine, s, t);
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto multiply = [&](int d, int next, int after) {   // the pieces one and two turns on
+        const Stage<TY, NSPP, NT>& x = st[d];
+        constexpr int SPS = 4 / NSPP;   // MFMA steps a scale
+        f4 part[MT][NT];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            pass(h ^ 1, h ? after * NB_PK : next * NB_PK + 64);
+#pragma unroll
+            for (int s = 2 * h; s < 2 * h + 2; ++s) {
+                AFrag<TY> fa[MT];
+#pragma unroll
+                for (int t = 0; t < MT; ++t) fa[t] = Act::operand(f[h][s & 1][t]);
+#pragma unroll
+                for (int u = 0; u < NT; ++u) {
+                    const uint32_t z = (x.zp[u] >> (4 * s)) & 15;
+                    if constexpr (TY == FT_F16) {
+                        const uint32_t o = (0x6400u + z) * 0x10001u;   // 1024 + zp, twice
+                        const h8 b = weights_f16(x.w[u][s], __builtin_bit_cast(h2, o));
+#pragma unroll
+                        for (int t = 0; t < MT; ++t)
+                            part[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                __builtin_bit_cast(h8, fa[t].p[0]), b, s % SPS ? part[t][u] : f4{0, 0, 0, 0}, 0, 0, 0);
+                    } else {
+                        const b8 b = weights_bf16(x.w[u][s], (float)z);
+#pragma unroll
+                        for (int t = 0; t < MT; ++t) {
+                            if (s % SPS == 0) part[t][u] = f4{0, 0, 0, 0};
+#pragma unroll
+                            for (int q = 0; q < kPieces<TY>; ++q)
+                                part[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, fa[t].p[q]), b,
+                                                                                     part[t][u], 0, 0, 0);
+                        }
+                    }
+                    if (s % SPS == SPS - 1) {
+                        const float sc = x.sc[u].get(s / SPS);
+#pragma unroll
+                        for (int t = 0; t < MT; ++t)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) acc[t][u][i] = __builtin_fmaf(part[t][u][i], sc, acc[t][u][i]);
+                    }
+                }
             }
         }
     };
-    auto load_a = [&](int s, int piece) {
+    act[0].template load<AM>(base, rows, min(wave, last) * NB_PK, p.K);
+    act[1].template load<AM>(base, rows, min(wave, last) * NB_PK + 64, p.K);
 #pragma unroll
-        for (int t = 0; t < MT; ++t) a[s][t].template load<AM>(row[t], piece * NB_PK + 32 * s + 8 * g, p.K);
+    for (int d = 0; d < D; ++d) load_w(d, min(wave + d * NB_WAVES, last));
+    pass(0, min(wave + NB_WAVES, last) * NB_PK);
+    int piece = wave;
+    for (; piece + D * NB_WAVES < p.P; piece += D * NB_WAVES)
+#pragma unroll
+        for (int d = 0; d < D; ++d) {
+            const int at = piece + d * NB_WAVES;
+            multiply(d, min(at + NB_WAVES, last), min(at + 2 * NB_WAVES, last));
+            __builtin_amdgcn_sched_barrier(0);
+            load_w(d, min(at + D * NB_WAVES, last));
+        }
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+        const int at = piece + d * NB_WAVES;
+        if (at < p.P) multiply(d, min(at + NB_WAVES, last), min(at + 2 * NB_WAVES, last));
+    }
+    __syncthreads();   // every wave is done with its stretch
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int u = 0; u < NT; ++u) red[wave][t * NT + u][lane] = acc[t][u];
+    __syncthreads();
+    // output (row, column) sits in lane 16 (row / 4) + column, element row % 4
+    const int nr = min(rows, 16 * MT);
+    for (int o = threadIdx.x; o < nr * (16 * NT); o += NB_WAVES * 64) {
+        const int r = o / (16 * NT), c = o % (16 * NT);
+        const int n = tile0 * 16 + c;
+        if (n >= p.N) continue;
+        const int t = (r >> 4) * NT + (c >> 4), l = (c & 15) + 16 * ((r & 15) >> 2);
+        float v = 0.0f;
+#pragma unroll
+        for (int q = 0; q < NB_WAVES; ++q) v += ((const float*)&red[q][t][l])[r & 3];
+        if (p.bias) v += load_f32<TY>(p.bias, n);
+        store_f32<TY>(p.y, (long long)(m0 + r) * p.N + n, v);
+    }
+}
+
+// Many rows. One block: MT x 16 rows, WN x NT x 16 columns; its waves are WN
+// columns groups times 8 / WN groups that take pieces of K in turn. Waves of one
+// K group share its activations: each loads a part of a chunk (64 K) and stores
+// it into LDS as 16-bit operands (fp32 as its three bf16 pieces), beside the
+// chunk that is being multiplied; one barrier a chunk, and two chunks on their
+// way (with one, a chunk took as long as its loads: 2600 cycles).
+template <int TY, int NSPP, int AM, int MT, int NT, int WN>
+__global__ __launch_bounds__(NB_WAVES * 64) void nbits_tile_kernel(NbitsArgs p) {
+    constexpr int KG = NB_WAVES / WN, NP = kPieces<TY>, ES = TY == FT_F32 ? 4 : 2, D = 2;
+    constexpr int PLANE = MT * 16 * 128;                    // bytes of 64 K of the rows, 16 bits each
+    constexpr int BUF = NP * PLANE;
+    constexpr int CELLS = 8, NL = MT * 16 * CELLS / (64 * WN);   // cells of 8 elements: a row's, a lane's
+    constexpr int V = TY == FT_F32 ? 2 : 1;                 // 16-byte loads a cell
+    constexpr int acts = 2 * KG * BUF, sums = NB_WAVES * MT * NT * 1024;
+    __shared__ __attribute__((aligned(16))) char lds[acts > sums ? acts : sums];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, g = lane >> 4, wn = wave % WN, kg = wave / WN;
+    const int tile0 = (blockIdx.x * WN + wn) * NT;
+    const int m0 = blockIdx.y * (16 * MT), rows = p.M - m0;
+    const char* const base = (const char*)p.a + (long long)m0 * p.K * ES;
+    const int last = p.P - 1, rounds = (p.P + KG - 1) / KG;
+    char* const mine = lds + kg * BUF;                      // buffer b: mine + b KG BUF
+
+    u4 act[2][NL][V];
+    auto load_a = [&](int b, int k0) {   // the wave's cells of the chunk at k0
+        const int k = k0 + (lane & 7) * 8;
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+            const uint32_t row = (uint32_t)min(((i * WN + wn) * 64 + lane) / CELLS, rows - 1) * (uint32_t)(p.K * ES);
+#pragma unroll
+            for (int h = 0; h < V; ++h) {
+                const int kk = k + 4 * h;   // (h: fp32 only)
+                if constexpr (AM == A_WHOLE) {
+                    act[b][i][h] = *(const u4*)(base + (row + (uint32_t)(kk * ES)));
+                } else {
+                    const bool in = kk < p.K;
+                    const u4 x = *(const u4*)(base + (row + (uint32_t)(in ? kk * ES : 0)));
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) act[b][i][h][j] = in ? x[j] : 0u;
+                }
+            }
+        }
     };
-    auto multiply = [&](const Stage<TY, NSPP, NT>& x, int next) {
-        f4 part[MT][NT];
+    auto store_a = [&](int b) {
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            AFrag<TY> f[MT];
+        for (int i = 0; i < NL; ++i) {
+            const int r = ((i * WN + wn) * 64 + lane) / CELLS;
+            char* to = mine + b * (KG * BUF) + (r * CELLS + ((lane & 7) ^ (r & 7))) * 16;
+            if constexpr (TY == FT_F32) {
+                float x[8];
 #pragma unroll
-            for (int t = 0; t < MT; ++t) f[t] = a[s][t].frag();
-            load_a(s, next);
-            constexpr int SPS = 4 / NSPP;   // MFMA steps a scale
+                for (int j = 0; j < 8; ++j) x[j] = __builtin_bit_cast(float, (uint32_t)act[b][i][j >> 2][j & 3]);
+                const AFrag<TY> f = split3(x);
+#pragma unroll
+                for (int q = 0; q < NP; ++q) *(u4*)(to + q * PLANE) = f.p[q];
+            } else {
+                *(u4*)to = act[b][i][0];
+            }
+        }
+    };
+    Stage<TY, NSPP, NT> st[D];
+    auto load_w = [&](int d, int piece) {
+        Stage<TY, NSPP, NT>& x = st[d];
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+            const long long pc = (long long)(tile0 + u) * p.P + piece;
+            x.w[u] = *(const u4*)((const char*)p.w + pc * 1024 + (uint32_t)(lane * 16));
+            x.sc[u].load((const char*)p.scales + pc * (16 * NSPP * ES), (uint32_t)col);
+            x.zp[u] = *(const uint16_t*)((const char*)p.zp + (pc & p.zp_mask) * 32 + (uint32_t)(col * 2));
+        }
+    };
+    f4 acc[MT][NT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int u = 0; u < NT; ++u) acc[t][u] = f4{0, 0, 0, 0};
+    constexpr int SPS = 4 / NSPP;   // MFMA steps a scale
+    f4 part[MT][NT];
+    auto half = [&](int d, int h) {   // buffer h
+        const Stage<TY, NSPP, NT>& x = st[d];
+        const char* from = mine + h * (KG * BUF);
+#pragma unroll
+        for (int s = 2 * h; s < 2 * h + 2; ++s) {
+            u4 f[MT][NP];
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int q = 0; q < NP; ++q) {
+                    const int r = 16 * t + col;
+                    f[t][q] = *(const u4*)(from + q * PLANE + (r * CELLS + ((4 * (s & 1) + g) ^ (r & 7))) * 16);
+                }
 #pragma unroll
             for (int u = 0; u < NT; ++u) {
                 const uint32_t z = (x.zp[u] >> (4 * s)) & 15;
-                if constexpr (TY == FT_F16) {
-                    const uint32_t o = (0x6400u + z) * 0x10001u;   // 1024 + zp, twice
-                    const h8 b = weights_f16(x.w[u][s], __builtin_bit_cast(h2, o));
+                h8 bh;
+                b8 bb;
+                if constexpr (TY == FT_F16) bh = weights_f16(x.w[u][s], __builtin_bit_cast(h2, (0x6400u + z) * 0x10001u));
+                else bb = weights_bf16(x.w[u][s], (float)z);
 #pragma unroll
-                    for (int t = 0; t < MT; ++t)
-                        part[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                            __builtin_bit_cast(h8, f[t].p[0]), b, s % SPS ? part[t][u] : f4{0, 0, 0, 0}, 0, 0, 0);
-                } else {
-                    const b8 b = weights_bf16(x.w[u][s], (float)z);
+                for (int t = 0; t < MT; ++t) {
+                    f4 c = s % SPS ? part[t][u] : f4{0, 0, 0, 0};
 #pragma unroll
-                    for (int t = 0; t < MT; ++t) {
-                        if (s % SPS == 0) part[t][u] = f4{0, 0, 0, 0};
-#pragma unroll
-                        for (int q = 0; q < kPieces<TY>; ++q)
-                            part[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                                __builtin_bit_cast(b8, f[t].p[q]), b, part[t][u], 0, 0, 0);
+                    for (int q = 0; q < NP; ++q) {
+                        if constexpr (TY == FT_F16)
+                            c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, f[t][q]), bh, c, 0, 0, 0);
+                        else
+                            c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, f[t][q]), bb, c, 0, 0, 0);
                     }
+                    part[t][u] = c;
                 }
                 if (s % SPS == SPS - 1) {
                     const float sc = x.sc[u].get(s / SPS);
@@ -254,40 +471,49 @@ __global__ __launch_bounds__(NB_WAVES * 64) void nbits_kernel(NbitsArgs p) {
                         for (int i = 0; i < 4; ++i) acc[t][u][i] = __builtin_fmaf(part[t][u][i], sc, acc[t][u][i]);
                 }
             }
-            if (NSPP == 4 && MT == 4) __builtin_amdgcn_sched_barrier(0);   // one step's block sums at a time, or registers spill
         }
     };
-    Stage<TY, NSPP, NT> cur[D];
-    load_w(cur, wave);
+    const auto piece_of = [&](int r) { return min(kg + r * KG, last); };
+    load_a(0, piece_of(0) * NB_PK);
 #pragma unroll
-    for (int s = 0; s < 4; ++s) load_a(s, min(wave, last));
-    int piece = wave;
-    for (; piece + D * NB_WAVES < p.P; piece += D * NB_WAVES) {
-        Stage<TY, NSPP, NT> nxt[D];
-        load_w(nxt, piece + D * NB_WAVES);
+    for (int d = 0; d < D; ++d) load_w(d, piece_of(d));
+    load_a(1, piece_of(0) * NB_PK + 64);
+    store_a(0);
+    load_a(0, piece_of(1) * NB_PK);
+    __syncthreads();
+    auto round = [&](int d, int r) {
 #pragma unroll
-        for (int d = 0; d < D; ++d) multiply(cur[d], min(piece + (d + 1) * NB_WAVES, last));
+        for (int h = 0; h < 2; ++h) {
+            store_a(h ^ 1);
+            __builtin_amdgcn_sched_barrier(0);
+            load_a(h ^ 1, h ? piece_of(r + 2) * NB_PK : piece_of(r + 1) * NB_PK + 64);   // three chunks on
+            __builtin_amdgcn_sched_barrier(0);
+            if (kg + r * KG < p.P) half(d, h);
+            __syncthreads();
+        }
+        load_w(d, piece_of(r + D));
+    };
+    for (int r = 0; r < rounds; r += D)
 #pragma unroll
-        for (int d = 0; d < D; ++d) cur[d] = nxt[d];
-    }
-#pragma unroll
-    for (int d = 0; d < D; ++d)
-        if (piece + d * NB_WAVES < p.P) multiply(cur[d], min(piece + (d + 1) * NB_WAVES, last));
+        for (int d = 0; d < D; ++d)
+            if (r + d < rounds) round(d, r + d);
+
+    f4(*red)[MT * NT][64] = (f4(*)[MT * NT][64])lds;
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
         for (int u = 0; u < NT; ++u) red[wave][t * NT + u][lane] = acc[t][u];
     __syncthreads();
-    // output (row, column) sits in lane 16 (row / 4) + column, element row % 4
-    const int rows = p.M - m0 < 16 * MT ? p.M - m0 : 16 * MT;
-    for (int o = threadIdx.x; o < rows * (16 * NT); o += NB_WAVES * 64) {
-        const int r = o / (16 * NT), c = o % (16 * NT);
-        const int n = tile0 * 16 + c;
+    constexpr int COLS = WN * NT * 16;
+    const int nr = min(rows, 16 * MT);
+    for (int o = threadIdx.x; o < nr * COLS; o += NB_WAVES * 64) {
+        const int r = o / COLS, c = o % COLS, w = c / (NT * 16);
+        const int n = blockIdx.x * COLS + c;
         if (n >= p.N) continue;
-        const int t = (r >> 4) * NT + (c >> 4), l = (c & 15) + 16 * ((r & 15) >> 2);
+        const int t = (r >> 4) * NT + (c % (NT * 16) >> 4), l = (c & 15) + 16 * ((r & 15) >> 2);
         float v = 0.0f;
 #pragma unroll
-        for (int q = 0; q < NB_WAVES; ++q) v += ((const float*)&red[q][t][l])[r & 3];
+        for (int q = 0; q < KG; ++q) v += ((const float*)&red[q * WN + w][t][l])[r & 3];
         if (p.bias) v += load_f32<TY>(p.bias, n);
         store_f32<TY>(p.y, (long long)(m0 + r) * p.N + n, v);
     }
@@ -337,15 +563,29 @@ hipError_t go(const NbitsArgs& a, hipStream_t s) {
     nbits_kernel<TY, NSPP, AM, MT, NT, D><<<grid, NB_WAVES * 64, 0, s>>>(a);
     return hipGetLastError();
 }
+template <int TY, int NSPP, int AM, int MT, int NT, int WN>
+hipError_t go_tile(const NbitsArgs& a, hipStream_t s) {
+    const dim3 grid((unsigned)((nbits_cols(a.N) / 16 + NT * WN - 1) / (NT * WN)), (unsigned)((a.M + 16 * MT - 1) / (16 * MT)));
+    nbits_tile_kernel<TY, NSPP, AM, MT, NT, WN><<<grid, NB_WAVES * 64, 0, s>>>(a);
+    return hipGetLastError();
+}
 template <int TY, int NSPP, int AM>
 hipError_t by_size(const NbitsArgs& a, hipStream_t s) {
+    const int tiles = nbits_cols(a.N) / 16;
     if constexpr (AM == A_ANY) {
         return a.M <= 16 ? go<TY, NSPP, AM, 1, 1, 2>(a, s) : go<TY, NSPP, AM, 2, 2, 1>(a, s);
     } else {
-        const int tiles = nbits_cols(a.N) / 16;
-        if (a.M <= 16) return tiles >= 1024 ? go<TY, NSPP, AM, 1, 2, 2>(a, s) : go<TY, NSPP, AM, 1, 1, 4>(a, s);
-        if constexpr (TY != FT_F32)   // (fp32 activations take twice the registers)
-            if (a.M > 32) return go<TY, NSPP, AM, 4, 2, 1>(a, s);
+        // (fp32 activations take twice the registers)
+        constexpr bool wide = TY == FT_F32;
+        if (a.M <= 16) return tiles >= 1024 ? go<TY, NSPP, AM, 1, 2, 3>(a, s) : go<TY, NSPP, AM, 1, 1, 4>(a, s);
+        if (a.M > 64) {
+            if constexpr (wide) return go_tile<TY, NSPP, AM, 4, 2, 4>(a, s);
+            else {
+                return go_tile<TY, NSPP, AM, 8, 2, 2>(a, s);
+            }
+        }
+        if constexpr (!wide)
+            if (a.M > 32) return go<TY, NSPP, AM, 4, 2, 2>(a, s);
         return go<TY, NSPP, AM, 2, 2, 2>(a, s);
     }
 }

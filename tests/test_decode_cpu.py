@@ -24,7 +24,7 @@ def nbits_desc(**kw):
     (dict(n=0), INVALID), (dict(k=-1), INVALID), (dict(block_size=48), INVALID), (dict(block_size=0), INVALID),
     (dict(b_host=None), INVALID), (dict(scales_host=None), INVALID), (dict(bits=8), UNSUPPORTED),
     (dict(block_size=16), UNSUPPORTED), (dict(dtype=_lib.U8), UNSUPPORTED), (dict(dtype=17), UNSUPPORTED),
-    (dict(k=(1 << 30) + 1), UNSUPPORTED), (dict(n=(1 << 31) - 1), UNSUPPORTED)])
+    (dict(k=(1 << 22) + 1), UNSUPPORTED), (dict(n=(1 << 31) - 1), UNSUPPORTED)])
 def test_nbits_create_refuses(kw, rc):
     h = C.c_void_p(5)
     d = nbits_desc(**kw)
