@@ -77,11 +77,11 @@ __device__ __forceinline__ TileAt tile_at(const KvCache& c, const KvTokens& t, i
     r.part = nullptr;
     r.in_page = 0;
     if (r.pos >= 0 && r.pos < r.end) {
-        const int pi = (int)(r.pos / c.page_size);
+        const int pi = (int)r.pos >> (31 - __builtin_clz((unsigned)c.page_size));
         const int id = t.table[(long long)b * t.max_pages + pi];
         if (id >= 0 && id < c.num_pages) {
             r.part = c.data + ((long long)id * c.heads + head) * kv_head_bytes(c.page_size, c.hd, c.bits);
-            r.in_page = (int)(r.pos - (long long)pi * c.page_size) / 32;
+            r.in_page = ((int)r.pos & (c.page_size - 1)) / 32;
         }
     }
     return r;
@@ -136,7 +136,6 @@ __device__ __forceinline__ u2 codes_of(const float* v, float s, float inv) {
     }
     return u2{lo, hi};
 }
-__device__ __forceinline__ uint32_t nibble(uint32_t w, int j) { return (w >> (4 * ((j >> 1) + 4 * (j & 1)))) & 15u; }
 // eight codes, a byte each, as a word of nibbles (j even: nibble j / 2, j odd: 4 + j / 2; turned)
 __device__ __forceinline__ uint32_t pack_nibbles(u2 q) {
     // bytes 0 4 1 5 below bytes 2 6 3 7
@@ -146,189 +145,171 @@ __device__ __forceinline__ uint32_t pack_nibbles(u2 q) {
 template <int BITS>
 __device__ __forceinline__ int scale_slot(int values, int t) { return BITS == 4 && !values ? kv_pair(t) : kv_slot(t); }
 
-// One wave a (tile of 32 positions, head, sequence, keys or values). Lanes read
-// 8 neighbouring elements of a token, form scales and codes, and store keys as
-// they are; values pass through LDS, where an element's tokens come together.
-// A tile whose tokens are not all written is merged with what it holds: no
-// other wave of the launch has this tile.
+// One block a (tile of 32 positions, head, sequence, keys or values), one wave
+// 32 elements of it: a block of the layout. Lanes read 8 neighbouring elements of
+// a token, form scales (at 8 bits with the other waves' maxima) and codes, and
+// store keys as they are; values pass through LDS, where an element's tokens come
+// together. A tile whose tokens are not all written is merged with what it holds:
+// nothing else of the launch has this tile. (A wave for all of a head's elements
+// ran 2000 instructions once, fetched for it: 3 x 1900 tokens of 8 x 128 elements
+// 18.6 us.)
 template <int TY, int BITS, int HD>
-__global__ __launch_bounds__(64) void kv_write_kernel(KvCache c, KvTokens t) {
+__global__ __launch_bounds__(HD * 2) void kv_write_kernel(KvCache c, KvTokens t) {
     constexpr int NC = HD / 32;
     constexpr float limit = BITS == 8 ? 127.0f : 7.0f;
     constexpr int BB = BITS == 8 ? 1024 : 512;   // bytes of a block
     typedef uint32_t vec __attribute__((ext_vector_type(BITS == 8 ? 4 : 2)));   // a lane's bytes of it
     __shared__ __attribute__((aligned(16))) uint8_t lds[HD * kLdsRow];
-    const int lane = threadIdx.x, g = lane >> 4;
+    __shared__ float tops[NC][32];
+    const int lane = threadIdx.x & 63, k = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
     const int values = blockIdx.y & 1, head = blockIdx.y >> 1, b = blockIdx.z;
     const TileAt w = tile_at(c, t, b, head, blockIdx.x);
     if (!w.part) return;
     const void* src = values ? t.v : t.k;
     const long long cb = kv_codes_bytes(c.page_size, HD, BITS);
-    uint8_t* blocks = w.part + (values ? cb : 0) + (long long)w.in_page * NC * BB;
-    bool in[2], half[2];   // this lane's tokens; has the wave any
-    float x[2][NC][8];
+    uint8_t* block = w.part + (values ? cb : 0) + ((long long)w.in_page * NC + k) * BB;
+    bool in[2];   // this lane's tokens
+    float x[2][8];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const int tok = (lane & 15) + 16 * h;
         in[h] = token_in(w, t.seq, tok);
-        half[h] = __any(in[h]);
-        const long long at = (long long)b * t.bstride + (w.pos + tok - w.p0) * t.tstride + (long long)head * HD + 8 * g;
 #pragma unroll
-        for (int k = 0; k < NC; ++k) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[h][k][j] = 0.0f;
-            if (in[h]) load8<TY>(src, at + 32 * k, x[h][k]);
-        }
+        for (int j = 0; j < 8; ++j) x[h][j] = 0.0f;
+        if (in[h])
+            load8<TY>(src, (long long)b * t.bstride + (w.pos + tok - w.p0) * t.tstride + (long long)head * HD + 32 * k + 8 * g,
+                      x[h]);
     }
     // values: what this lane's bytes hold beside the new tokens (slots 8 g .. 8 g + 7)
     uint32_t keep = 0;   // bit j: slot 8 g + j is not written
-    vec old[NC];
+    vec old;
     if (values) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
             if (!token_in(w, t.seq, 4 * g + (j & 3) + 16 * (j >> 2))) keep |= 1u << j;
-        if (keep != 0 && keep != 0xff)
+        if (keep != 0 && keep != 0xff) old = *(const vec*)(block + lane * sizeof(vec));
+    }
+    float m[2];
 #pragma unroll
-            for (int k = 0; k < NC; ++k) old[k] = *(const vec*)(blocks + k * BB + lane * sizeof(vec));
+    for (int h = 0; h < 2; ++h) {
+        m[h] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m[h] = fmaxf(m[h], finite_abs(x[h][j]));
+        m[h] = across_groups_max(m[h]);
+        if (BITS == 8 && g == 0) tops[k][(lane & 15) + 16 * h] = m[h];
+    }
+    if constexpr (BITS == 8) {
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < NC; ++i) m[h] = fmaxf(m[h], tops[i][(lane & 15) + 16 * h]);
     }
     __bf16* scales = (__bf16*)(w.part + 2 * cb) + (values ? (long long)c.page_size * kv_groups(HD, BITS) : 0);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        if (!half[h]) continue;
         const int tok = (lane & 15) + 16 * h;
-        float sc[NC], inv[NC], all = 0.0f;
+        const float sc = scale_of(m[h], limit), inv = sc > 0.0f ? 1.0f / sc : 0.0f;
+        if (in[h] && g == 0 && (BITS == 4 || k == 0))
+            scales[(long long)(BITS == 8 ? 0 : k) * c.page_size + w.in_page * 32 + scale_slot<BITS>(values, tok)] = (__bf16)sc;
+        const u2 q = codes_of<BITS>(x[h], sc, inv);
+        if (values) {
+            uint8_t* to = lds + (32 * k + 8 * g) * kLdsRow + kv_slot(tok);
 #pragma unroll
-        for (int k = 0; k < NC; ++k) {
-            float m = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) m = fmaxf(m, finite_abs(x[h][k][j]));
-            if (BITS == 8) all = fmaxf(all, m);
-            else sc[k] = scale_of(across_groups_max(m), limit);
-        }
-        if (BITS == 8) {
-            all = scale_of(across_groups_max(all), limit);
-#pragma unroll
-            for (int k = 0; k < NC; ++k) sc[k] = all;
-        }
-#pragma unroll
-        for (int k = 0; k < NC; ++k) inv[k] = BITS == 8 && k ? inv[0] : sc[k] > 0.0f ? 1.0f / sc[k] : 0.0f;
-        if (g == 0 && in[h])
-#pragma unroll
-            for (int k = 0; k < (BITS == 8 ? 1 : NC); ++k)
-                scales[(long long)k * c.page_size + w.in_page * 32 + scale_slot<BITS>(values, tok)] = (__bf16)sc[k];
-#pragma unroll
-        for (int k = 0; k < NC; ++k) {
-            const u2 q = codes_of<BITS>(x[h][k], sc[k], inv[k]);
-            if (values) {
-                uint8_t* to = lds + (32 * k + 8 * g) * kLdsRow + kv_slot(tok);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) to[j * kLdsRow] = (uint8_t)(q[j >> 2] >> (8 * (j & 3)));
-            } else if (in[h]) {
-                if constexpr (BITS == 8) *(u2*)(blocks + k * BB + lane * 16 + h * 8) = q;
-                else *(uint32_t*)(blocks + k * BB + lane * 8 + h * 4) = pack_nibbles(q);
-            }
+            for (int j = 0; j < 8; ++j) to[j * kLdsRow] = (uint8_t)(q[j >> 2] >> (8 * (j & 3)));
+        } else if (in[h]) {
+            if constexpr (BITS == 8) *(u2*)(block + lane * 16 + h * 8) = q;
+            else *(uint32_t*)(block + lane * 8 + h * 4) = pack_nibbles(q);
         }
     }
     if (!values) return;
     __syncthreads();
     if (keep == 0xff) return;
+    u2 e[2];
 #pragma unroll
-    for (int k = 0; k < NC; ++k) {
-        u2 e[2];
+    for (int h = 0; h < 2; ++h) e[h] = *(const u2*)(lds + (32 * k + (lane & 15) + 16 * h) * kLdsRow + 8 * g);
+    vec out, mask;
+    if constexpr (BITS == 8) {
+        out = vec{e[0][0], e[0][1], e[1][0], e[1][1]};
 #pragma unroll
-        for (int h = 0; h < 2; ++h) e[h] = *(const u2*)(lds + (32 * k + (lane & 15) + 16 * h) * kLdsRow + 8 * g);
-        vec out, m;
-        if constexpr (BITS == 8) {
-            out = vec{e[0][0], e[0][1], e[1][0], e[1][1]};
+        for (int i = 0; i < 4; ++i) {
+            mask[i] = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                m[i] = 0;
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (keep >> (4 * (i & 1) + j) & 1) m[i] |= 0xffu << (8 * j);
-            }
-        } else {
-            uint32_t mm = 0;
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (keep >> j & 1) mm |= 15u << (4 * ((j >> 1) + 4 * (j & 1)));
-            // (LDS holds anything where the wave has no token)
-            out = vec{pack_nibbles(e[0] & 0x0f0f0f0fu), pack_nibbles(e[1] & 0x0f0f0f0fu)};
-            m = vec{kv_turn(mm), kv_turn(mm)};
+            for (int j = 0; j < 4; ++j)
+                if (keep >> (4 * (i & 1) + j) & 1) mask[i] |= 0xffu << (8 * j);
         }
-        if (keep) out = (out & ~m) | (old[k] & m);
-        *(vec*)(blocks + k * BB + lane * sizeof(vec)) = out;
+    } else {
+        uint32_t mm = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (keep >> j & 1) mm |= 15u << (4 * ((j >> 1) + 4 * (j & 1)));
+        out = vec{pack_nibbles(e[0]), pack_nibbles(e[1])};
+        mask = vec{kv_turn(mm), kv_turn(mm)};
     }
+    if (keep) out = (out & ~mask) | (old & mask);
+    *(vec*)(block + lane * sizeof(vec)) = out;
 }
 
-// The same wave the other way; a position that holds no token reads as zeros.
+// The same block the other way; a position that holds no token reads as zeros.
 template <int TY, int BITS, int HD>
-__global__ __launch_bounds__(64) void kv_read_kernel(KvCache c, KvTokens t) {
+__global__ __launch_bounds__(HD * 2) void kv_read_kernel(KvCache c, KvTokens t) {
     constexpr int NC = HD / 32;
     constexpr int zero = BITS == 8 ? 128 : 8;
     constexpr int BB = BITS == 8 ? 1024 : 512;
     __shared__ __attribute__((aligned(16))) uint8_t lds[HD * kLdsRow];
-    const int lane = threadIdx.x, g = lane >> 4;
+    const int lane = threadIdx.x & 63, k = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
     const int values = blockIdx.y & 1, head = blockIdx.y >> 1, b = blockIdx.z;
     const TileAt w = tile_at(c, t, b, head, blockIdx.x);
     const long long cb = kv_codes_bytes(c.page_size, HD, BITS);
-    if (w.part && values) {
-        const uint8_t* blocks = w.part + cb + (long long)w.in_page * NC * BB;
+    u2 e[2] = {{0, 0}, {0, 0}};   // codes of a half's 8 elements or tokens, a byte each
+    float sc[2] = {0.0f, 0.0f};
+    bool in[2];
 #pragma unroll
-        for (int k = 0; k < NC; ++k) {
-            u2 e[2];
-            if constexpr (BITS == 8) {
-                const u4 v = *(const u4*)(blocks + k * BB + lane * 16);
-                e[0] = u2{v[0], v[1]};
-                e[1] = u2{v[2], v[3]};
-            } else {
-                const u2 v = *(const u2*)(blocks + k * BB + lane * 8);
+    for (int h = 0; h < 2; ++h) in[h] = token_in(w, t.seq, (lane & 15) + 16 * h);
+    if (w.part) {
+        const uint8_t* block = w.part + (values ? cb : 0) + ((long long)w.in_page * NC + k) * BB;
+        const __bf16* scales = (const __bf16*)(w.part + 2 * cb) + (values ? (long long)c.page_size * kv_groups(HD, BITS) : 0);
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    e[h] = u2{0, 0};
+        for (int h = 0; h < 2; ++h)
+            if (in[h])
+                sc[h] = (float)scales[(long long)(BITS == 8 ? 0 : k) * c.page_size + w.in_page * 32 +
+                                      scale_slot<BITS>(values, (lane & 15) + 16 * h)];
+        if constexpr (BITS == 8) {
+            const u4 v = *(const u4*)(block + lane * 16);
+            e[0] = u2{v[0], v[1]};
+            e[1] = u2{v[2], v[3]};
+        } else {
+            const u2 v = *(const u2*)(block + lane * 8);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) e[h][j >> 2] |= nibble(kv_unturn(v[h]), j) << (8 * (j & 3));
-                }
+            for (int h = 0; h < 2; ++h) {
+                // bytes 0 4 1 5 and 2 6 3 7
+                const uint32_t n = kv_unturn(v[h]), x = n & 0x0f0f0f0fu, y = n >> 4 & 0x0f0f0f0fu;
+                e[h] = u2{__builtin_amdgcn_perm(y, x, 0x06040200u), __builtin_amdgcn_perm(y, x, 0x07050301u)};
             }
-#pragma unroll
-            for (int h = 0; h < 2; ++h) *(u2*)(lds + (32 * k + (lane & 15) + 16 * h) * kLdsRow + 8 * g) = e[h];
         }
     }
-    __syncthreads();
+    if (values) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) *(u2*)(lds + (32 * k + (lane & 15) + 16 * h) * kLdsRow + 8 * g) = e[h];
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            e[h] = u2{0, 0};
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                e[h][j >> 2] |= (uint32_t)lds[(32 * k + 8 * g + j) * kLdsRow + kv_slot((lane & 15) + 16 * h)] << (8 * (j & 3));
+        }
+    }
     void* dst = values ? t.v : t.k;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        const int tok = (lane & 15) + 16 * h;
-        const long long s = w.pos + tok - w.p0;
+        const long long s = w.pos + (lane & 15) + 16 * h - w.p0;
         if (s < 0 || s >= t.seq) continue;
-        const bool in = token_in(w, t.seq, tok);
-        const long long at = (long long)b * t.bstride + s * t.tstride + (long long)head * HD + 8 * g;
-        const uint8_t* blocks = w.part + (long long)w.in_page * NC * BB;
-        const __bf16* scales = (const __bf16*)(w.part + 2 * cb) + (values ? (long long)c.page_size * kv_groups(HD, BITS) : 0);
+        float x[8];
 #pragma unroll
-        for (int k = 0; k < NC; ++k) {
-            float x[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = 0.0f;
-            if (in) {
-                const float sc = (float)scales[(long long)(BITS == 8 ? 0 : k) * c.page_size + w.in_page * 32 + scale_slot<BITS>(values, tok)];
-                u2 q = {0, 0};
-                uint32_t n = 0;
-                if (!values) {
-                    if constexpr (BITS == 8) q = *(const u2*)(blocks + k * BB + lane * 16 + h * 8);
-                    else n = kv_unturn(*(const uint32_t*)(blocks + k * BB + lane * 8 + h * 4));
-                }
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    int code;
-                    if (values) code = lds[(32 * k + 8 * g + j) * kLdsRow + kv_slot(tok)];
-                    else if constexpr (BITS == 8) code = (q[j >> 2] >> (8 * (j & 3))) & 0xff;
-                    else code = nibble(n, j);
-                    x[j] = (float)(code - zero) * sc;
-                }
-            }
-            store8<TY>(dst, at + 32 * k, x);
-        }
+        for (int j = 0; j < 8; ++j)
+            x[j] = in[h] ? (float)((int)((e[h][j >> 2] >> (8 * (j & 3))) & 0xff) - zero) * sc[h] : 0.0f;
+        store8<TY>(dst, (long long)b * t.bstride + s * t.tstride + (long long)head * HD + 32 * k + 8 * g, x);
     }
 }
 
@@ -336,8 +317,8 @@ template <int TY, int BITS, int HD>
 hipError_t go(bool write, const KvCache& c, const KvTokens& t, hipStream_t s) {
     // seq positions from anywhere in a tile on
     const dim3 grid((unsigned)(((long long)t.seq + 62) / 32), (unsigned)(2 * c.heads), (unsigned)t.batch);
-    if (write) kv_write_kernel<TY, BITS, HD><<<grid, 64, 0, s>>>(c, t);
-    else kv_read_kernel<TY, BITS, HD><<<grid, 64, 0, s>>>(c, t);
+    if (write) kv_write_kernel<TY, BITS, HD><<<grid, HD * 2, 0, s>>>(c, t);
+    else kv_read_kernel<TY, BITS, HD><<<grid, HD * 2, 0, s>>>(c, t);
     return hipGetLastError();
 }
 template <int TY, int BITS>
