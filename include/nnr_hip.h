@@ -592,10 +592,12 @@ typedef struct nnrh_matmul_nbits_desc {
     int bits;                     /* 4                                       */
     int block_size;
     int dtype;                    /* of a, the scales, the bias and y        */
-    const uint8_t* b_host;        /* [n][blocks][block_size / 2]             */
-    const void* scales_host;      /* [n][blocks]                             */
-    const uint8_t* zero_points_host;   /* [n][(blocks + 1) / 2], or NULL      */
-    const void* bias_host;        /* [n], or NULL                            */
+    int on_device;                /* the pointers below: 0 host, 1 device (b
+                                     4-byte aligned, written before the call) */
+    const uint8_t* b;             /* [n][blocks][block_size / 2]             */
+    const void* scales;           /* [n][blocks]                             */
+    const uint8_t* zero_points;   /* [n][(blocks + 1) / 2], or NULL          */
+    const void* bias;             /* [n], or NULL                            */
 } nnrh_matmul_nbits_desc;
 typedef struct nnrh_matmul_nbits* nnrh_matmul_nbits_t;
 int nnrh_matmul_nbits_create(nnrh_matmul_nbits_t* h, const nnrh_matmul_nbits_desc* d);

@@ -589,27 +589,40 @@ class MatMulNBits:
     rows), low nibble first. scales: torch tensor [n][blocks], float32, float16
     or bfloat16: the type of a, bias and y too. zero_points: uint8
     [n][(blocks + 1) // 2], two a byte, or None (8). bias: [n] or None.
-    Laid out on the current device at construction, or on `device`."""
+    Laid out at construction on `device`: the weights' where they are on one,
+    else the current one."""
 
     def __init__(self, b, scales, k, block_size, zero_points=None, bias=None, bits=4, device=None):
         import torch
-        host = lambda t, dt: None if t is None else torch.as_tensor(t).to("cpu", dt).contiguous()
+        self.device = torch.device("cuda" if device is None else device)
         if scales.dtype not in (torch.float32, torch.float16, torch.bfloat16):
             raise TypeError(f"scales of {scales.dtype}: float32, float16 or bfloat16")
         n, nb = int(b.shape[0]), -(-int(k) // int(block_size))
-        keep = [host(b, torch.uint8), host(scales, scales.dtype), host(zero_points, torch.uint8),
-                host(bias, scales.dtype)]
+        # what is on a device already does not go by way of the host
+        on_device = all(t is None or getattr(t, "is_cuda", False) for t in (b, scales, zero_points, bias))
+        at = scales.device if on_device else "cpu"
+        put = lambda t, dt: None if t is None else torch.as_tensor(t).to(at, dt).contiguous()
+        keep = [put(b, torch.uint8), put(scales, scales.dtype), put(zero_points, torch.uint8), put(bias, scales.dtype)]
+        if on_device:
+            if device is None:
+                self.device = scales.device
+            elif self.device.index is not None and self.device != scales.device:
+                raise ValueError(f"weights on {scales.device}, device {self.device}")
+            if keep[0].data_ptr() % 4:
+                keep[0] = keep[0].clone()
         for t, count, name in zip(keep, (n * nb * (block_size // 2), n * nb, n * ((nb + 1) // 2), n),
                                   ("b", "scales", "zero_points", "bias")):
             if t is not None and t.numel() != count:
                 raise ValueError(f"{name} has {t.numel()} elements, {count} expected")
         self.n, self.k, self.block_size, self.dtype = n, int(k), int(block_size), scales.dtype
-        self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
         if self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
-        desc = MatMulNBitsDesc(n, self.k, bits, self.block_size, _float_dt(self.dtype), *[ptr(t) for t in keep])
+        desc = MatMulNBitsDesc(n, self.k, bits, self.block_size, _float_dt(self.dtype), int(on_device),
+                               *[ptr(t) for t in keep])
         h = ct.c_void_p()
         with torch.cuda.device(self.device):
+            if on_device:
+                torch.cuda.current_stream().synchronize()
             check(lib().nnrh_matmul_nbits_create(ct.byref(h), ct.byref(desc)))
         self.h = h
 

@@ -97,8 +97,8 @@ class DqCodes(C.Structure):
 
 
 class MatMulNBitsDesc(C.Structure):
-    _fields_ = [(n, C.c_int) for n in ("n", "k", "bits", "block_size", "dtype")] + [
-        (n, C.c_void_p) for n in ("b_host", "scales_host", "zero_points_host", "bias_host")]
+    _fields_ = [(n, C.c_int) for n in ("n", "k", "bits", "block_size", "dtype", "on_device")] + [
+        (n, C.c_void_p) for n in ("b", "scales", "zero_points", "bias")]
 
 
 class KvCacheDesc(C.Structure):

@@ -2278,22 +2278,28 @@ struct Upload {
 int nbits_build(nnrh_matmul_nbits* h, const nnrh_matmul_nbits_desc* d) {
     const size_t nb = ((size_t)d->k + d->block_size - 1) / d->block_size, es = float_type_size(h->a.type);
     Upload raw, raw_scales, raw_zp;
+    const uint8_t *b = d->b, *scales = (const uint8_t*)d->scales, *zps = d->zero_points;
     int rc;
-    if ((rc = upload(&raw.p, d->b_host, (size_t)d->n * nb * (d->block_size / 2))) ||
-        (rc = upload(&raw_scales.p, (const uint8_t*)d->scales_host, (size_t)d->n * nb * es)))
-        return rc;
-    if (d->zero_points_host && (rc = upload(&raw_zp.p, d->zero_points_host, (size_t)d->n * ((nb + 1) / 2)))) return rc;
-    if (d->bias_host) {
-        uint8_t* b = nullptr;
-        if ((rc = upload(&b, (const uint8_t*)d->bias_host, (size_t)d->n * es))) return rc;
-        h->bias = b;
+    if (!d->on_device) {
+        if ((rc = upload(&raw.p, b, (size_t)d->n * nb * (d->block_size / 2))) ||
+            (rc = upload(&raw_scales.p, scales, (size_t)d->n * nb * es)) ||
+            (zps && (rc = upload(&raw_zp.p, zps, (size_t)d->n * ((nb + 1) / 2)))))
+            return rc;
+        b = raw.p;
+        scales = raw_scales.p;
+        zps = raw_zp.p;
+    }
+    if (d->bias) {
+        if ((rc = nnrh_malloc(&h->bias, (size_t)d->n * es))) return rc;
+        HIP_TRY(hipMemcpy(h->bias, d->bias, (size_t)d->n * es, d->on_device ? hipMemcpyDeviceToDevice : hipMemcpyHostToDevice),
+                "hipMemcpy");
     }
     const size_t pieces = (size_t)(nbits_cols(d->n) / 16) * h->a.P;
     if ((rc = nnrh_malloc((void**)&h->w, pieces * 1024)) ||
         (rc = nnrh_malloc(&h->scales, pieces * 16 * h->a.nspp * es)) ||
-        (rc = nnrh_malloc((void**)&h->zp, (d->zero_points_host ? pieces : 1) * 32)))
+        (rc = nnrh_malloc((void**)&h->zp, (zps ? pieces : 1) * 32)))
         return rc;
-    HIP_TRY(launch_nbits_pack(raw.p, raw_scales.p, raw_zp.p, d->n, d->k, d->block_size, h->a.type, h->w, h->scales,
+    HIP_TRY(launch_nbits_pack(b, scales, zps, d->n, d->k, d->block_size, h->a.type, h->w, h->scales,
                               h->zp, nullptr),
             "matmul_nbits: pack");
     // what was uploaded goes away with this call, and runs may come on any stream
@@ -2301,7 +2307,7 @@ int nbits_build(nnrh_matmul_nbits* h, const nnrh_matmul_nbits_desc* d) {
     h->a.w = h->w;
     h->a.scales = h->scales;
     h->a.zp = h->zp;
-    h->a.zp_mask = d->zero_points_host ? -1 : 0;
+    h->a.zp_mask = zps ? -1 : 0;
     h->a.bias = h->bias;
     return NNRH_OK;
 }
@@ -2311,7 +2317,7 @@ int nbits_build(nnrh_matmul_nbits* h, const nnrh_matmul_nbits_desc* d) {
 extern "C" int nnrh_matmul_nbits_create(nnrh_matmul_nbits_t* out, const nnrh_matmul_nbits_desc* d) {
     if (!out) return set_err(NNRH_ERR_INVALID, "matmul_nbits: handle NULL");
     *out = nullptr;
-    if (!d || !d->b_host || !d->scales_host) return set_err(NNRH_ERR_INVALID, "matmul_nbits: NULL argument");
+    if (!d || !d->b || !d->scales) return set_err(NNRH_ERR_INVALID, "matmul_nbits: NULL argument");
     if (d->n <= 0 || d->k <= 0) return set_err(NNRH_ERR_INVALID, "matmul_nbits: n %d, k %d", d->n, d->k);
     if (d->block_size <= 0 || (d->block_size & (d->block_size - 1)))
         return set_err(NNRH_ERR_INVALID, "matmul_nbits: block size %d is no power of two", d->block_size);
@@ -2321,6 +2327,9 @@ extern "C" int nnrh_matmul_nbits_create(nnrh_matmul_nbits_t* out, const nnrh_mat
     // bytes of a block's rows (64 fp32 ones) and columns of the last tile in an int
     if (d->k > (1 << 22) || d->n > (1 << 30) || d->block_size > (1 << 22))
         return set_err(NNRH_ERR_UNSUPPORTED, "matmul_nbits: n %d, k %d, block size %d", d->n, d->k, d->block_size);
+    if (d->on_device && (((uintptr_t)d->b & 3) || (((uintptr_t)d->scales | (uintptr_t)d->bias) &
+                                                   (float_type_size(float_type(d->dtype)) - 1))))
+        return set_err(NNRH_ERR_INVALID, "matmul_nbits: alignment");
     nnrh_matmul_nbits* h = new (std::nothrow) nnrh_matmul_nbits();
     if (!h) return set_err(NNRH_ERR_NOMEM, "matmul_nbits: host allocation");
     h->a.N = d->n;

@@ -221,8 +221,10 @@ template <int TY, int NSPP, int NT> struct Stage {
 // One block: MT x 16 rows, NT x 16 columns, all of K. Its waves take pieces of
 // K in turn, weights straight from memory into registers, asked for D pieces
 // ahead, activations through LDS, asked for a chunk ahead. The waves' sums meet
-// in LDS.
-template <int TY, int NSPP, int AM, int MT, int NT, int D>
+// in LDS. DIR (a row or two): operands straight from memory like the weights;
+// lanes that repeat a row cost no accesses of their own (1 x 4096 x 8192 bf16
+// 6.8 us, through LDS 7.8; 16 rows 18.6 and 11.7).
+template <int TY, int NSPP, int AM, int MT, int NT, int D, bool DIR>
 __global__ __launch_bounds__(NB_WAVES * 64) void nbits_kernel(NbitsArgs p) {
     typedef Activations<TY, MT> Act;
     constexpr int sums = NB_WAVES * MT * NT * 1024, acts = NB_WAVES * Act::BYTES;
@@ -243,7 +245,8 @@ __global__ __launch_bounds__(NB_WAVES * 64) void nbits_kernel(NbitsArgs p) {
 
     const int last = p.P - 1;
     Stage<TY, NSPP, NT> st[D];
-    Act act[2];
+    typename Act::Raw dir[DIR ? D : 1][4];
+    Act act;
     auto load_w = [&](int d, int piece) {
         Stage<TY, NSPP, NT>& x = st[d];
 #pragma unroll
@@ -253,15 +256,31 @@ __global__ __launch_bounds__(NB_WAVES * 64) void nbits_kernel(NbitsArgs p) {
             x.sc[u].load((const char*)p.scales + pc * (16 * NSPP * Act::ES), (uint32_t)col);
             x.zp[u] = *(const uint16_t*)((const char*)p.zp + (pc & p.zp_mask) * 32 + (uint32_t)(col * 2));
         }
+        if constexpr (DIR)
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+#pragma unroll
+                for (int i = 0; i < (TY == FT_F32 ? 2 : 1); ++i) {
+                    const int k = piece * NB_PK + 32 * s + 8 * (lane >> 4) + 4 * i;   // (i: fp32 only)
+                    const uint32_t row = (uint32_t)min(col, rows - 1) * (uint32_t)(p.K * Act::ES);
+                    if constexpr (AM == A_WHOLE) {
+                        dir[d][s].v[i] = *(const u4*)(base + (row + (uint32_t)(k * Act::ES)));
+                    } else {
+                        const bool in = k < p.K;
+                        const u4 v = *(const u4*)(base + (row + (uint32_t)(in ? k * Act::ES : 0)));
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) dir[d][s].v[i][j] = in ? v[j] : 0u;
+                    }
+                }
     };
     // Operands of the chunk at hand are in registers when its turn comes; the next
-    // one's go through LDS meanwhile, and the two after are on their way.
+    // one's go through LDS meanwhile, and the one after is on its way.
     typename Act::Raw f[2][2][MT];
-    auto pass = [&](int to, int k) {   // act[to] -> f[to]; act[to] <- the chunk at k
-        act[to].store(mine);
+    auto pass = [&](int to, int k) {   // act -> f[to]; act <- the chunk at k
+        act.store(mine);
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_sched_barrier(0);   // loads stay where they are asked for
-        act[to].template load<AM>(base, rows, k, p.K);
+        act.template load<AM>(base, rows, k, p.K);
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
@@ -269,18 +288,18 @@ __global__ __launch_bounds__(NB_WAVES * 64) void nbits_kernel(NbitsArgs p) {
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_sched_barrier(0);
     };
-    auto multiply = [&](int d, int next, int after) {   // the pieces one and two turns on
+    auto multiply = [&](int d, int next) {
         const Stage<TY, NSPP, NT>& x = st[d];
         constexpr int SPS = 4 / NSPP;   // MFMA steps a scale
         f4 part[MT][NT];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            pass(h ^ 1, h ? after * NB_PK : next * NB_PK + 64);
+            if constexpr (!DIR) pass(h ^ 1, next * NB_PK + 64 * h);
 #pragma unroll
             for (int s = 2 * h; s < 2 * h + 2; ++s) {
                 AFrag<TY> fa[MT];
 #pragma unroll
-                for (int t = 0; t < MT; ++t) fa[t] = Act::operand(f[h][s & 1][t]);
+                for (int t = 0; t < MT; ++t) fa[t] = Act::operand(DIR ? dir[DIR ? d : 0][s] : f[h][s & 1][t]);
 #pragma unroll
                 for (int u = 0; u < NT; ++u) {
                     const uint32_t z = (x.zp[u] >> (4 * s)) & 15;
@@ -313,24 +332,24 @@ __global__ __launch_bounds__(NB_WAVES * 64) void nbits_kernel(NbitsArgs p) {
             }
         }
     };
-    act[0].template load<AM>(base, rows, min(wave, last) * NB_PK, p.K);
-    act[1].template load<AM>(base, rows, min(wave, last) * NB_PK + 64, p.K);
+    if constexpr (!DIR) act.template load<AM>(base, rows, min(wave, last) * NB_PK, p.K);
 #pragma unroll
     for (int d = 0; d < D; ++d) load_w(d, min(wave + d * NB_WAVES, last));
-    pass(0, min(wave + NB_WAVES, last) * NB_PK);
+    if constexpr (!DIR) pass(0, min(wave, last) * NB_PK + 64);
     int piece = wave;
     for (; piece + D * NB_WAVES < p.P; piece += D * NB_WAVES)
 #pragma unroll
         for (int d = 0; d < D; ++d) {
             const int at = piece + d * NB_WAVES;
-            multiply(d, min(at + NB_WAVES, last), min(at + 2 * NB_WAVES, last));
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(d, min(at + NB_WAVES, last));
             __builtin_amdgcn_sched_barrier(0);
             load_w(d, min(at + D * NB_WAVES, last));
         }
 #pragma unroll
     for (int d = 0; d < D; ++d) {
         const int at = piece + d * NB_WAVES;
-        if (at < p.P) multiply(d, min(at + NB_WAVES, last), min(at + 2 * NB_WAVES, last));
+        if (at < p.P) multiply(d, min(at + NB_WAVES, last));
     }
     __syncthreads();   // every wave is done with its stretch
 #pragma unroll
@@ -357,8 +376,7 @@ __global__ __launch_bounds__(NB_WAVES * 64) void nbits_kernel(NbitsArgs p) {
 // columns groups times 8 / WN groups that take pieces of K in turn. Waves of one
 // K group share its activations: each loads a part of a chunk (64 K) and stores
 // it into LDS as 16-bit operands (fp32 as its three bf16 pieces), beside the
-// chunk that is being multiplied; one barrier a chunk, and two chunks on their
-// way (with one, a chunk took as long as its loads: 2600 cycles).
+// chunk that is being multiplied; one barrier a chunk.
 template <int TY, int NSPP, int AM, int MT, int NT, int WN>
 __global__ __launch_bounds__(NB_WAVES * 64) void nbits_tile_kernel(NbitsArgs p) {
     constexpr int KG = NB_WAVES / WN, NP = kPieces<TY>, ES = TY == FT_F32 ? 4 : 2, D = 2;
@@ -376,8 +394,8 @@ __global__ __launch_bounds__(NB_WAVES * 64) void nbits_tile_kernel(NbitsArgs p) 
     const int last = p.P - 1, rounds = (p.P + KG - 1) / KG;
     char* const mine = lds + kg * BUF;                      // buffer b: mine + b KG BUF
 
-    u4 act[2][NL][V];
-    auto load_a = [&](int b, int k0) {   // the wave's cells of the chunk at k0
+    u4 act[NL][V];
+    auto load_a = [&](int k0) {   // the wave's cells of the chunk at k0
         const int k = k0 + (lane & 7) * 8;
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
@@ -386,12 +404,12 @@ __global__ __launch_bounds__(NB_WAVES * 64) void nbits_tile_kernel(NbitsArgs p) 
             for (int h = 0; h < V; ++h) {
                 const int kk = k + 4 * h;   // (h: fp32 only)
                 if constexpr (AM == A_WHOLE) {
-                    act[b][i][h] = *(const u4*)(base + (row + (uint32_t)(kk * ES)));
+                    act[i][h] = *(const u4*)(base + (row + (uint32_t)(kk * ES)));
                 } else {
                     const bool in = kk < p.K;
                     const u4 x = *(const u4*)(base + (row + (uint32_t)(in ? kk * ES : 0)));
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) act[b][i][h][j] = in ? x[j] : 0u;
+                    for (int j = 0; j < 4; ++j) act[i][h][j] = in ? x[j] : 0u;
                 }
             }
         }
@@ -404,12 +422,12 @@ __global__ __launch_bounds__(NB_WAVES * 64) void nbits_tile_kernel(NbitsArgs p) 
             if constexpr (TY == FT_F32) {
                 float x[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] = __builtin_bit_cast(float, (uint32_t)act[b][i][j >> 2][j & 3]);
+                for (int j = 0; j < 8; ++j) x[j] = __builtin_bit_cast(float, (uint32_t)act[i][j >> 2][j & 3]);
                 const AFrag<TY> f = split3(x);
 #pragma unroll
                 for (int q = 0; q < NP; ++q) *(u4*)(to + q * PLANE) = f.p[q];
             } else {
-                *(u4*)to = act[b][i][0];
+                *(u4*)to = act[i][0];
             }
         }
     };
@@ -474,19 +492,18 @@ __global__ __launch_bounds__(NB_WAVES * 64) void nbits_tile_kernel(NbitsArgs p) 
         }
     };
     const auto piece_of = [&](int r) { return min(kg + r * KG, last); };
-    load_a(0, piece_of(0) * NB_PK);
+    load_a(piece_of(0) * NB_PK);
 #pragma unroll
     for (int d = 0; d < D; ++d) load_w(d, piece_of(d));
-    load_a(1, piece_of(0) * NB_PK + 64);
     store_a(0);
-    load_a(0, piece_of(1) * NB_PK);
+    load_a(piece_of(0) * NB_PK + 64);
     __syncthreads();
     auto round = [&](int d, int r) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             store_a(h ^ 1);
             __builtin_amdgcn_sched_barrier(0);
-            load_a(h ^ 1, h ? piece_of(r + 2) * NB_PK : piece_of(r + 1) * NB_PK + 64);   // three chunks on
+            load_a(piece_of(r + 1) * NB_PK + 64 * h);
             __builtin_amdgcn_sched_barrier(0);
             if (kg + r * KG < p.P) half(d, h);
             __syncthreads();
@@ -537,13 +554,12 @@ __global__ __launch_bounds__(256) void nbits_pack_kernel(const uint8_t* raw, con
         uint32_t z = 8;
         if (raw_zp && n < N && k0 < K) z = (raw_zp[n * ((nb + 1) / 2) + (b >> 1)] >> (4 * (b & 1))) & 15;
         zps |= z << (4 * s);
+        // eight neighbouring nibbles (behind K a block's filling, which meets zeros)
+        const int k = k0 + 8 * (lane >> 4);
+        uint32_t q = z * 0x11111111u;
+        if (n < N && k < nb * block) q = *(const uint32_t*)(raw + ((n * nb * block + k) >> 1));
         uint32_t word = 0;
-        for (int j = 0; j < 8; ++j) {
-            const int k = k0 + 8 * (lane >> 4) + j;
-            uint32_t q = z;
-            if (n < N && k < K) q = (raw[(n * nb * block + k) >> 1] >> (4 * (k & 1))) & 15;
-            word |= q << (4 * ((j >> 1) + 4 * (j & 1)));
-        }
+        for (int j = 0; j < 8; ++j) word |= (q >> (4 * j) & 15) << (4 * ((j >> 1) + 4 * (j & 1)));
         w[i * 4 + s] = word;
     }
     if (lane >= 16) return;
@@ -557,10 +573,10 @@ __global__ __launch_bounds__(256) void nbits_pack_kernel(const uint8_t* raw, con
     }
 }
 
-template <int TY, int NSPP, int AM, int MT, int NT, int D>
+template <int TY, int NSPP, int AM, int MT, int NT, int D, bool DIR = false>
 hipError_t go(const NbitsArgs& a, hipStream_t s) {
     const dim3 grid((unsigned)(nbits_cols(a.N) / 16 / NT), (unsigned)((a.M + 16 * MT - 1) / (16 * MT)));
-    nbits_kernel<TY, NSPP, AM, MT, NT, D><<<grid, NB_WAVES * 64, 0, s>>>(a);
+    nbits_kernel<TY, NSPP, AM, MT, NT, D, DIR><<<grid, NB_WAVES * 64, 0, s>>>(a);
     return hipGetLastError();
 }
 template <int TY, int NSPP, int AM, int MT, int NT, int WN>
@@ -571,19 +587,26 @@ hipError_t go_tile(const NbitsArgs& a, hipStream_t s) {
 }
 template <int TY, int NSPP, int AM>
 hipError_t by_size(const NbitsArgs& a, hipStream_t s) {
-    const int tiles = nbits_cols(a.N) / 16;
     if constexpr (AM == A_ANY) {
         return a.M <= 16 ? go<TY, NSPP, AM, 1, 1, 2>(a, s) : go<TY, NSPP, AM, 2, 2, 1>(a, s);
     } else {
-        // (fp32 activations take twice the registers)
-        constexpr bool wide = TY == FT_F32;
-        if (a.M <= 16) return tiles >= 1024 ? go<TY, NSPP, AM, 1, 2, 3>(a, s) : go<TY, NSPP, AM, 1, 1, 4>(a, s);
+        constexpr bool wide = TY == FT_F32;   // activations take twice the registers
+        const int cols = nbits_cols(a.N);
+        const auto blocks = [&](int m, int n) { return (long long)((a.M + m - 1) / m) * (cols / n); };
         if (a.M > 64) {
-            if constexpr (wide) return go_tile<TY, NSPP, AM, 4, 2, 4>(a, s);
-            else {
-                return go_tile<TY, NSPP, AM, 8, 2, 2>(a, s);
-            }
+            // Blocks of shared rows where they fill the chip (bf16, K 4096, blocks of
+            // 32: 512 x 4096 38 us, K split over waves 53; 256 x 4096 35 and 27);
+            // those of 128 columns where that is so twice over (4096 x 4096 235 us,
+            // 64 columns of 128 rows 279).
+            if (blocks(64, 128) >= (wide ? 192 : 512)) return go_tile<TY, NSPP, AM, 4, 2, 4>(a, s);
+            if constexpr (!wide)
+                if (blocks(128, 64) >= 192)   // (column tiles side by side spill with few scales: 41 us, 35)
+                    return NSPP == 4 ? go_tile<TY, NSPP, AM, 8, NSPP == 4 ? 2 : 1, NSPP == 4 ? 2 : 4>(a, s)
+                                     : go_tile<TY, NSPP, AM, 8, 1, 4>(a, s);
         }
+        if (a.M <= 2)
+            return cols >= 16384 ? go<TY, NSPP, AM, 1, 2, wide ? 2 : 3, true>(a, s) : go<TY, NSPP, AM, 1, 1, wide ? 3 : 4, true>(a, s);
+        if (a.M <= 16) return cols >= 16384 ? go<TY, NSPP, AM, 1, 2, 3>(a, s) : go<TY, NSPP, AM, 1, 1, 4>(a, s);
         if constexpr (!wide)
             if (a.M > 32) return go<TY, NSPP, AM, 4, 2, 2>(a, s);
         return go<TY, NSPP, AM, 2, 2, 2>(a, s);

@@ -15,15 +15,16 @@ MEM = [0x100000000 * (i + 1) for i in range(8)]
 
 
 def nbits_desc(**kw):
-    d = dict(n=16, k=64, bits=4, block_size=32, dtype=_lib.F32, b_host=MEM[0], scales_host=MEM[1])
+    d = dict(n=16, k=64, bits=4, block_size=32, dtype=_lib.F32, b=MEM[0], scales=MEM[1])
     d.update(kw)
     return _lib.MatMulNBitsDesc(**d)
 
 
 @pytest.mark.parametrize("kw,rc", [
     (dict(n=0), INVALID), (dict(k=-1), INVALID), (dict(block_size=48), INVALID), (dict(block_size=0), INVALID),
-    (dict(b_host=None), INVALID), (dict(scales_host=None), INVALID), (dict(bits=8), UNSUPPORTED),
+    (dict(b=None), INVALID), (dict(scales=None), INVALID), (dict(bits=8), UNSUPPORTED),
     (dict(block_size=16), UNSUPPORTED), (dict(dtype=_lib.U8), UNSUPPORTED), (dict(dtype=17), UNSUPPORTED),
+    (dict(on_device=1, b=MEM[0] + 2), INVALID), (dict(on_device=1, scales=MEM[1] + 1), INVALID),
     (dict(k=(1 << 22) + 1), UNSUPPORTED), (dict(n=(1 << 31) - 1), UNSUPPORTED)])
 def test_nbits_create_refuses(kw, rc):
     h = C.c_void_p(5)

@@ -49,7 +49,10 @@ def check_nbits(dev, m, n, k, block, t, zp, bias, a=None):
     (15, 48, 384, 256, True, False), (16, 333, 1000, 64, False, True), (17, 80, 257, 32, True, True),
     (31, 96, 512, 128, False, False), (33, 130, 640, 32, True, True), (64, 256, 2048, 32, True, False),
     (65, 67, 96, 512, False, True), (130, 200, 1500, 64, True, True), (300, 512, 1024, 32, False, False),
-    (1, 16500, 160, 32, True, True), (3, 20, 8192, 4096, True, False)])
+    (1, 16500, 160, 32, True, True), (3, 20, 8192, 4096, True, False), (2, 16400, 320, 64, True, True),
+    # grids of blocks that share rows: few column tiles a wave, many, one piece of K, uneven rounds
+    (130, 12300, 200, 32, True, True), (193, 8200, 1160, 128, False, True), (300, 16500, 160, 64, True, False),
+    (260, 16400, 64, 32, False, True), (1030, 4200, 640, 256, True, True), (513, 8250, 1096, 32, True, False)])
 def test_nbits(dev, t, m, n, k, block, zp, bias):
     check_nbits(dev, m, n, k, block, t, zp, bias)
 
@@ -96,6 +99,20 @@ def test_nbits_extreme_activations(dev, t):
     a[2, ::2] *= -1
     a[3, 1:] = 1e-4
     check_nbits(dev, 4, n, k, block, t, True, False, a=a)
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_nbits_weights_on_the_device(dev, t):
+    """The same handle from host and device memory, at odd addresses too"""
+    b, s, z, c = weights(11, 70, 300, 64, t, True, True)
+    x = torch.randn((9, 300), generator=torch.Generator().manual_seed(4)).to(t).to(dev)
+    ref = nnr_amd.MatMulNBits(b, s, 300, 64, zero_points=z, bias=c)(x)
+    odd = torch.empty(b.size + 1, dtype=torch.uint8, device=dev)[1:].reshape(b.shape)
+    odd.copy_(torch.from_numpy(b))
+    for w in (torch.from_numpy(b).to(dev), odd):
+        op = nnr_amd.MatMulNBits(w, s.to(dev), 300, 64, zero_points=torch.from_numpy(z).to(dev), bias=c.to(dev))
+        w.fill_(0)
+        assert torch.equal(op(x), ref)
 
 
 def test_nbits_empty_and_shapes(dev):
