@@ -1605,6 +1605,60 @@ struct MatMul_hip : operator_t {
     double num_ops() const override { return 2.0 * batch * M * (double)N * K; }
 };
 
+// com.microsoft MatMulNBits: 4-bit weights in blocks along K, constant. No
+// counterpart in the reference. A (fp32 or fp16) [.., K]; B [N][blocks]
+// [block_size / 2] uint8; scales of A's type; zero points packed like B or
+// none; an optional constant bias.
+struct MatMulNBits_hip : operator_t {
+    nnrh_matmul_nbits_t h = nullptr;
+    int n = 0, k = 0;
+    ~MatMulNBits_hip() override { nnrh_matmul_nbits_destroy(h); }
+    bool init() override {
+        k = (int)attribute("K", 0);
+        n = (int)attribute("N", 0);
+        return inputs.size() >= 3 && inputs.size() <= 6 && outputs.size() == 1 && k > 0 && n > 0;
+    }
+    bool reshape() override {
+        tensor_t *a = inputs[0], *b = inputs[1], *s = inputs[2], *zp = in(this, 3), *idx = in(this, 4), *bias = in(this, 5);
+        const int dt = a->type == NNR_DATA_TYPE_FLOAT32 ? NNRH_F32 : a->type == NNR_DATA_TYPE_FLOAT16 ? NNRH_F16 : -1;
+        if (dt < 0) return bad(this, "A must be fp32 or fp16");
+        if (a->ndim() < 1 || a->dims[a->ndim() - 1] != k) return bad(this, "A's last axis is not K");
+        std::vector<int> d(a->dims.begin(), a->dims.end() - 1);
+        d.push_back(n);
+        if (!outputs[0]->reshape(d, a->type)) return false;
+        if (ctx->shape_only) return true;
+        const int64_t block = attribute("block_size", 0), bits = attribute("bits", 4);
+        if (block < 16 || block > (1 << 22) || (block & (block - 1))) return bad(this, "block_size must be a power of two");
+        const size_t nb = ((size_t)k + block - 1) / block;
+        const auto constant = [](tensor_t* t, data_type_t type, size_t count) {
+            return t->has_host() && t->type == type && t->ndata == count;
+        };
+        if (idx && idx->ndata) return bad(this, "g_idx is not supported");
+        if (!constant(b, NNR_DATA_TYPE_UINT8, n * nb * (block / 2))) return bad(this, "B must be constant uint8 [N][blocks][block_size / 2]");
+        if (!constant(s, a->type, n * nb)) return bad(this, "scales must be constant, of A's type, [N][blocks]");
+        if (has_zp(zp) && !constant(zp, NNR_DATA_TYPE_UINT8, n * ((nb + 1) / 2)))
+            return bad(this, "zero points must be constant uint8, two a byte");
+        if (bias && bias->ndata && !constant(bias, a->type, n)) return bad(this, "the bias must be constant, of A's type, [N]");
+        nnrh_matmul_nbits_desc dsc{};
+        dsc.n = n;
+        dsc.k = k;
+        dsc.bits = (int)bits;
+        dsc.block_size = (int)block;
+        dsc.dtype = dt;
+        dsc.b = b->host.data();
+        dsc.scales = s->host.data();
+        dsc.zero_points = has_zp(zp) ? zp->host.data() : nullptr;
+        dsc.bias = bias && bias->ndata ? bias->host.data() : nullptr;
+        nnrh_matmul_nbits_destroy(h);
+        h = nullptr;
+        return ok(this, nnrh_matmul_nbits_create(&h, &dsc));
+    }
+    bool exec() override {
+        return ok(this, nnrh_matmul_nbits_run(h, inputs[0]->data, outputs[0]->data, (int)(inputs[0]->ndata / k), ctx->stream));
+    }
+    double num_ops() const override { return 2.0 * (double)inputs[0]->ndata * n; }
+};
+
 template <typename T>
 operator_t* make(int, pool_t& pool) { return pool_new<T>(pool); }
 operator_t* make_relu(int, pool_t& pool) {
@@ -1646,6 +1700,7 @@ const op_registrar_t reg[] = {
     {"Gelu", backend_t::HIP, make<Gelu_hip>},
     {"Transpose", backend_t::HIP, make<Transpose_hip>},
     {"MatMul", backend_t::HIP, make<MatMul_hip>},
+    {"MatMulNBits", backend_t::HIP, make<MatMulNBits_hip>},
 };
 
 }  // namespace

@@ -40,7 +40,7 @@ FIELDS = {
 ATTR_FLOAT, ATTR_INT, ATTR_STRING, ATTR_TENSOR, ATTR_FLOATS, ATTR_INTS = 1, 2, 3, 4, 6, 7
 # operators of the com.microsoft domain (ONNX Runtime contrib ops)
 MS_OPS = {"QLinearConcat", "QLinearGlobalAveragePool", "QLinearAveragePool", "QLinearMul",
-          "QLinearAdd", "MultiHeadAttention"}
+          "QLinearAdd", "MultiHeadAttention", "MatMulNBits"}
 
 
 def _varint(v: int) -> bytes:

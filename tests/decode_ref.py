@@ -88,3 +88,20 @@ def attention_tol(y, mag_tol, weighted, t):
     """mag_tol: attention()'s; weighted: sum p |v|, for the rounding of weights
     to one (fp16, bf16) or two fp16 pieces (fp32)."""
     return mag_tol + (2.0 ** -11 if t != torch.float32 else 2.0 ** -21) * weighted + HALF[t] * y.abs() + TINY[t]
+
+
+def nbits_graph(dt=np.float32, block=32, K=70, N=24, zp=True, bias=True, shape=(2, 3, 70), scale_dt=None, drop=0, attrs=()):
+    """A graph of one MatMulNBits node. drop: bytes missing from the weights."""
+    from nnr_amd.graph import Graph
+    rng = np.random.default_rng(1)
+    nb = -(-K // block)
+    g = Graph()
+    g.inputs["x"] = (dt, shape)
+    b = rng.integers(0, 256, (N, nb, block // 2), dtype=np.uint8)
+    ins = ["x", g.init("b", b.reshape(-1)[drop:] if drop else b),
+           g.init("s", rng.uniform(0.01, 0.1, (N, nb)).astype(scale_dt or dt)),
+           g.init("z", rng.integers(0, 256, (N, (nb + 1) // 2), dtype=np.uint8)) if zp else "", "",
+           g.init("c", rng.standard_normal(N).astype(dt)) if bias else ""]
+    g.node("MatMulNBits", ins, outputs="y", **{**dict(K=K, N=N, bits=4, block_size=block), **dict(attrs)})
+    g.outputs.append("y")
+    return g

@@ -8,6 +8,7 @@ import torch
 
 import decode_ref as R
 import nnr_amd
+from decode_ref import nbits_graph
 from nnr_amd import _lib
 
 INVALID, UNSUPPORTED = _lib.NNRH_ERR_INVALID, _lib.NNRH_ERR_UNSUPPORTED
@@ -171,3 +172,16 @@ def test_plain_quantizer():
     v, c, s = R.quantize(x * 7 / 127, 4)
     assert c[:2].tolist() == [7, -4]
     assert s[1].item() == 0.0
+
+
+def test_nbits_node_shapes():
+    from nnr_amd.graph import Session
+    s = Session(nbits_graph(), device=False)
+    assert s.tensor_info("y")[2] == (2, 3, 24) and [p["op"] for p in s.plan()] == ["MatMulNBits"]
+
+
+@pytest.mark.parametrize("kw", [dict(shape=(2, 3, 71)), dict(attrs=dict(K=0)), dict(attrs=dict(N=-1)), dict(dt=np.int8)])
+def test_nbits_node_refuses(kw):
+    from nnr_amd.graph import Session
+    with pytest.raises(RuntimeError):
+        Session(nbits_graph(**kw), device=False)

@@ -144,6 +144,40 @@ def test_nbits_streams_share_a_handle(dev):
         assert torch.equal(y, ref[i % 4])
 
 
+@pytest.mark.parametrize("dt", [np.float32, np.float16])
+@pytest.mark.parametrize("kw", [dict(), dict(zp=False, bias=False), dict(block=128, K=300, N=70, shape=(5, 300)),
+                                dict(shape=(70,))])
+@pytest.mark.parametrize("onnx", [False, True])
+def test_nbits_node(dev, dt, kw, onnx, tmp_path):
+    """The node in a graph, from memory and from an ONNX file; run twice (the
+    second time as a captured graph)"""
+    from nnr_amd import onnx_io
+    from nnr_amd.graph import Session
+    g = R.nbits_graph(dt=dt, **kw)
+    if onnx:
+        onnx_io.save(g, str(tmp_path / "m.onnx"))
+        s = Session(None, onnx=str(tmp_path / "m.onnx"))
+    else:
+        s = Session(g)
+    i, t = g.initializers, torch.float32 if dt == np.float32 else torch.float16
+    K, block = kw.get("K", 70), kw.get("block", 32)
+    for seed in (1, 2, 3):
+        x = np.random.default_rng(seed).standard_normal(g.inputs["x"][1]).astype(dt)
+        s.set_input("x", x)
+        s.run()
+        y = s.output("y")[0].astype(np.float64).reshape(-1, i["s"].shape[0])
+        ref, mag = R.nbits(x.reshape(-1, K), i["b"], i["s"], K, block, i.get("z"), i["c"].astype(np.float64) if "c" in i else None)
+        assert R.close(y, ref, R.nbits_tol(ref, mag, K, t), t).all()
+
+
+@pytest.mark.parametrize("kw", [dict(block=16), dict(scale_dt=np.float16), dict(drop=1), dict(attrs=dict(bits=8)),
+                                dict(attrs=dict(block_size=48))])
+def test_nbits_node_refuses(dev, kw):
+    from nnr_amd.graph import Session
+    with pytest.raises(RuntimeError, match="MatMulNBits|matmul_nbits"):
+        Session(R.nbits_graph(**kw))
+
+
 # ---------------------------------------------------------------------------
 # the cache
 
