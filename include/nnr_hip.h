@@ -579,14 +579,14 @@ int nnrh_clip_f32(const float* x_dev, float* y_dev, size_t n, float lo, float hi
 
 /* com.microsoft MatMulNBits with a constant B, bits = 4:
  *   y[m][n] = sum_k a[m][k] (q[n][k] - zp[n][k / block]) scale[n][k / block] + bias[n]
- * block_size: a power of two >= 32; K (at most 2^22) need not be a multiple of it. Column n's
- * ceil(k / block_size) blocks lie one after another, block_size / 2 bytes
- * each, the lower nibble first; zero points likewise, two a byte, a column's
- * rounded up to a whole byte (NULL: 8). run takes a of m x k and writes y of
- * m x n, both row-major and dense, any m >= 0, and uses no workspace: calls
- * on several streams may share a handle. y must not overlap a. a and y are
- * aligned to their element; rows of 16-byte multiples at 16-byte aligned
- * addresses are faster.                                                     */
+ * block_size: a power of two >= 32; k (at most 2^22; n at most 2^26, n k at
+ * most 2^36) need not be a multiple of it. Column n's ceil(k / block_size)
+ * blocks lie one after another, block_size / 2 bytes each, the lower nibble
+ * first; zero points likewise, two a byte, a column's rounded up to a whole
+ * byte (NULL: 8). run takes a of m x k and writes y of m x n, both row-major
+ * and dense, 0 <= m <= 2^20, and uses no workspace: calls on several streams
+ * may share a handle. y must not overlap a. a and y are aligned to their
+ * element; rows of 16-byte multiples at 16-byte aligned addresses are faster. */
 typedef struct nnrh_matmul_nbits_desc {
     int n, k;
     int bits;                     /* 4                                       */
@@ -621,12 +621,14 @@ int nnrh_matmul_nbits_destroy(nnrh_matmul_nbits_t h);
  * write: token s of `seq` new tokens of sequence b goes to position
  *   seq_lens[b] - seq + s. Tokens at negative positions (a batch padded at the
  *   front) and behind the last page are skipped. The pages that one call
- *   writes to must belong to one sequence each.
+ *   writes to must belong to one sequence each, and no other call may write to
+ *   them meanwhile: 32 tokens are read and written back together.
  * read: the same positions back, code * scale rounded to dtype; those that
  *   hold no token as zeros.
  * k and v are [batch][seq][kv_heads][head_dim] with batch and token strides in
  * elements (shared by k and v; heads are dense, tokens of an output do not
- * overlap); addresses and strides in bytes are multiples of 16.            */
+ * overlap); addresses and strides in bytes are multiples of 16. batch is at
+ * most 65535, seq 2^22, max_pages page_size 2^30.                           */
 typedef struct nnrh_kv_cache_desc {
     int num_pages;
     int page_size;                /* tokens: a power of two, 32 .. 4096      */
@@ -660,7 +662,7 @@ int nnrh_kv_cache_read(const nnrh_kv_cache_desc* c, const void* cache_dev, const
  * otherwise. Zero, one or several tokens a sequence, in any mixture of
  * lengths. workspace: nnrh_kv_attention_workspace bytes (a function of the
  * shapes, not of the lengths), 256-byte aligned, NULL where that is 0; calls
- * that may overlap need one each.                                          */
+ * that may overlap need one each. batch seq q_heads is at most 2^23.        */
 typedef struct nnrh_kv_attention_desc {
     int dtype;
     int batch, seq, q_heads;

@@ -550,29 +550,44 @@ def maxpool_u8_nhwc(x, kH, kW, sH, sW, pH, pW, oH, oW):
 # ---------------------------------------------------------------------------
 # a decoder's serving step
 
-def _float_dt(dtype) -> int:
+_FLOAT_DT = {}   # torch type -> NNRH_*; filled with torch's first use here
+_torch_C = None
+
+
+def _use_torch():
+    """torch, which this package imports where it is first needed."""
+    global _torch_C
     import torch
-    if dtype is torch.float16:
-        return F16
-    if dtype is torch.bfloat16:
-        return BF16
-    if dtype is torch.float32:
-        return F32
-    raise TypeError(f"{dtype}: float32, float16 or bfloat16")
+    if _torch_C is None:
+        _FLOAT_DT.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+        _torch_C = torch._C
+    return torch
 
 
-def _launch(index, stream, fn, *args):
-    """fn(*args, stream) with device `index` current, on its current stream
-    unless one is given."""
-    from torch import _C
-    if _C._cuda_getDevice() == index:
-        rc = fn(*args, _C._cuda_getCurrentRawStream(index) if stream is None else stream)
+def _float_dt(dtype) -> int:
+    dt = _FLOAT_DT.get(dtype)
+    if dt is None:
+        raise TypeError(f"{dtype}: float32, float16 or bfloat16")
+    return dt
+
+
+def _launch(index, fn, *args):
+    """fn(*args, stream) with device `index` current, on its current stream."""
+    if _torch_C._cuda_getDevice() == index:
+        rc = fn(*args, _torch_C._cuda_getCurrentRawStream(index))
     else:
         import torch
         with torch.cuda.device(index):
-            rc = fn(*args, _C._cuda_getCurrentRawStream(index) if stream is None else stream)
+            rc = fn(*args, _torch_C._cuda_getCurrentRawStream(index))
     if rc:
         check(rc)
+
+
+def _current(device, stream):
+    """A context in which `stream` (its handle) is current: what a call copies and
+    allocates belongs to the stream that it runs on."""
+    import torch
+    return torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device))
 
 
 def _on_device(device, **tensors):
@@ -593,7 +608,7 @@ class MatMulNBits:
     else the current one."""
 
     def __init__(self, b, scales, k, block_size, zero_points=None, bias=None, bits=4, device=None):
-        import torch
+        torch = _use_torch()
         self.device = torch.device("cuda" if device is None else device)
         if scales.dtype not in (torch.float32, torch.float16, torch.bfloat16):
             raise TypeError(f"scales of {scales.dtype}: float32, float16 or bfloat16")
@@ -624,10 +639,13 @@ class MatMulNBits:
             if on_device:
                 torch.cuda.current_stream().synchronize()
             check(lib().nnrh_matmul_nbits_create(ct.byref(h), ct.byref(desc)))
-        self.h = h
+        self.h, self._run, self._index = h, lib().nnrh_matmul_nbits_run, self.device.index
 
     def __call__(self, a, y=None, stream=None):
         """a [..., k] -> y [..., n]"""
+        if stream is not None:
+            with _current(self.device, stream):
+                return self(a, y)
         shape = a.shape
         if a.dtype != self.dtype or shape[-1] != self.k:
             raise ValueError(f"a must be {self.dtype} [..., {self.k}]")
@@ -640,8 +658,7 @@ class MatMulNBits:
             y = a.new_empty(shape)
         elif y.shape != shape or y.dtype != self.dtype or y.device != self.device or not y.is_contiguous():
             raise ValueError(f"y must be contiguous {self.dtype} of shape {shape} on {self.device}")
-        _launch(self.device.index, stream, lib().nnrh_matmul_nbits_run, self.h, a.data_ptr(), y.data_ptr(),
-                a.numel() // self.k)
+        _launch(self._index, self._run, self.h, a.data_ptr(), y.data_ptr(), a.numel() // self.k)
         return y
 
     def __del__(self):
@@ -664,26 +681,29 @@ class KVCache:
     be strided (a slice of a fused projection's output)."""
 
     def __init__(self, num_pages, kv_heads, head_dim, page_size=64, bits=8, device=None):
-        import torch
+        torch = _use_torch()
         self.desc = KvCacheDesc(int(num_pages), int(page_size), int(kv_heads), int(head_dim), int(bits))
         n = ct.c_size_t()
         check(lib().nnrh_kv_cache_bytes(ct.byref(self.desc), ct.byref(n)))
         self.data = torch.zeros(n.value, dtype=torch.uint8, device="cuda" if device is None else device)
         self.device = self.data.device
+        self._torch, self._index, self._L = torch, self.device.index, lib()
         self.num_pages, self.page_size, self.kv_heads = int(num_pages), int(page_size), int(kv_heads)
         self.head_dim, self.bits = int(head_dim), int(bits)
 
     def _tables(self, batch, page_table, seq_lens):
-        from torch import int32
-        if page_table.dtype != int32 or page_table.dim() != 2 or page_table.shape[0] != batch:
+        int32 = self._torch.int32
+        if page_table.dtype is not int32 or page_table.dim() != 2 or page_table.shape[0] != batch:
             raise ValueError(f"page_table must be int32 [{batch}][pages]")
-        if seq_lens.dtype != int32 or seq_lens.shape != (batch,):
+        if seq_lens.dtype is not int32 or seq_lens.shape != (batch,):
             raise ValueError(f"seq_lens must be int32 [{batch}]")
         if page_table.device != self.device or seq_lens.device != self.device:
             _on_device(self.device, page_table=page_table, seq_lens=seq_lens)
         if not page_table.is_contiguous():
             page_table = page_table.contiguous()
-        return page_table, seq_lens.contiguous()
+        if not seq_lens.is_contiguous():
+            seq_lens = seq_lens.contiguous()
+        return page_table, seq_lens
 
     def _rows(self, name, t, heads):
         """t with dense heads and 16-byte steps: itself, or a copy."""
@@ -700,31 +720,37 @@ class KVCache:
         return t
 
     def _tokens(self, k, page_table, seq_lens):
-        B, S = k.shape[:2]
+        B, S, _, _ = k.shape
         st = k.stride()
         return KvTokens(_float_dt(k.dtype), B, S, st[0], st[1], page_table.data_ptr(), page_table.shape[1],
                         seq_lens.data_ptr())
 
     def write(self, k, v, page_table, seq_lens, stream=None):
         """Token s of sequence b to position seq_lens[b] - seq + s; tokens at
-        negative positions are skipped."""
+        negative positions are skipped. 32 tokens are read and written back
+        together: a page is one sequence's, and one call's at a time."""
+        if stream is not None:
+            with _current(self.device, stream):
+                return self.write(k, v, page_table, seq_lens)
         k, v = self._rows("k", k, self.kv_heads), self._rows("v", v, self.kv_heads)
         if k.shape != v.shape or k.dtype != v.dtype:
             raise ValueError("k and v must agree in shape and type")
         if k.stride() != v.stride():
             k, v = k.contiguous(), v.contiguous()
         page_table, seq_lens = self._tables(k.shape[0], page_table, seq_lens)
-        _launch(self.device.index, stream, lib().nnrh_kv_cache_write, self.desc, self.data.data_ptr(),
+        _launch(self._index, self._L.nnrh_kv_cache_write, self.desc, self.data.data_ptr(),
                 self._tokens(k, page_table, seq_lens), k.data_ptr(), v.data_ptr())
 
     def read(self, seq, page_table, seq_lens, dtype, stream=None):
         """(k, v) of positions seq_lens[b] - seq .. seq_lens[b] - 1 as `dtype`; zeros
         where there is no token."""
-        import torch
+        if stream is not None:
+            with _current(self.device, stream):
+                return self.read(seq, page_table, seq_lens, dtype)
         B = page_table.shape[0]
         page_table, seq_lens = self._tables(B, page_table, seq_lens)
-        k, v = torch.empty((2, B, seq, self.kv_heads, self.head_dim), dtype=dtype, device=self.device).unbind(0)
-        _launch(self.device.index, stream, lib().nnrh_kv_cache_read, self.desc, self.data.data_ptr(),
+        k, v = self._torch.empty((2, B, seq, self.kv_heads, self.head_dim), dtype=dtype, device=self.device).unbind(0)
+        _launch(self._index, self._L.nnrh_kv_cache_read, self.desc, self.data.data_ptr(),
                 self._tokens(k, page_table, seq_lens), k.data_ptr(), v.data_ptr())
         return k, v
 
@@ -741,9 +767,11 @@ class KVCache:
         (b, s) sees the first prefix_len tokens of the pages in prefix_table
         (int32 [pages], shared by the batch) and positions up to seq_lens[b] -
         seq + s of its own. workspace: a uint8 tensor of attention_workspace's
-        size, 256-byte aligned, made by the call unless given (a call on a
-        stream that is not current should bring it)."""
-        import torch
+        size, 256-byte aligned, made by the call unless given."""
+        if stream is not None:
+            with _current(self.device, stream):
+                return self.attention(q, page_table, seq_lens, scale, prefix_table, prefix_len, y, workspace)
+        torch = self._torch
         if q.dim() != 4:
             raise ValueError("q must be [batch, seq, heads, head_dim]")
         B, S, Hq, _ = q.shape
@@ -766,7 +794,7 @@ class KVCache:
                             self.head_dim ** -0.5 if scale is None else float(scale), page_table.data_ptr(),
                             page_table.shape[1], seq_lens.data_ptr(), pt, int(prefix_len))
         n = ct.c_size_t()
-        rc = lib().nnrh_kv_attention_workspace(self.desc, d, n)
+        rc = self._L.nnrh_kv_attention_workspace(self.desc, d, n)
         if rc:
             check(rc)
         ws = None
@@ -777,6 +805,5 @@ class KVCache:
                     not workspace.is_contiguous():
                 raise ValueError(f"workspace must be contiguous uint8 of at least {n.value} elements on {self.device}")
             ws = workspace.data_ptr()
-        _launch(self.device.index, stream, lib().nnrh_kv_attention, self.desc, self.data.data_ptr(), d, q.data_ptr(),
-                y.data_ptr(), ws)
+        _launch(self._index, self._L.nnrh_kv_attention, self.desc, self.data.data_ptr(), d, q.data_ptr(), y.data_ptr(), ws)
         return y

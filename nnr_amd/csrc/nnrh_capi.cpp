@@ -2324,9 +2324,11 @@ extern "C" int nnrh_matmul_nbits_create(nnrh_matmul_nbits_t* out, const nnrh_mat
     if (d->bits != 4 || d->block_size < 32 || float_type(d->dtype) < 0)
         return set_err(NNRH_ERR_UNSUPPORTED, "matmul_nbits: bits %d, block size %d, type %d (4 bits, blocks of 32 and "
                                              "more, fp32 / fp16 / bf16)", d->bits, d->block_size, d->dtype);
-    // bytes of a block's rows (64 fp32 ones) and columns of the last tile in an int
-    if (d->k > (1 << 22) || d->n > (1 << 30) || d->block_size > (1 << 22))
-        return set_err(NNRH_ERR_UNSUPPORTED, "matmul_nbits: n %d, k %d, block size %d", d->n, d->k, d->block_size);
+    // bytes of a block's rows (64 fp32 ones) in an int; threads of a launch, 32 for a
+    // column and one for 32 codes, under the runtime's 2^32
+    if (d->k > (1 << 22) || d->n > (1 << 26) || d->block_size > (1 << 22) || (long long)d->n * d->k > (1LL << 36))
+        return set_err(NNRH_ERR_UNSUPPORTED, "matmul_nbits: n %d, k %d, block size %d (at most 2^26, 2^22, 2^22; n k at "
+                                             "most 2^36)", d->n, d->k, d->block_size);
     if (d->on_device && (((uintptr_t)d->b & 3) || (((uintptr_t)d->scales | (uintptr_t)d->bias) &
                                                    (float_type_size(float_type(d->dtype)) - 1))))
         return set_err(NNRH_ERR_INVALID, "matmul_nbits: alignment");
@@ -2348,7 +2350,8 @@ extern "C" int nnrh_matmul_nbits_create(nnrh_matmul_nbits_t* out, const nnrh_mat
 
 extern "C" int nnrh_matmul_nbits_run(nnrh_matmul_nbits_t h, const void* a, void* y, int m, void* stream) {
     if (!h || m < 0 || (m && (!a || !y))) return set_err(NNRH_ERR_INVALID, "matmul_nbits_run: bad argument");
-    if (m > (1 << 22)) return set_err(NNRH_ERR_UNSUPPORTED, "matmul_nbits_run: %d rows (at most %d)", m, 1 << 22);
+    // blocks of 32 rows and more in a grid's second dimension, 65535 long
+    if (m > (1 << 20)) return set_err(NNRH_ERR_UNSUPPORTED, "matmul_nbits_run: %d rows (at most %d)", m, 1 << 20);
     const size_t es = float_type_size(h->a.type);
     if (((uintptr_t)a | (uintptr_t)y) & (es - 1)) return set_err(NNRH_ERR_INVALID, "matmul_nbits_run: alignment");
     if (overlap(a, (size_t)m * h->a.K * es, y, (size_t)m * h->a.N * es))
@@ -2397,8 +2400,11 @@ int kv_batch(const char* what, int batch, int seq, int max_pages, int page_size,
              const int32_t* lens) {
     if (batch < 0 || seq < 0 || max_pages < 0)
         return set_err(NNRH_ERR_INVALID, "%s: batch %d, seq %d, pages %d", what, batch, seq, max_pages);
-    if (batch > 65535 || seq > (1 << 30) || (long long)max_pages * page_size > (1 << 30))
-        return set_err(NNRH_ERR_UNSUPPORTED, "%s: batch %d (at most 65535), seq %d, %d pages of %d tokens (at most 2^30)",
+    // seq: a launch's threads, 512 for 32 tokens, under the runtime's 2^32, and an
+    // extent in bytes at the longest strides in 64 bits
+    if (batch > 65535 || seq > (1 << 22) || (long long)max_pages * page_size > (1 << 30))
+        return set_err(NNRH_ERR_UNSUPPORTED,
+                       "%s: batch %d (at most 65535), seq %d (at most 2^22), %d pages of %d tokens (at most 2^30)",
                        what, batch, seq, max_pages, page_size);
     if (!batch || !seq) return NNRH_OK;
     if (!lens || (max_pages && !table)) return set_err(NNRH_ERR_INVALID, "%s: NULL table or lengths", what);
@@ -2410,7 +2416,7 @@ int kv_strides(const char* what, int type, int batch, int seq, long long width, 
     const long long per16 = 16 / float_type_size(type);
     if (bs < 0 || ts < 0 || (batch > 1 && bs % per16) || (seq > 1 && ts % per16))
         return set_err(NNRH_ERR_INVALID, "%s: strides %lld, %lld (multiples of 16 bytes)", what, bs, ts);
-    if (bs > (1LL << 40) || ts > (1LL << 40)) return set_err(NNRH_ERR_UNSUPPORTED, "%s: strides %lld, %lld", what, bs, ts);
+    if (bs > (1LL << 38) || ts > (1LL << 38)) return set_err(NNRH_ERR_UNSUPPORTED, "%s: strides %lld, %lld", what, bs, ts);
     // one of the two orders, each row or sequence behind the one before
     const bool rows = seq <= 1 || ts >= width, seqs = batch <= 1 || bs >= (seq - 1) * ts + width;
     const bool inner = batch <= 1 || bs >= width, outer = seq <= 1 || ts >= (batch - 1) * bs + width;
@@ -2437,8 +2443,9 @@ int kv_tokens(const char* what, const KvCache& c, const nnrh_kv_tokens* t, const
     const size_t all = (size_t)c.num_pages * kv_page_bytes(c);
     if (overlap(k, extent, c.data, all) || overlap(v, extent, c.data, all))
         return set_err(NNRH_ERR_INVALID, "%s: k or v lies over the cache", what);
-    // k and v may alternate in one tensor; the same rows are two results in one place
-    if (out && k == v) return set_err(NNRH_ERR_INVALID, "%s: k and v are one tensor", what);
+    // k and v may alternate in one tensor; rows over each other are two results in one place
+    const size_t row = width * float_type_size(type);
+    if (out && overlap(k, row, v, row)) return set_err(NNRH_ERR_INVALID, "%s: k lies over v", what);
     return NNRH_OK;
 }
 
@@ -2487,8 +2494,9 @@ int kv_attention_args(const nnrh_kv_cache_desc* d, const void* cache, const nnrh
         return set_err(NNRH_ERR_INVALID, "kv_attention: %d query heads over %d", a->q_heads, c->heads);
     if (a->prefix_len < 0 || a->batch < 0 || a->seq < 0)
         return set_err(NNRH_ERR_INVALID, "kv_attention: batch %d, seq %d, prefix of %d", a->batch, a->seq, a->prefix_len);
-    // rows, and blocks of rows times splits, in an int
-    if (a->prefix_len > (1 << 30) || (double)a->batch * a->seq * a->q_heads * c->hd > 17179869184.0)
+    // a launch's threads, 256 for a row of a block of its own, under the runtime's 2^32
+    // with room for the prefix's blocks and the splits
+    if (a->prefix_len > (1 << 30) || (double)a->batch * a->seq * a->q_heads > (1 << 23))
         return set_err(NNRH_ERR_UNSUPPORTED, "kv_attention: batch %d, seq %d, %d heads, prefix of %d", a->batch, a->seq,
                        a->q_heads, a->prefix_len);
     *r = KvAttention{nullptr, nullptr, type, a->q_batch_stride, a->q_token_stride, a->batch, a->seq, a->q_heads,
@@ -2530,13 +2538,13 @@ extern "C" int nnrh_kv_attention(const nnrh_kv_cache_desc* d, const void* cache,
     const size_t qsize = ((a->batch - 1) * bs + (a->seq - 1) * ts + width) * es;
     const bool dense = (a->seq == 1 || ts == width) && (a->batch == 1 || bs == a->seq * width);
     if (overlap(q, qsize, y, ysize) && !(q == y && dense)) return set_err(NNRH_ERR_INVALID, "kv_attention: y lies over q");
-    if (overlap(y, ysize, c.data, (size_t)c.num_pages * kv_page_bytes(c)))
-        return set_err(NNRH_ERR_INVALID, "kv_attention: y lies over the cache");
+    const size_t all = (size_t)c.num_pages * kv_page_bytes(c);
+    if (overlap(y, ysize, c.data, all)) return set_err(NNRH_ERR_INVALID, "kv_attention: y lies over the cache");
     const size_t need = kv_attention_workspace(c, r);
     if (need && !workspace) return set_err(NNRH_ERR_INVALID, "kv_attention: this shape needs a workspace of %zu bytes", need);
     if ((uintptr_t)workspace & 255) return set_err(NNRH_ERR_INVALID, "kv_attention: the workspace must be 256-byte aligned");
-    if (overlap(workspace, need, q, qsize) || overlap(workspace, need, y, ysize))
-        return set_err(NNRH_ERR_INVALID, "kv_attention: the workspace lies over q or y");
+    if (overlap(workspace, need, q, qsize) || overlap(workspace, need, y, ysize) || overlap(workspace, need, c.data, all))
+        return set_err(NNRH_ERR_INVALID, "kv_attention: the workspace lies over q, y or the cache");
     r.q = q;
     r.y = y;
     ProfScope ps("kv_attention", S(stream));

@@ -155,6 +155,44 @@ def test_attention_refuses_memory():
     assert run(MEM[0], None, None, None) == 0
 
 
+@pytest.mark.parametrize("kw", [dict(n=(1 << 26) + 1), dict(n=1 << 25, k=4096)])
+def test_nbits_create_refuses_sizes(kw):
+    """Launches that would pass 2^32 threads: from shapes alone, before any pointer is read"""
+    d = dict(n=16, k=64, bits=4, block_size=32, dtype=_lib.F16, on_device=1, b=MEM[0], scales=MEM[1])
+    h = C.c_void_p()
+    assert _lib.lib().nnrh_matmul_nbits_create(C.byref(h), C.byref(_lib.MatMulNBitsDesc(**{**d, **kw}))) == UNSUPPORTED
+    assert not h.value
+
+
+@pytest.mark.parametrize("kw", [dict(seq=(1 << 22) + 1), dict(batch_stride=(1 << 38) + 8)])
+def test_calls_refuse_sizes(kw):
+    L, c, t = _lib.lib(), cache_desc(), tokens_desc(**kw)
+    assert L.nnrh_kv_cache_write(C.byref(c), MEM[0], C.byref(t), MEM[1], MEM[2], None) == UNSUPPORTED
+    assert L.nnrh_kv_cache_read(C.byref(c), MEM[0], C.byref(t), MEM[1], MEM[2], None) == UNSUPPORTED
+
+
+def test_attention_refuses_rows():
+    L, c, n = _lib.lib(), cache_desc(kv_heads=1), C.c_size_t()
+    for batch, seq, heads, rc in ((64, 4096, 32, 0), (64, 4097, 32, UNSUPPORTED), (1, 1, (1 << 23) + 1, UNSUPPORTED)):
+        a = attention_desc(batch=batch, seq=seq, q_heads=heads, q_token_stride=heads * 128, q_batch_stride=seq * heads * 128)
+        assert L.nnrh_kv_attention_workspace(C.byref(c), C.byref(a), C.byref(n)) == rc
+        if rc:
+            assert L.nnrh_kv_attention(C.byref(c), MEM[0], C.byref(a), MEM[1], MEM[2], MEM[6], None) == rc
+
+
+def test_read_refuses_rows_over_each_other():
+    """v's rows may lie between k's, not over them."""
+    L, c = _lib.lib(), cache_desc()
+    t = tokens_desc(token_stride=1024, batch_stride=4096)
+    for at in (-496, -16, 16, 496):
+        assert L.nnrh_kv_cache_read(C.byref(c), MEM[0], C.byref(t), MEM[1] + 512, MEM[1] + 512 + at, None) == INVALID
+
+
+def test_attention_refuses_a_workspace_in_the_cache():
+    L, c, a = _lib.lib(), cache_desc(), attention_desc()
+    assert L.nnrh_kv_attention(C.byref(c), MEM[0], C.byref(a), MEM[1], MEM[2], MEM[0] + 256, None) == INVALID
+
+
 def test_python_refuses_types():
     with pytest.raises(TypeError):
         nnr_amd.MatMulNBits(np.zeros((4, 2, 16), np.uint8), torch.zeros(4, 2, dtype=torch.float64), 64, 32)

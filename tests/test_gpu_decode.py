@@ -127,6 +127,51 @@ def test_nbits_empty_and_shapes(dev):
     assert torch.equal(op(wide[:, 3:99]), op(wide[:, 3:99].contiguous()))
 
 
+@pytest.mark.parametrize("t,k", [(torch.float32, 33), (torch.float16, 64)])
+def test_nbits_most_rows(dev, t, k):
+    """2^20 rows, the most that a call takes, by row loads of either kind; one more is refused."""
+    b, s, z, c = weights(2, 16, k, 32, t, True, True)
+    op = nnr_amd.MatMulNBits(b, s, k, 32, zero_points=z, bias=c)
+    a = torch.randn(((1 << 20) + 1, k), device=dev).to(t)
+    y = op(a[:-1])
+    for i in (0, 77777, (1 << 20) - 300):
+        ref = op(a[i:i + 300])   # both: k 2^-24 of the terms' sum, and half a step of y
+        assert ((y[i:i + 300] - ref).abs() <= 1e-2 * ref.abs() + 1e-2).all()
+    with pytest.raises(nnr_amd.NnrHipError):
+        op(a)
+
+
+def test_calls_on_a_given_stream(dev):
+    """Each call by a stream's handle while the current stream is busy: copies of
+    rows and tables that the call makes are made on that stream."""
+    st = torch.cuda.Stream()
+    H, hd, page, B, S = 2, 64, 32, 2, 40
+    b, s, z, c = weights(5, 24, 96, 32, torch.float16, True, True)
+    op = nnr_amd.MatMulNBits(b, s, 96, 32, zero_points=z, bias=c)
+    a = torch.randn((5, 200), device=dev).half()[:, 3:99]
+    caches = [filled(dev, 8, H, hd, page_size=page) for _ in "ab"]
+    k, v = (x.to(dev) for x in tokens(1, B, S, H, hd, torch.float16))
+    k, v = k.transpose(1, 2).contiguous().transpose(1, 2), v.transpose(1, 2).contiguous().transpose(1, 2)
+    q = torch.randn((B, 4 * H, S, hd), device=dev).half().transpose(1, 2)
+    td = torch.arange(16, dtype=torch.int32, device=dev).reshape(8, 2)[:, 0].reshape(2, 4).t()[:2]
+    lens = torch.tensor([40, 9, 33, 9], dtype=torch.int32, device=dev)[::2]
+    td = torch.stack((td[:, 0] // 2, td[:, 1] // 2 + 1), 1).t().contiguous().t()
+
+    def run(cache, **kw):
+        y = op(a, **kw)
+        cache.write(k, v, td, lens, **kw)
+        return (y, *cache.read(S, td, lens, torch.float16, **kw), cache.attention(q, td, lens, **kw),
+                cache.attention(q, td, lens, prefix_table=td[1], prefix_len=33, **kw))
+    ref = run(caches[0])
+    torch.cuda.synchronize()
+    torch.cuda._sleep(50_000_000)
+    got = run(caches[1], stream=st.cuda_stream)
+    st.synchronize()
+    torch.cuda.synchronize()
+    for x, y in zip(got, ref):
+        assert torch.equal(x, y)
+
+
 def test_nbits_streams_share_a_handle(dev):
     b, s, z, c = weights(5, 512, 1024, 32, torch.bfloat16, True, False)
     op = nnr_amd.MatMulNBits(b, s, 1024, 32, zero_points=z)
@@ -438,6 +483,57 @@ def test_attention_pages_that_do_not_exist(dev, bits):
     assert ((y[0].double() - ref).abs() <= R.attention_tol(ref, tol, mag, torch.float32)).all()
     none = cache.attention(q.to(dev), torch.tensor([[-1, 4, 5]], dtype=torch.int32, device=dev), lens)
     assert not none.any()
+
+
+@pytest.mark.parametrize("hd,S,heads,prefix", [(64, 1, 1, 0), (128, 1, 8, 40), (128, 40, 2, 40), (256, 9, 4, 100)])
+def test_attention_without_keys(dev, hd, S, heads, prefix):
+    """No pages at all, and tables of no pages: zeros for every query."""
+    q = torch.randn((3, S, heads, hd), device=dev).half()
+    lens = torch.tensor([0, 50, 2 ** 31 - 1], dtype=torch.int32, device=dev)
+    pt = torch.tensor([0, 1, 5, -1], dtype=torch.int32, device=dev)
+    for pages, per in ((0, 4), (0, 0), (2, 0)):
+        cache = filled(dev, pages, 1, hd, page_size=32)
+        td = torch.zeros((3, per), dtype=torch.int32, device=dev)
+        assert not cache.attention(q, td, lens).any()
+        if pages == 0 and prefix:
+            assert not cache.attention(q, td, lens, prefix_table=pt, prefix_len=prefix).any()
+        k = torch.randn((3, S, 1, hd), device=dev)
+        cache.write(k, k, td, lens)
+        assert not any(x.any() for x in cache.read(S, td, lens, torch.float32))
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_attention_splits_in_a_graph(dev, bits):
+    """Prefix, many rows and splits captured; replays after the lengths and the
+    queries changed, eager calls between, two graphs over one workspace in turn."""
+    H, hd, page, B, S, G = 2, 128, 64, 3, 3, 8
+    cache = filled(dev, 70, H, hd, page_size=page, bits=bits)
+    td = torch.arange(60, dtype=torch.int32, device=dev).reshape(3, 20)
+    pt = torch.arange(60, 70, dtype=torch.int32, device=dev)
+    lens = torch.tensor([1280, 700, 64], dtype=torch.int32, device=dev)
+    for tab, n in ((td, 1280), (pt.reshape(1, 10), 640)):
+        k, v = (x.to(dev) for x in tokens(n, len(tab), n, H, hd, torch.float16))
+        cache.write(k, v, tab, torch.full((len(tab),), n, dtype=torch.int32, device=dev))
+    q = torch.randn((B, S, H * G, hd), device=dev).half()
+    size = cache.attention_workspace(B, S, H * G, 20, 600)
+    assert size > 0
+    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    cache.attention(q, td, lens, prefix_table=pt, prefix_len=600, workspace=ws)
+    torch.cuda.synchronize()
+    graphs, ys = [], []
+    for prefix in (600, 64):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            ys.append(cache.attention(q, td, lens, prefix_table=pt, prefix_len=prefix, workspace=ws))
+        graphs.append(g)
+    for i in range(4):
+        q.copy_(torch.randn(q.shape, generator=torch.Generator().manual_seed(i)).half())
+        lens.copy_(torch.tensor([1280 - 100 * i, 3 + i, 64 * i], dtype=torch.int32))
+        for g in graphs:
+            g.replay()
+        for y, prefix in zip(ys, (600, 64)):
+            assert torch.equal(y, cache.attention(q, td, lens, prefix_table=pt, prefix_len=prefix))
+        torch.cuda.synchronize()
 
 
 @pytest.mark.parametrize("t", TYPES)
