@@ -12,12 +12,24 @@
 // Codes are exact in fp16. A query row is scaled by a power of two to below
 // 2^15, where fp16 and bf16 elements are exact (those under 2^-38 of the
 // row's largest lose their last bits); an fp32 row is the sum of two fp16
-// pieces, 22 bits and more. Weights p = exp(s - max) enter as p * 2^15, and
-// with them, at 8 bits, the values' scales divided by their largest power of
-// two so far: 11 significant bits (two pieces, 22, for fp32 tensors) over 39
-// binary orders. At 4 bits scale (8 bits) times code (3 bits) is exact in
-// fp16 and is formed in the operand. Sums, maxima and the running total are
-// fp32.
+// pieces, 22 bits and more. Weights p = exp(s - max) enter as 2^11 p, where
+// max may be one that up to 2^4 outgrow, or for fp32 tensors as 2^15 p in two
+// pieces; with them, at 8 bits, the values' scales over their largest power of
+// two so far: 11 significant bits (22) over 35 binary orders and more. At 4
+// bits scale (8 bits) times code (3 bits) is exact in fp16 and is formed in
+// the operand, over the largest power of two so far as well (eu for values, ek
+// for keys: the units, which sums and scores follow when they move). Sums,
+// maxima and the running total are fp32.
+//
+// Up to 16 rows (few): the block's waves take tiles in turn, operands go from
+// memory to registers, and a tile's registers are asked for again as soon as
+// they are used; bound by memory: 48 sequences of up to 8192 tokens, 32 heads
+// over 8 of 128, 8 bits, 409 MB in 80 us and 4 of joining (a copy's rate: 79).
+// More rows (many): the waves take rows, and a tile's codes are turned into
+// operands once, in LDS. Bound by the instructions between the products: 128
+// sequences after a prefix of 32768, 4 bits, 69 GFLOP in 121 us (a large
+// library product's rate: 57): products are a quarter of a tile's cycles, the
+// rest weights, conversion, and waiting at the tile's barrier.
 //
 // Keys are split over blocks; each leaves (max, total, O) of its rows, which
 // a second kernel joins in a fixed order. One block that sees everything
@@ -52,7 +64,7 @@ struct AttnArgs {
     int rows;                      // batch * seq * q_heads
     int slots, pre_slots;          // partial results a row: prefix ones first
     int pre_chunk, own_chunk;      // tiles of a split
-    int pre_groups, own_groups;    // row groups (of 16 NR rows)
+    int pre_groups, own_groups;    // row groups: of 16 rows, or of a block's with many
     int page_shift;                // log2(page_size / 32)
     float* part_o;                 // [rows][slots][hd]
     float2* part_ml;               // [rows][slots]
@@ -679,7 +691,9 @@ __device__ __forceinline__ void few(const AttnArgs& p, Job& job, char* lds) {
 template <int HD> constexpr int kFewLds = 2 * (HD / 16) * 1024 + 2 * AW * 64;
 
 // ---- many rows: the block's waves split its rows ------------------------------
-constexpr int kManyTiles = 2;   // tiles between two barriers
+// Tiles between two barriers: two, or one where two would not leave enough
+// registers (32 sequences after a prefix of 8192: 27.0 us, with two 27.5).
+template <int HD, int BITS> constexpr int kManyTiles = HD == 128 && BITS == 8 ? 1 : 2;
 
 // A tile is turned into operands once, a part by each wave, and lies in LDS
 // for all of them; the next tile is written beside it meanwhile, and the codes
@@ -747,7 +761,7 @@ template <int HD, int BITS> struct Parts {
 
 template <int HD, int BITS, int NP, int NR>
 __device__ __forceinline__ void many(const AttnArgs& p, Job& job, char* lds) {
-    constexpr int NC = HD / 32, NU = Parts<HD, BITS>::NU, KT = kManyTiles;
+    constexpr int NC = HD / 32, NU = Parts<HD, BITS>::NU, KT = kManyTiles<HD, BITS>;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15;
     h8(*frag)[KT][4 * NC][64] = (h8(*)[KT][4 * NC][64])lds;   // [2]: a tile's keys (c, i), then its values (c, i)
@@ -884,7 +898,7 @@ __device__ __forceinline__ void many(const AttnArgs& p, Job& job, char* lds) {
     }
     put_rows(p, job, row0, w, m, l);
 }
-template <int HD> constexpr int kManyLds = 2 * kManyTiles * 4 * (HD / 32) * 1024;
+template <int HD, int BITS> constexpr int kManyLds = 2 * kManyTiles<HD, BITS> * 4 * (HD / 32) * 1024;
 
 // row tiles of a wave with many rows: two where they fit beside the rest
 template <int HD, int NP> constexpr int kManyRows = HD <= 128 && NP == 1 ? 2 : 1;
@@ -894,7 +908,7 @@ template <int HD, int NP> constexpr int kManyRows = HD <= 128 && NP == 1 ? 2 : 1
 // many rows.
 template <int HD, int BITS, int NP, bool PM, bool OM>
 __global__ __launch_bounds__(AW * 64, HD <= 128 ? 2 : 1) void kv_attn_kernel(AttnArgs p) {
-    constexpr int few_lds = PM && OM ? 0 : kFewLds<HD>, many_lds = PM || OM ? kManyLds<HD> : 0;
+    constexpr int few_lds = PM && OM ? 0 : kFewLds<HD>, many_lds = PM || OM ? kManyLds<HD, BITS> : 0;
     __shared__ __attribute__((aligned(16))) char lds[few_lds > many_lds ? few_lds : many_lds];
     constexpr int NR = kManyRows<HD, NP>;
     const KvAttention& a = p.a;
@@ -1004,22 +1018,26 @@ Plan plan(const KvCache& c, const KvAttention& a) {
     p.pre_groups = a.prefix_len ? ceil_div(pre_rows, p.pre_many ? many : 16) : 0;
     const long long pre_items = (long long)p.pre_groups * c.heads, own_items = (long long)p.own_groups * c.heads * a.batch;
     const long long pre_tiles = (a.prefix_len + 31) / 32, own_tiles = (long long)a.max_pages * c.page_size / 32;
-    // Blocks with many rows: no more than run at once, of 8 tiles or more. (128
-    // sequences after a prefix of 32768: 512 blocks 139 us, 384 147, 768 154.)
-    const long long at_once = c.hd <= 128 ? 512 : 256;
-    long long chunk = 8;
-    for (;; chunk += 2) {
-        const long long pre = p.pre_many ? pre_items * ceil_div(pre_tiles, chunk) : 0;
-        const long long own = p.own_many ? own_items * ceil_div(own_tiles, chunk) : 0;
-        if (pre + own <= at_once || chunk >= std::max(pre_tiles, own_tiles)) break;
-        chunk += chunk / 16 * 2;
-    }
-    // Those with few: 32 tiles or more, and short ones whole. (A split of 8 tiles a
-    // block, and its join: 48 sequences of 8192 87 us instead of 85, 16 of 1000
-    // 14 instead of 12.7, 4 of 8192 20 instead of 16, one of 700 13.7 instead of 10.)
+    // Blocks with few rows: 32 tiles or more, and short ones whole. (A split of 8
+    // tiles a block, and its join: 48 sequences of 8192 87 us instead of 85, 16 of
+    // 1000 14 instead of 12.7, 4 of 8192 20 instead of 16, one of 700 13.7 instead
+    // of 10.)
     const auto few = [](long long items, long long tiles) {
         return tiles <= 32 ? std::max(tiles, 1ll) : std::max(items * tiles / 1024, 32ll);
     };
+    // Those with many: no more than run at once, of 8 tiles or more. (128 sequences
+    // after a prefix of 32768: 512 blocks 139 us, 384 147, 768 154.) Of 4 where that
+    // is a block a CU, and two with the rest: such a block waits for most of a tile's
+    // 0.8 us. (32 sequences after a prefix of 1024: 19.2 us, of 8 tiles 22.8; 4096:
+    // 21.9 and 24.1. Beyond: 8192 36 and 27, 128 sequences after 512 30.4 and 28.8.)
+    const long long at_once = c.hd <= 128 ? 512 : 256;
+    const auto many_blocks = [&](long long chunk) {
+        return (p.pre_many ? pre_items * ceil_div(pre_tiles, chunk) : 0) + (p.own_many ? own_items * ceil_div(own_tiles, chunk) : 0);
+    };
+    const long long rest = (p.pre_many ? 0 : pre_items * ceil_div(pre_tiles, few(pre_items, pre_tiles))) +
+                           (p.own_many ? 0 : own_items * ceil_div(own_tiles, few(own_items, own_tiles)));
+    long long chunk = many_blocks(4) <= 256 && many_blocks(4) + rest <= 512 ? 4 : 8;
+    while (many_blocks(chunk) > at_once && chunk < std::max(pre_tiles, own_tiles)) chunk += 2 + chunk / 16 * 2;
     const long long pre_c = p.pre_many ? chunk : few(pre_items, pre_tiles), own_c = p.own_many ? chunk : few(own_items, own_tiles);
     p.pre_slots = p.pre_groups ? ceil_div(pre_tiles, pre_c) : 0;
     p.own_slots = own_tiles ? ceil_div(own_tiles, own_c) : 1;

@@ -7,6 +7,15 @@
 // No weight is rounded. fp16 activations run on fp16 MFMAs, bf16 ones on bf16
 // MFMAs; an fp32 activation is the exact sum of three bf16 pieces, one MFMA
 // each.
+//
+// Up to 64 rows a block is a few columns with all of K split over its waves:
+// every weight is read once, and there are blocks for all CUs. One row x 4096
+// x 8192 columns, bf16: 18 MB in 6.5 us (a copy's rate: 3.5), bound by how long
+// the first loads take; 64 x 8192 x 8192, fp16: 37 MB and 8.6 GFLOP in 19 us (7.1
+// and 7.5), bound by turning codes into operands, which 64 rows share. Beyond,
+// blocks of up to 128 rows share operands of activations through LDS: 512 x 4096
+// x 4096, bf16: 17 GFLOP in 33 us (14.1), bound by the same conversion and the
+// blocks' scales in fp32.
 #include "nnrh_decode.h"
 
 namespace nnrh {
