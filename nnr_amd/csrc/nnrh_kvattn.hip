@@ -28,8 +28,8 @@
 // More rows (many): the waves take rows, and a tile's codes are turned into
 // operands once, in LDS. Bound by the instructions between the products: 128
 // sequences after a prefix of 32768, 4 bits, 69 GFLOP in 121 us (a large
-// library product's rate: 57): products are a quarter of a tile's cycles, the
-// rest weights, conversion, and waiting at the tile's barrier.
+// library product's rate: 57): matrix units 25 % busy, vector units 50 with
+// weights and conversion, the rest waits for LDS and at the tile's barrier.
 //
 // Keys are split over blocks; each leaves (max, total, O) of its rows, which
 // a second kernel joins in a fixed order. One block that sees everything

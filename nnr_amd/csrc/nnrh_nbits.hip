@@ -12,10 +12,12 @@
 // every weight is read once, and there are blocks for all CUs. One row x 4096
 // x 8192 columns, bf16: 18 MB in 6.5 us (a copy's rate: 3.5), bound by how long
 // the first loads take; 64 x 8192 x 8192, fp16: 37 MB and 8.6 GFLOP in 19 us (7.1
-// and 7.5), bound by turning codes into operands, which 64 rows share. Beyond,
-// blocks of up to 128 rows share operands of activations through LDS: 512 x 4096
-// x 4096, bf16: 17 GFLOP in 33 us (14.1), bound by the same conversion and the
-// blocks' scales in fp32.
+// and 7.5), bound by loads: each of 256 blocks reads the 64 rows whole, 1 MB, beside
+// 0.14 MB of weights (vector units 30 % busy, matrix units 18). Beyond, blocks of
+// up to 128 rows share activations through LDS, and a wave's weights serve all of
+// them: 512 x 4096 x 4096, bf16: 17 GFLOP in 33 us (14.1), bound by conversion,
+// the blocks' scales in fp32 and the barrier of each chunk at two waves a SIMD
+// (vector units 45 % busy, matrix units 20).
 #include "nnrh_decode.h"
 
 namespace nnrh {
