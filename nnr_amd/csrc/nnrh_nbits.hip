@@ -416,6 +416,20 @@ __global__ __launch_bounds__(NB_WAVES * 64) void nbits_tile_kernel(NbitsArgs p) 
                 const int kk = k + 4 * h;   // (h: fp32 only)
                 if constexpr (AM == A_WHOLE) {
                     act[i][h] = *(const u4*)(base + (row + (uint32_t)(kk * ES)));
+                } else if constexpr (AM == A_ANY) {
+                    if (k0 + 64 <= p.K) {
+                        act[i][h] = *(const u4_any*)(base + (row + (uint32_t)(kk * ES)));
+                    } else {
+                        u4 x = {0, 0, 0, 0};
+#pragma unroll
+                        for (int j = 0; j < 16 / ES; ++j) {
+                            const bool in = kk + j < p.K;
+                            const uint32_t at = row + (uint32_t)(in ? (kk + j) * ES : 0);
+                            if constexpr (TY == FT_F32) x[j] = in ? *(const uint32_t*)(base + at) : 0u;
+                            else x[j >> 1] |= (in ? (uint32_t)*(const uint16_t*)(base + at) : 0u) << (16 * (j & 1));
+                        }
+                        act[i][h] = x;
+                    }
                 } else {
                     const bool in = kk < p.K;
                     const u4 x = *(const u4*)(base + (row + (uint32_t)(in ? kk * ES : 0)));
@@ -598,23 +612,23 @@ hipError_t go_tile(const NbitsArgs& a, hipStream_t s) {
 }
 template <int TY, int NSPP, int AM>
 hipError_t by_size(const NbitsArgs& a, hipStream_t s) {
+    constexpr bool wide = TY == FT_F32;   // activations take twice the registers
+    const int cols = nbits_cols(a.N);
+    const auto blocks = [&](int m, int n) { return (long long)((a.M + m - 1) / m) * (cols / n); };
+    if (a.M > 64) {
+        // Blocks of shared rows where they fill the chip (bf16, K 4096, blocks of
+        // 32: 512 x 4096 38 us, K split over waves 53; 256 x 4096 35 and 27);
+        // those of 128 columns where that is so twice over (4096 x 4096 235 us,
+        // 64 columns of 128 rows 279). Rows of any address too (512 x 4095 x 4096
+        // bf16 57 us, K split over waves 90; fp32 74 and 156).
+        if (blocks(64, 128) >= (wide ? 192 : 512)) return go_tile<TY, NSPP, AM, 4, 2, 4>(a, s);
+        if constexpr (!wide)
+            if (blocks(128, 64) >= 192)   // (column tiles side by side spill with few scales: 41 us, 35)
+                return go_tile<TY, NSPP, AM, 8, NSPP == 4 ? 2 : 1, NSPP == 4 ? 2 : 4>(a, s);
+    }
     if constexpr (AM == A_ANY) {
         return a.M <= 16 ? go<TY, NSPP, AM, 1, 1, 2>(a, s) : go<TY, NSPP, AM, 2, 2, 1>(a, s);
     } else {
-        constexpr bool wide = TY == FT_F32;   // activations take twice the registers
-        const int cols = nbits_cols(a.N);
-        const auto blocks = [&](int m, int n) { return (long long)((a.M + m - 1) / m) * (cols / n); };
-        if (a.M > 64) {
-            // Blocks of shared rows where they fill the chip (bf16, K 4096, blocks of
-            // 32: 512 x 4096 38 us, K split over waves 53; 256 x 4096 35 and 27);
-            // those of 128 columns where that is so twice over (4096 x 4096 235 us,
-            // 64 columns of 128 rows 279).
-            if (blocks(64, 128) >= (wide ? 192 : 512)) return go_tile<TY, NSPP, AM, 4, 2, 4>(a, s);
-            if constexpr (!wide)
-                if (blocks(128, 64) >= 192)   // (column tiles side by side spill with few scales: 41 us, 35)
-                    return NSPP == 4 ? go_tile<TY, NSPP, AM, 8, NSPP == 4 ? 2 : 1, NSPP == 4 ? 2 : 4>(a, s)
-                                     : go_tile<TY, NSPP, AM, 8, 1, 4>(a, s);
-        }
         if (a.M <= 2)
             return cols >= 16384 ? go<TY, NSPP, AM, 1, 2, wide ? 2 : 3, true>(a, s) : go<TY, NSPP, AM, 1, 1, wide ? 3 : 4, true>(a, s);
         if (a.M <= 16) return cols >= 16384 ? go<TY, NSPP, AM, 1, 2, 3>(a, s) : go<TY, NSPP, AM, 1, 1, 4>(a, s);

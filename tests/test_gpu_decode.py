@@ -127,6 +127,14 @@ def test_nbits_empty_and_shapes(dev):
     assert torch.equal(op(wide[:, 3:99]), op(wide[:, 3:99].contiguous()))
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("block", [32, 64, 256])
+@pytest.mark.parametrize("m,n,k", [(450, 3201, 191), (200, 6401, 65), (1700, 2500, 193)])
+def test_nbits_many_unaligned_rows(dev, t, block, m, n, k):
+    """Rows of odd lengths where blocks share rows: a chunk of 64 k whole, cut short, and with nothing left in it"""
+    check_nbits(dev, m, n, k, block, t, True, block == 64)
+
+
 @pytest.mark.parametrize("t,k", [(torch.float32, 33), (torch.float16, 64)])
 def test_nbits_most_rows(dev, t, k):
     """2^20 rows, the most that a call takes, by row loads of either kind; one more is refused."""
