@@ -661,8 +661,9 @@ int nnrh_kv_cache_read(const nnrh_kv_cache_desc* c, const void* cache_dev, const
  * aligned; y may be q itself where q is dense, and must not overlap it
  * otherwise. Zero, one or several tokens a sequence, in any mixture of
  * lengths. workspace: nnrh_kv_attention_workspace bytes (a function of the
- * shapes, not of the lengths), 256-byte aligned, NULL where that is 0; calls
- * that may overlap need one each. batch seq q_heads is at most 2^23.        */
+ * shapes and the type, not of the lengths: a buffer that serves several types
+ * is as large as the largest asks), 256-byte aligned, NULL where that is 0;
+ * calls that may overlap need one each. batch seq q_heads is at most 2^23.        */
 typedef struct nnrh_kv_attention_desc {
     int dtype;
     int batch, seq, q_heads;

@@ -754,12 +754,17 @@ class KVCache:
                 self._tokens(k, page_table, seq_lens), k.data_ptr(), v.data_ptr())
         return k, v
 
-    def attention_workspace(self, batch, seq, q_heads, max_pages, prefix_len=0):
-        """Bytes of workspace that such an attention takes, whatever the lengths."""
-        d = KvAttentionDesc(F32, batch, seq, q_heads, 0, 0, 1.0, None, max_pages, None, None, int(prefix_len))
-        n = ct.c_size_t()
-        check(lib().nnrh_kv_attention_workspace(self.desc, d, n))
-        return n.value
+    def attention_workspace(self, batch, seq, q_heads, max_pages, prefix_len=0, dtype=None):
+        """Bytes of workspace that such an attention takes, whatever the lengths: of
+        queries of type `dtype`, or enough for any type. (Keys are split by how
+        many rows a block holds, and that goes by the type.)"""
+        sizes = []
+        for dt in (F32, F16, BF16) if dtype is None else (_float_dt(dtype),):
+            d = KvAttentionDesc(dt, batch, seq, q_heads, 0, 0, 1.0, None, max_pages, None, None, int(prefix_len))
+            n = ct.c_size_t()
+            check(lib().nnrh_kv_attention_workspace(self.desc, d, n))
+            sizes.append(n.value)
+        return max(sizes)
 
     def attention(self, q, page_table, seq_lens, scale=None, prefix_table=None, prefix_len=0, y=None, workspace=None,
                   stream=None):

@@ -1,0 +1,42 @@
+"""What the decoder operators say of sizes, from the host alone."""
+import ctypes as C
+
+import pytest
+import torch
+
+import nnr_amd
+from nnr_amd import _lib
+
+TYPES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+
+
+def workspace(cache, t, batch, seq, heads, pages, prefix):
+    """What the C function says for a type."""
+    a = _lib.KvAttentionDesc(dtype=TYPES[t], batch=batch, seq=seq, q_heads=heads, max_pages=pages, prefix_len=prefix)
+    n = C.c_size_t()
+    assert _lib.lib().nnrh_kv_attention_workspace(C.byref(cache.desc), C.byref(a), C.byref(n)) == 0
+    return n.value
+
+
+# batch, seq, heads, pages a sequence, prefix
+SHAPES = [(32, 1, 32, 8, 4096), (8, 64, 32, 64, 0), (128, 1, 32, 5, 32768), (1, 1024, 32, 128, 0), (1, 1, 32, 4, 0),
+          (3, 3, 16, 20, 600), (64, 1, 8, 100, 0)]
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_attention_workspace_by_type(shape):
+    """A type's own size where it is named, enough for any type where it is not."""
+    cache = nnr_amd.KVCache(1, 8, 128, page_size=64, device="cpu")
+    need = {t: workspace(cache, t, *shape) for t in TYPES}
+    for t in TYPES:
+        assert cache.attention_workspace(*shape, dtype=t) == need[t]
+    assert cache.attention_workspace(*shape) == max(need.values())
+
+
+def test_attention_workspace_differs_by_type():
+    """(the shapes above tell the types apart)"""
+    cache = nnr_amd.KVCache(1, 8, 128, page_size=64, device="cpu")
+    sizes = [[workspace(cache, t, *s) for t in TYPES] for s in SHAPES]
+    assert any(f32 < f16 for f32, f16, _ in sizes) and all(f16 == bf16 for _, f16, bf16 in sizes)
+    with pytest.raises(TypeError):
+        cache.attention_workspace(1, 1, 8, 4, dtype=torch.float64)
