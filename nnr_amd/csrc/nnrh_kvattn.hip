@@ -66,8 +66,8 @@ struct AttnArgs {
     int pre_chunk, own_chunk;      // tiles of a split
     int pre_groups, own_groups;    // row groups: of 16 rows, or of a block's with many
     int page_shift;                // log2(page_size / 32)
-    float* part_o;                 // [rows][slots][hd]
-    float2* part_ml;               // [rows][slots]
+    float* part_o;                 // [rows][slots][hd]: means over a split's keys
+    float2* part_ml;               // [rows][slots]: maximum and total of its weights
 };
 
 // Tables and lengths are read through the scalar cache: a wait for a vector
@@ -596,25 +596,31 @@ __device__ __forceinline__ void few_tile(const AttnArgs& p, Rows<HD, NP, 1>& w, 
         });
 }
 
-// the results of a wave's rows: into the call's result, or among the parts
+// The results of a wave's rows, sums in units of 2^unit: into the call's result,
+// or among the parts. Divided by the total first: a sum of values and weights of
+// up to 2^15 may pass the largest number where their mean does not.
 template <int HD, int NP, int NR>
-__device__ __forceinline__ void put_rows(const AttnArgs& p, const Job& job, int row0, const Rows<HD, NP, NR>& w,
+__device__ __forceinline__ void put_rows(const AttnArgs& p, const Job& job, int row0, const Rows<HD, NP, NR>& w, int unit,
                                          const float* m, const float* l) {
     const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
 #pragma unroll
     for (int t = 0; t < NR; ++t) {
         if (row0 + 16 * t + col >= job.nrows) continue;
         const bool none = m[t] == kNegInf && l[t] == 0.0f;
+        const float inv = none ? 0.0f : 1.0f / l[t];
+        const auto mean = [&](int d) {
+            const f4 o = w.o[t][d] * inv;
+            return f4{ldexpf(o[0], unit), ldexpf(o[1], unit), ldexpf(o[2], unit), ldexpf(o[3], unit)};
+        };
         if (p.slots > 1) {
             const long long at = (long long)w.at[t] * p.slots + job.slot;
             if (g == 0) p.part_ml[at] = float2{m[t], l[t]};
             if (none) continue;
 #pragma unroll
-            for (int d = 0; d < HD / 16; ++d) *(f4*)(p.part_o + at * HD + 16 * d + 4 * g) = w.o[t][d];
+            for (int d = 0; d < HD / 16; ++d) *(f4*)(p.part_o + at * HD + 16 * d + 4 * g) = mean(d);
         } else {
-            const float inv = none ? 0.0f : 1.0f / l[t];
 #pragma unroll
-            for (int d = 0; d < HD / 16; ++d) store_y4(p.a, (long long)w.at[t] * HD + 16 * d + 4 * g, w.o[t][d] * inv);
+            for (int d = 0; d < HD / 16; ++d) store_y4(p.a, (long long)w.at[t] * HD + 16 * d + 4 * g, mean(d));
         }
     }
 }
@@ -648,16 +654,18 @@ __device__ __forceinline__ void few(const AttnArgs& p, Job& job, char* lds) {
     } else {
         clear_rows<BITS>(w);
     }
-    // join the waves: first everyone's maximum, then sums in the units of it
+    // join the waves: first everyone's maximum and unit, then sums in these
     f4(*buf)[ND][64] = (f4(*)[ND][64])lds;                       // [2]
     float(*sm)[16] = (float(*)[16])(lds + 2 * sizeof(*buf));     // [AW]
     float(*sl)[16] = sm + AW;
+    int* su = (int*)(sl + AW);                                   // [AW]
     const float lw = row_total<BITS>(w.l[0]);
     const float top = w.m[0] == kNegInf ? kNegInf : w.m[0] * w.rk[0];   // (rk is not set where there was no tile)
     if (g == 0) {
         sm[wave][col] = top;
         sl[wave][col] = lw;
     }
+    if (lane == 0) su[wave] = w.eu;
     __syncthreads();
     float mall = kNegInf, lall = 0.0f;
 #pragma unroll
@@ -665,7 +673,10 @@ __device__ __forceinline__ void few(const AttnArgs& p, Job& job, char* lds) {
     const float base = mall == kNegInf ? 0.0f : mall;
 #pragma unroll
     for (int v = 0; v < AW; ++v) lall += sl[v][col] * exp2_(sm[v][col] - base);
-    const float f = ldexpf(exp2_(top - base), w.eu);
+    int unit = kNoUnit;
+#pragma unroll
+    for (int v = 0; v < AW; ++v) unit = max(unit, su[v]);
+    const float f = ldexpf(exp2_(top - base), w.eu - unit);
 #pragma unroll
     for (int d = 0; d < ND; ++d) w.o[0][d] *= f;
     if (wave >= 2) {
@@ -686,9 +697,9 @@ __device__ __forceinline__ void few(const AttnArgs& p, Job& job, char* lds) {
     if (wave != 0) return;
 #pragma unroll
     for (int d = 0; d < ND; ++d) w.o[0][d] += buf[0][d][lane];
-    put_rows(p, job, job.row0, w, &mall, &lall);
+    put_rows(p, job, job.row0, w, unit, &mall, &lall);
 }
-template <int HD> constexpr int kFewLds = 2 * (HD / 16) * 1024 + 2 * AW * 64;
+template <int HD> constexpr int kFewLds = 2 * (HD / 16) * 1024 + 2 * AW * 64 + AW * 4;
 
 // ---- many rows: the block's waves split its rows ------------------------------
 // Tiles between two barriers: two, or one where two would not leave enough
@@ -892,11 +903,8 @@ __device__ __forceinline__ void many(const AttnArgs& p, Job& job, char* lds) {
     for (int t = 0; t < NR; ++t) {
         l[t] = row_total<BITS>(w.l[t]);
         m[t] = w.m[t] == kNegInf ? kNegInf : w.m[t] * w.rk[t];
-        const float f = ldexpf(1.0f, w.eu);
-#pragma unroll
-        for (int d = 0; d < HD / 16; ++d) w.o[t][d] *= f;
     }
-    put_rows(p, job, row0, w, m, l);
+    put_rows(p, job, row0, w, w.eu, m, l);
 }
 template <int HD, int BITS> constexpr int kManyLds = 2 * kManyTiles<HD, BITS> * 4 * (HD / 32) * 1024;
 
@@ -957,8 +965,8 @@ __global__ __launch_bounds__(AW * 64, HD <= 128 ? 2 : 1) void kv_attn_kernel(Att
     }
 }
 
-// One wave a row: its partial results joined in a fixed order, several slots
-// side by side where a row is shorter than the wave.
+// One wave a row: the mean of its partial results, by their totals, in a fixed
+// order, several slots side by side where a row is shorter than the wave.
 template <int HD>
 __global__ __launch_bounds__(256) void kv_join_kernel(AttnArgs p) {
     constexpr int L = HD / 4, W = 64 / L;   // lanes of a row, slots at a time
@@ -970,34 +978,36 @@ __global__ __launch_bounds__(256) void kv_join_kernel(AttnArgs p) {
     for (int i = lane; i < p.slots; i += 64) mx = fmaxf(mx, ml[i].x);
     mx = max16_32(max_16(mx));
     const float base = mx == kNegInf ? 0.0f : mx;
-    const int part = lane / L, at = (lane - part * L) * 4;
+    // what a slot counts for; of an empty one (whose mean is not written) nothing
+    const auto weight = [&](float2 v) { return v.x == kNegInf && v.y == 0.0f ? 0.0f : exp2_(v.x - base) * v.y; };
     float total = 0.0f;
+    for (int i = lane; i < p.slots; i += 64) total += weight(ml[i]);
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) total += __shfl_xor(total, o);
+    const bool none = mx == kNegInf && total == 0.0f;
+    const float inv = none ? 0.0f : 1.0f / total;
+    const int part = lane / L, at = (lane - part * L) * 4;
     f4 o = {0, 0, 0, 0};
     if (part < W) {
         const float* src = p.part_o + (long long)row * p.slots * HD + at;
 #pragma unroll 4
         for (int i = part; i < p.slots; i += W) {
             const float2 v = ml[i];
-            const f4 x = *(const f4*)(src + (long long)i * HD);   // (not written where the slot is empty)
+            const f4 x = *(const f4*)(src + (long long)i * HD);
             const bool some = !(v.x == kNegInf && v.y == 0.0f);
-            const float w = some ? exp2_(v.x - base) : 0.0f;
-            total += some ? w * v.y : 0.0f;
+            const float w = weight(v) * inv;
 #pragma unroll
             for (int j = 0; j < 4; ++j) o[j] += some ? x[j] * w : 0.0f;
         }
     }
-    const float total1 = total;
     const f4 o1 = o;
 #pragma unroll
     for (int s = 1; s < W; ++s) {   // into the first lanes, in order
         const int from = (lane % L) + s * L;
-        total += __shfl(total1, from);
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[j] += __shfl(o1[j], from);
     }
     if (part != 0) return;
-    const bool none = mx == kNegInf && total == 0.0f;
-    o *= 1.0f / total;
     store_y4(p.a, (long long)row * HD + at, none ? f4{0, 0, 0, 0} : o);
 }
 

@@ -2,6 +2,8 @@
 import pytest
 import torch
 
+import decode_range_ref as D
+import decode_ref as R
 import nnr_amd
 
 pytestmark = pytest.mark.gpu
@@ -29,3 +31,48 @@ def test_workspace_made_before_the_call(dev, t, typed):
         y = cache.attention(q, td, lens, workspace=buf[:n], **kw)
         assert torch.equal(y, cache.attention(q, td, lens, **kw))
         assert (buf[n:] == 77).all()
+
+
+def run_attention(dev, t, bits, shape, q, k, v, pk, pv, scale=None):
+    """(result, float64's, how far it may be off), each [rows, hd]"""
+    lens, S, H, G, hd, P, per = D.SHAPES[shape]
+    B, n, page = len(lens), max(lens), 32
+    pre = -(-P // page)
+    order = torch.randperm(B * per + pre + 1, generator=torch.Generator().manual_seed(5)).to(torch.int32)
+    td, pt = order[:B * per].reshape(B, per).to(dev), order[B * per:B * per + pre].to(dev)
+    cache = nnr_amd.KVCache(len(order), H, hd, page_size=page, bits=bits)
+    cache.data.fill_(255)
+    ld = torch.tensor(lens, dtype=torch.int32, device=dev)
+    cache.write(k.to(dev), v.to(dev), td, ld)
+    if P:
+        cache.write(pk.to(dev), pv.to(dev), pt[None], torch.tensor([P], dtype=torch.int32, device=dev))
+    y = cache.attention(q.to(dev), td, ld, scale=scale, prefix_table=pt, prefix_len=P).cpu()
+    sc = torch.tensor(hd ** -0.5 if scale is None else scale, dtype=torch.float32).item()
+    out = []
+    for h in range(H):
+        pkx, pvx = (R.quantize(x[0, :, h], bits)[0] for x in (pk, pv))
+        for b in range(B):
+            kx = torch.cat((pkx, R.quantize(k[b, n - lens[b]:, h], bits)[0]))
+            vx = torch.cat((pvx, R.quantize(v[b, n - lens[b]:, h], bits)[0]))
+            vis = [P + max(0, lens[b] - S + s + 1) for s in range(S)]
+            ref, tol = D.attention(q[b, :, h * G:(h + 1) * G], kx, vx, sc, vis, bits)
+            out.append([x.reshape(-1, hd) for x in (y[b, :, h * G:(h + 1) * G].double(), ref, tol)])
+    return [torch.cat(x) for x in zip(*out)]
+
+
+@pytest.mark.parametrize("shape", list(D.SHAPES))
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("bits", [8, 4])
+def test_attention_large_values(dev, t, bits, shape):
+    """Results that fit their type, of values next to its largest number"""
+    lens, S, H, G, hd, P, _ = D.SHAPES[shape]
+    top = {torch.float32: 3e38, torch.float16: 6e4, torch.bfloat16: 3e38}[t]
+    g = torch.Generator().manual_seed(1)
+    r = lambda *s: torch.rand(s, generator=g, dtype=torch.float64) * 2 - 1
+    q, k, pk = r(len(lens), S, H * G, hd), r(len(lens), max(lens), H, hd), r(1, P, H, hd)
+    v, pv = r(len(lens), max(lens), H, hd) * top, r(1, P, H, hd) * top
+    # (a token's largest element stands for up to 2^-8 more than it is)
+    v, pv = v.clamp(-0.95 * top, 0.95 * top), pv.clamp(-0.95 * top, 0.95 * top)
+    y, ref, tol = run_attention(dev, t, bits, shape, *(x.to(t) for x in (q, k, v, pk, pv)))
+    assert torch.isfinite(y).all()
+    assert ((y - ref).abs() <= tol).all(), ((y - ref).abs() / tol).max()
