@@ -657,6 +657,12 @@ int nnrh_kv_cache_read(const nnrh_kv_cache_desc* c, const void* cache_dev, const
  *   positions 0 .. seq_lens[b] - seq + s of its own sequence,
  * with key/value head h / (q_heads / kv_heads):
  *   y = sum_j softmax_j(scale q k_j) v_j.   A query that sees no key gives 0.
+ * Sums are fp32. The softmax's weights meet the values with 11 bits (as they
+ * would in an fp16 tensor), and for fp32 tensors with 22, as do their queries.
+ * Rows for which scales lie too far apart for the matrix instructions (4 bits: a
+ * group's 2^17 below another's of the same split; 8 bits: values 2^12 above all
+ * that the row looks at; keys' of 2^64 and more) are computed again in fp32:
+ * right as well, and some 50 times as slow.
  * q: [batch][seq][q_heads][head_dim], strides as above; y dense, 16-byte
  * aligned; y may be q itself where q is dense, and must not overlap it
  * otherwise. Zero, one or several tokens a sequence, in any mixture of

@@ -15,11 +15,18 @@
 // pieces, 22 bits and more. Weights p = exp(s - max) enter as 2^11 p, where
 // max may be one that up to 2^4 outgrow, or for fp32 tensors as 2^15 p in two
 // pieces; with them, at 8 bits, the values' scales over their largest power of
-// two so far: 11 significant bits (22) over 35 binary orders and more. At 4
-// bits scale (8 bits) times code (3 bits) is exact in fp16 and is formed in
-// the operand, over the largest power of two so far as well (eu for values, ek
-// for keys: the units, which sums and scores follow when they move). Sums,
-// maxima and the running total are fp32.
+// two so far. That rounds a weight to 11 bits (22): a 16-bit result is rounded to as
+// many or fewer, and a second piece would be a second product. At 4 bits scale
+// (8 bits) times code (3 bits) is formed in the operand, over the largest power of
+// two so far as well (eu for values, ek for keys: the units, which sums and scores
+// follow when they move). Sums, maxima and the running total are fp32.
+//
+// A unit serves all of a block's rows, tokens and groups, so what is far below it
+// would lose its bits, though a row may see nothing else. Such rows are computed
+// again in fp32 (slow_rows): at 4 bits all of a block's where a scale is under
+// 2^-17 of the unit, beyond which it and its products are no longer exact; at 8
+// bits those whose largest weight times scale is under 2^-12 of it (2^-16 in two
+// pieces), where fp16's least step would count for more than an fp32 sum's.
 //
 // Up to 16 rows (few): the block's waves take tiles in turn, operands go from
 // memory to registers, and a tile's registers are asked for again as soon as
@@ -54,6 +61,15 @@ constexpr int AW = 4;              // waves of a block
 // the sums of 32 rows is then rare instead of usual.
 constexpr float kTop = 15.0f, kSlack = 4.0f;
 constexpr int kNoUnit = -126;      // the least unit of scales (they are 0 or normal)
+// What the products carry; rows beyond it are computed again (slow_rows). A 4-bit
+// scale has 8 bits: it and its products with codes are fp16 numbers down to 2^-17
+// of the unit. A weight of 8 bits has an fp16 step of 2^-24 whatever its size,
+// half of which is 2^-24 of the row's largest where that is 2^-1, an fp32 sum's
+// rounding. Raw scores of 8 bits fit fp32 up to scales of 2^64, with room for the
+// least factor below.
+constexpr int kFarScale = 17;
+constexpr float kFarWeight = 0.5f;
+constexpr uint32_t kLargeScale = (127 + 64) << 7;   // as bf16
 constexpr float kLeast = 1e-37f;   // a factor of 0 would make NaN of a masked score, -inf
 constexpr float kNegInf = -__builtin_inff();
 
@@ -116,6 +132,46 @@ __device__ __forceinline__ uint32_t umax_16(uint32_t u) {
 __device__ __forceinline__ int ceil_exp(uint32_t bf16, int none) {
     return bf16 ? (int)((bf16 + 0x7fu) >> 7) - 127 : none;
 }
+typedef uint16_t us2 __attribute__((ext_vector_type(2)));
+typedef int16_t ss2 __attribute__((ext_vector_type(2)));
+// the larger of two pairs of bf16 scales, as bits
+__device__ __forceinline__ uint32_t pair_max(uint32_t a, uint32_t b) {
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(us2, a), __builtin_bit_cast(us2, b)));
+}
+__device__ __forceinline__ uint32_t half_max(uint32_t a) { return umax(a & 0xffffu, a >> 16); }
+
+// What is kept of the scales that a wave has seen, to know whether the products
+// carried them: at 4 bits the least of keys and values (0 aside), at 8 the
+// largest of keys, pairs a lane. (As signed numbers: memory that no token was
+// written to may hold a sign.)
+template <int BITS> struct Seen;
+template <> struct Seen<8> {
+    uint32_t k = 0;
+    __device__ __forceinline__ void add(u4 w) {
+        const auto m = [](uint32_t a, uint32_t b) {
+            return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(ss2, a), __builtin_bit_cast(ss2, b)));
+        };
+        k = m(k, m(m(w[0], w[1]), m(w[2], w[3])));
+    }
+    __device__ __forceinline__ bool far(int, int) const { return half_max(k) >= kLargeScale; }
+};
+template <> struct Seen<4> {
+    uint32_t k = 0xffffffffu, v = 0xffffffffu;   // of bits less 1, where 0 is the largest
+    __device__ __forceinline__ static uint32_t least(uint32_t a, uint32_t w) {
+        return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(us2, a), __builtin_bit_cast(us2, w) - us2{1, 1}));
+    }
+    __device__ __forceinline__ void add_k(uint32_t w) { k = least(k, w); }
+    __device__ __forceinline__ void add_v(u2 w) { v = least(least(v, w[0]), w[1]); }
+    __device__ __forceinline__ void add(u2 wk, u2 wv) {
+        add_k(wk[0]);
+        add_k(wk[1]);
+        add_v(wv);
+    }
+    __device__ __forceinline__ static bool below(uint32_t a, int unit) {
+        return min(a & 0xffffu, a >> 16) < (uint32_t)(max(unit - kFarScale + 127, 1) << 7) - 1;
+    }
+    __device__ __forceinline__ bool far(int ek, int eu) const { return below(k, ek) || below(v, eu); }
+};
 // keeps the compiler from computing both sides of a branch that a tile hardly ever takes
 __device__ __forceinline__ void stay_a_branch() { asm volatile(""); }
 
@@ -192,6 +248,7 @@ template <int HD, int NP, int NR> struct Rows {
     f4 l[NR];
     f4 o[NR][ND];       // sums of kTop p v in units of 2^eu
     int eu;
+    float x[NR];        // 8 bits: the largest weight with its value's scale so far, this lane's
     int lim[NR];        // keys that the row sees
     int at[NR];         // its place among all rows
     int lo, hi;         // least and largest limit of the wave's rows
@@ -244,6 +301,7 @@ __device__ __forceinline__ void clear_rows(Rows<HD, NP, NR>& w) {
     for (int t = 0; t < NR; ++t) {
         w.m[t] = kNegInf;
         w.l[t] = f4{0, 0, 0, 0};
+        w.x[t] = 0.0f;
 #pragma unroll
         for (int d = 0; d < HD / 16; ++d) w.o[t][d] = f4{0, 0, 0, 0};
     }
@@ -382,6 +440,7 @@ __device__ __forceinline__ void tile_step(Rows<HD, NP, NR>& w, int key0, const i
             w.m[t] = m;
             w.l[t] *= al;
             const float f = ldexpf(al, w.eu - en);
+            if constexpr (BITS == 8) w.x[t] *= f;
 #pragma unroll
             for (int d = 0; d < ND; ++d) w.o[t][d] *= f;
         }
@@ -415,6 +474,7 @@ __device__ __forceinline__ void tile_step(Rows<HD, NP, NR>& w, int key0, const i
 #pragma unroll
             for (int t = 0; t < NR; ++t) {
                 const float x = BITS == 8 ? s[t][z][j] * vu : s[t][z][j];
+                if constexpr (BITS == 8) w.x[t] = fmaxf(w.x[t], x);
                 const _Float16 h = (_Float16)x;
                 pf[0][t][j] = h;
                 if constexpr (NP == 2) pf[1][t][j] = (_Float16)(x - (float)h);
@@ -479,27 +539,42 @@ __device__ __forceinline__ u4 held_scales(u4 w, int held) {
     return w;
 }
 // the largest of a lane's 8 scales, as bits of bf16
-__device__ __forceinline__ uint32_t top8(u4 w) {
-    typedef uint16_t us2 __attribute__((ext_vector_type(2)));
-    const auto m = [](uint32_t a, uint32_t b) {
-        return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(us2, a), __builtin_bit_cast(us2, b)));
-    };
-    const uint32_t x = m(m(w[0], w[1]), m(w[2], w[3]));
-    return umax(x & 0xffffu, x >> 16);
+__device__ __forceinline__ uint32_t top8(u4 w) { return half_max(pair_max(pair_max(w[0], w[1]), pair_max(w[2], w[3]))); }
+// Scales of a tile, all groups', 4 a lane (4 bits): those of keys or of values
+__device__ __forceinline__ u2 all_scales(const uint16_t* first, int page, int groups) {
+    const int lane = threadIdx.x & 63, grp = lane >> 3 < groups ? lane >> 3 : 0;
+    return *(const u2*)(first + grp * page + (lane & 7) * 4);
 }
-// scales of keys col and col + 16 (4 bits), as floats' bits; 0 past `held`
-__device__ __forceinline__ void held_pair(uint32_t w, int held, uint32_t* s) {
-    s[0] = w << 16;
-    s[1] = w & 0xffff0000u;
+// without what the tile's tokens do not hold
+__device__ __forceinline__ u2 of_tokens(u2 w, int held, bool key) {
+    if (held < 32) {
+        stay_a_branch();
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int slot = (lane & 7) * 4 + q;
+            const int tok = key ? (slot >> 1) + 16 * (slot & 1) : 16 * ((slot >> 2) & 1) + 4 * (slot >> 3) + (slot & 3);
+            if (tok >= held) w[q >> 1] &= q & 1 ? 0xffffu : 0xffff0000u;
+        }
+    }
+    return w;
+}
+// the unit of a tile's scales, at least `unit`
+__device__ __forceinline__ int unit_of(uint32_t pairs, int unit) {
+    return max(unit, ceil_exp(__builtin_amdgcn_readfirstlane(umax16_32(umax_16(half_max(pairs)))), kNoUnit));
+}
+// the pair of scales of keys col and col + 16 (4 bits); 0 past `held`
+__device__ __forceinline__ uint32_t held_pair(uint32_t w, int held) {
     if (held < 32) {
         stay_a_branch();
         const int col = threadIdx.x & 15;
-        if (col >= held) s[0] = 0;
-        if (col + 16 >= held) s[1] = 0;
+        if (col >= held) w &= 0xffff0000u;
+        if (col + 16 >= held) w &= 0xffffu;
     }
+    return w;
 }
-__device__ __forceinline__ h8 key4(uint32_t codes, uint32_t scale, float unit) {
-    const _Float16 x = (_Float16)(__builtin_bit_cast(float, scale) * unit);
+__device__ __forceinline__ h8 key4(uint32_t codes, float scale, float unit) {
+    const _Float16 x = (_Float16)(scale * unit);
     Scale4 s;
     s.set(x, x);
     return codes4(codes, s, s, s, s);
@@ -523,13 +598,16 @@ template <int HD, int BITS> struct RawTile {
     u4 vs[BITS == 8 ? 1 : NC];
     u4 ks;                        // 8 bits
     uint32_t ks4[NC];             // 4 bits
+    u2 all_v;                     // 4 bits: the values', 4 a lane
     __device__ __forceinline__ void load_keys(const AttnArgs& p, const TilePtr& t) {
         constexpr int BB = BITS == 8 ? 1024 : 512;
         const int lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
-        if constexpr (BITS == 8) ks = *(const u4*)(t.scales + 8 * g);
-        else
+        if constexpr (BITS == 8) {
+            ks = *(const u4*)(t.scales + 8 * g);
+        } else {
 #pragma unroll
             for (int c = 0; c < NC; ++c) ks4[c] = *(const uint32_t*)(t.scales + c * p.c.page_size + 2 * col);
+        }
 #pragma unroll
         for (int c = 0; c < NC; ++c) k[c] = *(const vec*)(t.codes + c * BB + lane * sizeof(vec));
     }
@@ -538,6 +616,7 @@ template <int HD, int BITS> struct RawTile {
         const int lane = threadIdx.x & 63, g = lane >> 4;
         const uint8_t* vc = t.codes + kv_codes_bytes(p.c.page_size, HD, BITS);
         const uint16_t* vsp = t.scales + (long long)p.c.page_size * kv_groups(HD, BITS);
+        if constexpr (BITS == 4) all_v = all_scales(vsp, p.c.page_size, NC);
 #pragma unroll
         for (int c = 0; c < (BITS == 8 ? 1 : NC); ++c) vs[c] = *(const u4*)(vsp + c * p.c.page_size + 8 * g);
 #pragma unroll
@@ -547,35 +626,37 @@ template <int HD, int BITS> struct RawTile {
 
 // next: the tile to load meanwhile
 template <int HD, int BITS, int NP>
-__device__ __forceinline__ void few_tile(const AttnArgs& p, Rows<HD, NP, 1>& w, RawTile<HD, BITS>& r, int tile, int held,
-                                         const TilePtr& next) {
+__device__ __forceinline__ void few_tile(const AttnArgs& p, Rows<HD, NP, 1>& w, Seen<BITS>& scales, RawTile<HD, BITS>& r,
+                                         int tile, int held, const TilePtr& next) {
     constexpr int NC = HD / 32;
     u4 vs[BITS == 8 ? 1 : NC];
-    uint32_t vtop = 0;
 #pragma unroll
-    for (int c = 0; c < (BITS == 8 ? 1 : NC); ++c) {
-        vs[c] = held_scales(r.vs[c], held);
-        vtop = umax(vtop, top8(vs[c]));
-    }
-    const int en = max(w.eu, ceil_exp(__builtin_amdgcn_readfirstlane(umax16_32(vtop)), kNoUnit));
-    int ek = 0;
+    for (int c = 0; c < (BITS == 8 ? 1 : NC); ++c) vs[c] = held_scales(r.vs[c], held);
+    int ek = 0, en;
     const u4 ks = r.ks;
-    uint32_t kb[NC][2];
+    uint32_t kb[NC];
     if constexpr (BITS == 4) {
+        const u2 v = of_tokens(r.all_v, held, false);
+        scales.add_v(v);
         uint32_t top = 0;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            held_pair(r.ks4[c], held, kb[c]);
-            top = umax(top, umax(kb[c][0], kb[c][1]));
+            kb[c] = held_pair(r.ks4[c], held);
+            scales.add_k(kb[c]);
+            top = pair_max(top, kb[c]);
         }
-        ek = max(w.ek, ceil_exp(__builtin_amdgcn_readfirstlane(umax_16(top) >> 16), kNoUnit));
+        ek = max(w.ek, ceil_exp(__builtin_amdgcn_readfirstlane(umax_16(half_max(top))), kNoUnit));
+        en = unit_of(pair_max(v[0], v[1]), w.eu);
+    } else {
+        scales.add(ks);
+        en = max(w.eu, ceil_exp(__builtin_amdgcn_readfirstlane(umax16_32(top8(vs[0]))), kNoUnit));
     }
     const float fk = ldexpf(1.0f, -ek), fv = ldexpf(1.0f, -en);
     tile_step<HD, BITS, NP, 1, 1>(
         w, tile * 32, &held, held < 32, &ks, vs, ek, en,
         [&](int, int j) {
             if constexpr (BITS == 8) return codes8(r.k[j >> 1][2 * (j & 1)], r.k[j >> 1][2 * (j & 1) + 1]);
-            else return key4(r.k[j >> 1][j & 1], kb[j >> 1][j & 1], fk);
+            else return key4(r.k[j >> 1][j & 1], j & 1 ? bf16_hi(kb[j >> 1]) : bf16_lo(kb[j >> 1]), fk);
         },
         [&](int, int j) {
             if constexpr (BITS == 8) {
@@ -598,14 +679,15 @@ __device__ __forceinline__ void few_tile(const AttnArgs& p, Rows<HD, NP, 1>& w, 
 
 // The results of a wave's rows, sums in units of 2^unit: into the call's result,
 // or among the parts. Divided by the total first: a sum of values and weights of
-// up to 2^15 may pass the largest number where their mean does not.
+// up to 2^15 may pass the largest number where their mean does not. Not those
+// that are computed again.
 template <int HD, int NP, int NR>
 __device__ __forceinline__ void put_rows(const AttnArgs& p, const Job& job, int row0, const Rows<HD, NP, NR>& w, int unit,
-                                         const float* m, const float* l) {
+                                         const float* m, const float* l, const bool* again) {
     const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
 #pragma unroll
     for (int t = 0; t < NR; ++t) {
-        if (row0 + 16 * t + col >= job.nrows) continue;
+        if (row0 + 16 * t + col >= job.nrows || again[t]) continue;
         const bool none = m[t] == kNegInf && l[t] == 0.0f;
         const float inv = none ? 0.0f : 1.0f / l[t];
         const auto mean = [&](int d) {
@@ -625,6 +707,110 @@ __device__ __forceinline__ void put_rows(const AttnArgs& p, const Job& job, int 
     }
 }
 
+// ---- rows that the products do not carry --------------------------------------
+// One row by one wave in fp32, from the codes: a lane scores half of a key's
+// elements, and holds elements 64 apart of the result, the mean so far. As near
+// to a sum in fp32 as that comes whatever the sizes of queries, keys and values,
+// and some 50 times as slow as the products.
+template <int HD, int BITS, int NP>
+__device__ __forceinline__ void slow_row(const AttnArgs& p, const Job& job, int row, int lim) {
+    constexpr int NC = HD / 32, BB = BITS == 8 ? 1024 : 512, NE = (HD + 63) / 64;
+    const KvAttention& a = p.a;
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));   // nothing of this path in registers before it
+    const int tok = lane & 31, half = lane >> 5;
+    const int bt = row / a.q_heads, hq = row - bt * a.q_heads, bq = bt / a.seq;
+    const long long q0 = (long long)bq * a.q_bstride + (long long)(bt - bq * a.seq) * a.q_tstride + (long long)hq * HD;
+    const long long vcodes = kv_codes_bytes(p.c.page_size, HD, BITS), vscales = (long long)p.c.page_size * kv_groups(HD, BITS);
+    float m = kNegInf, l = 0.0f, y[NE];
+#pragma unroll
+    for (int i = 0; i < NE; ++i) y[i] = 0.0f;
+    const int t1 = min(job.t1, (lim + 31) / 32);
+    for (int tile = job.t0; tile < t1; ++tile) {
+        const TilePtr t = tile_ptr<HD, BITS>(p, job.head, page_id(job, p, tile), tile);
+        if (!t.ok) continue;
+        const int seen = min(lim - 32 * tile, 32);   // (a row's limit is within what the source holds)
+        float s = 0.0f;
+#pragma unroll 1
+        for (int c = 0; c < NC; ++c) {
+            const uint32_t sb = t.scales[BITS == 8 ? kv_slot(tok) : c * p.c.page_size + kv_pair(tok)];
+            const float scale = bf16_lo(sb);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int oct = 2 * half + i;
+                const uint8_t* from = t.codes + c * BB + ((tok & 15) + 16 * oct) * (BITS == 8 ? 16 : 8) + (tok >> 4) * (BITS == 8 ? 8 : 4);
+                float q[8];
+                load_q8(a, q0 + 32 * c + 8 * oct, q);
+                u2 w = {0, 0};
+                if constexpr (BITS == 8) w = *(const u2*)from;
+                else w[0] = kv_unturn(*(const uint32_t*)from);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int code = BITS == 8 ? (int)((w[j >> 2] >> (8 * (j & 3))) & 255u) - 128
+                                               : (int)((w[0] >> (4 * ((j >> 1) + 4 * (j & 1)))) & 15u) - 8;
+                    s = __builtin_fmaf(q[j] * a.scale, (float)code * scale, s);
+                }
+            }
+        }
+        s = (s + __shfl_xor(s, 32)) * 1.44269504088896341f;
+        if (tok >= seen) s = kNegInf;
+        const float top = fmaxf(m, max16_32(max_16(s)));
+        const float base = top == kNegInf ? 0.0f : top;
+        const float w = exp2_(s - base);
+        float sum = tok >= seen || half ? 0.0f : w;
+#pragma unroll
+        for (int o = 1; o < 64; o *= 2) sum += __shfl_xor(sum, o);
+        const float old = l * exp2_(m - base);
+        l = old + sum;
+        m = top;
+        const float inv = 1.0f / l;
+#pragma unroll
+        for (int i = 0; i < NE; ++i) y[i] *= old * inv;
+#pragma unroll 1
+        for (int k = 0; k < seen; ++k) {
+            const float wk = __shfl(w, k) * inv;
+            const int slot = kv_slot(k);
+#pragma unroll
+            for (int i = 0; i < NE; ++i) {
+                const int e = min(lane + 64 * i, HD - 1), c = e >> 5;
+                const float scale = bf16_lo(t.scales[vscales + (BITS == 8 ? 0 : c * p.c.page_size) + slot]);
+                const uint8_t* from = t.codes + vcodes + c * BB + ((e & 15) + 16 * (slot >> 3)) * (BITS == 8 ? 16 : 8) +
+                                      ((e >> 4) & 1) * (BITS == 8 ? 8 : 4);
+                int code;
+                if constexpr (BITS == 8) code = (int)from[slot & 7] - 128;
+                else code = (int)((kv_unturn(*(const uint32_t*)from) >> (4 * (((slot & 7) >> 1) + 4 * (slot & 1)))) & 15u) - 8;
+                y[i] = __builtin_fmaf(wk, (float)code * scale, y[i]);
+            }
+        }
+    }
+    // as the products leave it: totals are of weights with their largest at 2^top
+    constexpr float unit = NP == 1 ? kTop - kSlack : kTop;
+    const long long part = (long long)row * p.slots + job.slot;
+    if (p.slots > 1 && lane == 0) p.part_ml[part] = float2{m, ldexpf(l, (int)unit)};
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+        const int e = lane + 64 * i;
+        if (HD % 64 && e >= HD) break;
+        if (p.slots > 1) p.part_o[part * HD + e] = y[i];
+        else if (a.type == FT_F32) ((float*)a.y)[(long long)row * HD + e] = y[i];
+        else if (a.type == FT_F16) ((_Float16*)a.y)[(long long)row * HD + e] = (_Float16)y[i];
+        else ((__bf16*)a.y)[(long long)row * HD + e] = (__bf16)y[i];
+    }
+}
+// of 16 rows (one a lane of the first group) those that are asked for, every `of`th from `first` on
+template <int HD, int BITS, int NP>
+__device__ __forceinline__ void slow_rows(const Job& job, int at, int lim, bool again, int first, int of) {
+    const uint32_t todo = (uint32_t)__ballot(again) & 0xffffu;
+    if (!todo) return;
+    // (read anew from the kernel's arguments, its only ones, so that none of them stay in registers for this path)
+    uintptr_t args = (uintptr_t)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(args));
+    const AttnArgs& p = *(const AttnArgs*)args;
+#pragma unroll 1
+    for (int i = first; i < 16; i += of)
+        if (todo >> i & 1) slow_row<HD, BITS, NP>(p, job, __builtin_amdgcn_readlane(at, i), __builtin_amdgcn_readlane(lim, i));
+}
+
 template <int HD, int BITS, int NP>
 __device__ __forceinline__ void few(const AttnArgs& p, Job& job, char* lds) {
     constexpr int ND = HD / 16;
@@ -634,6 +820,7 @@ __device__ __forceinline__ void few(const AttnArgs& p, Job& job, char* lds) {
     set_rows(p, job, job.row0, w);
     job.t1 = min(job.t1, (w.hi + 31) / 32);
     int tile = job.t0 + wave;
+    Seen<BITS> scales;
     RawTile<HD, BITS> raw;
     // (past the last tile its own are loaded again, for nothing)
     const auto at = [&](int x) {
@@ -647,7 +834,7 @@ __device__ __forceinline__ void few(const AttnArgs& p, Job& job, char* lds) {
         load_rows<BITS>(p, w);
         for (; tile < job.t1; tile += AW) {
             const TilePtr after = at(tile + 2 * AW);
-            few_tile<HD, BITS, NP>(p, w, raw, tile, cur.ok ? (int)min(job.len - (long long)tile * 32, 32ll) : 0, next);
+            few_tile<HD, BITS, NP>(p, w, scales, raw, tile, cur.ok ? (int)min(job.len - (long long)tile * 32, 32ll) : 0, next);
             cur = next;
             next = after;
         }
@@ -658,14 +845,21 @@ __device__ __forceinline__ void few(const AttnArgs& p, Job& job, char* lds) {
     f4(*buf)[ND][64] = (f4(*)[ND][64])lds;                       // [2]
     float(*sm)[16] = (float(*)[16])(lds + 2 * sizeof(*buf));     // [AW]
     float(*sl)[16] = sm + AW;
-    int* su = (int*)(sl + AW);                                   // [AW]
+    float(*sx)[16] = sl + AW;
+    float(*sf)[16] = sx + AW;
+    int* su = (int*)(sf + AW);                                   // [AW]
+    int* sfar = su + AW;
     const float lw = row_total<BITS>(w.l[0]);
     const float top = w.m[0] == kNegInf ? kNegInf : w.m[0] * w.rk[0];   // (rk is not set where there was no tile)
     if (g == 0) {
         sm[wave][col] = top;
         sl[wave][col] = lw;
     }
-    if (lane == 0) su[wave] = w.eu;
+    const bool wave_far = __any(scales.far(w.ek, w.eu));
+    if (lane == 0) {
+        su[wave] = w.eu;
+        sfar[wave] = wave_far;
+    }
     __syncthreads();
     float mall = kNegInf, lall = 0.0f;
 #pragma unroll
@@ -674,9 +868,20 @@ __device__ __forceinline__ void few(const AttnArgs& p, Job& job, char* lds) {
 #pragma unroll
     for (int v = 0; v < AW; ++v) lall += sl[v][col] * exp2_(sm[v][col] - base);
     int unit = kNoUnit;
+    bool again = false;
 #pragma unroll
-    for (int v = 0; v < AW; ++v) unit = max(unit, su[v]);
+    for (int v = 0; v < AW; ++v) {
+        unit = max(unit, su[v]);
+        again |= sfar[v] != 0;
+    }
     const float f = ldexpf(exp2_(top - base), w.eu - unit);
+    if constexpr (BITS == 8) {
+        const float x = max16_32(w.x[0]) * f;
+        if (g == 0) {
+            sx[wave][col] = x;
+            sf[wave][col] = f;
+        }
+    }
 #pragma unroll
     for (int d = 0; d < ND; ++d) w.o[0][d] *= f;
     if (wave >= 2) {
@@ -684,6 +889,15 @@ __device__ __forceinline__ void few(const AttnArgs& p, Job& job, char* lds) {
         for (int d = 0; d < ND; ++d) buf[wave - 2][d][lane] = w.o[0][d];
     }
     __syncthreads();
+    if constexpr (BITS == 8) {   // of all waves: the largest weight against the largest step
+        float x = 0.0f, step = 0.0f;
+#pragma unroll
+        for (int v = 0; v < AW; ++v) {
+            x = fmaxf(x, sx[v][col]);
+            step = fmaxf(step, sf[v][col]);
+        }
+        again |= x < kFarWeight * step && unit != kNoUnit && lall > 0.0f;
+    }
     if (wave < 2) {
 #pragma unroll
         for (int d = 0; d < ND; ++d) w.o[0][d] += buf[wave][d][lane];
@@ -694,12 +908,14 @@ __device__ __forceinline__ void few(const AttnArgs& p, Job& job, char* lds) {
         for (int d = 0; d < ND; ++d) buf[0][d][lane] = w.o[0][d];
     }
     __syncthreads();
-    if (wave != 0) return;
+    if (wave == 0) {
 #pragma unroll
-    for (int d = 0; d < ND; ++d) w.o[0][d] += buf[0][d][lane];
-    put_rows(p, job, job.row0, w, unit, &mall, &lall);
+        for (int d = 0; d < ND; ++d) w.o[0][d] += buf[0][d][lane];
+        put_rows(p, job, job.row0, w, unit, &mall, &lall, &again);
+    }
+    slow_rows<HD, BITS, NP>(job, w.at[0], w.lim[0], again && job.row0 + col < job.nrows, wave, AW);
 }
-template <int HD> constexpr int kFewLds = 2 * (HD / 16) * 1024 + 2 * AW * 64 + AW * 4;
+template <int HD> constexpr int kFewLds = 2 * (HD / 16) * 1024 + 4 * AW * 64 + 2 * AW * 4;
 
 // ---- many rows: the block's waves split its rows ------------------------------
 // Tiles between two barriers: two, or one where two would not leave enough
@@ -748,25 +964,9 @@ template <int HD, int BITS> struct Parts {
             ks = *(const u4*)(t.scales + 8 * g);
             vs = *(const u4*)(vsp + 8 * g);
         } else {
-            const int grp = lane >> 3 < NC ? lane >> 3 : 0;
-            all_k = *(const u2*)(t.scales + grp * p.c.page_size + (lane & 7) * 4);
-            all_v = *(const u2*)(vsp + grp * p.c.page_size + (lane & 7) * 4);
+            all_k = all_scales(t.scales, p.c.page_size, NC);
+            all_v = all_scales(vsp, p.c.page_size, NC);
         }
-    }
-    // largest scale of a tile's tokens, from all_k or all_v, as bits of bf16
-    __device__ __forceinline__ static uint32_t top(u2 w, int held, bool key) {
-        const int lane = threadIdx.x & 63;
-        uint32_t f[4] = {w[0] & 0xffffu, w[0] >> 16, w[1] & 0xffffu, w[1] >> 16};
-        if (held < 32) {
-            stay_a_branch();
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int slot = (lane & 7) * 4 + q;
-                const int tok = key ? (slot >> 1) + 16 * (slot & 1) : 16 * ((slot >> 2) & 1) + 4 * (slot >> 3) + (slot & 3);
-                if (tok >= held) f[q] = 0;
-            }
-        }
-        return umax(umax(f[0], f[1]), umax(f[2], f[3]));
     }
 };
 
@@ -793,6 +993,7 @@ __device__ __forceinline__ void many(const AttnArgs& p, Job& job, char* lds) {
     Parts<HD, BITS> raw[KT] = {};
     int id[KT], held[KT], held_next[KT], ek = kNoUnit, ek_next = kNoUnit, en = kNoUnit, en_next = kNoUnit;
     u4 ks_next[KT], vs_next[KT];   // 8 bits
+    Seen<BITS> scales;
     auto ids = [&](int tile) {
 #pragma unroll
         for (int z = 0; z < KT; ++z) id[z] = tile + z < job.t1 ? page_id(job, p, tile + z) : -1;
@@ -812,15 +1013,21 @@ __device__ __forceinline__ void many(const AttnArgs& p, Job& job, char* lds) {
         }
         if constexpr (BITS == 4) {
             uint32_t tk = 0, tv = 0;
+            u2 k[KT], v[KT];
 #pragma unroll
             for (int z = 0; z < KT; ++z) {
-                tk = umax(tk, raw[z].top(raw[z].all_k, held_next[z], true));
-                tv = umax(tv, raw[z].top(raw[z].all_v, held_next[z], false));
+                k[z] = of_tokens(raw[z].all_k, held_next[z], true);
+                v[z] = of_tokens(raw[z].all_v, held_next[z], false);
+                tk = pair_max(tk, pair_max(k[z][0], k[z][1]));
+                tv = pair_max(tv, pair_max(v[z][0], v[z][1]));
             }
-            tk = __builtin_amdgcn_readfirstlane(umax16_32(umax_16(tk)));
-            tv = __builtin_amdgcn_readfirstlane(umax16_32(umax_16(tv)));
-            ek_next = max(ek_next, ceil_exp(tk, kNoUnit));
-            en_next = max(en_next, ceil_exp(tv, kNoUnit));
+            ek_next = unit_of(tk, ek_next);
+            en_next = unit_of(tv, en_next);
+            if ((tile / KT) % AW == wave) {   // (one wave of the block is enough)
+                stay_a_branch();
+#pragma unroll
+                for (int z = 0; z < KT; ++z) scales.add(k[z], v[z]);
+            }
             fk = ldexpf(1.0f, -ek_next);
             fv = ldexpf(1.0f, -en_next);
         }
@@ -835,10 +1042,9 @@ __device__ __forceinline__ void many(const AttnArgs& p, Job& job, char* lds) {
 #pragma unroll
                     for (int i = 0; i < 2; ++i) to[64 * i] = codes8(raw[z].code[u][2 * i], raw[z].code[u][2 * i + 1]);
                 } else if (Parts<HD, BITS>::keys(u, b)) {
-                    uint32_t s[2];
-                    held_pair(raw[z].sc[u][0], held_next[z], s);
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) to[64 * i] = key4(raw[z].code[u][i], s[i], fk);
+                    const uint32_t s = held_pair(raw[z].sc[u][0], held_next[z]);
+                    to[0] = key4(raw[z].code[u][0], bf16_lo(s), fk);
+                    to[64] = key4(raw[z].code[u][1], bf16_hi(s), fk);
                 } else {
                     Scale4 s[4];
                     value_scales(held_scales(raw[z].sc[u], held_next[z]), fv, s);
@@ -880,6 +1086,11 @@ __device__ __forceinline__ void many(const AttnArgs& p, Job& job, char* lds) {
                 vs_raw[z] = held_scales(vs_raw[z], held[z]);
                 vtop = umax(vtop, top8(vs_raw[z]));
             }
+            if ((tile / KT) % AW == wave) {
+                stay_a_branch();
+#pragma unroll
+                for (int z = 0; z < KT; ++z) scales.add(ks_raw[z]);
+            }
             ek = 0;
             en = max(w.eu, ceil_exp(__builtin_amdgcn_readfirstlane(umax16_32(vtop)), kNoUnit));
         }
@@ -897,14 +1108,26 @@ __device__ __forceinline__ void many(const AttnArgs& p, Job& job, char* lds) {
             [] {});
         __syncthreads();
     }
+    int* sfar = (int*)lds;   // (past the loop's last barrier)
+    const bool wave_far = __any(scales.far(w.ek, w.eu));
+    if (lane == 0) sfar[wave] = wave_far;
+    __syncthreads();
+    bool any_far = false;
+#pragma unroll
+    for (int v = 0; v < AW; ++v) any_far |= sfar[v] != 0;
     if (row0 >= job.nrows) return;
     float m[NR], l[NR];
+    bool again[NR];
 #pragma unroll
     for (int t = 0; t < NR; ++t) {
         l[t] = row_total<BITS>(w.l[t]);
         m[t] = w.m[t] == kNegInf ? kNegInf : w.m[t] * w.rk[t];
+        again[t] = any_far || (BITS == 8 && max16_32(w.x[t]) < kFarWeight && w.eu != kNoUnit && l[t] > 0.0f);
     }
-    put_rows(p, job, row0, w, w.eu, m, l);
+    put_rows(p, job, row0, w, w.eu, m, l, again);
+#pragma unroll
+    for (int t = 0; t < NR; ++t)
+        slow_rows<HD, BITS, NP>(job, w.at[t], w.lim[t], again[t] && row0 + 16 * t + col < job.nrows, 0, 1);
 }
 template <int HD, int BITS> constexpr int kManyLds = 2 * kManyTiles<HD, BITS> * 4 * (HD / 32) * 1024;
 
@@ -915,7 +1138,7 @@ template <int HD, int NP> constexpr int kManyRows = HD <= 128 && NP == 1 ? 2 : 1
 // a sequence's tokens. PM, OM: the prefix's and the sequences' blocks have
 // many rows.
 template <int HD, int BITS, int NP, bool PM, bool OM>
-__global__ __launch_bounds__(AW * 64, HD <= 128 ? 2 : 1) void kv_attn_kernel(AttnArgs p) {
+__global__ __launch_bounds__(AW * 64, HD <= 128 ? (!PM && !OM && NP == 1 ? 3 : 2) : 1) void kv_attn_kernel(AttnArgs p) {
     constexpr int few_lds = PM && OM ? 0 : kFewLds<HD>, many_lds = PM || OM ? kManyLds<HD, BITS> : 0;
     __shared__ __attribute__((aligned(16))) char lds[few_lds > many_lds ? few_lds : many_lds];
     constexpr int NR = kManyRows<HD, NP>;

@@ -76,3 +76,62 @@ def test_attention_large_values(dev, t, bits, shape):
     y, ref, tol = run_attention(dev, t, bits, shape, *(x.to(t) for x in (q, k, v, pk, pv)))
     assert torch.isfinite(y).all()
     assert ((y - ref).abs() <= tol).all(), ((y - ref).abs() / tol).max()
+
+
+@pytest.mark.parametrize("shape", list(D.SHAPES))
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("size", [1e-30, 1e25, 1e36])
+def test_attention_large_and_small_keys(dev, t, bits, shape, size):
+    """Scores of ordinary size out of keys and queries that are not"""
+    lens, S, H, G, hd, P, _ = D.SHAPES[shape]
+    q, k, v, pk, pv = D.inputs("", shape, torch.float64)
+    y, ref, tol = run_attention(dev, t, bits, shape, (q / size).to(t), *(x.to(t) for x in (k * size, v, pk * size, pv)))
+    assert ((y - ref).abs() <= tol).all(), ((y - ref).abs() / tol).max()
+
+
+@pytest.mark.parametrize("shape", list(D.SHAPES))
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("pattern", D.PATTERNS)
+def test_attention_sizes_far_apart(dev, t, bits, shape, pattern):
+    """Groups, tokens and rows that another's size may not cost their bits"""
+    y, ref, tol = run_attention(dev, t, bits, shape, *D.inputs(pattern, shape, t))
+    assert torch.isfinite(ref).all() and ((y - ref).abs() <= tol).all(), ((y - ref).abs() / tol).max()
+
+
+@pytest.mark.parametrize("shape", ["one block", "splits", "prompt"])
+@pytest.mark.parametrize("bits", [8, 4])
+def test_attention_sizes_far_apart_repeats(dev, bits, shape):
+    """Such rows too: the same from call to call, over their own queries, and in a
+    graph whose values grow apart and come together again"""
+    lens, S, H, G, hd, P, per = D.SHAPES[shape]
+    B, n, t = len(lens), max(lens), torch.bfloat16
+    cache = nnr_amd.KVCache(B * per + 8, H, hd, page_size=32, bits=bits)
+    td = torch.arange(B * per, dtype=torch.int32, device=dev).reshape(B, per)
+    pt = torch.arange(B * per, B * per + 7, dtype=torch.int32, device=dev)
+    ld = torch.tensor(lens, dtype=torch.int32, device=dev)
+
+    def fill(pattern):
+        q, k, v, pk, pv = (x.to(dev) for x in D.inputs(pattern, shape, t))
+        cache.write(k, v, td, ld)
+        if P:
+            cache.write(pk, pv, pt[None], torch.tensor([P], dtype=torch.int32, device=dev))
+        return q
+    q = fill("value tokens")
+    kw = dict(prefix_table=pt, prefix_len=P)
+    first = cache.attention(q, td, ld, **kw)
+    for _ in range(3):
+        assert torch.equal(cache.attention(q, td, ld, **kw), first)
+    over = q.clone()
+    assert torch.equal(cache.attention(over, td, ld, y=over, **kw), first)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = cache.attention(q, td, ld, **kw)
+    for pattern in ("", "key tokens", "value tokens", "", "seen later"):
+        q.copy_(fill(pattern))
+        graph.replay()
+        got = y.clone()
+        assert torch.equal(got, cache.attention(q, td, ld, **kw))
+        torch.cuda.synchronize()
