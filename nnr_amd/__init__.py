@@ -590,6 +590,13 @@ def _current(device, stream):
     return torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device))
 
 
+def _int32(**sizes):
+    """Whole numbers that go to the library as 32 bits (ctypes would cut them)."""
+    for name, v in sizes.items():
+        if not -2 ** 31 <= v < 2 ** 31:
+            raise ValueError(f"{name} of {v} does not fit 32 bits")
+
+
 def _on_device(device, **tensors):
     for name, t in tensors.items():
         if t.device != device:
@@ -613,6 +620,7 @@ class MatMulNBits:
         if scales.dtype not in (torch.float32, torch.float16, torch.bfloat16):
             raise TypeError(f"scales of {scales.dtype}: float32, float16 or bfloat16")
         n, nb = int(b.shape[0]), -(-int(k) // int(block_size))
+        _int32(n=n, k=k, block_size=block_size, bits=bits)
         # what is on a device already does not go by way of the host
         on_device = all(t is None or getattr(t, "is_cuda", False) for t in (b, scales, zero_points, bias))
         at = scales.device if on_device else "cpu"
@@ -654,11 +662,14 @@ class MatMulNBits:
         if not a.is_contiguous():
             a = a.contiguous()
         shape = (*shape[:-1], self.n)
+        m = a.numel() // self.k
+        if m > 0x7fffffff:
+            _int32(rows=m)
         if y is None:
             y = a.new_empty(shape)
         elif y.shape != shape or y.dtype != self.dtype or y.device != self.device or not y.is_contiguous():
             raise ValueError(f"y must be contiguous {self.dtype} of shape {shape} on {self.device}")
-        _launch(self._index, self._run, self.h, a.data_ptr(), y.data_ptr(), a.numel() // self.k)
+        _launch(self._index, self._run, self.h, a.data_ptr(), y.data_ptr(), m)
         return y
 
     def __del__(self):
@@ -682,6 +693,7 @@ class KVCache:
 
     def __init__(self, num_pages, kv_heads, head_dim, page_size=64, bits=8, device=None):
         torch = _use_torch()
+        _int32(num_pages=num_pages, page_size=page_size, kv_heads=kv_heads, head_dim=head_dim, bits=bits)
         self.desc = KvCacheDesc(int(num_pages), int(page_size), int(kv_heads), int(head_dim), int(bits))
         n = ct.c_size_t()
         check(lib().nnrh_kv_cache_bytes(ct.byref(self.desc), ct.byref(n)))
@@ -721,6 +733,8 @@ class KVCache:
 
     def _tokens(self, k, page_table, seq_lens):
         B, S, _, _ = k.shape
+        if max(B, S, page_table.shape[1]) > 0x7fffffff:
+            _int32(batch=B, seq=S, pages=page_table.shape[1])
         st = k.stride()
         return KvTokens(_float_dt(k.dtype), B, S, st[0], st[1], page_table.data_ptr(), page_table.shape[1],
                         seq_lens.data_ptr())
@@ -758,6 +772,7 @@ class KVCache:
         """Bytes of workspace that such an attention takes, whatever the lengths: of
         queries of type `dtype`, or enough for any type. (Keys are split by how
         many rows a block holds, and that goes by the type.)"""
+        _int32(batch=batch, seq=seq, q_heads=q_heads, max_pages=max_pages, prefix_len=prefix_len)
         sizes = []
         for dt in (F32, F16, BF16) if dtype is None else (_float_dt(dtype),):
             d = KvAttentionDesc(dt, batch, seq, q_heads, 0, 0, 1.0, None, max_pages, None, None, int(prefix_len))
@@ -780,6 +795,8 @@ class KVCache:
         if q.dim() != 4:
             raise ValueError("q must be [batch, seq, heads, head_dim]")
         B, S, Hq, _ = q.shape
+        if max(B, S, Hq, abs(prefix_len), page_table.shape[-1]) > 0x7fffffff:
+            _int32(batch=B, seq=S, heads=Hq, prefix_len=prefix_len, pages=page_table.shape[-1])
         q = self._rows("q", q, Hq)
         page_table, seq_lens = self._tables(B, page_table, seq_lens)
         if y is None:

@@ -40,3 +40,33 @@ def test_attention_workspace_differs_by_type():
     assert any(f32 < f16 for f32, f16, _ in sizes) and all(f16 == bf16 for _, f16, bf16 in sizes)
     with pytest.raises(TypeError):
         cache.attention_workspace(1, 1, 8, 4, dtype=torch.float64)
+
+
+BIG = 2 ** 32
+
+
+def test_whole_numbers_past_32_bits():
+    """None is taken for its remainder."""
+    for kw in (dict(num_pages=BIG + 4), dict(page_size=BIG + 64), dict(kv_heads=BIG + 8), dict(head_dim=BIG + 128), dict(bits=BIG + 8)):
+        with pytest.raises(ValueError, match="32 bits"):
+            nnr_amd.KVCache(**{**dict(num_pages=1, kv_heads=8, head_dim=128, page_size=64, bits=8, device="cpu"), **kw})
+    b = torch.zeros((1, 1, 1), dtype=torch.uint8).expand(1, (BIG + 64) // 32, 16)
+    for k, block in ((BIG + 64, 32), (64, BIG + 32), (64 - BIG, 32)):
+        with pytest.raises(ValueError, match="32 bits"):
+            nnr_amd.MatMulNBits(b, torch.zeros(1, 1), k, block)
+
+
+def test_calls_past_32_bits():
+    cache = nnr_amd.KVCache(1, 1, 64, page_size=4096, device="cpu")
+    one = torch.zeros((1, 1, 1, 64))
+    many = one.expand(1, BIG + 1, 1, 64)
+    table, lens = torch.zeros((1, 1), dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    pt = torch.zeros(BIG // 4096 + 1, dtype=torch.int32)
+    for call in (lambda: cache.write(many, many, table, lens), lambda: cache.attention(many, table, lens, y=many.detach()),
+                 lambda: cache.attention(one, table, lens, prefix_table=pt, prefix_len=BIG),
+                 lambda: cache.attention(one, table, lens, prefix_table=pt, prefix_len=-BIG)):
+        with pytest.raises(ValueError, match="32 bits"):
+            call()
+    for args in ((BIG + 1, 1, 1, 1), (1, BIG + 1, 1, 1), (1, 1, BIG + 1, 1), (1, 1, 1, BIG + 1), (1, 1, 1, 1, BIG)):
+        with pytest.raises(ValueError, match="32 bits"):
+            cache.attention_workspace(*args)

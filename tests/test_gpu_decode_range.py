@@ -135,3 +135,10 @@ def test_attention_sizes_far_apart_repeats(dev, bits, shape):
         got = y.clone()
         assert torch.equal(got, cache.attention(q, td, ld, **kw))
         torch.cuda.synchronize()
+
+
+def test_nbits_rows_past_32_bits(dev):
+    """Refused, not taken for their remainder"""
+    op = nnr_amd.MatMulNBits(torch.zeros((1, 1, 16), dtype=torch.uint8), torch.ones((1, 1), dtype=torch.float16), 1, 32)
+    with pytest.raises(ValueError, match="32 bits"):
+        op(torch.empty((2 ** 32 + 5, 1), dtype=torch.float16, device=dev))
