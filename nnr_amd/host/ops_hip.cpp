@@ -4,6 +4,7 @@
 // false on a device error) and crosses into device code only through the C
 // ABI of include/nnr_hip.h on the context's stream.
 #include <algorithm>
+#include <climits>
 #include <cmath>
 #include <cstdio>
 #include <cstring>
@@ -1614,21 +1615,28 @@ struct MatMulNBits_hip : operator_t {
     int n = 0, k = 0;
     ~MatMulNBits_hip() override { nnrh_matmul_nbits_destroy(h); }
     bool init() override {
-        k = (int)attribute("K", 0);
-        n = (int)attribute("N", 0);
-        return inputs.size() >= 3 && inputs.size() <= 6 && outputs.size() == 1 && k > 0 && n > 0;
+        const int64_t kk = attribute("K", 0), nn = attribute("N", 0);
+        const auto is = [&](size_t i) { return in(this, i) != nullptr; };
+        if (inputs.size() > 6 || !is(0) || !is(1) || !is(2) || outputs.size() != 1 || kk <= 0 || nn <= 0 || kk > INT_MAX || nn > INT_MAX)
+            return false;
+        k = (int)kk;
+        n = (int)nn;
+        return true;
     }
     bool reshape() override {
+        if (!k) return bad(this, "needs A, B and scales, one output, and K and N of 31 bits");   // (what init refused)
         tensor_t *a = inputs[0], *b = inputs[1], *s = inputs[2], *zp = in(this, 3), *idx = in(this, 4), *bias = in(this, 5);
         const int dt = a->type == NNR_DATA_TYPE_FLOAT32 ? NNRH_F32 : a->type == NNR_DATA_TYPE_FLOAT16 ? NNRH_F16 : -1;
         if (dt < 0) return bad(this, "A must be fp32 or fp16");
         if (a->ndim() < 1 || a->dims[a->ndim() - 1] != k) return bad(this, "A's last axis is not K");
         std::vector<int> d(a->dims.begin(), a->dims.end() - 1);
         d.push_back(n);
+        if (a->ndata / k > (1u << 20)) return bad(this, "more than 2^20 rows");
+        const int64_t block = attribute("block_size", 0);
+        if (attribute("bits", 4) != 4) return bad(this, "bits must be 4");
+        if (block < 16 || block > (1 << 22) || (block & (block - 1))) return bad(this, "block_size must be a power of two");
         if (!outputs[0]->reshape(d, a->type)) return false;
         if (ctx->shape_only) return true;
-        const int64_t block = attribute("block_size", 0), bits = attribute("bits", 4);
-        if (block < 16 || block > (1 << 22) || (block & (block - 1))) return bad(this, "block_size must be a power of two");
         const size_t nb = ((size_t)k + block - 1) / block;
         const auto constant = [](tensor_t* t, data_type_t type, size_t count) {
             return t->has_host() && t->type == type && t->ndata == count;
@@ -1642,7 +1650,7 @@ struct MatMulNBits_hip : operator_t {
         nnrh_matmul_nbits_desc dsc{};
         dsc.n = n;
         dsc.k = k;
-        dsc.bits = (int)bits;
+        dsc.bits = 4;
         dsc.block_size = (int)block;
         dsc.dtype = dt;
         dsc.b = b->host.data();

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import nnr_amd
+from decode_ref import nbits_graph
 from nnr_amd import _lib
 
 TYPES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
@@ -70,3 +71,21 @@ def test_calls_past_32_bits():
     for args in ((BIG + 1, 1, 1, 1), (1, BIG + 1, 1, 1), (1, 1, BIG + 1, 1), (1, 1, 1, BIG + 1), (1, 1, 1, 1, BIG)):
         with pytest.raises(ValueError, match="32 bits"):
             cache.attention_workspace(*args)
+
+
+@pytest.mark.parametrize("kw", [dict(attrs=dict(K=BIG + 70)), dict(attrs=dict(N=BIG + 24)), dict(shape=(2 ** 20 + 1, 70)),
+                                dict(shape=(2 ** 26, 2 ** 6, 70)), dict(attrs=dict(bits=BIG + 4))])
+def test_nbits_node_past_its_range(kw):
+    from nnr_amd.graph import Session
+    with pytest.raises(RuntimeError):
+        Session(nbits_graph(**kw), device=False)
+
+
+@pytest.mark.parametrize("ins", [["x"], ["x", "b"], ["x", "", "s"], ["x", "b", ""]])
+def test_nbits_node_without_its_inputs(ins):
+    from nnr_amd.graph import Session
+    g = nbits_graph()
+    node = g.nodes[-1]
+    node.inputs[:] = ins
+    with pytest.raises(RuntimeError, match="MatMulNBits"):
+        Session(g, device=False)
