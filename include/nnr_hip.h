@@ -616,7 +616,8 @@ int nnrh_matmul_nbits_destroy(nnrh_matmul_nbits_t h);
  * order: position i in page page_table[b][i / page_size]. An entry outside 0
  * .. num_pages - 1 is a page that does not exist: nothing is written to it
  * and it holds no tokens. seq_lens[b] counts sequence b's tokens up to and
- * with the newest. Both are int32 in device memory, read when the kernels run.
+ * with the newest. Both are int32 in device memory, read when the kernels run,
+ * and lie in nothing that the call writes.
  *
  * write: token s of `seq` new tokens of sequence b goes to position
  *   seq_lens[b] - seq + s. Tokens at negative positions (a batch padded at the

@@ -2411,6 +2411,10 @@ int kv_batch(const char* what, int batch, int seq, int max_pages, int page_size,
     if (((uintptr_t)table | (uintptr_t)lens) & 3) return set_err(NNRH_ERR_INVALID, "%s: table alignment", what);
     return NNRH_OK;
 }
+// a result over the tables that a call's kernels read
+bool over_tables(const void* p, size_t bytes, const int32_t* table, long long entries, const int32_t* lens, int batch) {
+    return overlap(p, bytes, table, (size_t)entries * 4) || overlap(p, bytes, lens, (size_t)batch * 4);
+}
 // rows of `width` dense elements at strides; out: rows must not overlap
 int kv_strides(const char* what, int type, int batch, int seq, long long width, long long bs, long long ts, bool out) {
     const long long per16 = 16 / float_type_size(type);
@@ -2446,6 +2450,10 @@ int kv_tokens(const char* what, const KvCache& c, const nnrh_kv_tokens* t, const
     // k and v may alternate in one tensor; rows over each other are two results in one place
     const size_t row = width * float_type_size(type);
     if (out && overlap(k, row, v, row)) return set_err(NNRH_ERR_INVALID, "%s: k lies over v", what);
+    const long long entries = (long long)t->batch * t->max_pages;
+    for (const void* p : {out ? k : c.data, out ? v : c.data})
+        if (over_tables(p, out ? extent : all, t->page_table_dev, entries, t->seq_lens_dev, t->batch))
+            return set_err(NNRH_ERR_INVALID, "%s: results over the page table or the lengths", what);
     return NNRH_OK;
 }
 
@@ -2545,6 +2553,11 @@ extern "C" int nnrh_kv_attention(const nnrh_kv_cache_desc* d, const void* cache,
     if ((uintptr_t)workspace & 255) return set_err(NNRH_ERR_INVALID, "kv_attention: the workspace must be 256-byte aligned");
     if (overlap(workspace, need, q, qsize) || overlap(workspace, need, y, ysize) || overlap(workspace, need, c.data, all))
         return set_err(NNRH_ERR_INVALID, "kv_attention: the workspace lies over q, y or the cache");
+    const size_t prefix_entries = ((size_t)a->prefix_len + c.page_size - 1) / c.page_size;
+    for (const auto& [p, bytes] : {std::pair<const void*, size_t>(y, ysize), std::pair<const void*, size_t>(workspace, need)})
+        if (over_tables(p, bytes, a->page_table_dev, (long long)a->batch * a->max_pages, a->seq_lens_dev, a->batch) ||
+            overlap(p, bytes, a->prefix_table_dev, prefix_entries * 4))
+            return set_err(NNRH_ERR_INVALID, "kv_attention: y or the workspace lies over a table or the lengths");
     r.q = q;
     r.y = y;
     ProfScope ps("kv_attention", S(stream));

@@ -89,3 +89,29 @@ def test_nbits_node_without_its_inputs(ins):
     node.inputs[:] = ins
     with pytest.raises(RuntimeError, match="MatMulNBits"):
         Session(g, device=False)
+
+
+MEM = [0x100000000 * (i + 1) for i in range(8)]
+
+
+def test_results_over_tables():
+    """Tables and lengths are read while a call writes: none may lie in its results."""
+    L, inv = _lib.lib(), _lib.NNRH_ERR_INVALID
+    c = _lib.KvCacheDesc(4, 64, 2, 128, 8)
+
+    def tokens(table, lens):
+        return _lib.KvTokens(dtype=_lib.F16, batch=2, seq=3, batch_stride=768, token_stride=256, page_table_dev=table, max_pages=2,
+                             seq_lens_dev=lens)
+
+    def attention(table, lens, prefix):
+        return _lib.KvAttentionDesc(dtype=_lib.F16, batch=2, seq=1, q_heads=8, q_batch_stride=1024, q_token_stride=1024, scale=0.1,
+                                    page_table_dev=table, max_pages=2, seq_lens_dev=lens, prefix_table_dev=prefix, prefix_len=100)
+    last = 2 * 3 * 256 * 2 - 4   # of k's or v's extent
+    for at in (MEM[1], MEM[1] + last, MEM[2] + 16):
+        for table, lens in ((at, MEM[4]), (MEM[3], at)):
+            assert L.nnrh_kv_cache_read(C.byref(c), MEM[0], C.byref(tokens(table, lens)), MEM[1], MEM[2], None) == inv
+    for table, lens in ((MEM[0] + 64, MEM[4]), (MEM[3], MEM[0] + 64)):
+        assert L.nnrh_kv_cache_write(C.byref(c), MEM[0], C.byref(tokens(table, lens)), MEM[1], MEM[2], None) == inv
+    for at in (MEM[2], MEM[2] + 4092, MEM[6] + 256):
+        for tables in ((at, MEM[4], MEM[5]), (MEM[3], at, MEM[5]), (MEM[3], MEM[4], at)):
+            assert L.nnrh_kv_attention(C.byref(c), MEM[0], C.byref(attention(*tables)), MEM[1], MEM[2], MEM[6], None) == inv
