@@ -68,11 +68,15 @@ SHAPES = {
 }
 
 
+def sizes(shape):
+    return shape if isinstance(shape, tuple) else SHAPES[shape]
+
+
 def inputs(pattern, shape, t, seed=0):
     """q [B, S, H G, hd], own k and v [B, longest, H, hd] (a sequence's last tokens are its own) and the
     prefix's [1, P, H, hd]. Every key is 1/4 of the way to a query of ones, so that a token of
     -1s is hardly seen."""
-    lens, S, H, G, hd, P, _ = SHAPES[shape]
+    lens, S, H, G, hd, P, _ = sizes(shape)
     B, n = len(lens), max(lens)
     g = torch.Generator().manual_seed(seed)
     r = lambda *s: torch.randn(s, generator=g, dtype=torch.float64)

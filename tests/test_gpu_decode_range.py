@@ -1,4 +1,5 @@
 """Operators of a decoder's step where ranges, sizes and rows are far apart, against float64."""
+import numpy as np
 import pytest
 import torch
 
@@ -35,7 +36,7 @@ def test_workspace_made_before_the_call(dev, t, typed):
 
 def run_attention(dev, t, bits, shape, q, k, v, pk, pv, scale=None):
     """(result, float64's, how far it may be off), each [rows, hd]"""
-    lens, S, H, G, hd, P, per = D.SHAPES[shape]
+    lens, S, H, G, hd, P, per = D.sizes(shape)
     B, n, page = len(lens), max(lens), 32
     pre = -(-P // page)
     order = torch.randperm(B * per + pre + 1, generator=torch.Generator().manual_seed(5)).to(torch.int32)
@@ -65,7 +66,7 @@ def run_attention(dev, t, bits, shape, q, k, v, pk, pv, scale=None):
 @pytest.mark.parametrize("bits", [8, 4])
 def test_attention_large_values(dev, t, bits, shape):
     """Results that fit their type, of values next to its largest number"""
-    lens, S, H, G, hd, P, _ = D.SHAPES[shape]
+    lens, S, H, G, hd, P, _ = D.sizes(shape)
     top = {torch.float32: 3e38, torch.float16: 6e4, torch.bfloat16: 3e38}[t]
     g = torch.Generator().manual_seed(1)
     r = lambda *s: torch.rand(s, generator=g, dtype=torch.float64) * 2 - 1
@@ -84,7 +85,7 @@ def test_attention_large_values(dev, t, bits, shape):
 @pytest.mark.parametrize("size", [1e-30, 1e25, 1e36])
 def test_attention_large_and_small_keys(dev, t, bits, shape, size):
     """Scores of ordinary size out of keys and queries that are not"""
-    lens, S, H, G, hd, P, _ = D.SHAPES[shape]
+    lens, S, H, G, hd, P, _ = D.sizes(shape)
     q, k, v, pk, pv = D.inputs("", shape, torch.float64)
     y, ref, tol = run_attention(dev, t, bits, shape, (q / size).to(t), *(x.to(t) for x in (k * size, v, pk * size, pv)))
     assert ((y - ref).abs() <= tol).all(), ((y - ref).abs() / tol).max()
@@ -105,7 +106,7 @@ def test_attention_sizes_far_apart(dev, t, bits, shape, pattern):
 def test_attention_sizes_far_apart_repeats(dev, bits, shape):
     """Such rows too: the same from call to call, over their own queries, and in a
     graph whose values grow apart and come together again"""
-    lens, S, H, G, hd, P, per = D.SHAPES[shape]
+    lens, S, H, G, hd, P, per = D.sizes(shape)
     B, n, t = len(lens), max(lens), torch.bfloat16
     cache = nnr_amd.KVCache(B * per + 8, H, hd, page_size=32, bits=bits)
     td = torch.arange(B * per, dtype=torch.int32, device=dev).reshape(B, per)
@@ -142,3 +143,50 @@ def test_nbits_rows_past_32_bits(dev):
     op = nnr_amd.MatMulNBits(torch.zeros((1, 1, 16), dtype=torch.uint8), torch.ones((1, 1), dtype=torch.float16), 1, 32)
     with pytest.raises(ValueError, match="32 bits"):
         op(torch.empty((2 ** 32 + 5, 1), dtype=torch.float16, device=dev))
+
+
+# ---------------------------------------------------------------------------
+# sizes that the kernels tell apart
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("k,block", [(33, 32), (64, 32), (96, 64)])
+def test_nbits_most_rows_values(dev, t, k, block):
+    """2^20 rows against float64, at both ends, in the middle and across a block's end"""
+    m, n = 1 << 20, 20
+    rng = np.random.default_rng(k)
+    nb = -(-k // block)
+    b, z = rng.integers(0, 256, (n, nb, block // 2), dtype=np.uint8), rng.integers(0, 256, (n, (nb + 1) // 2), dtype=np.uint8)
+    s, c = torch.from_numpy(rng.uniform(0.01, 0.1, (n, nb))).to(t), torch.from_numpy(rng.standard_normal(n)).to(t)
+    op = nnr_amd.MatMulNBits(b, s, k, block, zero_points=z, bias=c)
+    a = torch.randn((m, k), device=dev).to(t)
+    y = op(a)
+    for i in (0, 77777, (1 << 19) - 150, m - 300):
+        f = lambda x: x.detach().cpu().double().numpy()
+        ref, mag = R.nbits(f(a[i:i + 300]), b, f(s), k, block, z, f(c))
+        tol = R.nbits_tol(ref, mag, k, t)
+        assert R.close(f(y[i:i + 300]), ref, tol, t).all()
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("hd", [64, 96, 128])
+@pytest.mark.parametrize("lens,S,G,prefix", [
+    ([300], 300, 1, 0),                  # a prompt: rows of 128 a block and what is left of them
+    ([520, 417], 260, 2, 0),             # the second part of one, 520 rows
+    ([64, 70, 33], 50, 4, 190),          # 600 rows of a prefix, 200 of each sequence
+    ([5] * 130, 1, 2, 130),              # 260 rows of a prefix, few of each sequence
+    ([129], 129, 1, 0), ([128], 128, 1, 1)])
+def test_attention_prompts(dev, t, bits, hd, lens, S, G, prefix):
+    """More rows of a head than a block holds"""
+    shape = (lens, S, 1, G, hd, prefix, -(-max(lens) // 32))
+    y, ref, tol = run_attention(dev, t, bits, shape, *D.inputs("", shape, t))
+    assert ((y - ref).abs() <= tol).all(), ((y - ref).abs() / tol).max()
+
+
+@pytest.mark.parametrize("t", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("bits", [8, 4])
+def test_attention_long_prompt(dev, t, bits):
+    """1200 new tokens over splits of their own and of a prefix"""
+    shape = ([1200], 1200, 1, 2, 128, 700, 40)
+    y, ref, tol = run_attention(dev, t, bits, shape, *D.inputs("", shape, t))
+    assert ((y - ref).abs() <= tol).all(), ((y - ref).abs() / tol).max()
