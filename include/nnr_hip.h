@@ -610,8 +610,8 @@ int nnrh_matmul_nbits_destroy(nnrh_matmul_nbits_t h);
  * and stands for code * scale. Elements that are not finite do not enter the
  * maximum; a NaN is held as 0, an infinity as its sign's last code. A scale
  * that is no normal float is 0.
- * The cache is one device buffer of nnrh_kv_cache_bytes, 16-byte aligned, of
- * the caller; its layout is the library's. Zero it before its first use.
+ * The cache is one device buffer of nnrh_kv_cache_bytes (2^56 at most), 16-byte
+ * aligned, of the caller; its layout is the library's. Zero it before its first use.
  * A sequence's tokens lie in the pages that its row of page_table names, in
  * order: position i in page page_table[b][i / page_size]. An entry outside 0
  * .. num_pages - 1 is a page that does not exist: nothing is written to it

@@ -2372,6 +2372,8 @@ extern "C" int nnrh_matmul_nbits_destroy(nnrh_matmul_nbits_t h) {
 
 namespace {
 
+long long kv_page_bytes(const KvCache& c) { return c.heads * kv_head_bytes(c.page_size, c.hd, c.bits); }
+
 // the cache's description; data may be NULL
 int kv_cache(const nnrh_kv_cache_desc* c, const void* data, KvCache* out) {
     if (!c) return set_err(NNRH_ERR_INVALID, "kv_cache: NULL description");
@@ -2391,10 +2393,12 @@ int kv_cache(const nnrh_kv_cache_desc* c, const void* data, KvCache* out) {
     out->heads = c->kv_heads;
     out->hd = c->head_dim;
     out->bits = c->bits;
+    // (beyond any memory; more pages' bytes would pass 64 bits)
+    if (c->num_pages > (1LL << 56) / kv_page_bytes(*out))
+        return set_err(NNRH_ERR_UNSUPPORTED, "kv_cache: %d pages of %lld bytes (2^56 bytes at most)", c->num_pages,
+                       kv_page_bytes(*out));
     return NNRH_OK;
 }
-long long kv_page_bytes(const KvCache& c) { return c.heads * kv_head_bytes(c.page_size, c.hd, c.bits); }
-
 // what write, read and attention ask of a batch's tables
 int kv_batch(const char* what, int batch, int seq, int max_pages, int page_size, const int32_t* table,
              const int32_t* lens) {

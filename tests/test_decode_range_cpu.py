@@ -115,3 +115,16 @@ def test_results_over_tables():
     for at in (MEM[2], MEM[2] + 4092, MEM[6] + 256):
         for tables in ((at, MEM[4], MEM[5]), (MEM[3], at, MEM[5]), (MEM[3], MEM[4], at)):
             assert L.nnrh_kv_attention(C.byref(c), MEM[0], C.byref(attention(*tables)), MEM[1], MEM[2], MEM[6], None) == inv
+
+
+@pytest.mark.parametrize("kw,rc", [
+    (dict(num_pages=2 ** 31 - 1, page_size=4096, kv_heads=32767, head_dim=256, bits=8), _lib.NNRH_ERR_UNSUPPORTED),
+    (dict(num_pages=2 ** 30, page_size=4096, kv_heads=16384, head_dim=128, bits=4), _lib.NNRH_ERR_UNSUPPORTED),
+    (dict(num_pages=2 ** 31 - 1, page_size=32, kv_heads=8, head_dim=128, bits=8), 0)])
+def test_cache_bytes_past_64_bits(kw, rc):
+    """A cache larger than any memory has no size, and no page of it is taken for one."""
+    c, n = _lib.KvCacheDesc(**kw), C.c_size_t(7)
+    assert _lib.lib().nnrh_kv_cache_bytes(C.byref(c), C.byref(n)) == rc
+    groups = 1 if kw["bits"] == 8 else kw["head_dim"] // 32
+    each = 2 * kw["kv_heads"] * kw["page_size"] * (kw["head_dim"] * kw["bits"] // 8 + 2 * groups)
+    assert n.value == (7 if rc else kw["num_pages"] * each)
