@@ -585,7 +585,8 @@ int nnrh_clip_f32(const float* x_dev, float* y_dev, size_t n, float lo, float hi
  * first; zero points likewise, two a byte, a column's rounded up to a whole
  * byte (NULL: 8). run takes a of m x k and writes y of m x n, both row-major
  * and dense, 0 <= m <= 2^20, and uses no workspace: calls on several streams
- * may share a handle. y must not overlap a. a and y are aligned to their
+ * may share a handle. Elements of a are below 2^117 (a block's products are summed
+ * in fp32 before its scale). y must not overlap a. a and y are aligned to their
  * element; rows of 16-byte multiples at 16-byte aligned addresses are faster. */
 typedef struct nnrh_matmul_nbits_desc {
     int n, k;

@@ -1,6 +1,6 @@
 // nnrh_decode.h -- operators of a decoder's serving step: products with 4-bit
-// weights (nnrh_nbits.hip), the quantized key/value cache and the attention
-// that reads it (nnrh_kvcache.hip). Shared with the C-ABI layer.
+// weights (nnrh_nbits.hip), the quantized key/value cache (nnrh_kvcache.hip) and
+// the attention that reads it (nnrh_kvattn.hip). Shared with the C-ABI layer.
 #pragma once
 
 #include <hip/hip_runtime.h>

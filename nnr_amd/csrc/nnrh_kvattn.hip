@@ -31,14 +31,15 @@
 // Up to 16 rows (few): the block's waves take tiles in turn, operands go from
 // memory to registers, and a tile's registers are asked for again as soon as
 // they are used; bound by memory: 48 sequences of up to 8192 tokens, 32 heads
-// over 8 of 128, 8 bits, 409 MB in 80 us and 4 of joining (a copy's rate: 79).
+// over 8 of 128, 8 bits, 409 MB in 82 us and 5 of joining, the two back to back 84
+// to 86 (a copy's rate: 79).
 // More rows (many): the waves take rows, and a tile's codes are turned into
 // operands once, in LDS. Bound by the instructions between the products: 128
-// sequences after a prefix of 32768, 4 bits, 69 GFLOP in 121 us (a large
-// library product's rate: 57): matrix units 25 % busy, vector units 50 with
+// sequences after a prefix of 32768, 4 bits, 69 GFLOP in 125 us, the join with it (a
+// large library product's rate: 57): matrix units 25 % busy, vector units 50 with
 // weights and conversion, the rest waits for LDS and at the tile's barrier.
 //
-// Keys are split over blocks; each leaves (max, total, O) of its rows, which
+// Keys are split over blocks; each leaves (max, total, mean) of its rows, which
 // a second kernel joins in a fixed order. One block that sees everything
 // writes the result itself.
 #include "nnrh_decode.h"
@@ -919,7 +920,7 @@ template <int HD> constexpr int kFewLds = 2 * (HD / 16) * 1024 + 4 * AW * 64 + 2
 
 // ---- many rows: the block's waves split its rows ------------------------------
 // Tiles between two barriers: two, or one where two would not leave enough
-// registers (32 sequences after a prefix of 8192: 27.0 us, with two 27.5).
+// registers (32 sequences after a prefix of 8192: 26.8 us, with two 30.1).
 template <int HD, int BITS> constexpr int kManyTiles = HD == 128 && BITS == 8 ? 1 : 2;
 
 // A tile is turned into operands once, a part by each wave, and lies in LDS
@@ -1251,18 +1252,18 @@ Plan plan(const KvCache& c, const KvAttention& a) {
     p.pre_groups = a.prefix_len ? ceil_div(pre_rows, p.pre_many ? many : 16) : 0;
     const long long pre_items = (long long)p.pre_groups * c.heads, own_items = (long long)p.own_groups * c.heads * a.batch;
     const long long pre_tiles = (a.prefix_len + 31) / 32, own_tiles = (long long)a.max_pages * c.page_size / 32;
-    // Blocks with few rows: 32 tiles or more, and short ones whole. (A split of 8
-    // tiles a block, and its join: 48 sequences of 8192 87 us instead of 85, 16 of
-    // 1000 14 instead of 12.7, 4 of 8192 20 instead of 16, one of 700 13.7 instead
-    // of 10.)
+    // Blocks with few rows: 32 tiles or more, and short ones whole. (Splits of 8
+    // tiles, and their join: 48 sequences of 8192 120 us instead of 86, 16 of 1000
+    // 13.6 instead of 12.8, 4 of 8192 21 instead of 16.5, one of 700 13.6 instead of
+    // 10.4.)
     const auto few = [](long long items, long long tiles) {
         return tiles <= 32 ? std::max(tiles, 1ll) : std::max(items * tiles / 1024, 32ll);
     };
     // Those with many: no more than run at once, of 8 tiles or more. (128 sequences
-    // after a prefix of 32768: 512 blocks 139 us, 384 147, 768 154.) Of 4 where that
+    // after a prefix of 32768: 512 blocks 134 us, 384 150, 768 141.) Of 4 where that
     // is a block a CU, and two with the rest: such a block waits for most of a tile's
-    // 0.8 us. (32 sequences after a prefix of 1024: 19.2 us, of 8 tiles 22.8; 4096:
-    // 21.9 and 24.1. Beyond: 8192 36 and 27, 128 sequences after 512 30.4 and 28.8.)
+    // 0.8 us. (32 sequences after a prefix of 1024: 20.0 us, of 8 tiles 23.5; 4096:
+    // 22.8 and 24.9. Beyond: 8192 35.6 and 27.2, 128 sequences after 512 31.8 and 30.2.)
     const long long at_once = c.hd <= 128 ? 512 : 256;
     const auto many_blocks = [&](long long chunk) {
         return (p.pre_many ? pre_items * ceil_div(pre_tiles, chunk) : 0) + (p.own_many ? own_items * ceil_div(own_tiles, chunk) : 0);

@@ -4,7 +4,8 @@
 // q - zp is a whole number of at most 15 and so exact in 16 bits: the MFMA
 // multiplies activations by q - zp, sums a block's (or 32 k's) products in
 // fp32, and the block's scale enters in fp32 when they join the running sum.
-// No weight is rounded. fp16 activations run on fp16 MFMAs, bf16 ones on bf16
+// No weight is rounded. (So that sums before the scale fit fp32, activations are to
+// be below 2^117: 128 of them times 15.) fp16 activations run on fp16 MFMAs, bf16 ones on bf16
 // MFMAs; an fp32 activation is the exact sum of three bf16 pieces, one MFMA
 // each.
 //
@@ -15,9 +16,9 @@
 // and 7.5), bound by loads: each of 256 blocks reads the 64 rows whole, 1 MB, beside
 // 0.14 MB of weights (vector units 30 % busy, matrix units 18). Beyond, blocks of
 // up to 128 rows share activations through LDS, and a wave's weights serve all of
-// them: 512 x 4096 x 4096, bf16: 17 GFLOP in 33 us (14.1), bound by conversion,
-// the blocks' scales in fp32 and the barrier of each chunk at two waves a SIMD
-// (vector units 45 % busy, matrix units 20).
+// them: 512 x 4096 x 4096, bf16: 17 GFLOP in 33 to 38 us over machines (14.1), bound
+// by how little two waves a SIMD can put beside each other between the barriers of
+// two chunks: neither vector units (45 % busy) nor matrix units (20) are full.
 #include "nnrh_decode.h"
 
 namespace nnrh {
@@ -234,7 +235,7 @@ template <int TY, int NSPP, int NT> struct Stage {
 // ahead, activations through LDS, asked for a chunk ahead. The waves' sums meet
 // in LDS. DIR (a row or two): operands straight from memory like the weights;
 // lanes that repeat a row cost no accesses of their own (1 x 4096 x 8192 bf16
-// 6.8 us, through LDS 7.8; 16 rows 18.6 and 11.7).
+// 6.6 us, through LDS 7.7; 16 rows 10.7 and 8.1).
 template <int TY, int NSPP, int AM, int MT, int NT, int D, bool DIR>
 __global__ __launch_bounds__(NB_WAVES * 64) void nbits_kernel(NbitsArgs p) {
     typedef Activations<TY, MT> Act;
@@ -617,10 +618,10 @@ hipError_t by_size(const NbitsArgs& a, hipStream_t s) {
     const auto blocks = [&](int m, int n) { return (long long)((a.M + m - 1) / m) * (cols / n); };
     if (a.M > 64) {
         // Blocks of shared rows where they fill the chip (bf16, K 4096, blocks of
-        // 32: 512 x 4096 38 us, K split over waves 53; 256 x 4096 35 and 27);
-        // those of 128 columns where that is so twice over (4096 x 4096 235 us,
-        // 64 columns of 128 rows 279). Rows of any address too (512 x 4095 x 4096
-        // bf16 57 us, K split over waves 90; fp32 74 and 156).
+        // 32, one machine: 512 x 4096 38 us, K split over waves 52; 256 x 4096 33 and
+        // 25); those of 128 columns where that is so twice over (4096 x 4096 213 us,
+        // 64 columns of 128 rows 251). Rows of any address too (512 x 4095 x 4096
+        // bf16 54 us, K split over waves 86; fp32 73 and 156).
         if (blocks(64, 128) >= (wide ? 192 : 512)) return go_tile<TY, NSPP, AM, 4, 2, 4>(a, s);
         if constexpr (!wide)
             if (blocks(128, 64) >= 192)   // (column tiles side by side spill with few scales: 41 us, 35)
