@@ -336,7 +336,8 @@ __device__ __forceinline__ void load_rows(const AttnArgs& p, Rows<HD, NP, NR>& w
         for (int k = 0; k < NC; ++k)
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float s = ldexpf(neg ? -v[k][j] : v[k][j], e);
+                float s = ldexpf(neg ? -v[k][j] : v[k][j], e);
+                if constexpr (NP == 2) asm("" : "+v"(s));   // (both pieces are of this, as below)
                 const _Float16 h = (_Float16)s;
                 w.q[0][t][k][j] = h;
                 if constexpr (NP == 2) w.q[1][t][k][j] = (_Float16)(s - (float)h);
@@ -474,7 +475,11 @@ __device__ __forceinline__ void tile_step(Rows<HD, NP, NR>& w, int key0, const i
             const float vu = BITS == 8 ? bf16_at(vs[z], j) * fv : 1.0f;
 #pragma unroll
             for (int t = 0; t < NR; ++t) {
-                const float x = BITS == 8 ? s[t][z][j] * vu : s[t][z][j];
+                float x = BITS == 8 ? s[t][z][j] * vu : s[t][z][j];
+                // Both pieces are of x as fp32 holds it. Left to itself the compiler takes
+                // the second from an fp16 of the product, rounded once, and next to a tie
+                // that is not the first.
+                if constexpr (NP == 2) asm("" : "+v"(x));
                 if constexpr (BITS == 8) w.x[t] = fmaxf(w.x[t], x);
                 const _Float16 h = (_Float16)x;
                 pf[0][t][j] = h;

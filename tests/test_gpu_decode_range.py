@@ -190,3 +190,34 @@ def test_attention_long_prompt(dev, t, bits):
     shape = ([1200], 1200, 1, 2, 128, 700, 40)
     y, ref, tol = run_attention(dev, t, bits, shape, *D.inputs("", shape, t))
     assert ((y - ref).abs() <= tol).all(), ((y - ref).abs() / tol).max()
+
+
+@pytest.mark.parametrize("own", [False, True])
+@pytest.mark.parametrize("bits", [8, 4])
+def test_attention_weights_next_to_ties(dev, bits, own):
+    """Weights of fp32 tensors in two pieces: their sum is the weight also where it
+    lies beside the middle of two fp16 numbers. Two keys, the second's value 0, so
+    that nothing hides the first's weight; 2^16 of them."""
+    hd, n = 64, 1 << 16
+    g = torch.Generator().manual_seed(2)
+    k, v = torch.randn((1, 2, 1, hd), generator=g), torch.randn((1, 2, 1, hd), generator=g)
+    v[:, 1] = 0
+    cache = nnr_amd.KVCache(1, 1, hd, page_size=32, bits=bits)
+    two = torch.full((1,), 2, dtype=torch.int32, device=dev)
+    cache.write(k.to(dev), v.to(dev), torch.zeros((1, 1), dtype=torch.int32, device=dev), two)
+    kx, vx = (R.quantize(x[0, :, 0], bits)[0] for x in (k, v))
+    if own:     # 16384 sequences of those tokens, 4 queries each
+        q, lens = 0.3 * torch.randn((n // 4, 1, 4, hd), generator=g), torch.full((n // 4,), 2, dtype=torch.int32, device=dev)
+        y = cache.attention(q.to(dev), torch.zeros((n // 4, 1), dtype=torch.int32, device=dev), lens)
+    else:       # a prefix that 2^16 queries see
+        q, lens = 0.3 * torch.randn((1, n // 4, 4, hd), generator=g), torch.zeros(1, dtype=torch.int32, device=dev)
+        y = cache.attention(q.to(dev), torch.zeros((1, 1), dtype=torch.int32, device=dev), lens,
+                            prefix_table=torch.zeros(1, dtype=torch.int32, device=dev), prefix_len=2)
+    q, y = q.reshape(n, hd).double(), y.reshape(n, hd).cpu().double()
+    p = torch.softmax(q @ kx.T * hd ** -0.5, -1)[:, :1]
+    # of both keys' scores, each in p and in the total; the weight's two pieces and what is left of
+    # the second (2^-21); maximum, exponential, total, division and result, an operation each
+    e = hd ** -0.5 * ((hd + 16) * R.U + 2.0 ** -22) * (q.abs() @ kx.abs().T).sum(-1, keepdim=True)
+    tol = (2 * e + 2.0 ** -21 + 16 * R.U) * (p * vx[0]).abs()
+    assert tol.max() < 2.0 ** -12 * vx.abs().max()
+    assert ((y - p * vx[0]).abs() <= tol).all(), ((y - p * vx[0]).abs() / tol).nan_to_num(0).max()
