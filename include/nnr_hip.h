@@ -687,6 +687,101 @@ int nnrh_kv_attention_workspace(const nnrh_kv_cache_desc* c, const nnrh_kv_atten
 int nnrh_kv_attention(const nnrh_kv_cache_desc* c, const void* cache_dev, const nnrh_kv_attention_desc* a,
                       const void* q_dev, void* y_dev, void* workspace_dev, void* stream);
 
+/* The same where the `seq` newest tokens are drafts that form a tree (or any
+ * other relation): query (b, s, h) sees the prefix, positions 0 .. seq_lens[b] -
+ * seq - 1, and of the drafts those j (at position seq_lens[b] - seq + j) with
+ * tree[b * tree_batch_stride + s * seq + j] != 0: itself too only if so. One byte a
+ * pair, in device memory, read when the kernels run, over nothing that the call
+ * writes; a stride of 0: one tree for the batch. At most 4096 drafts. Workspace
+ * and everything else as nnrh_kv_attention has it.                          */
+int nnrh_kv_tree_attention(const nnrh_kv_cache_desc* c, const void* cache_dev, const nnrh_kv_attention_desc* a,
+                           const uint8_t* tree_dev, long long tree_batch_stride, const void* q_dev, void* y_dev,
+                           void* workspace_dev, void* stream);
+
+/* Page source[i] copied to page destination[i], i < n, in each of `layers`
+ * caches of one description (`caches`: a host array of their device buffers, which
+ * do not overlap; one launch for 64 of them): a sequence is forked by copying its
+ * last page, or a cache compacted. int32 page numbers in device memory, read when
+ * the kernels run; a pair with a number outside 0 .. num_pages - 1 is skipped, and
+ * so is a page copied to itself. Pages are copied in no order: none may be the
+ * destination of two pairs, or the destination of one and the source of another
+ * (a chain takes several calls). At most 1024 caches.                       */
+int nnrh_kv_copy_pages(const nnrh_kv_cache_desc* c, void* const* caches, int layers, const int32_t* source_dev,
+                       const int32_t* destination_dev, int n, void* stream);
+
+/* Tokens moved within their sequences, in each of `layers` caches as above: what
+ * position source[b][i] of sequence b holds, codes and scales as they are, goes to
+ * position destination[b][i]. All of a sequence's are read before any is written, so
+ * that a call may permute them (the accepted drafts of a tree to the front). int32 in
+ * device memory, read when the kernels run. A pair with a position that is negative,
+ * behind the last page or on a page that does not exist is skipped (sequences that
+ * move fewer). A sequence's destinations are distinct; the pages that they lie on are
+ * one sequence's each, and no other call writes to them meanwhile. count is at
+ * most 128, batch 65535, max_pages page_size 2^30, batch kv_heads layers (of 64 at
+ * once) 2^22.                                                               */
+typedef struct nnrh_kv_moves {
+    int batch, count;
+    const int32_t* page_table_dev;   /* [batch][max_pages]                   */
+    int max_pages;
+    const int32_t* source_dev;       /* [batch][count]                       */
+    const int32_t* destination_dev;  /* [batch][count]                       */
+} nnrh_kv_moves;
+int nnrh_kv_move_tokens(const nnrh_kv_cache_desc* c, void* const* caches, int layers, const nnrh_kv_moves* m,
+                        void* stream);
+
+/* Rotary positions: queries and keys [batch][seq][heads][head_dim] turned by their
+ * tokens' positions. Of a head's first rotary_dim elements (even; the rest is copied)
+ * the pairs (x[2i], x[2i + 1]) if interleaved, or else (x[i], x[i + rotary_dim / 2]),
+ * become
+ *   (a c - b s, b c + a s),   c, s = table[position][i],
+ * in fp32, rounded once. table: [max_positions][rotary_dim / 2] pairs (cosine, sine)
+ * in fp32, which the caller makes (scaled for long contexts or not). positions:
+ * int32 [batch][seq], read when the kernel runs. A token at a negative position
+ * (padding) is copied as it is; one at max_positions or beyond gives NaN.
+ * Strides in elements; heads are dense. Results go to qy and ky, which may be q and
+ * k at the same strides, and whose rows otherwise share no memory with q, k and each
+ * other (rows of q and k may lie side by side in one tensor). Addresses are aligned
+ * to the element; of 16-byte multiples they are faster. 0 heads: no such tensor. Fewer than
+ * 2^31 elements.                                                            */
+typedef struct nnrh_rotary_desc {
+    int dtype;
+    int batch, seq, q_heads, k_heads;
+    int head_dim, rotary_dim;
+    int interleaved;
+    long long q_batch_stride, q_token_stride, k_batch_stride, k_token_stride;
+    long long qy_batch_stride, qy_token_stride, ky_batch_stride, ky_token_stride;
+    const int32_t* positions_dev;    /* [batch][seq]                         */
+    const float* table_dev;          /* [max_positions][rotary_dim / 2][2]   */
+    int max_positions;
+} nnrh_rotary_desc;
+int nnrh_rotary(const nnrh_rotary_desc* d, const void* q_dev, const void* k_dev, void* qy_dev, void* ky_dev,
+                void* stream);
+
+/* Attention of prompts to themselves: sequence b is tokens starts[b] .. starts[b +
+ * 1] - 1 of q, k, v and y (starts: int32 [seqs + 1] in device memory, ascending,
+ * within 0 .. tokens, read when the kernel runs; sequences may be empty). Query (i,
+ * h) of a sequence sees its tokens 0 .. i (causal) or all of them, with key/value
+ * head h / (q_heads / kv_heads):
+ *   y = sum_j softmax_j(scale q k_j) v_j.
+ * What a token does not see has no effect, infinities and NaNs included. Tokens
+ * before the first sequence and behind the last are left as they are in y.
+ * Scores, totals and sums are fp32; weights meet 16-bit values rounded to their
+ * type. Values are such that 2^20 times the largest stays below 2^128 (fp16: any).
+ * q [tokens][q_heads][head_dim], k and v [tokens][kv_heads][head_dim] with token
+ * strides in elements (at most 2^22; heads are dense), y dense; addresses and strides
+ * in bytes are multiples of 16. y may be q itself where q is dense, and overlaps
+ * nothing else. head_dim 64, 96, 128 or 256. No workspace.                  */
+typedef struct nnrh_prompt_attention_desc {
+    int dtype;
+    int tokens, seqs, q_heads, kv_heads, head_dim;
+    long long q_stride, k_stride, v_stride;
+    float scale;
+    int causal;
+    const int32_t* starts_dev;
+} nnrh_prompt_attention_desc;
+int nnrh_prompt_attention(const nnrh_prompt_attention_desc* d, const void* q_dev, const void* k_dev, const void* v_dev,
+                          void* y_dev, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

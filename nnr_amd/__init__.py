@@ -14,12 +14,13 @@ import ctypes as ct
 import numpy as np
 
 from ._lib import (BF16, BRANCH_NAMES, F16, F32, I32, NNRH_ERR_UNSUPPORTED, S8, U8, NnrHipError,  # noqa: F401
-                   KvAttentionDesc, KvCacheDesc, KvTokens, MatMulNBitsDesc, QConvDesc,
-                   QMatMulDesc, check, cur_stream, lib, ptr)
+                   KvAttentionDesc, KvCacheDesc, KvMoves, KvTokens, MatMulNBitsDesc, PromptAttentionDesc, QConvDesc,
+                   QMatMulDesc, RotaryDesc, check, cur_stream, lib, ptr)
 
 __all__ = ["QLinearConv", "QLinearMatMul", "MatMulIntegerScaled", "MatMulInteger", "quantize_linear",
            "dequantize_linear", "dynamic_quantize_linear", "qlinear_add", "maxpool_u8_nhwc",
-           "conv_dispatch", "MatMulNBits", "KVCache", "NnrHipError", "lib"]
+           "conv_dispatch", "MatMulNBits", "KVCache", "copy_pages", "move_tokens", "RotaryEmbedding", "prompt_attention",
+           "NnrHipError", "lib"]
 
 
 def _dt(np_dtype) -> int:
@@ -782,15 +783,18 @@ class KVCache:
         return max(sizes)
 
     def attention(self, q, page_table, seq_lens, scale=None, prefix_table=None, prefix_len=0, y=None, workspace=None,
-                  stream=None):
+                  stream=None, tree=None):
         """softmax(scale q K^T) V, scale 1 / sqrt(head_dim) unless given. Query
         (b, s) sees the first prefix_len tokens of the pages in prefix_table
         (int32 [pages], shared by the batch) and positions up to seq_lens[b] -
         seq + s of its own. workspace: a uint8 tensor of attention_workspace's
-        size, 256-byte aligned, made by the call unless given."""
+        size, 256-byte aligned, made by the call unless given.
+        tree: bool [batch, seq, seq], or [seq, seq] for the whole batch. The seq
+        newest tokens are drafts, then: query (b, s) sees the prefix, all positions
+        before the drafts, and draft j where tree[b, s, j] (itself only if so)."""
         if stream is not None:
             with _current(self.device, stream):
-                return self.attention(q, page_table, seq_lens, scale, prefix_table, prefix_len, y, workspace)
+                return self.attention(q, page_table, seq_lens, scale, prefix_table, prefix_len, y, workspace, tree=tree)
         torch = self._torch
         if q.dim() != 4:
             raise ValueError("q must be [batch, seq, heads, head_dim]")
@@ -815,6 +819,15 @@ class KVCache:
         d = KvAttentionDesc(_float_dt(q.dtype), B, S, Hq, st[0], st[1],
                             self.head_dim ** -0.5 if scale is None else float(scale), page_table.data_ptr(),
                             page_table.shape[1], seq_lens.data_ptr(), pt, int(prefix_len))
+        if tree is not None:
+            if tree.dtype is not torch.bool or tree.shape not in ((S, S), (B, S, S)):
+                raise ValueError(f"tree must be bool [{S}, {S}] or [{B}, {S}, {S}]")
+            if tree.device != self.device:
+                _on_device(self.device, tree=tree)
+            if tree.dim() == 3 and tree.stride(0) == 0:   # one that was expanded
+                tree = tree[0]
+            if not tree.is_contiguous():
+                tree = tree.contiguous()
         n = ct.c_size_t()
         rc = self._L.nnrh_kv_attention_workspace(self.desc, d, n)
         if rc:
@@ -827,5 +840,218 @@ class KVCache:
                     not workspace.is_contiguous():
                 raise ValueError(f"workspace must be contiguous uint8 of at least {n.value} elements on {self.device}")
             ws = workspace.data_ptr()
-        _launch(self._index, self._L.nnrh_kv_attention, self.desc, self.data.data_ptr(), d, q.data_ptr(), y.data_ptr(), ws)
+        if tree is not None:
+            _launch(self._index, self._L.nnrh_kv_tree_attention, self.desc, self.data.data_ptr(), d, tree.data_ptr(),
+                    S * S if tree.dim() == 3 else 0, q.data_ptr(), y.data_ptr(), ws)
+        else:
+            _launch(self._index, self._L.nnrh_kv_attention, self.desc, self.data.data_ptr(), d, q.data_ptr(), y.data_ptr(), ws)
         return y
+
+
+def _layers(caches):
+    """(the first, how many, their buffers) of one cache or several equal ones"""
+    if isinstance(caches, KVCache):
+        caches = (caches,)
+    if not caches:
+        raise ValueError("no caches")
+    first = caches[0]
+    shape = (first.num_pages, first.page_size, first.kv_heads, first.head_dim, first.bits)
+    for c in caches[1:]:
+        if (c.num_pages, c.page_size, c.kv_heads, c.head_dim, c.bits) != shape or c.device != first.device:
+            raise ValueError("the caches must agree in shape, bits and device")
+    return first, len(caches), (ct.c_void_p * len(caches))(*[c.data.data_ptr() for c in caches])
+
+
+def _int32_tensor(name, t, device, dim):
+    import torch
+    if t.dtype is not torch.int32 or t.dim() != dim:
+        raise ValueError(f"{name} must be int32, of {dim} dimension{'s' * (dim > 1)}")
+    if t.device != device:
+        _on_device(device, **{name: t})
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def copy_pages(caches, source, destination, stream=None):
+    """Page source[i] to page destination[i] (int32 tensors [n] on the caches'
+    device) in a KVCache, or in each of a sequence of equal ones (a model's layers):
+    a sequence is forked by copying its last page. Pairs with a page that does not
+    exist are skipped. No page may be the destination of two pairs, or the
+    destination of one and the source of another."""
+    cache, n, data = _layers(caches)
+    if stream is not None:
+        with _current(cache.device, stream):
+            return copy_pages(caches, source, destination)
+    source, destination = (_int32_tensor(name, t, cache.device, 1)
+                           for name, t in (("source", source), ("destination", destination)))
+    if source.shape != destination.shape:
+        raise ValueError(f"{source.numel()} sources, {destination.numel()} destinations")
+    _int32(pages=source.numel())
+    _launch(cache._index, cache._L.nnrh_kv_copy_pages, cache.desc, data, n, source.data_ptr(), destination.data_ptr(),
+            source.numel())
+
+
+def move_tokens(caches, page_table, source, destination, stream=None):
+    """What position source[b, i] of sequence b holds to position destination[b, i]
+    (int32 [batch, n], n up to 128), in a KVCache or in each of a sequence of equal
+    ones. Nothing is quantized again. All of a sequence's sources are read before
+    anything is written; pairs with a negative position or one that no page holds are
+    skipped. Destinations are distinct, on pages that are one sequence's each."""
+    cache, n, data = _layers(caches)
+    if stream is not None:
+        with _current(cache.device, stream):
+            return move_tokens(caches, page_table, source, destination)
+    page_table, source, destination = (
+        _int32_tensor(name, t, cache.device, 2)
+        for name, t in (("page_table", page_table), ("source", source), ("destination", destination)))
+    if source.shape != destination.shape or source.shape[0] != page_table.shape[0]:
+        raise ValueError(f"page_table, source and destination are of {page_table.shape[0]}, {tuple(source.shape)} and "
+                         f"{tuple(destination.shape)}")
+    _int32(batch=source.shape[0], count=source.shape[1], pages=page_table.shape[1])
+    moves = KvMoves(source.shape[0], source.shape[1], page_table.data_ptr(), page_table.shape[1], source.data_ptr(),
+                    destination.data_ptr())
+    _launch(cache._index, cache._L.nnrh_kv_move_tokens, cache.desc, data, n, moves)
+
+
+class RotaryEmbedding:
+    """Rotary positions of queries and keys: the pairs of a head's first
+    rotary_dim elements (all unless given; the rest is left alone) are turned by
+    position * f_i, f_i = base^(-2 i / rotary_dim). interleaved: pairs are (2 i,
+    2 i + 1), or else (i, i + rotary_dim / 2).
+
+    scaling, for contexts `factor` times as long as the `original_positions` (max_positions / factor
+    unless given) that a model was trained at:
+      "linear"  f_i / factor
+      "ntk"     the base times factor^(r / (r - 2)), r = rotary_dim: the lowest frequency is divided by factor
+      "yarn"    f_i where a pair turns 32 times and more within original_positions, f_i / factor where
+                not even once, a linear ramp between; cosines and sines times 0.1 ln(factor) + 1
+    frequencies: rotary_dim / 2 numbers in place of all that, with `magnitude` a
+    factor of cosines and sines (1 unless given). Tables are formed in 64 bits and held in 32, on
+    `device` or the current one."""
+
+    def __init__(self, head_dim, max_positions, base=10000.0, rotary_dim=None, interleaved=False, scaling=None,
+                 factor=1.0, original_positions=None, frequencies=None, magnitude=None, device=None):
+        torch = _use_torch()
+        r = head_dim if rotary_dim is None else rotary_dim
+        _int32(head_dim=head_dim, max_positions=max_positions, rotary_dim=r)
+        if head_dim <= 0 or max_positions <= 0 or not 0 <= r <= head_dim or r % 2:
+            raise ValueError(f"rotary_dim {r} of heads of {head_dim}, {max_positions} positions")
+        self.head_dim, self.max_positions, self.rotary_dim = int(head_dim), int(max_positions), int(r)
+        self.interleaved = bool(interleaved)
+        if frequencies is None:
+            if original_positions is None:
+                original_positions = max_positions / factor
+            frequencies, m = rotary_frequencies(r, base, scaling, factor, original_positions)
+            magnitude = m if magnitude is None else magnitude
+        f = torch.as_tensor(np.asarray(frequencies, np.float64))
+        if f.shape != (r // 2,):
+            raise ValueError(f"{tuple(f.shape)} frequencies, {r // 2} expected")
+        device = torch.device("cuda" if device is None else device)
+        angles = torch.arange(max_positions, dtype=torch.float64, device=device)[:, None] * f.to(device)
+        m = 1.0 if magnitude is None else float(magnitude)
+        self.table = torch.stack((angles.cos() * m, angles.sin() * m), -1).float()
+        self.device, self._index = self.table.device, self.table.device.index
+
+    def _dense(self, name, t):
+        if t.dim() != 4 or t.shape[3] != self.head_dim:
+            raise ValueError(f"{name} must be [batch, seq, heads, {self.head_dim}]")
+        if t.device != self.device:
+            _on_device(self.device, **{name: t})
+        st = t.stride()
+        return st[3] == 1 and (t.shape[2] <= 1 or st[2] == self.head_dim)
+
+    def __call__(self, q, k, positions, out=None, stream=None):
+        """(q, k) turned: q [batch, seq, heads, head_dim], k with heads of its own,
+        positions int32 [batch, seq] (negative: padding, left as it is; from
+        max_positions on: NaN). The first two axes may be strided. out: two tensors
+        for the results, (q, k) themselves to work in place; new ones unless given."""
+        if stream is not None:
+            with _current(self.device, stream):
+                return self(q, k, positions, out)
+        torch = _use_torch()
+        q, k = (t if self._dense(name, t) else t.contiguous() for name, t in (("q", q), ("k", k)))
+        B, S = q.shape[:2]
+        if k.shape[:2] != (B, S) or k.dtype != q.dtype:
+            raise ValueError("q and k must agree in batch, seq and type")
+        if positions.dtype is not torch.int32 or positions.shape != (B, S):
+            raise ValueError(f"positions must be int32 [{B}, {S}]")
+        if positions.device != self.device:
+            _on_device(self.device, positions=positions)
+        if not positions.is_contiguous():
+            positions = positions.contiguous()
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=q.dtype, device=q.device)
+        else:
+            for name, y, x in zip(("out[0]", "out[1]"), out, (q, k)):
+                if not self._dense(name, y) or y.shape != x.shape or y.dtype != q.dtype:
+                    raise ValueError(f"{name} must be {q.dtype} of {tuple(x.shape)} with dense heads")
+        if max(B, S, q.shape[2], k.shape[2]) > 0x7fffffff:
+            _int32(batch=B, seq=S, q_heads=q.shape[2], k_heads=k.shape[2])
+        d = RotaryDesc(_float_dt(q.dtype), B, S, q.shape[2], k.shape[2], self.head_dim, self.rotary_dim, self.interleaved,
+                       *[s for t in (q, k, *out) for s in t.stride()[:2]], positions.data_ptr(), self.table.data_ptr(),
+                       self.max_positions)
+        _launch(self._index, lib().nnrh_rotary, d, q.data_ptr(), k.data_ptr(), out[0].data_ptr(), out[1].data_ptr())
+        return tuple(out)
+
+
+def rotary_frequencies(rotary_dim, base=10000.0, scaling=None, factor=1.0, original_positions=None):
+    """(angles a position of the rotary_dim / 2 pairs, a factor for cosines and
+    sines) in 64 bits, as RotaryEmbedding says."""
+    if scaling not in (None, "none", "linear", "ntk", "yarn"):
+        raise ValueError(f"scaling {scaling!r}: linear, ntk or yarn")
+    if not (base > 0 and factor > 0):
+        raise ValueError(f"base {base}, factor {factor}")
+    r = rotary_dim
+    if scaling == "ntk" and r > 2:
+        base = base * factor ** (r / (r - 2))
+    f = float(base) ** (-np.arange(0, r, 2, dtype=np.float64) / max(r, 1))
+    if scaling == "linear":
+        return f / factor, 1.0
+    if scaling == "yarn":
+        if original_positions is None:
+            raise ValueError("yarn needs original_positions")
+        keep = np.clip((f * original_positions / (2 * np.pi) - 1) / 31, 0, 1)
+        return f * keep + f / factor * (1 - keep), 0.1 * float(np.log(factor)) + 1 if factor > 1 else 1.0
+    return f, 1.0
+
+
+def prompt_attention(q, k, v, starts, scale=None, causal=True, y=None, stream=None):
+    """softmax(scale q k^T) v of packed prompts to themselves, scale 1 /
+    sqrt(head_dim) unless given. q [tokens, q_heads, head_dim], k and v [tokens,
+    kv_heads, head_dim] in float32, float16 or bfloat16; tokens may be strided (slices of a fused
+    projection's output). Sequence b is tokens starts[b] .. starts[b + 1] - 1 (int32 [sequences +
+    1] on q's device, ascending); a token sees its sequence's tokens up to itself, or all
+    of them where causal is False. Tokens of no sequence are left as they are in
+    y, which is new memory unless it is given."""
+    torch = _use_torch()
+    if stream is not None:
+        with _current(q.device, stream):
+            return prompt_attention(q, k, v, starts, scale, causal, y)
+    if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2] or v.shape != k.shape:
+        raise ValueError("q, k and v must be [tokens, heads, head_dim], k and v with the same heads")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError("q, k and v must agree in type")
+    dt = _float_dt(q.dtype)
+    starts = _int32_tensor("starts", starts, q.device, 1)
+    if starts.numel() < 1:
+        raise ValueError("starts must name the first sequence's start and every one's end")
+    _on_device(q.device, k=k, v=v)
+    rows = []
+    for t in (q, k, v):
+        st = t.stride()
+        if st[2] != 1 or (t.shape[1] > 1 and st[1] != t.shape[2]) or t.data_ptr() % 16 or st[0] * t.element_size() % 16:
+            t = t.contiguous()
+            if t.data_ptr() % 16:
+                t = t.clone()
+        rows.append(t)
+    q, k, v = rows
+    if y is None:
+        y = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif y.shape != q.shape or y.dtype != q.dtype or y.device != q.device or not y.is_contiguous():
+        raise ValueError("y must be contiguous, of q's shape, type and device")
+    tokens, heads, hd = q.shape
+    if max(tokens, heads, hd, starts.numel()) > 0x7fffffff:
+        _int32(tokens=tokens, heads=heads, head_dim=hd, sequences=starts.numel())
+    d = PromptAttentionDesc(dt, tokens, starts.numel() - 1, heads, k.shape[1], hd, q.stride(0), k.stride(0), v.stride(0),
+                            hd ** -0.5 if scale is None else float(scale), bool(causal), starts.data_ptr())
+    _launch(q.device.index, lib().nnrh_prompt_attention, d, q.data_ptr(), k.data_ptr(), v.data_ptr(), y.data_ptr())
+    return y

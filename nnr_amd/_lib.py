@@ -49,7 +49,8 @@ EXPORTS = [
     "nnrh_gelu_f32", "nnrh_hardswish_f32", "nnrh_transpose_f32",
     "nnrh_matmul_nbits_create", "nnrh_matmul_nbits_run", "nnrh_matmul_nbits_destroy",
     "nnrh_kv_cache_bytes", "nnrh_kv_cache_write", "nnrh_kv_cache_read",
-    "nnrh_kv_attention_workspace", "nnrh_kv_attention",
+    "nnrh_kv_attention_workspace", "nnrh_kv_attention", "nnrh_kv_tree_attention",
+    "nnrh_kv_copy_pages", "nnrh_kv_move_tokens", "nnrh_rotary", "nnrh_prompt_attention",
 ]
 
 
@@ -116,6 +117,24 @@ class KvAttentionDesc(C.Structure):
         ("q_batch_stride", C.c_longlong), ("q_token_stride", C.c_longlong), ("scale", C.c_float),
         ("page_table_dev", C.c_void_p), ("max_pages", C.c_int), ("seq_lens_dev", C.c_void_p),
         ("prefix_table_dev", C.c_void_p), ("prefix_len", C.c_int)]
+
+
+class KvMoves(C.Structure):
+    _fields_ = [("batch", C.c_int), ("count", C.c_int), ("page_table_dev", C.c_void_p), ("max_pages", C.c_int),
+                ("source_dev", C.c_void_p), ("destination_dev", C.c_void_p)]
+
+
+class RotaryDesc(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("dtype", "batch", "seq", "q_heads", "k_heads", "head_dim", "rotary_dim",
+                                        "interleaved")] + [
+        (f"{t}_{n}_stride", C.c_longlong) for t in ("q", "k", "qy", "ky") for n in ("batch", "token")] + [
+        ("positions_dev", C.c_void_p), ("table_dev", C.c_void_p), ("max_positions", C.c_int)]
+
+
+class PromptAttentionDesc(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("dtype", "tokens", "seqs", "q_heads", "kv_heads", "head_dim")] + [
+        (n, C.c_longlong) for n in ("q_stride", "k_stride", "v_stride")] + [
+        ("scale", C.c_float), ("causal", C.c_int), ("starts_dev", C.c_void_p)]
 
 
 _lib = None
@@ -233,6 +252,11 @@ def lib():
         "nnrh_kv_cache_read": (i, [P(KvCacheDesc), vp, P(KvTokens), vp, vp, vp]),
         "nnrh_kv_attention_workspace": (i, [P(KvCacheDesc), P(KvAttentionDesc), P(sz)]),
         "nnrh_kv_attention": (i, [P(KvCacheDesc), vp, P(KvAttentionDesc), vp, vp, vp, vp]),
+        "nnrh_kv_tree_attention": (i, [P(KvCacheDesc), vp, P(KvAttentionDesc), vp, ll, vp, vp, vp, vp]),
+        "nnrh_kv_copy_pages": (i, [P(KvCacheDesc), P(vp), i, vp, vp, i, vp]),
+        "nnrh_kv_move_tokens": (i, [P(KvCacheDesc), P(vp), i, P(KvMoves), vp]),
+        "nnrh_rotary": (i, [P(RotaryDesc), vp, vp, vp, vp, vp]),
+        "nnrh_prompt_attention": (i, [P(PromptAttentionDesc), vp, vp, vp, vp, vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)

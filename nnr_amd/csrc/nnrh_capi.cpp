@@ -2530,8 +2530,11 @@ extern "C" int nnrh_kv_attention_workspace(const nnrh_kv_cache_desc* d, const nn
     return NNRH_OK;
 }
 
-extern "C" int nnrh_kv_attention(const nnrh_kv_cache_desc* d, const void* cache, const nnrh_kv_attention_desc* a,
-                                 const void* q, void* y, void* workspace, void* stream) {
+namespace {
+
+// tree: NULL (causal) or [batch][seq][seq] bytes, a sequence's tree_bs after the one before
+int kv_attention(const nnrh_kv_cache_desc* d, const void* cache, const nnrh_kv_attention_desc* a, const void* q, void* y,
+                 void* workspace, const uint8_t* tree, long long tree_bs, void* stream) {
     KvCache c;
     KvAttention r;
     int rc = kv_attention_args(d, cache, a, &c, &r);
@@ -2562,9 +2565,272 @@ extern "C" int nnrh_kv_attention(const nnrh_kv_cache_desc* d, const void* cache,
         if (over_tables(p, bytes, a->page_table_dev, (long long)a->batch * a->max_pages, a->seq_lens_dev, a->batch) ||
             overlap(p, bytes, a->prefix_table_dev, prefix_entries * 4))
             return set_err(NNRH_ERR_INVALID, "kv_attention: y or the workspace lies over a table or the lengths");
+    if (tree) {
+        const size_t tsize = (size_t)(a->batch - 1) * tree_bs + (size_t)a->seq * a->seq;
+        if (overlap(tree, tsize, y, ysize) || overlap(tree, tsize, workspace, need))
+            return set_err(NNRH_ERR_INVALID, "kv_tree_attention: y or the workspace lies over the tree");
+    }
     r.q = q;
     r.y = y;
+    r.tree = tree;
+    r.tree_bstride = tree_bs;
     ProfScope ps("kv_attention", S(stream));
     HIP_TRY(launch_kv_attention(c, r, workspace, S(stream)), "kv_attention");
+    return NNRH_OK;
+}
+
+}  // namespace
+
+extern "C" int nnrh_kv_attention(const nnrh_kv_cache_desc* d, const void* cache, const nnrh_kv_attention_desc* a,
+                                 const void* q, void* y, void* workspace, void* stream) {
+    return kv_attention(d, cache, a, q, y, workspace, nullptr, 0, stream);
+}
+
+extern "C" int nnrh_kv_tree_attention(const nnrh_kv_cache_desc* d, const void* cache, const nnrh_kv_attention_desc* a,
+                                      const uint8_t* tree, long long tree_batch_stride, const void* q, void* y,
+                                      void* workspace, void* stream) {
+    if (!a) return set_err(NNRH_ERR_INVALID, "kv_tree_attention: NULL description");
+    if (a->batch > 0 && a->seq > 0) {
+        if (!tree) return set_err(NNRH_ERR_INVALID, "kv_tree_attention: NULL tree");
+        if (a->seq > 4096) return set_err(NNRH_ERR_UNSUPPORTED, "kv_tree_attention: %d drafts (at most 4096)", a->seq);
+        if (tree_batch_stride != 0 && tree_batch_stride < (long long)a->seq * a->seq)
+            return set_err(NNRH_ERR_INVALID, "kv_tree_attention: trees of %d x %d drafts at a stride of %lld", a->seq, a->seq,
+                           tree_batch_stride);
+        if (tree_batch_stride > (1LL << 38))
+            return set_err(NNRH_ERR_UNSUPPORTED, "kv_tree_attention: a stride of %lld", tree_batch_stride);
+    }
+    return kv_attention(d, cache, a, q, y, workspace, tree, tree_batch_stride, stream);
+}
+
+namespace {
+
+// equal caches, each in a buffer of its own
+int kv_layers(const char* what, const KvCache& c, void* const* caches, int layers) {
+    if (layers < 0) return set_err(NNRH_ERR_INVALID, "%s: %d caches", what, layers);
+    // (distinct ones, as a block of each would write the same place: looked at pair by pair)
+    if (layers > 1024) return set_err(NNRH_ERR_UNSUPPORTED, "%s: %d caches (at most 1024)", what, layers);
+    if (layers && !caches) return set_err(NNRH_ERR_INVALID, "%s: NULL caches", what);
+    const size_t all = (size_t)c.num_pages * kv_page_bytes(c);
+    for (int i = 0; i < layers; ++i) {
+        if (!caches[i] && c.num_pages) return set_err(NNRH_ERR_INVALID, "%s: cache %d is NULL", what, i);
+        if ((uintptr_t)caches[i] & 15) return set_err(NNRH_ERR_INVALID, "%s: cache %d must be 16-byte aligned", what, i);
+        for (int j = 0; j < i; ++j)
+            if (overlap(caches[i], all, caches[j], all)) return set_err(NNRH_ERR_INVALID, "%s: caches %d and %d overlap", what, j, i);
+    }
+    return NNRH_OK;
+}
+int kv_clear_of(const char* what, const KvCache& c, void* const* caches, int layers, const void* p, long long entries) {
+    for (int i = 0; i < layers; ++i)
+        if (overlap(caches[i], (size_t)c.num_pages * kv_page_bytes(c), p, (size_t)entries * 4))
+            return set_err(NNRH_ERR_INVALID, "%s: cache %d lies over the call's page numbers or positions", what, i);
+    return NNRH_OK;
+}
+// fn(layers of a launch, how many)
+template <class F> int by_layers(void* const* caches, int layers, F fn) {
+    for (int at = 0; at < layers; at += KV_LAYERS) {
+        KvLayers l{};
+        const int n = std::min(layers - at, KV_LAYERS);
+        for (int i = 0; i < n; ++i) l.data[i] = (uint8_t*)caches[at + i];
+        const int rc = fn(l, n);
+        if (rc != NNRH_OK) return rc;
+    }
+    return NNRH_OK;
+}
+
+}  // namespace
+
+extern "C" int nnrh_kv_copy_pages(const nnrh_kv_cache_desc* d, void* const* caches, int layers, const int32_t* src,
+                                  const int32_t* dst, int n, void* stream) {
+    KvCache c;
+    int rc = kv_cache(d, nullptr, &c);
+    if (rc != NNRH_OK || (rc = kv_layers("kv_copy_pages", c, caches, layers)) != NNRH_OK) return rc;
+    if (n < 0) return set_err(NNRH_ERR_INVALID, "kv_copy_pages: %d pages", n);
+    if (!n || !layers) return NNRH_OK;
+    if (!src || !dst || (((uintptr_t)src | (uintptr_t)dst) & 3))
+        return set_err(NNRH_ERR_INVALID, "kv_copy_pages: page numbers NULL or not aligned");
+    if ((rc = kv_clear_of("kv_copy_pages", c, caches, layers, src, n)) ||
+        (rc = kv_clear_of("kv_copy_pages", c, caches, layers, dst, n)))
+        return rc;
+    ProfScope ps("kv_copy_pages", S(stream));
+    return by_layers(caches, layers, [&](const KvLayers& l, int count) {
+        HIP_TRY(launch_kv_copy_pages(c, l, count, src, dst, n, S(stream)), "kv_copy_pages");
+        return (int)NNRH_OK;
+    });
+}
+
+extern "C" int nnrh_kv_move_tokens(const nnrh_kv_cache_desc* d, void* const* caches, int layers, const nnrh_kv_moves* m,
+                                   void* stream) {
+    KvCache c;
+    int rc = kv_cache(d, nullptr, &c);
+    if (rc != NNRH_OK || (rc = kv_layers("kv_move_tokens", c, caches, layers)) != NNRH_OK) return rc;
+    if (!m) return set_err(NNRH_ERR_INVALID, "kv_move_tokens: NULL description");
+    if (m->batch < 0 || m->count < 0 || m->max_pages < 0)
+        return set_err(NNRH_ERR_INVALID, "kv_move_tokens: batch %d, %d tokens, %d pages", m->batch, m->count, m->max_pages);
+    // (a launch's threads, 256 a sequence, head and layer, under the runtime's 2^32)
+    if (m->batch > 65535 || m->count > KV_MOVES || (long long)m->max_pages * c.page_size > (1 << 30) ||
+        (long long)m->batch * 2 * c.heads * std::min(layers, KV_LAYERS) > (1 << 23))
+        return set_err(NNRH_ERR_UNSUPPORTED,
+                       "kv_move_tokens: batch %d (at most 65535), %d tokens (%d), %d pages of %d tokens (2^30), %d heads "
+                       "and %d caches (2^22 heads of sequences and caches)",
+                       m->batch, m->count, KV_MOVES, m->max_pages, c.page_size, c.heads, layers);
+    if (!m->batch || !m->count || !layers || !m->max_pages || !c.num_pages) return NNRH_OK;
+    if (!m->page_table_dev || !m->source_dev || !m->destination_dev ||
+        (((uintptr_t)m->page_table_dev | (uintptr_t)m->source_dev | (uintptr_t)m->destination_dev) & 3))
+        return set_err(NNRH_ERR_INVALID, "kv_move_tokens: table or positions NULL or not aligned");
+    const long long entries = (long long)m->batch * m->count;
+    if ((rc = kv_clear_of("kv_move_tokens", c, caches, layers, m->page_table_dev, (long long)m->batch * m->max_pages)) ||
+        (rc = kv_clear_of("kv_move_tokens", c, caches, layers, m->source_dev, entries)) ||
+        (rc = kv_clear_of("kv_move_tokens", c, caches, layers, m->destination_dev, entries)))
+        return rc;
+    const KvMoves a{m->page_table_dev, m->max_pages, m->batch, m->count, m->source_dev, m->destination_dev};
+    ProfScope ps("kv_move_tokens", S(stream));
+    return by_layers(caches, layers, [&](const KvLayers& l, int count) {
+        HIP_TRY(launch_kv_move_tokens(c, l, count, a, S(stream)), "kv_move_tokens");
+        return (int)NNRH_OK;
+    });
+}
+
+// ---------------------------------------------------------------------------
+// Rotary positions, attention of prompts
+
+namespace {
+
+// `width` elements at strides bs, ts, in bytes from `at` on
+struct Lines {
+    uintptr_t at;
+    size_t width, bs, ts;
+    int batch, seq;
+    size_t extent() const { return (batch - 1) * bs + (seq - 1) * ts + width; }
+    // one step that leads through all lines
+    bool even() const { return batch == 1 || seq == 1 || bs == seq * ts; }
+    size_t step() const { return seq > 1 ? ts : batch > 1 ? bs : 0; }
+};
+// Do lines of a and b share memory? Those of one wider tensor's rows (equal, even
+// steps) may lie between each other; of other patterns whose extents meet it is
+// taken for granted.
+bool share(const Lines& a, const Lines& b) {
+    if (!overlap((void*)a.at, a.extent(), (void*)b.at, b.extent())) return false;
+    const size_t step = a.step();
+    if (!a.even() || !b.even() || step != b.step() || step == 0) return true;
+    const size_t d = a.at <= b.at ? (b.at - a.at) % step : (step - (a.at - b.at) % step) % step;
+    return d < a.width || d + b.width > step;
+}
+
+}  // namespace
+
+extern "C" int nnrh_rotary(const nnrh_rotary_desc* d, const void* q, const void* k, void* qy, void* ky, void* stream) {
+    if (!d) return set_err(NNRH_ERR_INVALID, "rotary: NULL description");
+    const int type = float_type(d->dtype);
+    if (type < 0) return set_err(NNRH_ERR_UNSUPPORTED, "rotary: type %d (fp32, fp16 or bf16)", d->dtype);
+    if (d->batch < 0 || d->seq < 0 || d->q_heads < 0 || d->k_heads < 0 || d->head_dim <= 0 || d->max_positions <= 0)
+        return set_err(NNRH_ERR_INVALID, "rotary: batch %d, seq %d, %d and %d heads of %d, %d positions", d->batch, d->seq,
+                       d->q_heads, d->k_heads, d->head_dim, d->max_positions);
+    if (d->rotary_dim < 0 || d->rotary_dim > d->head_dim || d->rotary_dim % 2)
+        return set_err(NNRH_ERR_INVALID, "rotary: %d of %d elements (an even number)", d->rotary_dim, d->head_dim);
+    const long long heads = (long long)d->q_heads + d->k_heads;
+    // threads of a launch, one an element at most, in 31 bits
+    if (heads > (1 << 20) || d->head_dim > (1 << 16) ||
+        (double)d->batch * d->seq * (double)heads * d->head_dim >= (double)(1LL << 31))
+        return set_err(NNRH_ERR_UNSUPPORTED, "rotary: batch %d, seq %d, %lld heads of %d (2^31 elements)", d->batch, d->seq,
+                       heads, d->head_dim);
+    if (!d->batch || !d->seq || !heads) return NNRH_OK;
+    if ((d->q_heads && (!q || !qy)) || (d->k_heads && (!k || !ky)) || !d->positions_dev || (d->rotary_dim && !d->table_dev))
+        return set_err(NNRH_ERR_INVALID, "rotary: NULL argument");
+    const size_t es = float_type_size(type);
+    if ((((uintptr_t)q | (uintptr_t)k | (uintptr_t)qy | (uintptr_t)ky) & (es - 1)) || ((uintptr_t)d->positions_dev & 3) ||
+        ((uintptr_t)d->table_dev & 7))
+        return set_err(NNRH_ERR_INVALID, "rotary: alignment");
+    const struct { const void* p; int heads; long long bs, ts; bool out; } parts[4] = {
+        {q, d->q_heads, d->q_batch_stride, d->q_token_stride, false},
+        {k, d->k_heads, d->k_batch_stride, d->k_token_stride, false},
+        {qy, d->q_heads, d->qy_batch_stride, d->qy_token_stride, true},
+        {ky, d->k_heads, d->ky_batch_stride, d->ky_token_stride, true}};
+    Lines l[4];
+    for (int i = 0; i < 4; ++i) {
+        const long long width = (long long)parts[i].heads * d->head_dim, bs = parts[i].bs, ts = parts[i].ts;
+        if (!width) continue;
+        if (bs < 0 || ts < 0) return set_err(NNRH_ERR_INVALID, "rotary: strides %lld, %lld", bs, ts);
+        if (bs > (1LL << 38) || ts > (1LL << 38)) return set_err(NNRH_ERR_UNSUPPORTED, "rotary: strides %lld, %lld", bs, ts);
+        const bool rows = d->seq <= 1 || ts >= width, seqs = d->batch <= 1 || bs >= (d->seq - 1) * ts + width;
+        const bool inner = d->batch <= 1 || bs >= width, outer = d->seq <= 1 || ts >= (d->batch - 1) * bs + width;
+        if (parts[i].out && !(rows && seqs) && !(inner && outer))
+            return set_err(NNRH_ERR_INVALID, "rotary: rows at strides %lld, %lld overlap", bs, ts);
+        l[i] = Lines{(uintptr_t)parts[i].p, (size_t)width * es, (size_t)bs * es, (size_t)ts * es, d->batch, d->seq};
+    }
+    const size_t entries = (size_t)d->batch * d->seq;
+    for (int o = 2; o < 4; ++o) {
+        if (!parts[o].heads) continue;
+        for (int i = 0; i < o; ++i) {
+            if (!parts[i].heads) continue;
+            const bool same = i == o - 2 && l[i].at == l[o].at && (d->batch == 1 || l[i].bs == l[o].bs) &&
+                              (d->seq == 1 || l[i].ts == l[o].ts);   // in place
+            if (!same && share(l[i], l[o]))
+                return set_err(NNRH_ERR_INVALID, "rotary: a result lies over another tensor of the call");
+        }
+        if (overlap((void*)l[o].at, l[o].extent(), d->positions_dev, entries * 4) ||
+            overlap((void*)l[o].at, l[o].extent(), d->table_dev, (size_t)d->max_positions * d->rotary_dim * 4))
+            return set_err(NNRH_ERR_INVALID, "rotary: a result lies over the positions or the table");
+    }
+    Rotary r{};
+    if (d->q_heads)
+        r.r[0] = RotaryRows{q, qy, d->q_heads, d->q_batch_stride, d->q_token_stride, d->qy_batch_stride, d->qy_token_stride};
+    if (d->k_heads)
+        r.r[1] = RotaryRows{k, ky, d->k_heads, d->k_batch_stride, d->k_token_stride, d->ky_batch_stride, d->ky_token_stride};
+    for (RotaryRows& x : r.r) {   // (steps that are not taken say nothing)
+        if (d->batch == 1) x.xb = x.yb = 0;
+        if (d->seq == 1) x.xt = x.yt = 0;
+    }
+    r.type = type;
+    r.batch = d->batch;
+    r.seq = d->seq;
+    r.hd = d->head_dim;
+    r.rotary = d->rotary_dim;
+    r.interleaved = d->interleaved != 0;
+    r.positions = d->positions_dev;
+    r.table = (const float2*)d->table_dev;
+    r.held = d->max_positions;
+    ProfScope ps("rotary", S(stream));
+    HIP_TRY(launch_rotary(r, S(stream)), "rotary");
+    return NNRH_OK;
+}
+
+extern "C" int nnrh_prompt_attention(const nnrh_prompt_attention_desc* d, const void* q, const void* k, const void* v,
+                                     void* y, void* stream) {
+    if (!d) return set_err(NNRH_ERR_INVALID, "prompt_attention: NULL description");
+    const int type = float_type(d->dtype);
+    if (type < 0) return set_err(NNRH_ERR_UNSUPPORTED, "prompt_attention: type %d (fp32, fp16 or bf16)", d->dtype);
+    if (d->tokens < 0 || d->seqs < 0) return set_err(NNRH_ERR_INVALID, "prompt_attention: %d tokens, %d sequences", d->tokens, d->seqs);
+    if (d->kv_heads <= 0 || d->q_heads <= 0 || d->q_heads % d->kv_heads)
+        return set_err(NNRH_ERR_INVALID, "prompt_attention: %d query heads over %d", d->q_heads, d->kv_heads);
+    if (d->head_dim != 64 && d->head_dim != 96 && d->head_dim != 128 && d->head_dim != 256)
+        return set_err(NNRH_ERR_UNSUPPORTED, "prompt_attention: head size %d (64, 96, 128 or 256)", d->head_dim);
+    // rows and blocks (256 threads for 128 rows, and one block a sequence and head) in 31 bits and under 2^32 threads
+    if (d->kv_heads > 32767 || (double)d->tokens * d->q_heads >= (double)(1LL << 31) ||
+        (double)d->tokens * d->q_heads / 128 + (double)d->seqs * d->kv_heads > (double)(1 << 23))
+        return set_err(NNRH_ERR_UNSUPPORTED, "prompt_attention: %d tokens, %d sequences, %d heads over %d", d->tokens,
+                       d->seqs, d->q_heads, d->kv_heads);
+    if (!d->tokens || !d->seqs) return NNRH_OK;
+    if (!q || !k || !v || !y || !d->starts_dev) return set_err(NNRH_ERR_INVALID, "prompt_attention: NULL argument");
+    if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)y) & 15)
+        return set_err(NNRH_ERR_INVALID, "prompt_attention: q, k, v and y must be 16-byte aligned");
+    if ((uintptr_t)d->starts_dev & 3) return set_err(NNRH_ERR_INVALID, "prompt_attention: alignment of the starts");
+    const size_t es = float_type_size(type);
+    const size_t qw = (size_t)d->q_heads * d->head_dim * es, kw = (size_t)d->kv_heads * d->head_dim * es, n = d->tokens;
+    for (const long long st : {d->q_stride, d->k_stride, d->v_stride}) {
+        if (st < 0 || (n > 1 && st * es % 16))
+            return set_err(NNRH_ERR_INVALID, "prompt_attention: a stride of %lld (multiples of 16 bytes)", st);
+        // (64 rows of a tile in 31 bits)
+        if (st > (1 << 22)) return set_err(NNRH_ERR_UNSUPPORTED, "prompt_attention: a stride of %lld (at most 2^22)", st);
+    }
+    const size_t ysize = n * qw;
+    const auto extent = [&](long long st, size_t w) { return (n - 1) * st * es + w; };
+    const bool in_place = y == q && (n == 1 || (size_t)d->q_stride * es == qw);
+    if ((!in_place && overlap(y, ysize, q, extent(d->q_stride, qw))) || overlap(y, ysize, k, extent(d->k_stride, kw)) ||
+        overlap(y, ysize, v, extent(d->v_stride, kw)) || overlap(y, ysize, d->starts_dev, ((size_t)d->seqs + 1) * 4))
+        return set_err(NNRH_ERR_INVALID, "prompt_attention: y lies over q, k, v or the starts");
+    const PromptAttention a{q, k, v, y, type, d->q_stride, d->k_stride, d->v_stride, d->tokens, d->seqs, d->q_heads,
+                            d->kv_heads, d->head_dim, d->scale, d->causal != 0, d->starts_dev};
+    ProfScope ps("prompt_attention", S(stream));
+    HIP_TRY(launch_prompt_attention(a, S(stream)), "prompt_attention");
     return NNRH_OK;
 }

@@ -1,6 +1,8 @@
 // nnrh_decode.h -- operators of a decoder's serving step: products with 4-bit
-// weights (nnrh_nbits.hip), the quantized key/value cache (nnrh_kvcache.hip) and
-// the attention that reads it (nnrh_kvattn.hip). Shared with the C-ABI layer.
+// weights (nnrh_nbits.hip), rotary positions (nnrh_rotary.hip), attention of
+// prompts to themselves (nnrh_prompt.hip), the quantized key/value cache
+// (nnrh_kvcache.hip), pages and tokens moved within it (nnrh_kvmove.hip) and the
+// attention that reads it (nnrh_kvattn.hip). Shared with the C-ABI layer.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -99,9 +101,58 @@ struct KvAttention {
     const int32_t* lens;
     const int32_t* prefix_table;
     int prefix_len;
+    // drafts: does new token s see new token j, [seq][seq] bytes a sequence; NULL: causal
+    const uint8_t* tree;
+    long long tree_bstride;
 };
 // bytes of partial results; 0: one block sees all keys of its rows
 size_t kv_attention_workspace(const KvCache& c, const KvAttention& a);
 hipError_t launch_kv_attention(const KvCache& c, const KvAttention& a, void* workspace, hipStream_t s);
+
+// ---- pages and tokens moved within caches --------------------------------------
+constexpr int KV_LAYERS = 64;              // caches of a launch
+struct KvLayers { uint8_t* data[KV_LAYERS]; };
+constexpr int KV_MOVES = 128;              // tokens of a sequence that one call moves
+// pages src[i] -> dst[i], i < n, of every layer
+hipError_t launch_kv_copy_pages(const KvCache& c, const KvLayers& l, int layers, const int32_t* src, const int32_t* dst,
+                                int n, hipStream_t s);
+struct KvMoves {
+    const int32_t* table;
+    int max_pages, batch, n;
+    const int32_t* src;                    // [batch][n] positions
+    const int32_t* dst;
+};
+hipError_t launch_kv_move_tokens(const KvCache& c, const KvLayers& l, int layers, const KvMoves& m, hipStream_t s);
+
+// ---- rotary positions ----------------------------------------------------------
+struct RotaryRows {
+    const void* x;
+    void* y;
+    int heads;
+    long long xb, xt, yb, yt;              // strides of sequences and tokens, elements
+};
+struct Rotary {
+    RotaryRows r[2];                       // queries, keys
+    int type, batch, seq, hd;
+    int rotary;                            // elements that turn, the head's first
+    int interleaved;                       // pairs are neighbours, or else rotary / 2 apart
+    const int32_t* positions;              // [batch][seq]
+    const float2* table;                   // [held][rotary / 2]: cosine, sine
+    int held;
+};
+hipError_t launch_rotary(const Rotary& a, hipStream_t s);
+
+// ---- attention of packed prompts to themselves -----------------------------------
+struct PromptAttention {
+    const void *q, *k, *v;
+    void* y;                               // [tokens][q_heads][hd]
+    int type;
+    long long qs, ks, vs;                  // strides of tokens, elements
+    int tokens, seqs, q_heads, kv_heads, hd;
+    float scale;
+    int causal;
+    const int32_t* starts;                 // [seqs + 1]
+};
+hipError_t launch_prompt_attention(const PromptAttention& a, hipStream_t s);
 
 }  // namespace nnrh

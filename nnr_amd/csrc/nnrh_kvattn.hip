@@ -264,9 +264,12 @@ struct Job {
     long long len;               // tokens that the source holds
     int t0, t1;                  // tiles
     const int32_t* table;
+    int drafts;                  // position of the first draft (may be negative); with a prefix's rows, or none: the largest
 };
 
-template <int HD, int NP, int NR>
+// With drafts (TREE) a row's limit is its sequence's end, and of the tokens from
+// job.drafts on it sees those that its line of the tree names.
+template <bool TREE, int HD, int NP, int NR>
 __device__ __forceinline__ void set_rows(const AttnArgs& p, const Job& job, int row0, Rows<HD, NP, NR>& w) {
     const KvAttention& a = p.a;
     const int col = threadIdx.x & 15;
@@ -279,7 +282,7 @@ __device__ __forceinline__ void set_rows(const AttnArgs& p, const Job& job, int 
         const int tok = r / p.G, hq = job.head * p.G + (r - tok * p.G);   // tok counts over the batch in the prefix's rows
         w.at[t] = (job.pre ? tok : job.b * a.seq + tok) * a.q_heads + hq;
         long long l = job.len;
-        if (!job.pre) {
+        if (!job.pre && !TREE) {
             const long long last = (long long)scalar_load(a.lens, job.b) - a.seq + tok + 1;
             l = last < l ? last : l;
         }
@@ -293,6 +296,7 @@ __device__ __forceinline__ void set_rows(const AttnArgs& p, const Job& job, int 
         w.hi = max(w.hi, __shfl_xor(w.hi, o));
     }
     w.lo = __builtin_amdgcn_readfirstlane(w.lo);
+    if (TREE) w.lo = min(w.lo, max(job.drafts, 0));
     w.hi = __builtin_amdgcn_readfirstlane(w.hi);
 }
 
@@ -356,13 +360,27 @@ __device__ __forceinline__ float bf16_at(u4 w, int j) { return j & 1 ? bf16_hi(w
 // at 4 bits scales are in the operands, keys' over 2^ek, values' over 2^en). ek,
 // en: the units from here on. held: tokens in each tile; some: not all have 32.
 // after_keys, after_values: what can be done while the first are on their way.
-template <int HD, int BITS, int NP, int NR, int KT, class Key, class Value, class AfterKeys, class AfterValues>
-__device__ __forceinline__ void tile_step(Rows<HD, NP, NR>& w, int key0, const int* held, bool some, const u4* ks,
+// seen(t, key): whether row t sees the draft there (TREE).
+template <int HD, int BITS, int NP, int NR, int KT, bool TREE, class Seen_, class Key, class Value, class AfterKeys, class AfterValues>
+__device__ __forceinline__ void tile_step(Rows<HD, NP, NR>& w, Seen_ seen, int key0, const int* held, bool some, const u4* ks,
                                           const u4* vs, int ek, int en, Key key, Value value, AfterKeys after_keys,
                                           AfterValues after_values) {
     constexpr int NC = HD / 32, ND = HD / 16;
     constexpr float slack = NP == 1 ? kSlack : 0.0f, top = NP == 1 ? kTop - kSlack : kTop;
     const int g = (threadIdx.x & 63) >> 4;
+    // drafts that a row does not see, a bit each of a tile's: here, where registers are free
+    uint32_t hides = 0;
+    static_assert(NR * KT <= 4, "8 bits each");
+    if constexpr (TREE) {
+        if (key0 + 32 * KT > w.lo) {
+            stay_a_branch();
+#pragma unroll
+            for (int i = 0; i < NR * KT; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    hides |= (uint32_t)!seen(i / KT, key0 + 32 * (i % KT) + 16 * (j >> 2) + 4 * g + (j & 3)) << (8 * i + j);
+        }
+    }
     h8 kf[2 * NC];
 #pragma unroll
     for (int j = 0; j < 2 * NC; ++j) kf[j] = key(0, j);
@@ -417,7 +435,7 @@ __device__ __forceinline__ void tile_step(Rows<HD, NP, NR>& w, int key0, const i
                 const int end = min(w.lim[t] - key0 - 32 * z, held[z]) - 4 * g;
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    if (16 * (j >> 2) + (j & 3) >= end) s[t][z][j] = kNegInf;
+                    if ((16 * (j >> 2) + (j & 3) >= end) | (TREE && (hides >> (8 * (t * KT + z) + j) & 1))) s[t][z][j] = kNegInf;
             }
     }
     // running maximum: moved on only where a score outgrows it by more than the slack
@@ -630,9 +648,22 @@ template <int HD, int BITS> struct RawTile {
     }
 };
 
+// Does the row (its place among all) see the token at `key`, as far as the tree has
+// a say (key: of a tile that exists, maybe past the sequence's end). A byte is loaded
+// for any key, the first draft's where it is none, so that a tile's loads run side by
+// side; the prefix's rows, which see all, load the tree's first.
+__device__ __forceinline__ bool tree_sees(const AttnArgs& p, const Job& job, int row, int key) {
+    const int line = job.pre ? 0 : (row / p.a.q_heads - job.b * p.a.seq) * p.a.seq;
+    const int d = key - job.drafts;
+    const bool draft = key >= job.drafts && (unsigned)d < (unsigned)p.a.seq;
+    const uint8_t* tree = p.a.tree + job.b * p.a.tree_bstride;
+    const uint8_t sees = tree[(uint32_t)(line + (draft ? d : 0))];
+    return (!draft) | (sees != 0);
+}
+
 // next: the tile to load meanwhile
-template <int HD, int BITS, int NP>
-__device__ __forceinline__ void few_tile(const AttnArgs& p, Rows<HD, NP, 1>& w, Seen<BITS>& scales, RawTile<HD, BITS>& r,
+template <int HD, int BITS, int NP, bool TREE>
+__device__ __forceinline__ void few_tile(const AttnArgs& p, const Job& job, Rows<HD, NP, 1>& w, Seen<BITS>& scales, RawTile<HD, BITS>& r,
                                          int tile, int held, const TilePtr& next) {
     constexpr int NC = HD / 32;
     u4 vs[BITS == 8 ? 1 : NC];
@@ -658,8 +689,8 @@ __device__ __forceinline__ void few_tile(const AttnArgs& p, Rows<HD, NP, 1>& w, 
         en = max(w.eu, ceil_exp(__builtin_amdgcn_readfirstlane(umax16_32(top8(vs[0]))), kNoUnit));
     }
     const float fk = ldexpf(1.0f, -ek), fv = ldexpf(1.0f, -en);
-    tile_step<HD, BITS, NP, 1, 1>(
-        w, tile * 32, &held, held < 32, &ks, vs, ek, en,
+    tile_step<HD, BITS, NP, 1, 1, TREE>(
+        w, [&](int t, int key) { return tree_sees(p, job, w.at[t], key); }, tile * 32, &held, held < 32, &ks, vs, ek, en,
         [&](int, int j) {
             if constexpr (BITS == 8) return codes8(r.k[j >> 1][2 * (j & 1)], r.k[j >> 1][2 * (j & 1) + 1]);
             else return key4(r.k[j >> 1][j & 1], j & 1 ? bf16_hi(kb[j >> 1]) : bf16_lo(kb[j >> 1]), fk);
@@ -718,7 +749,7 @@ __device__ __forceinline__ void put_rows(const AttnArgs& p, const Job& job, int 
 // elements, and holds elements 64 apart of the result, the mean so far. As near
 // to a sum in fp32 as that comes whatever the sizes of queries, keys and values,
 // and some 50 times as slow as the products.
-template <int HD, int BITS, int NP>
+template <int HD, int BITS, int NP, bool TREE>
 __device__ __forceinline__ void slow_row(const AttnArgs& p, const Job& job, int row, int lim) {
     constexpr int NC = HD / 32, BB = BITS == 8 ? 1024 : 512, NE = (HD + 63) / 64;
     const KvAttention& a = p.a;
@@ -759,7 +790,9 @@ __device__ __forceinline__ void slow_row(const AttnArgs& p, const Job& job, int 
             }
         }
         s = (s + __shfl_xor(s, 32)) * 1.44269504088896341f;
-        if (tok >= seen) s = kNegInf;
+        bool hidden = tok >= seen;
+        if constexpr (TREE) hidden |= !tree_sees(p, job, row, 32 * tile + tok);
+        s = hidden ? kNegInf : s;
         const float top = fmaxf(m, max16_32(max_16(s)));
         const float base = top == kNegInf ? 0.0f : top;
         const float w = exp2_(s - base);
@@ -769,7 +802,7 @@ __device__ __forceinline__ void slow_row(const AttnArgs& p, const Job& job, int 
         const float old = l * exp2_(m - base);
         l = old + sum;
         m = top;
-        const float inv = 1.0f / l;
+        const float inv = TREE && l == 0.0f ? 0.0f : 1.0f / l;   // (a tile may hold nothing that a draft sees)
 #pragma unroll
         for (int i = 0; i < NE; ++i) y[i] *= old * inv;
 #pragma unroll 1
@@ -804,7 +837,7 @@ __device__ __forceinline__ void slow_row(const AttnArgs& p, const Job& job, int 
     }
 }
 // of 16 rows (one a lane of the first group) those that are asked for, every `of`th from `first` on
-template <int HD, int BITS, int NP>
+template <int HD, int BITS, int NP, bool TREE>
 __device__ __forceinline__ void slow_rows(const Job& job, int at, int lim, bool again, int first, int of) {
     const uint32_t todo = (uint32_t)__ballot(again) & 0xffffu;
     if (!todo) return;
@@ -814,16 +847,16 @@ __device__ __forceinline__ void slow_rows(const Job& job, int at, int lim, bool 
     const AttnArgs& p = *(const AttnArgs*)args;
 #pragma unroll 1
     for (int i = first; i < 16; i += of)
-        if (todo >> i & 1) slow_row<HD, BITS, NP>(p, job, __builtin_amdgcn_readlane(at, i), __builtin_amdgcn_readlane(lim, i));
+        if (todo >> i & 1) slow_row<HD, BITS, NP, TREE>(p, job, __builtin_amdgcn_readlane(at, i), __builtin_amdgcn_readlane(lim, i));
 }
 
-template <int HD, int BITS, int NP>
+template <int HD, int BITS, int NP, bool TREE>
 __device__ __forceinline__ void few(const AttnArgs& p, Job& job, char* lds) {
     constexpr int ND = HD / 16;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
     Rows<HD, NP, 1> w;
-    set_rows(p, job, job.row0, w);
+    set_rows<TREE>(p, job, job.row0, w);
     job.t1 = min(job.t1, (w.hi + 31) / 32);
     int tile = job.t0 + wave;
     Seen<BITS> scales;
@@ -840,7 +873,7 @@ __device__ __forceinline__ void few(const AttnArgs& p, Job& job, char* lds) {
         load_rows<BITS>(p, w);
         for (; tile < job.t1; tile += AW) {
             const TilePtr after = at(tile + 2 * AW);
-            few_tile<HD, BITS, NP>(p, w, scales, raw, tile, cur.ok ? (int)min(job.len - (long long)tile * 32, 32ll) : 0, next);
+            few_tile<HD, BITS, NP, TREE>(p, job, w, scales, raw, tile, cur.ok ? (int)min(job.len - (long long)tile * 32, 32ll) : 0, next);
             cur = next;
             next = after;
         }
@@ -919,14 +952,15 @@ __device__ __forceinline__ void few(const AttnArgs& p, Job& job, char* lds) {
         for (int d = 0; d < ND; ++d) w.o[0][d] += buf[0][d][lane];
         put_rows(p, job, job.row0, w, unit, &mall, &lall, &again);
     }
-    slow_rows<HD, BITS, NP>(job, w.at[0], w.lim[0], again && job.row0 + col < job.nrows, wave, AW);
+    slow_rows<HD, BITS, NP, TREE>(job, w.at[0], w.lim[0], again && job.row0 + col < job.nrows, wave, AW);
 }
 template <int HD> constexpr int kFewLds = 2 * (HD / 16) * 1024 + 4 * AW * 64 + 2 * AW * 4;
 
 // ---- many rows: the block's waves split its rows ------------------------------
 // Tiles between two barriers: two, or one where two would not leave enough
-// registers (32 sequences after a prefix of 8192: 26.8 us, with two 30.1).
-template <int HD, int BITS> constexpr int kManyTiles = HD == 128 && BITS == 8 ? 1 : 2;
+// registers (32 sequences after a prefix of 8192: 26.8 us, with two 30.1), as
+// beside a tree's bits.
+template <int HD, int BITS, bool TREE> constexpr int kManyTiles = (HD == 128 && BITS == 8) || (TREE && HD >= 96 && HD <= 128) ? 1 : 2;
 
 // A tile is turned into operands once, a part by each wave, and lies in LDS
 // for all of them; the next tile is written beside it meanwhile, and the codes
@@ -976,9 +1010,9 @@ template <int HD, int BITS> struct Parts {
     }
 };
 
-template <int HD, int BITS, int NP, int NR>
+template <int HD, int BITS, int NP, int NR, bool TREE>
 __device__ __forceinline__ void many(const AttnArgs& p, Job& job, char* lds) {
-    constexpr int NC = HD / 32, NU = Parts<HD, BITS>::NU, KT = kManyTiles<HD, BITS>;
+    constexpr int NC = HD / 32, NU = Parts<HD, BITS>::NU, KT = kManyTiles<HD, BITS, TREE>;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15;
     h8(*frag)[KT][4 * NC][64] = (h8(*)[KT][4 * NC][64])lds;   // [2]: a tile's keys (c, i), then its values (c, i)
@@ -988,13 +1022,13 @@ __device__ __forceinline__ void many(const AttnArgs& p, Job& job, char* lds) {
     {
         const int last = min(job.row0 + AW * 16 * NR, job.nrows) - 1;
         long long hi = job.len;
-        if (!job.pre) {
+        if (!job.pre && !TREE) {
             const long long seen = (long long)scalar_load(p.a.lens, job.b) - p.a.seq + last / p.G + 1;
             hi = seen < hi ? seen : hi;
         }
         job.t1 = min(job.t1, hi > 0 ? (int)((hi + 31) / 32) : 0);
     }
-    set_rows(p, job, row0, w);   // (a wave past the rows repeats the last one)
+    set_rows<TREE>(p, job, row0, w);   // (a wave past the rows repeats the last one)
 
     Parts<HD, BITS> raw[KT] = {};
     int id[KT], held[KT], held_next[KT], ek = kNoUnit, ek_next = kNoUnit, en = kNoUnit, en_next = kNoUnit;
@@ -1101,8 +1135,8 @@ __device__ __forceinline__ void many(const AttnArgs& p, Job& job, char* lds) {
             en = max(w.eu, ceil_exp(__builtin_amdgcn_readfirstlane(umax16_32(vtop)), kNoUnit));
         }
         const h8(*f)[4 * NC][64] = frag[at];
-        tile_step<HD, BITS, NP, NR, KT>(
-            w, tile * 32, held, some, ks_raw, vs_raw, ek, en,
+        tile_step<HD, BITS, NP, NR, KT, TREE>(
+            w, [&](int t, int key) { return tree_sees(p, job, w.at[t], key); }, tile * 32, held, some, ks_raw, vs_raw, ek, en,
             [&](int z, int j) { return f[z][j][lane]; }, [&](int z, int j) { return f[z][2 * NC + j][lane]; },
             [&] {   // past the last tile for nothing: without a branch
                 convert(tile + KT, at ^ 1);
@@ -1133,9 +1167,9 @@ __device__ __forceinline__ void many(const AttnArgs& p, Job& job, char* lds) {
     put_rows(p, job, row0, w, w.eu, m, l, again);
 #pragma unroll
     for (int t = 0; t < NR; ++t)
-        slow_rows<HD, BITS, NP>(job, w.at[t], w.lim[t], again[t] && row0 + 16 * t + col < job.nrows, 0, 1);
+        slow_rows<HD, BITS, NP, TREE>(job, w.at[t], w.lim[t], again[t] && row0 + 16 * t + col < job.nrows, 0, 1);
 }
-template <int HD, int BITS> constexpr int kManyLds = 2 * kManyTiles<HD, BITS> * 4 * (HD / 32) * 1024;
+template <int HD, int BITS, bool TREE> constexpr int kManyLds = 2 * kManyTiles<HD, BITS, TREE> * 4 * (HD / 32) * 1024;
 
 // row tiles of a wave with many rows: two where they fit beside the rest
 template <int HD, int NP> constexpr int kManyRows = HD <= 128 && NP == 1 ? 2 : 1;
@@ -1143,9 +1177,10 @@ template <int HD, int NP> constexpr int kManyRows = HD <= 128 && NP == 1 ? 2 : 1
 // One block: rows of one key/value head against one split of the prefix or of
 // a sequence's tokens. PM, OM: the prefix's and the sequences' blocks have
 // many rows.
-template <int HD, int BITS, int NP, bool PM, bool OM>
+// TREE: the newest tokens are drafts.
+template <int HD, int BITS, int NP, bool PM, bool OM, bool TREE>
 __global__ __launch_bounds__(AW * 64, HD <= 128 ? (!PM && !OM && NP == 1 ? 3 : 2) : 1) void kv_attn_kernel(AttnArgs p) {
-    constexpr int few_lds = PM && OM ? 0 : kFewLds<HD>, many_lds = PM || OM ? kManyLds<HD, BITS> : 0;
+    constexpr int few_lds = PM && OM ? 0 : kFewLds<HD>, many_lds = PM || OM ? kManyLds<HD, BITS, TREE> : 0;
     __shared__ __attribute__((aligned(16))) char lds[few_lds > many_lds ? few_lds : many_lds];
     constexpr int NR = kManyRows<HD, NP>;
     const KvAttention& a = p.a;
@@ -1182,15 +1217,17 @@ __global__ __launch_bounds__(AW * 64, HD <= 128 ? (!PM && !OM && NP == 1 ? 3 : 2
         const long long cap = (long long)a.max_pages * p.c.page_size, len = scalar_load(a.lens, job.b);
         job.len = len < cap ? len : cap;
     }
+    job.drafts = 0x7fffffff;
+    if (TREE && !job.pre) job.drafts = scalar_load(a.lens, job.b) - a.seq;
     const int chunk = job.pre ? p.pre_chunk : p.own_chunk;
     job.t0 = job.split * chunk;
     job.t1 = job.t0 + chunk;   // cut to what the rows see further on
     const bool is_many = job.pre ? PM : OM;
     job.row0 = group * (is_many ? AW * 16 * NR : 16);
     if (is_many) {
-        if constexpr (PM || OM) many<HD, BITS, NP, NR>(p, job, lds);
+        if constexpr (PM || OM) many<HD, BITS, NP, NR, TREE>(p, job, lds);
     } else {
-        if constexpr (!(PM && OM)) few<HD, BITS, NP>(p, job, lds);
+        if constexpr (!(PM && OM)) few<HD, BITS, NP, TREE>(p, job, lds);
     }
 }
 
@@ -1285,11 +1322,16 @@ Plan plan(const KvCache& c, const KvAttention& a) {
     return p;
 }
 
+template <int HD, int BITS, int NP, bool TREE>
+void start(const AttnArgs& p, const Plan& pl, unsigned blocks, hipStream_t s) {
+    if (pl.own_many) kv_attn_kernel<HD, BITS, NP, true, true, TREE><<<blocks, AW * 64, 0, s>>>(p);
+    else if (pl.pre_many) kv_attn_kernel<HD, BITS, NP, true, false, TREE><<<blocks, AW * 64, 0, s>>>(p);
+    else kv_attn_kernel<HD, BITS, NP, false, false, TREE><<<blocks, AW * 64, 0, s>>>(p);
+}
 template <int HD, int BITS, int NP>
 hipError_t go(const AttnArgs& p, const Plan& pl, unsigned blocks, hipStream_t s) {
-    if (pl.own_many) kv_attn_kernel<HD, BITS, NP, true, true><<<blocks, AW * 64, 0, s>>>(p);
-    else if (pl.pre_many) kv_attn_kernel<HD, BITS, NP, true, false><<<blocks, AW * 64, 0, s>>>(p);
-    else kv_attn_kernel<HD, BITS, NP, false, false><<<blocks, AW * 64, 0, s>>>(p);
+    if (p.a.tree) start<HD, BITS, NP, true>(p, pl, blocks, s);
+    else start<HD, BITS, NP, false>(p, pl, blocks, s);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.slots == 1) return e;
     kv_join_kernel<HD><<<(unsigned)ceil_div(p.rows, 4), 256, 0, s>>>(p);

@@ -1,0 +1,468 @@
+// nnrh_prompt.hip -- attention of packed prompts to themselves, before their keys
+// and values go into a cache: row (token i, head) of a sequence of n tokens sees
+// tokens 0 .. i (or all n):
+//   y = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale (q k_j - m)).
+// One pass over the keys with a running maximum m and total (sums are rescaled when
+// m moves).
+//
+// The rows of one key/value head are its tokens' query heads side by side (token
+// major), so that a tile of keys serves all heads of a group, and a block's rows
+// see almost the same keys. A block has 4 waves of 32 rows; 64 keys (fp32: 32) are
+// brought into LDS by direct loads while the tile before is worked on.
+//   S^T = K Q^T (keys x rows),   O^T = V^T P^T (elements x rows)
+// by 32x32 MFMAs: a lane of S^T holds 16 scores of one row, 4 neighbouring keys at
+// a time, which are its part of the second product's operand as they are. V^T comes
+// out of LDS by transposing reads (16 bits) or one element a lane (fp32).
+//
+// fp32 tensors meet in fp32 MFMAs. 16-bit ones in 16-bit MFMAs with fp32 sums: the
+// weights p are rounded to the tensors' type (11 or 8 bits), which is as far off
+// as rounding the result is, and would cost a second product to avoid. They are
+// held as 2^top p: fp16 has no small numbers (p <= 2^15 there, and weights down to
+// 2^-35 of the largest keep a bit); in bf16 and fp32 a sum of largest numbers must
+// not pass them (2^20 equal weights of such values still do not).
+#include "nnrh_decode.h"
+
+#include <type_traits>
+
+namespace nnrh {
+namespace {
+
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef uint16_t us2 __attribute__((ext_vector_type(2)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+#define NNRH_LDS __attribute__((address_space(3)))
+
+constexpr int PW = 4, PR = 32;              // waves of a block, rows of a wave
+constexpr float kSlack = 4.0f;              // powers of two by which scores may outgrow the maximum that they refer to
+constexpr float kNegInf = -__builtin_inff();
+constexpr float kLeast = 1e-37f;            // a factor of 0 would make NaN of a masked score, -inf
+
+template <int TY> struct Type;
+template <> struct Type<FT_F32> {
+    static constexpr int size = 4, keys = 32;
+    static constexpr float top = -24.0f;
+};
+template <> struct Type<FT_F16> {
+    typedef h4 v4;
+    typedef h8 v8;
+    static constexpr int size = 2, keys = 64;
+    static constexpr float top = 11.0f;
+    static constexpr uint32_t inf = 0x7c00;
+    __device__ static __forceinline__ f16v mfma(u4 a, u4 b, f16v c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+    }
+};
+template <> struct Type<FT_BF16> {
+    typedef b4 v4;
+    typedef b8 v8;
+    static constexpr int size = 2, keys = 64;
+    static constexpr float top = -24.0f;
+    static constexpr uint32_t inf = 0x7f80;
+    __device__ static __forceinline__ f16v mfma(u4 a, u4 b, f16v c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+    }
+};
+
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float max_halves(float m) {   // over lanes 32 apart
+    const uint32_t u = __builtin_bit_cast(uint32_t, m);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+}
+// keeps the compiler from computing both sides of a branch that is hardly ever taken
+__device__ __forceinline__ void stay_a_branch() { asm volatile(""); }
+// the lane, for what is rarely done: nothing that follows from it is kept in registers before
+__device__ __forceinline__ int lane_here() {
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
+    return lane;
+}
+
+// ---- which rows a block has -------------------------------------------------------
+// Blocks of rows are numbered over all sequences: sequence b's begin at number
+// starts[b] G / BM + b, as rounding up adds at most one block each; numbers that no
+// rows are left for do nothing.
+struct Job {
+    int s, len;        // first token, tokens
+    int row0, nrows;   // the block's first row, rows of the sequence
+};
+__device__ __forceinline__ long long first_block(const PromptAttention& a, int G, int b) {
+    const int s = a.starts[b];
+    return (long long)min(max(s, 0), a.tokens) * G / (PW * PR) + b;
+}
+__device__ __forceinline__ bool find_job(const PromptAttention& a, int G, int number, Job& job) {
+    // the last sequence that does not begin after it: 64 looked at at once
+    const int lane = threadIdx.x & 63;
+    int lo = 0, n = a.seqs;
+    while (true) {
+        const int step = (n + 63) / 64;
+        const bool le = lane * step < n && first_block(a, G, lo + lane * step) <= number;
+        const int count = __popcll(__ballot(le));
+        if (!count) return false;
+        lo += (count - 1) * step;
+        n = min(step, n - (count - 1) * step);
+        if (n <= 1) break;
+    }
+    const int b = __builtin_amdgcn_readfirstlane(lo);
+    const int s = min(max(a.starts[b], 0), a.tokens), e = min(max(a.starts[b + 1], s), a.tokens);
+    job.s = __builtin_amdgcn_readfirstlane(s);
+    job.len = __builtin_amdgcn_readfirstlane(e - s);
+    const long long row0 = (number - first_block(a, G, b)) * (PW * PR), nrows = (long long)job.len * G;
+    if (row0 >= nrows) return false;
+    job.row0 = __builtin_amdgcn_readfirstlane((int)row0);
+    job.nrows = (int)nrows;
+    return true;
+}
+
+// ---- tiles of keys and values in LDS -------------------------------------------------
+// A row of 16-byte chunks a token, at a place that is the chunk's number with some
+// bits turned by the token's, so that neither product's reads meet in a bank.
+template <int TY, int HD> struct Lds {
+    static constexpr int N = Type<TY>::keys;
+    static constexpr int real = HD * Type<TY>::size / 16;         // chunks of a row
+    static constexpr int CH = HD == 96 ? real * 4 / 3 : real;     // held, a power of two
+    static constexpr int tile = N * CH * 16;
+    static constexpr int loads = N * CH / (PW * 64);              // of a thread
+    // the keys' reads: 32 rows, one chunk
+    static __device__ __forceinline__ int key(int row) { return CH == 8 ? row >> 1 & 7 : row & 15; }
+    // the values': 16 bits: rows r .. r + 3 (and 4 further), 64 bytes of each; fp32:
+    // rows r and r + 4, 128 bytes of each
+    static __device__ __forceinline__ int value(int row) {
+        if (TY == FT_F32) return (row >> 2 & 1) << 3;
+        return CH == 8 ? (row >> 1 & 1) << 2 : (row & 3) << 2 | (row >> 2 & 3);
+    }
+};
+// A thread's loads of a tile: bytes from the tile's first row
+template <int TY, int HD> struct Loads {
+    uint32_t at[Lds<TY, HD>::loads];
+    __device__ __forceinline__ void set(uint32_t stride, bool values) {
+        typedef Lds<TY, HD> L;
+#pragma unroll
+        for (int i = 0; i < L::loads; ++i) {
+            const int id = i * PW * 64 + threadIdx.x, row = id / L::CH;
+            const int chunk = id % L::CH ^ (values ? L::value(row) : L::key(row));
+            at[i] = chunk < L::real ? row * stride + chunk * 16 : 0xfffffff0u;   // (none: nothing is read there)
+        }
+    }
+    // rows: those that are left from the tile's first on; what is past them reads as 0
+    __device__ __forceinline__ void load(const uint8_t* first, uint32_t stride, int rows, uint8_t* lds) const {
+        typedef Lds<TY, HD> L;
+        const uint32_t bytes = (uint32_t)(min(rows, L::N) - 1) * stride + HD * Type<TY>::size;
+        const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)first, (short)0, (int)bytes, 0x00020000);
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+        for (int i = 0; i < L::loads; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (NNRH_LDS void*)(lds + (i * PW + wave) * 1024), 16, (int)at[i], 0, 0, 0);
+    }
+};
+
+// ---- a wave's rows ---------------------------------------------------------------------
+template <int TY, int HD> struct Rows {
+    static constexpr int ND = HD / 32;
+    static constexpr int NQ = TY == FT_F32 ? HD / 8 : HD / 16;
+    u4 q[NQ];          // 16 bits: elements 16 i + 8 half ..; fp32: 8 i + 4 half ..
+    f16v o[ND];        // sums of 2^top p v: elements 32 d + 8 (r / 4) + 4 half + r % 4
+    float m, l;        // the raw score that weights refer to; the lane's total of 2^top p
+    float rk;          // scale log2 e > 0
+    int lim;           // keys that the row sees
+};
+
+// Scores of NB x 16 keys a lane, raw, to weights 2^top p. key0: of the tile;
+// masked: some row does not see all of it.
+template <int TY, int HD, int NB>
+__device__ __forceinline__ void weigh(Rows<TY, HD>& w, f16v* s, int key0, bool masked) {
+    const int half = (threadIdx.x & 63) >> 5;
+    if (masked) {
+        stay_a_branch();
+        const int end = w.lim - key0 - 4 * half;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (32 * b + 8 * (r >> 2) + (r & 3) >= end) s[b][r] = kNegInf;
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[b][r]);
+    mx = max_halves(mx);
+    // the maximum moves on only where a score outgrows it by more than the slack (a row's
+    // by itself: what other rows see has no part in its rounding)
+    const bool up = mx * w.rk > __builtin_fmaf(w.m, w.rk, kSlack);
+    if (__any(up)) {
+        stay_a_branch();
+        const float al = up ? exp2_((w.m - mx) * w.rk) : 1.0f;
+        w.m = up ? mx : w.m;
+        w.l *= al;
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d) w.o[d] *= al;
+    }
+    const float base = w.m == kNegInf ? 0.0f : w.m;
+    constexpr float top = Type<TY>::top;
+    float sum[2] = {0.0f, 0.0f};
+    const float off = top - base * w.rk;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            // (the difference first in fp32: of large scores' products little would be left)
+            const float x = TY == FT_F32 ? __builtin_fmaf(s[b][r] - base, w.rk, top) : __builtin_fmaf(s[b][r], w.rk, off);
+            s[b][r] = exp2_(x);
+            sum[r & 1] += s[b][r];
+        }
+    w.l += sum[0] + sum[1];
+}
+
+// V^T of a 16-bit tile: elements 32 d .. of keys 16 m + 8 (j / 4) + 4 half + j % 4
+template <int TY, int HD>
+__device__ __forceinline__ u4 value_operand(const uint8_t* v, int lane, int m, int d) {
+    typedef Lds<TY, HD> L;
+    const int half = lane >> 5, in = lane & 15;
+    u2 x[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        // 16 lanes read 4 rows of 16 elements, and get an element of 4 rows each
+        const int row = 16 * m + 8 * i + 4 * half + (in >> 2), e = 32 * d + (lane & 16) + 4 * (in & 3);
+        const uint8_t* at = v + row * L::CH * 16 + ((e >> 3 ^ L::value(row)) << 4) + (e & 4) * 2;
+        x[i] = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((NNRH_LDS s4*)at));
+    }
+    return u4{x[0][0], x[0][1], x[1][0], x[1][1]};
+}
+
+// Are there infinities or NaNs among the tile's values?
+template <int TY, int HD>
+__device__ __forceinline__ bool any_bad(const uint8_t* v) {
+    typedef Lds<TY, HD> L;
+    const int lane = lane_here();
+    us2 top = {0, 0};
+    bool bad = false;
+#pragma unroll 4
+    for (int i = lane; i < L::N * L::real; i += 64) {
+        const int row = i / L::real;
+        const u4 x = *(const u4*)(v + (row * L::CH + (i % L::real ^ L::value(row))) * 16);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (TY == FT_F32) bad |= (x[j] & 0x7fffffffu) >= 0x7f800000u;
+            else top = __builtin_elementwise_max(top, __builtin_bit_cast(us2, x[j] & 0x7fff7fffu));
+        }
+    }
+    if constexpr (TY != FT_F32) bad = top[0] >= Type<TY>::inf || top[1] >= Type<TY>::inf;
+    return __any(bad);
+}
+
+// O^T += V^T P^T over a tile. FINITE: of its finite values alone.
+template <int TY, int HD, bool FINITE>
+__device__ __forceinline__ void add_values(Rows<TY, HD>& w, const f16v* s, const uint8_t* v, int lane) {
+    const int half = lane >> 5;
+    if constexpr (TY == FT_F32) {
+        typedef Lds<TY, HD> L;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int row = 8 * (r >> 2) + 4 * half + (r & 3);
+#pragma unroll
+            for (int d = 0; d < HD / 32; ++d) {
+                const int e = 32 * d + (lane & 31);
+                float x = *(const float*)(v + (row * L::CH + (e >> 2 ^ L::value(row))) * 16 + (e & 3) * 4);
+                if (FINITE) x = fabsf(x) < __builtin_inff() ? x : 0.0f;
+                w.o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, s[0][r], w.o[d], 0, 0, 0);
+            }
+        }
+    } else {
+        typedef typename Type<TY>::v8 v8;
+#pragma unroll
+        for (int m = 0; m < Type<TY>::keys / 16; ++m) {
+            v8 p;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) p[j] = s[m >> 1][8 * (m & 1) + j];
+#pragma unroll
+            for (int d = 0; d < HD / 32; ++d) {
+                u4 x = value_operand<TY, HD>(v, lane, m, d);
+                if (FINITE) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {   // (an exponent of ones carries into the sign's place)
+                        const uint32_t bad = ((x[j] & 0x7fff7fffu) + (0x8000u - Type<TY>::inf) * 0x10001u) >> 15 & 0x10001u;
+                        x[j] &= ~(bad * 0xffffu);
+                    }
+                }
+                w.o[d] = Type<TY>::mfma(x, __builtin_bit_cast(u4, p), w.o[d]);
+            }
+        }
+    }
+}
+// What a row sees of a tile's infinities and NaNs
+template <int TY, int HD>
+__device__ __forceinline__ void add_others(Rows<TY, HD>& w, const uint8_t* v, int key0) {
+    typedef Lds<TY, HD> L;
+    const int half = lane_here() >> 5;
+#pragma unroll 1
+    for (int row = 0; row < L::N; ++row) {
+        if (!__any(key0 + row < w.lim)) break;
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int e = 32 * d + 8 * i + 4 * half, c = e * Type<TY>::size / 16;
+                const uint8_t* at = v + (row * L::CH + (c ^ L::value(row))) * 16 + e * Type<TY>::size % 16;
+                float x[4];
+                if constexpr (TY == FT_F32) {
+                    const f4 y = *(const f4*)at;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) x[r] = y[r];
+                } else {
+                    const typename Type<TY>::v4 y = *(const typename Type<TY>::v4*)at;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) x[r] = (float)y[r];
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (!(fabsf(x[r]) < __builtin_inff()) && key0 + row < w.lim) w.o[d][4 * i + r] += x[r];
+            }
+    }
+}
+
+template <int TY, int HD>
+__device__ __forceinline__ void raw_scores(const Rows<TY, HD>& w, f16v* s, const uint8_t* k, int lane) {
+    typedef Lds<TY, HD> L;
+    const int half = lane >> 5;
+#pragma unroll
+    for (int b = 0; b < L::N / 32; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[b][r] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < Rows<TY, HD>::NQ; ++i)
+#pragma unroll
+        for (int b = 0; b < L::N / 32; ++b) {
+            const int row = 32 * b + (lane & 31);
+            const u4 x = *(const u4*)(k + (row * L::CH + (2 * i + half ^ L::key(row))) * 16);
+            if constexpr (TY == FT_F32) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    s[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(__builtin_bit_cast(float, (uint32_t)x[j]),
+                                                                __builtin_bit_cast(float, (uint32_t)w.q[i][j]), s[b], 0, 0, 0);
+            } else {
+                s[b] = Type<TY>::mfma(x, w.q[i], s[b]);
+            }
+        }
+}
+
+template <int TY, int HD>
+__global__ __launch_bounds__(PW * 64, HD <= 128 ? 2 : 1) void prompt_kernel(PromptAttention a, int G, int blocks) {
+    typedef Lds<TY, HD> L;
+    constexpr int ES = Type<TY>::size;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[2][2][L::tile];
+    // Heads first, so that a head's blocks stay on an XCD where heads are a multiple
+    // of 8; a sequence's last rows, which see most keys, begin first.
+    const int head = blockIdx.x % a.kv_heads;
+    Job job;
+    if (!find_job(a, G, blocks - 1 - (int)(blockIdx.x / a.kv_heads), job)) return;
+    const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    Rows<TY, HD> w;
+    const int row = min(job.row0 + wave * PR + col, job.nrows - 1);
+    const int tok = row / G, hq = head * G + row - tok * G;
+    w.lim = a.causal ? tok + 1 : job.len;
+    // keys that some row of the block sees, that all of them do, that some row of the wave does
+    const int block_hi = a.causal ? (min(job.row0 + PW * PR, job.nrows) - 1) / G + 1 : job.len;
+    const int block_lo = a.causal ? job.row0 / G + 1 : job.len;
+    const int hi = __builtin_amdgcn_readlane(w.lim, 31);
+
+    Loads<TY, HD> kl, vl;
+    const uint32_t ks = (uint32_t)(a.ks * ES), vs = (uint32_t)(a.vs * ES);
+    kl.set(ks, false);
+    vl.set(vs, true);
+    const uint8_t* k = (const uint8_t*)a.k + (job.s * a.ks + (long long)head * HD) * ES;
+    const uint8_t* v = (const uint8_t*)a.v + (job.s * a.vs + (long long)head * HD) * ES;
+    const auto load = [&](int key0, int at) {
+        kl.load(k + (long long)key0 * ks, ks, job.len - key0, lds[at][0]);
+        vl.load(v + (long long)key0 * vs, vs, job.len - key0, lds[at][1]);
+    };
+    load(0, 0);
+    {
+        const uint8_t* q = (const uint8_t*)a.q + ((job.s + (long long)tok) * a.qs + (long long)hq * HD) * ES + 16 * half;
+        const uint32_t sign = a.scale < 0.0f ? (TY == FT_F32 ? 0x80000000u : 0x80008000u) : 0u;   // (so that rk is positive)
+#pragma unroll
+        for (int i = 0; i < Rows<TY, HD>::NQ; ++i) w.q[i] = *(const u4*)(q + 32 * i) ^ u4{sign, sign, sign, sign};
+    }
+    w.rk = fmaxf(fabsf(a.scale) * 1.44269504088896341f, kLeast);
+    w.m = kNegInf;
+    w.l = 0.0f;
+#pragma unroll
+    for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) w.o[d][r] = 0.0f;
+
+    int at = 0, key0 = 0;
+    const auto next = [&] {
+        // this tile is there, and the one before has been read by all
+        __builtin_amdgcn_s_waitcnt(0);
+        asm volatile("s_barrier" ::: "memory");
+        if (key0 + L::N < block_hi) load(key0 + L::N, at ^ 1);
+    };
+    f16v s[L::N / 32];
+    for (; key0 + L::N <= block_lo; key0 += L::N, at ^= 1) {
+        next();
+        raw_scores<TY, HD>(w, s, lds[at][0], lane);
+        weigh<TY, HD, L::N / 32>(w, s, key0, false);
+        add_values<TY, HD, false>(w, s, lds[at][1], lane);
+    }
+    // the tiles that some of the block's rows see in part or not at all
+    for (; key0 < block_hi; key0 += L::N, at ^= 1) {
+        next();
+        if (key0 >= hi) continue;
+        raw_scores<TY, HD>(w, s, lds[at][0], lane_here());
+        weigh<TY, HD, L::N / 32>(w, s, key0, true);
+        if (any_bad<TY, HD>(lds[at][1])) {
+            stay_a_branch();
+            add_values<TY, HD, true>(w, s, lds[at][1], lane_here());
+            add_others<TY, HD>(w, lds[at][1], key0);
+        } else {
+            add_values<TY, HD, false>(w, s, lds[at][1], lane_here());
+        }
+    }
+    const float inv = 1.0f / (w.l + __shfl_xor(w.l, 32));
+    if (job.row0 + wave * PR + col >= job.nrows) return;
+    const long long y = ((job.s + (long long)tok) * a.q_heads + hq) * HD + 4 * half;
+#pragma unroll
+    for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f4 x;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[r] = w.o[d][4 * i + r] * inv;
+            const long long e = y + 32 * d + 8 * i;
+            if constexpr (TY == FT_F32) *(f4*)((float*)a.y + e) = x;
+            else if constexpr (TY == FT_F16) *(h4*)((_Float16*)a.y + e) = h4{(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3]};
+            else *(b4*)((__bf16*)a.y + e) = b4{(__bf16)x[0], (__bf16)x[1], (__bf16)x[2], (__bf16)x[3]};
+        }
+}
+
+template <int TY>
+hipError_t by_head(const PromptAttention& a, hipStream_t s) {
+    const int G = a.q_heads / a.kv_heads, blocks = (int)((long long)a.tokens * G / (PW * PR)) + a.seqs;
+    const unsigned grid = (unsigned)blocks * a.kv_heads;
+    switch (a.hd) {
+    case 64: prompt_kernel<TY, 64><<<grid, PW * 64, 0, s>>>(a, G, blocks); break;
+    case 96: prompt_kernel<TY, 96><<<grid, PW * 64, 0, s>>>(a, G, blocks); break;
+    case 128: prompt_kernel<TY, 128><<<grid, PW * 64, 0, s>>>(a, G, blocks); break;
+    case 256: prompt_kernel<TY, 256><<<grid, PW * 64, 0, s>>>(a, G, blocks); break;
+    default: return hipErrorInvalidValue;
+    }
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_prompt_attention(const PromptAttention& a, hipStream_t s) {
+    if (a.tokens == 0 || a.seqs == 0) return hipSuccess;
+    return a.type == FT_F32 ? by_head<FT_F32>(a, s) : a.type == FT_F16 ? by_head<FT_F16>(a, s) : by_head<FT_BF16>(a, s);
+}
+
+}  // namespace nnrh
