@@ -174,6 +174,24 @@ template <int TY, int HD> struct Rows {
     int lim;           // keys that the row sees
 };
 
+// The sums of wide heads lie in the accumulator half of the register file, which
+// products read and write but no other instruction does. Left to itself the compiler
+// takes all of them to the other half and back at every tile for this one that hardly
+// ever runs. (The waits are for a product's result, and before the next one.)
+template <int HD> __device__ __forceinline__ void scale_acc(f16v* o, float al) {
+    asm volatile("s_nop 15\n\ts_nop 15");
+#pragma unroll
+    for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            float x = o[d][r], y;
+            asm volatile("v_accvgpr_read_b32 %1, %0\n\ts_nop 1\n\tv_mul_f32 %1, %1, %2\n\ts_nop 1\n\tv_accvgpr_write_b32 %0, %1"
+                         : "+a"(x), "=&v"(y) : "v"(al));
+            o[d][r] = x;
+        }
+    asm volatile("s_nop 7");
+}
+
 // Scores of NB x 16 keys a lane, raw, to weights 2^top p. key0: of the tile;
 // masked: some row does not see all of it.
 template <int TY, int HD, int NB>
@@ -197,13 +215,17 @@ __device__ __forceinline__ void weigh(Rows<TY, HD>& w, f16v* s, int key0, bool m
     // the maximum moves on only where a score outgrows it by more than the slack (a row's
     // by itself: what other rows see has no part in its rounding)
     const bool up = mx * w.rk > __builtin_fmaf(w.m, w.rk, kSlack);
-    if (__any(up)) {
+    if (__builtin_expect(__any(up), 0)) {
         stay_a_branch();
         const float al = up ? exp2_((w.m - mx) * w.rk) : 1.0f;
         w.m = up ? mx : w.m;
         w.l *= al;
+        if constexpr (HD > 128) {
+            scale_acc<HD>(w.o, al);
+        } else {
 #pragma unroll
-        for (int d = 0; d < HD / 32; ++d) w.o[d] *= al;
+            for (int d = 0; d < HD / 32; ++d) w.o[d] *= al;
+        }
     }
     const float base = w.m == kNegInf ? 0.0f : w.m;
     constexpr float top = Type<TY>::top;
@@ -419,7 +441,7 @@ __global__ __launch_bounds__(PW * 64, HD <= 128 ? 2 : 1) void prompt_kernel(Prom
         if (key0 >= hi) continue;
         raw_scores<TY, HD>(w, s, lds[at][0], lane_here());
         weigh<TY, HD, L::N / 32>(w, s, key0, true);
-        if (any_bad<TY, HD>(lds[at][1])) {
+        if (__builtin_expect(any_bad<TY, HD>(lds[at][1]), 0)) {
             stay_a_branch();
             add_values<TY, HD, true>(w, s, lds[at][1], lane_here());
             add_others<TY, HD>(w, lds[at][1], key0);
