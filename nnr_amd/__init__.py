@@ -552,17 +552,17 @@ def maxpool_u8_nhwc(x, kH, kW, sH, sW, pH, pW, oH, oW):
 # a decoder's serving step
 
 _FLOAT_DT = {}   # torch type -> NNRH_*; filled with torch's first use here
-_torch_C = None
+_torch = _torch_C = None
 
 
 def _use_torch():
     """torch, which this package imports where it is first needed."""
-    global _torch_C
-    import torch
-    if _torch_C is None:
+    global _torch, _torch_C
+    if _torch is None:
+        import torch
         _FLOAT_DT.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
-        _torch_C = torch._C
-    return torch
+        _torch, _torch_C = torch, torch._C
+    return _torch
 
 
 def _float_dt(dtype) -> int:
@@ -703,6 +703,7 @@ class KVCache:
         self._torch, self._index, self._L = torch, self.device.index, lib()
         self.num_pages, self.page_size, self.kv_heads = int(num_pages), int(page_size), int(kv_heads)
         self.head_dim, self.bits = int(head_dim), int(bits)
+        self._shape = (self.num_pages, self.page_size, self.kv_heads, self.head_dim, self.bits, self.device)
 
     def _tables(self, batch, page_table, seq_lens):
         int32 = self._torch.int32
@@ -764,7 +765,8 @@ class KVCache:
                 return self.read(seq, page_table, seq_lens, dtype)
         B = page_table.shape[0]
         page_table, seq_lens = self._tables(B, page_table, seq_lens)
-        k, v = self._torch.empty((2, B, seq, self.kv_heads, self.head_dim), dtype=dtype, device=self.device).unbind(0)
+        k = self._torch.empty((B, seq, self.kv_heads, self.head_dim), dtype=dtype, device=self.device)
+        v = self._torch.empty_like(k)
         _launch(self._index, self._L.nnrh_kv_cache_read, self.desc, self.data.data_ptr(),
                 self._tokens(k, page_table, seq_lens), k.data_ptr(), v.data_ptr())
         return k, v
@@ -804,7 +806,7 @@ class KVCache:
         q = self._rows("q", q, Hq)
         page_table, seq_lens = self._tables(B, page_table, seq_lens)
         if y is None:
-            y = torch.empty((B, S, Hq, self.head_dim), dtype=q.dtype, device=self.device)
+            y = torch.empty_like(q, memory_format=torch.contiguous_format)
         elif y.shape != q.shape or y.dtype != q.dtype or y.device != self.device or not y.is_contiguous():
             raise ValueError("y must be contiguous, of q's shape, type and device")
         pt = None
@@ -854,17 +856,15 @@ def _layers(caches):
         caches = (caches,)
     if not caches:
         raise ValueError("no caches")
-    first = caches[0]
-    shape = (first.num_pages, first.page_size, first.kv_heads, first.head_dim, first.bits)
-    for c in caches[1:]:
-        if (c.num_pages, c.page_size, c.kv_heads, c.head_dim, c.bits) != shape or c.device != first.device:
+    first, n = caches[0], len(caches)
+    for c in caches:
+        if c._shape != first._shape:
             raise ValueError("the caches must agree in shape, bits and device")
-    return first, len(caches), (ct.c_void_p * len(caches))(*[c.data.data_ptr() for c in caches])
+    return first, n, (ct.c_void_p * n)(*[c.data.data_ptr() for c in caches])
 
 
 def _int32_tensor(name, t, device, dim):
-    import torch
-    if t.dtype is not torch.int32 or t.dim() != dim:
+    if t.dtype is not _use_torch().int32 or t.dim() != dim:
         raise ValueError(f"{name} must be int32, of {dim} dimension{'s' * (dim > 1)}")
     if t.device != device:
         _on_device(device, **{name: t})
@@ -881,13 +881,14 @@ def copy_pages(caches, source, destination, stream=None):
     if stream is not None:
         with _current(cache.device, stream):
             return copy_pages(caches, source, destination)
-    source, destination = (_int32_tensor(name, t, cache.device, 1)
-                           for name, t in (("source", source), ("destination", destination)))
-    if source.shape != destination.shape:
-        raise ValueError(f"{source.numel()} sources, {destination.numel()} destinations")
-    _int32(pages=source.numel())
-    _launch(cache._index, cache._L.nnrh_kv_copy_pages, cache.desc, data, n, source.data_ptr(), destination.data_ptr(),
-            source.numel())
+    source = _int32_tensor("source", source, cache.device, 1)
+    destination = _int32_tensor("destination", destination, cache.device, 1)
+    count = source.shape[0]
+    if destination.shape[0] != count:
+        raise ValueError(f"{count} sources, {destination.shape[0]} destinations")
+    if count > 0x7fffffff:
+        _int32(pages=count)
+    _launch(cache._index, cache._L.nnrh_kv_copy_pages, cache.desc, data, n, source.data_ptr(), destination.data_ptr(), count)
 
 
 def move_tokens(caches, page_table, source, destination, stream=None):
@@ -900,15 +901,15 @@ def move_tokens(caches, page_table, source, destination, stream=None):
     if stream is not None:
         with _current(cache.device, stream):
             return move_tokens(caches, page_table, source, destination)
-    page_table, source, destination = (
-        _int32_tensor(name, t, cache.device, 2)
-        for name, t in (("page_table", page_table), ("source", source), ("destination", destination)))
-    if source.shape != destination.shape or source.shape[0] != page_table.shape[0]:
-        raise ValueError(f"page_table, source and destination are of {page_table.shape[0]}, {tuple(source.shape)} and "
-                         f"{tuple(destination.shape)}")
-    _int32(batch=source.shape[0], count=source.shape[1], pages=page_table.shape[1])
-    moves = KvMoves(source.shape[0], source.shape[1], page_table.data_ptr(), page_table.shape[1], source.data_ptr(),
-                    destination.data_ptr())
+    page_table = _int32_tensor("page_table", page_table, cache.device, 2)
+    source = _int32_tensor("source", source, cache.device, 2)
+    destination = _int32_tensor("destination", destination, cache.device, 2)
+    (B, count), (rows, pages) = source.shape, page_table.shape
+    if destination.shape != source.shape or rows != B:
+        raise ValueError(f"page_table, source and destination are of {rows}, {(B, count)} and {tuple(destination.shape)}")
+    if max(B, count, pages) > 0x7fffffff:
+        _int32(batch=B, count=count, pages=pages)
+    moves = KvMoves(B, count, page_table.data_ptr(), pages, source.data_ptr(), destination.data_ptr())
     _launch(cache._index, cache._L.nnrh_kv_move_tokens, cache.desc, data, n, moves)
 
 
@@ -950,14 +951,16 @@ class RotaryEmbedding:
         m = 1.0 if magnitude is None else float(magnitude)
         self.table = torch.stack((angles.cos() * m, angles.sin() * m), -1).float()
         self.device, self._index = self.table.device, self.table.device.index
+        self._torch, self._table, self._run = torch, self.table.data_ptr(), lib().nnrh_rotary
 
     def _dense(self, name, t):
-        if t.dim() != 4 or t.shape[3] != self.head_dim:
+        """Do t's heads lie one behind another? Refuses what is no [batch, seq, heads, head_dim] on the device."""
+        shape, st = t.shape, t.stride()
+        if len(shape) != 4 or shape[3] != self.head_dim:
             raise ValueError(f"{name} must be [batch, seq, heads, {self.head_dim}]")
         if t.device != self.device:
             _on_device(self.device, **{name: t})
-        st = t.stride()
-        return st[3] == 1 and (t.shape[2] <= 1 or st[2] == self.head_dim)
+        return st[3] == 1 and (st[2] == self.head_dim or shape[2] <= 1)
 
     def __call__(self, q, k, positions, out=None, stream=None):
         """(q, k) turned: q [batch, seq, heads, head_dim], k with heads of its own,
@@ -967,10 +970,13 @@ class RotaryEmbedding:
         if stream is not None:
             with _current(self.device, stream):
                 return self(q, k, positions, out)
-        torch = _use_torch()
-        q, k = (t if self._dense(name, t) else t.contiguous() for name, t in (("q", q), ("k", k)))
-        B, S = q.shape[:2]
-        if k.shape[:2] != (B, S) or k.dtype != q.dtype:
+        torch, dtype = self._torch, q.dtype
+        if not self._dense("q", q):
+            q = q.contiguous()
+        if not self._dense("k", k):
+            k = k.contiguous()
+        (B, S, Hq, hd), (Bk, Sk, Hk, _) = q.shape, k.shape
+        if Bk != B or Sk != S or k.dtype is not dtype:
             raise ValueError("q and k must agree in batch, seq and type")
         if positions.dtype is not torch.int32 or positions.shape != (B, S):
             raise ValueError(f"positions must be int32 [{B}, {S}]")
@@ -979,18 +985,20 @@ class RotaryEmbedding:
         if not positions.is_contiguous():
             positions = positions.contiguous()
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=q.dtype, device=q.device)
+            dense = torch.contiguous_format
+            qy, ky = torch.empty_like(q, memory_format=dense), torch.empty_like(k, memory_format=dense)
         else:
-            for name, y, x in zip(("out[0]", "out[1]"), out, (q, k)):
-                if not self._dense(name, y) or y.shape != x.shape or y.dtype != q.dtype:
-                    raise ValueError(f"{name} must be {q.dtype} of {tuple(x.shape)} with dense heads")
-        if max(B, S, q.shape[2], k.shape[2]) > 0x7fffffff:
-            _int32(batch=B, seq=S, q_heads=q.shape[2], k_heads=k.shape[2])
-        d = RotaryDesc(_float_dt(q.dtype), B, S, q.shape[2], k.shape[2], self.head_dim, self.rotary_dim, self.interleaved,
-                       *[s for t in (q, k, *out) for s in t.stride()[:2]], positions.data_ptr(), self.table.data_ptr(),
-                       self.max_positions)
-        _launch(self._index, lib().nnrh_rotary, d, q.data_ptr(), k.data_ptr(), out[0].data_ptr(), out[1].data_ptr())
-        return tuple(out)
+            qy, ky = out
+            for name, y, x in (("out[0]", qy, q), ("out[1]", ky, k)):
+                if not self._dense(name, y) or y.shape != x.shape or y.dtype is not dtype:
+                    raise ValueError(f"{name} must be {dtype} of {tuple(x.shape)} with dense heads")
+        if max(B, S, Hq, Hk) > 0x7fffffff:
+            _int32(batch=B, seq=S, q_heads=Hq, k_heads=Hk)
+        a, b, c, e = q.stride(), k.stride(), qy.stride(), ky.stride()
+        d = RotaryDesc(_float_dt(dtype), B, S, Hq, Hk, hd, self.rotary_dim, self.interleaved, a[0], a[1], b[0], b[1],
+                       c[0], c[1], e[0], e[1], positions.data_ptr(), self._table, self.max_positions)
+        _launch(self._index, self._run, d, q.data_ptr(), k.data_ptr(), qy.data_ptr(), ky.data_ptr())
+        return qy, ky
 
 
 def rotary_frequencies(rotary_dim, base=10000.0, scaling=None, factor=1.0, original_positions=None):
@@ -1022,36 +1030,45 @@ def prompt_attention(q, k, v, starts, scale=None, causal=True, y=None, stream=No
     1] on q's device, ascending); a token sees its sequence's tokens up to itself, or all
     of them where causal is False. Tokens of no sequence are left as they are in
     y, which is new memory unless it is given."""
-    torch = _use_torch()
     if stream is not None:
         with _current(q.device, stream):
             return prompt_attention(q, k, v, starts, scale, causal, y)
-    if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2] or v.shape != k.shape:
+    torch = _use_torch()
+    shape, dtype, device = q.shape, q.dtype, q.device
+    dt = _float_dt(dtype)
+    if len(shape) != 3 or k.dim() != 3 or k.shape[0] != shape[0] or k.shape[2] != shape[2] or v.shape != k.shape:
         raise ValueError("q, k and v must be [tokens, heads, head_dim], k and v with the same heads")
-    if k.dtype != q.dtype or v.dtype != q.dtype:
+    if k.dtype is not dtype or v.dtype is not dtype:
         raise ValueError("q, k and v must agree in type")
-    dt = _float_dt(q.dtype)
-    starts = _int32_tensor("starts", starts, q.device, 1)
-    if starts.numel() < 1:
+    if k.device != device or v.device != device:
+        _on_device(device, k=k, v=v)
+    starts = _int32_tensor("starts", starts, device, 1)
+    seqs = starts.shape[0] - 1
+    if seqs < 0:
         raise ValueError("starts must name the first sequence's start and every one's end")
-    _on_device(q.device, k=k, v=v)
-    rows = []
-    for t in (q, k, v):
-        st = t.stride()
-        if st[2] != 1 or (t.shape[1] > 1 and st[1] != t.shape[2]) or t.data_ptr() % 16 or st[0] * t.element_size() % 16:
-            t = t.contiguous()
-            if t.data_ptr() % 16:
-                t = t.clone()
-        rows.append(t)
-    q, k, v = rows
+    q, qs = _dense_heads(q)
+    k, ks = _dense_heads(k)
+    v, vs = _dense_heads(v)
     if y is None:
-        y = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    elif y.shape != q.shape or y.dtype != q.dtype or y.device != q.device or not y.is_contiguous():
+        y = torch.empty_like(q, memory_format=torch.contiguous_format)
+    elif y.shape != shape or y.dtype is not dtype or y.device != device or not y.is_contiguous():
         raise ValueError("y must be contiguous, of q's shape, type and device")
-    tokens, heads, hd = q.shape
-    if max(tokens, heads, hd, starts.numel()) > 0x7fffffff:
-        _int32(tokens=tokens, heads=heads, head_dim=hd, sequences=starts.numel())
-    d = PromptAttentionDesc(dt, tokens, starts.numel() - 1, heads, k.shape[1], hd, q.stride(0), k.stride(0), v.stride(0),
+    tokens, heads, hd = shape
+    if max(tokens, heads, hd, seqs) > 0x7fffffff:
+        _int32(tokens=tokens, heads=heads, head_dim=hd, sequences=seqs)
+    d = PromptAttentionDesc(dt, tokens, seqs, heads, k.shape[1], hd, qs, ks, vs,
                             hd ** -0.5 if scale is None else float(scale), bool(causal), starts.data_ptr())
-    _launch(q.device.index, lib().nnrh_prompt_attention, d, q.data_ptr(), k.data_ptr(), v.data_ptr(), y.data_ptr())
+    _launch(device.index, lib().nnrh_prompt_attention, d, q.data_ptr(), k.data_ptr(), v.data_ptr(), y.data_ptr())
     return y
+
+
+def _dense_heads(t):
+    """[tokens, heads, head_dim] with dense heads and 16-byte steps, itself or a copy, and the tokens' step"""
+    st, shape = t.stride(), t.shape
+    if (st[2] != 1 or (st[1] != shape[2] and shape[1] > 1) or t.data_ptr() % 16 or
+            (st[0] * t.element_size() % 16 and shape[0] > 1)):
+        t = t.contiguous()
+        if t.data_ptr() % 16:
+            t = t.clone()
+        st = t.stride()
+    return t, st[0]

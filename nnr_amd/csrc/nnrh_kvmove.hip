@@ -48,29 +48,33 @@ __device__ __forceinline__ TokenAt token_at(const KvCache& c, const KvMoves& m, 
     return r;
 }
 
-// One block a sequence, head, keys or values, layer. All of its tokens are read
-// before any is written, so that a call may permute them. Keys move in words of
-// 8 elements; of values, where neighbours in memory are a tile's tokens, a token's
-// byte is stored by itself, and its nibble turned into the new one by an
-// exclusive-or with what is there: the word's other nibbles stay as they are whoever
-// else changes them, and whatever the order.
+// One block a sequence, head, keys or values, layer; its waves take its tokens in
+// turn, four at a time in flight. All of them are read before any is written, so
+// that a call may permute them. Keys move in words of 8 elements; of values, where
+// neighbours in memory are a tile's tokens, a token's byte is stored by itself, and
+// its nibble turned into the new one by an exclusive-or with what is there: the
+// word's other nibbles stay as they are whoever else changes them, and whatever the
+// order.
+constexpr int MU = 4;
 template <int BITS>
 __global__ __launch_bounds__(256) void kv_move_tokens_kernel(KvCache c, KvLayers l, KvMoves m) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     constexpr int BB = BITS == 8 ? 1024 : 512, KW = BITS == 8 ? 2 : 1;   // KW: words of 8 key codes
+    typedef uint32_t key_t __attribute__((ext_vector_type(KW)));
     const int head = blockIdx.y >> 1, values = blockIdx.y & 1, b = blockIdx.x;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const int NC = c.hd / 32, groups = BITS == 8 ? 1 : NC;
     uint8_t* data = l.data[blockIdx.z];
     TokenAt* from = (TokenAt*)lds;
     TokenAt* to = from + m.n;
-    uint16_t* scales = (uint16_t*)(to + m.n);                   // [n][groups]
-    uint32_t* codes = (uint32_t*)(scales + (m.n * groups + 1) / 2 * 2);   // keys: [n][hd / 8][KW]; values: a byte each
-    if ((int)threadIdx.x < m.n) {
-        const long long i = (long long)b * m.n + threadIdx.x;
-        TokenAt x = token_at(c, m, b, head, m.src[i]), y = token_at(c, m, b, head, m.dst[i]);
+    uint16_t* scales = (uint16_t*)(to + m.n);                             // [n][groups]
+    uint8_t* codes = (uint8_t*)(scales + (m.n * groups + 3) / 4 * 4);     // keys: [n][hd / 8][KW] words; values: a byte each
+    for (int i = threadIdx.x; i < m.n; i += blockDim.x) {
+        const long long at = (long long)b * m.n + i;
+        TokenAt x = token_at(c, m, b, head, m.src[at]), y = token_at(c, m, b, head, m.dst[at]);
         if (y.part < 0) x.part = -1;
-        from[threadIdx.x] = x;
-        to[threadIdx.x] = y;
+        from[i] = x;
+        to[i] = y;
     }
     __syncthreads();
     const long long cb = kv_codes_bytes(c.page_size, c.hd, BITS);
@@ -83,8 +87,7 @@ __global__ __launch_bounds__(256) void kv_move_tokens_kernel(KvCache c, KvLayers
     // eight key elements of a token
     const auto key_place = [&](const TokenAt& t, int oct) {
         const int in = t.tok & 31;
-        return (uint32_t*)(data + t.part + ((long long)(t.tok >> 5) * NC + (oct >> 2)) * BB) +
-               ((in & 15) + 16 * (oct & 3)) * 2 * KW + (in >> 4) * KW;
+        return (key_t*)(data + t.part + ((long long)(t.tok >> 5) * NC + (oct >> 2)) * BB) + ((in & 15) + 16 * (oct & 3)) * 2 + (in >> 4);
     };
     // the word that holds a token's value e, and which of its bytes or nibbles that is
     const auto value_place = [&](const TokenAt& t, int e, int* which) {
@@ -94,60 +97,63 @@ __global__ __launch_bounds__(256) void kv_move_tokens_kernel(KvCache c, KvLayers
         *which = BITS == 8 ? j & 3 : (j >> 1) + 4 * (j & 1);
         return BITS == 8 ? w + (j >> 2) : w;
     };
-    for (int i = threadIdx.x; i < m.n * groups; i += 256) {
-        const TokenAt t = from[i / groups];
-        if (t.part >= 0) scales[i] = *scale_place(t, i % groups);
-    }
-    if (!values) {
-        const int octs = c.hd / 8;
-        for (int i = threadIdx.x; i < m.n * octs; i += 256) {
-            const TokenAt t = from[i / octs];
-            if (t.part < 0) continue;
-            const uint32_t* p = key_place(t, i % octs);
+    // fn(token, place of the lane's element) over the wave's tokens and the elements `width` of a token, `load` first
+    // for MU of them
+    const auto each = [&](int width, auto load, auto store) {
+        for (int e = lane; e < width; e += 64)
+            for (int t0 = wave; t0 < m.n; t0 += MU * waves) {
+                decltype(load(0, 0)) x[MU];
+                bool some[MU];
 #pragma unroll
-            for (int k = 0; k < KW; ++k) codes[i * KW + k] = p[k];
-        }
-    } else {
-        for (int i = threadIdx.x; i < m.n * c.hd; i += 256) {
-            const TokenAt t = from[i / c.hd];
-            if (t.part < 0) continue;
-            int which;
-            const uint32_t w = *value_place(t, i % c.hd, &which);
-            ((uint8_t*)codes)[i] = (uint8_t)(BITS == 8 ? w >> (8 * which) : kv_unturn(w) >> (4 * which) & 15u);
-        }
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < m.n * groups; i += 256)
-        if (from[i / groups].part >= 0) *scale_place(to[i / groups], i % groups) = scales[i];
-    if (!values) {
-        const int octs = c.hd / 8;
-        for (int i = threadIdx.x; i < m.n * octs; i += 256) {
-            if (from[i / octs].part < 0) continue;
-            uint32_t* p = key_place(to[i / octs], i % octs);
+                for (int u = 0; u < MU; ++u) {
+                    const int t = t0 + u * waves;
+                    some[u] = t < m.n && from[t].part >= 0;
+                    if (some[u]) x[u] = load(t, e);
+                }
 #pragma unroll
-            for (int k = 0; k < KW; ++k) p[k] = codes[i * KW + k];
-        }
-    } else {
-        for (int i = threadIdx.x; i < m.n * c.hd; i += 256) {
-            if (from[i / c.hd].part < 0) continue;
-            int which;
-            uint32_t* p = value_place(to[i / c.hd], i % c.hd, &which);
-            const uint8_t code = ((const uint8_t*)codes)[i];
-            if constexpr (BITS == 8) {
-                ((uint8_t*)p)[which] = code;
-            } else {
-                // (what another thread does to the word meanwhile leaves this nibble)
-                const uint32_t old = kv_unturn(__hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) >> (4 * which) & 15u;
-                const uint32_t flip = kv_turn((old ^ code) << (4 * which));
-                if (flip) __hip_atomic_fetch_xor(p, flip, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                for (int u = 0; u < MU; ++u)
+                    if (some[u]) store(t0 + u * waves, e, x[u]);
             }
-        }
-    }
+    };
+    each(groups, [&](int t, int g) { return *scale_place(from[t], g); }, [&](int t, int g, uint16_t x) { scales[t * groups + g] = x; });
+    if (!values)
+        each(c.hd / 8, [&](int t, int o) { return *key_place(from[t], o); },
+             [&](int t, int o, key_t x) { ((key_t*)codes)[t * (c.hd / 8) + o] = x; });
+    else
+        each(c.hd,
+             [&](int t, int e) {
+                 int which;
+                 const uint32_t w = *value_place(from[t], e, &which);
+                 return BITS == 8 ? w >> (8 * which) & 255u : kv_unturn(w) >> (4 * which) & 15u;
+             },
+             [&](int t, int e, uint32_t x) { codes[t * c.hd + e] = (uint8_t)x; });
+    __syncthreads();
+    each(groups, [&](int t, int g) { return scales[t * groups + g]; }, [&](int t, int g, uint16_t x) { *scale_place(to[t], g) = x; });
+    if (!values)
+        each(c.hd / 8, [&](int t, int o) { return ((const key_t*)codes)[t * (c.hd / 8) + o]; },
+             [&](int t, int o, key_t x) { *key_place(to[t], o) = x; });
+    else
+        each(c.hd,
+             [&](int t, int e) {
+                 int which;
+                 const uint32_t* p = value_place(to[t], e, &which);
+                 const uint32_t code = codes[t * c.hd + e];
+                 if constexpr (BITS == 8) return code;
+                 // (what another thread does to the word meanwhile leaves this nibble)
+                 const uint32_t old = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                 return kv_turn((kv_unturn(old) >> (4 * which) & 15u ^ code) << (4 * which));
+             },
+             [&](int t, int e, uint32_t x) {
+                 int which;
+                 uint32_t* p = value_place(to[t], e, &which);
+                 if constexpr (BITS == 8) ((uint8_t*)p)[which] = (uint8_t)x;
+                 else if (x) __hip_atomic_fetch_xor(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+             });
 }
 
 size_t move_lds(const KvCache& c, int n) {
     const int groups = kv_groups(c.hd, c.bits);
-    return (size_t)n * 2 * sizeof(TokenAt) + (n * groups + 1) / 2 * 4 + (size_t)n * c.hd;
+    return (size_t)n * 2 * sizeof(TokenAt) + (n * groups + 3) / 4 * 8 + (size_t)n * c.hd;
 }
 
 }  // namespace
@@ -170,8 +176,9 @@ hipError_t launch_kv_copy_pages(const KvCache& c, const KvLayers& l, int layers,
 hipError_t launch_kv_move_tokens(const KvCache& c, const KvLayers& l, int layers, const KvMoves& m, hipStream_t s) {
     const dim3 grid((unsigned)m.batch, (unsigned)(2 * c.heads), (unsigned)layers);
     const size_t lds = move_lds(c, m.n);
-    if (c.bits == 8) kv_move_tokens_kernel<8><<<grid, 256, lds, s>>>(c, l, m);
-    else kv_move_tokens_kernel<4><<<grid, 256, lds, s>>>(c, l, m);
+    const int threads = 64 * std::min(4, (m.n + 7) / 8);
+    if (c.bits == 8) kv_move_tokens_kernel<8><<<grid, threads, lds, s>>>(c, l, m);
+    else kv_move_tokens_kernel<4><<<grid, threads, lds, s>>>(c, l, m);
     return hipGetLastError();
 }
 

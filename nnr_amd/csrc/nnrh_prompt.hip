@@ -22,7 +22,6 @@
 // not pass them (2^20 equal weights of such values still do not).
 #include "nnrh_decode.h"
 
-#include <type_traits>
 
 namespace nnrh {
 namespace {
@@ -40,19 +39,23 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 #define NNRH_LDS __attribute__((address_space(3)))
 
 constexpr int PW = 4, PR = 32;              // waves of a block, rows of a wave
+// A block's waves are KG groups: waves of different groups take different keys of a
+// tile for the same rows, and are joined at the end.
+template <int KG> constexpr int kBlockRows = PW / KG * PR;
+template <int TY, int KG> constexpr int kWaveKeys = TY != FT_F32 && KG == 1 ? 64 : 32;   // of a tile
 constexpr float kSlack = 4.0f;              // powers of two by which scores may outgrow the maximum that they refer to
 constexpr float kNegInf = -__builtin_inff();
 constexpr float kLeast = 1e-37f;            // a factor of 0 would make NaN of a masked score, -inf
 
 template <int TY> struct Type;
 template <> struct Type<FT_F32> {
-    static constexpr int size = 4, keys = 32;
+    static constexpr int size = 4;
     static constexpr float top = -24.0f;
 };
 template <> struct Type<FT_F16> {
     typedef h4 v4;
     typedef h8 v8;
-    static constexpr int size = 2, keys = 64;
+    static constexpr int size = 2;
     static constexpr float top = 11.0f;
     static constexpr uint32_t inf = 0x7c00;
     __device__ static __forceinline__ f16v mfma(u4 a, u4 b, f16v c) {
@@ -62,7 +65,7 @@ template <> struct Type<FT_F16> {
 template <> struct Type<FT_BF16> {
     typedef b4 v4;
     typedef b8 v8;
-    static constexpr int size = 2, keys = 64;
+    static constexpr int size = 2;
     static constexpr float top = -24.0f;
     static constexpr uint32_t inf = 0x7f80;
     __device__ static __forceinline__ f16v mfma(u4 a, u4 b, f16v c) {
@@ -86,35 +89,89 @@ __device__ __forceinline__ int lane_here() {
 }
 
 // ---- which rows a block has -------------------------------------------------------
-// Blocks of rows are numbered over all sequences: sequence b's begin at number
-// starts[b] G / BM + b, as rounding up adds at most one block each; numbers that no
-// rows are left for do nothing.
 struct Job {
     int s, len;        // first token, tokens
     int row0, nrows;   // the block's first row, rows of the sequence
 };
-__device__ __forceinline__ long long first_block(const PromptAttention& a, int G, int b) {
-    const int s = a.starts[b];
-    return (long long)min(max(s, 0), a.tokens) * G / (PW * PR) + b;
+// blocks of BM rows that tokens s .. e - 1 have
+template <int BM>
+__device__ __forceinline__ int blocks_of(const PromptAttention& a, int G, int s, int e) {
+    s = min(max(s, 0), a.tokens);
+    return (int)(((long long)(min(max(e, s), a.tokens) - s) * G + BM - 1) / BM);
 }
-__device__ __forceinline__ bool find_job(const PromptAttention& a, int G, int number, Job& job) {
-    // the last sequence that does not begin after it: 64 looked at at once
+template <int CTRL> __device__ __forceinline__ int dpp(int x) { return __builtin_amdgcn_update_dpp(x, x, CTRL, 0xf, 0xf, false); }
+// fn over all 64 lanes, in all of them: quads, halves and rows of 16 mirrored, then rows and halves exchanged
+template <class F> __device__ __forceinline__ int over_lanes(int x, F fn) {
+    x = fn(x, dpp<0xb1>(x));
+    x = fn(x, dpp<0x4e>(x));
+    x = fn(x, dpp<0x141>(x));
+    x = fn(x, dpp<0x140>(x));
+    const auto r = __builtin_amdgcn_permlane16_swap((uint32_t)x, (uint32_t)x, false, false);
+    x = fn((int)r[0], (int)r[1]);
+    const auto q = __builtin_amdgcn_permlane32_swap((uint32_t)x, (uint32_t)x, false, false);
+    return __builtin_amdgcn_readfirstlane(fn((int)q[0], (int)q[1]));
+}
+__device__ __forceinline__ int sum_lanes(int x) {
+    return over_lanes(x, [](int a, int b) { return a + b; });
+}
+template <int BM>
+__device__ __forceinline__ long long first_number(const PromptAttention& a, int G, int b) {
+    return (long long)min(max(a.starts[b], 0), a.tokens) * G / BM + b;
+}
+// Block `number` of a launch: sequence b and its block. Up to 64 sequences (a lane
+// each): all sequences' blocks by their place, the last places first, so that long
+// ones begin first wherever they are. More: sequence by sequence from the last one on;
+// one's blocks begin at number starts[b] G / BM + b, as rounding up adds at most one
+// each. Numbers that no rows are left for do nothing.
+template <int BM>
+__device__ __forceinline__ bool find_job(const PromptAttention& a, int G, int number, int numbers, Job& job) {
     const int lane = threadIdx.x & 63;
-    int lo = 0, n = a.seqs;
-    while (true) {
-        const int step = (n + 63) / 64;
-        const bool le = lane * step < n && first_block(a, G, lo + lane * step) <= number;
-        const int count = __popcll(__ballot(le));
-        if (!count) return false;
-        lo += (count - 1) * step;
-        n = min(step, n - (count - 1) * step);
-        if (n <= 1) break;
+    int b, block;
+    if (a.seqs <= 64) {
+        const int n = lane < a.seqs ? blocks_of<BM>(a, G, a.starts[lane], a.starts[lane + 1]) : 0;
+        // the place p with C(p + 1) <= number < C(p), C(p) = blocks at places p and up
+        int p = 0, above = 0;
+        if (a.seqs == 1) {
+            p = __builtin_amdgcn_readfirstlane(n) - 1 - number;
+            if (p < 0) return false;
+            above = number;
+        } else {
+            if (number >= sum_lanes(n)) return false;
+            int hi = over_lanes(n, [](int a, int b) { return max(a, b); });
+            while (hi - p > 1) {   // C(p) > number >= C(hi)
+                const int mid = (p + hi) >> 1, c = sum_lanes(max(n - mid, 0));
+                if (c > number) p = mid;
+                else hi = mid;
+            }
+            above = sum_lanes(max(n - p - 1, 0));
+        }
+        const unsigned long long have = __ballot(n > p);
+        const int rank = __builtin_amdgcn_mbcnt_hi((uint32_t)(have >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)have, 0));
+        const unsigned long long mine = __ballot(n > p && rank == number - above);
+        if (!mine) return false;   // (not reached: lanes past the sequences have no blocks)
+        b = __builtin_ctzll(mine);
+        block = p;
+    } else {
+        number = numbers - 1 - number;
+        // the last sequence that does not begin after it: 64 looked at at once
+        int lo = 0, n = a.seqs;
+        while (true) {
+            const int step = (n + 63) / 64;
+            const bool le = lane * step < n && first_number<BM>(a, G, lo + lane * step) <= number;
+            const int count = __popcll(__ballot(le));
+            if (!count) return false;
+            lo += (count - 1) * step;
+            n = min(step, n - (count - 1) * step);
+            if (n <= 1) break;
+        }
+        b = lo;
+        block = (int)(number - first_number<BM>(a, G, b));
     }
-    const int b = __builtin_amdgcn_readfirstlane(lo);
+    b = __builtin_amdgcn_readfirstlane(b);
     const int s = min(max(a.starts[b], 0), a.tokens), e = min(max(a.starts[b + 1], s), a.tokens);
     job.s = __builtin_amdgcn_readfirstlane(s);
     job.len = __builtin_amdgcn_readfirstlane(e - s);
-    const long long row0 = (number - first_block(a, G, b)) * (PW * PR), nrows = (long long)job.len * G;
+    const long long row0 = (long long)block * BM, nrows = (long long)job.len * G;
     if (row0 >= nrows) return false;
     job.row0 = __builtin_amdgcn_readfirstlane((int)row0);
     job.nrows = (int)nrows;
@@ -124,11 +181,11 @@ __device__ __forceinline__ bool find_job(const PromptAttention& a, int G, int nu
 // ---- tiles of keys and values in LDS -------------------------------------------------
 // A row of 16-byte chunks a token, at a place that is the chunk's number with some
 // bits turned by the token's, so that neither product's reads meet in a bank.
-template <int TY, int HD> struct Lds {
-    static constexpr int N = Type<TY>::keys;
+template <int TY, int HD, int KG> struct Lds {
+    static constexpr int NW = kWaveKeys<TY, KG>, N = KG * NW;     // tokens of a tile: a wave's, all
     static constexpr int real = HD * Type<TY>::size / 16;         // chunks of a row
     static constexpr int CH = HD == 96 ? real * 4 / 3 : real;     // held, a power of two
-    static constexpr int tile = N * CH * 16;
+    static constexpr int tile = N * CH * 16, part = NW * CH * 16;
     static constexpr int loads = N * CH / (PW * 64);              // of a thread
     // the keys' reads: 32 rows, one chunk
     static __device__ __forceinline__ int key(int row) { return CH == 8 ? row >> 1 & 7 : row & 15; }
@@ -140,10 +197,10 @@ template <int TY, int HD> struct Lds {
     }
 };
 // A thread's loads of a tile: bytes from the tile's first row
-template <int TY, int HD> struct Loads {
-    uint32_t at[Lds<TY, HD>::loads];
+template <int TY, int HD, int KG> struct Loads {
+    uint32_t at[Lds<TY, HD, KG>::loads];
     __device__ __forceinline__ void set(uint32_t stride, bool values) {
-        typedef Lds<TY, HD> L;
+        typedef Lds<TY, HD, KG> L;
 #pragma unroll
         for (int i = 0; i < L::loads; ++i) {
             const int id = i * PW * 64 + threadIdx.x, row = id / L::CH;
@@ -153,7 +210,7 @@ template <int TY, int HD> struct Loads {
     }
     // rows: those that are left from the tile's first on; what is past them reads as 0
     __device__ __forceinline__ void load(const uint8_t* first, uint32_t stride, int rows, uint8_t* lds) const {
-        typedef Lds<TY, HD> L;
+        typedef Lds<TY, HD, KG> L;
         const uint32_t bytes = (uint32_t)(min(rows, L::N) - 1) * stride + HD * Type<TY>::size;
         const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)first, (short)0, (int)bytes, 0x00020000);
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -244,9 +301,9 @@ __device__ __forceinline__ void weigh(Rows<TY, HD>& w, f16v* s, int key0, bool m
 }
 
 // V^T of a 16-bit tile: elements 32 d .. of keys 16 m + 8 (j / 4) + 4 half + j % 4
-template <int TY, int HD>
+template <int TY, int HD, int KG>
 __device__ __forceinline__ u4 value_operand(const uint8_t* v, int lane, int m, int d) {
-    typedef Lds<TY, HD> L;
+    typedef Lds<TY, HD, KG> L;
     const int half = lane >> 5, in = lane & 15;
     u2 x[2];
 #pragma unroll
@@ -259,15 +316,15 @@ __device__ __forceinline__ u4 value_operand(const uint8_t* v, int lane, int m, i
     return u4{x[0][0], x[0][1], x[1][0], x[1][1]};
 }
 
-// Are there infinities or NaNs among the tile's values?
-template <int TY, int HD>
+// Are there infinities or NaNs among the values of a wave's part of the tile?
+template <int TY, int HD, int KG>
 __device__ __forceinline__ bool any_bad(const uint8_t* v) {
-    typedef Lds<TY, HD> L;
+    typedef Lds<TY, HD, KG> L;
     const int lane = lane_here();
     us2 top = {0, 0};
     bool bad = false;
 #pragma unroll 4
-    for (int i = lane; i < L::N * L::real; i += 64) {
+    for (int i = lane; i < L::NW * L::real; i += 64) {
         const int row = i / L::real;
         const u4 x = *(const u4*)(v + (row * L::CH + (i % L::real ^ L::value(row))) * 16);
 #pragma unroll
@@ -281,11 +338,11 @@ __device__ __forceinline__ bool any_bad(const uint8_t* v) {
 }
 
 // O^T += V^T P^T over a tile. FINITE: of its finite values alone.
-template <int TY, int HD, bool FINITE>
+template <int TY, int HD, int KG, bool FINITE>
 __device__ __forceinline__ void add_values(Rows<TY, HD>& w, const f16v* s, const uint8_t* v, int lane) {
     const int half = lane >> 5;
     if constexpr (TY == FT_F32) {
-        typedef Lds<TY, HD> L;
+        typedef Lds<TY, HD, KG> L;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const int row = 8 * (r >> 2) + 4 * half + (r & 3);
@@ -300,13 +357,13 @@ __device__ __forceinline__ void add_values(Rows<TY, HD>& w, const f16v* s, const
     } else {
         typedef typename Type<TY>::v8 v8;
 #pragma unroll
-        for (int m = 0; m < Type<TY>::keys / 16; ++m) {
+        for (int m = 0; m < kWaveKeys<TY, KG> / 16; ++m) {
             v8 p;
 #pragma unroll
             for (int j = 0; j < 8; ++j) p[j] = s[m >> 1][8 * (m & 1) + j];
 #pragma unroll
             for (int d = 0; d < HD / 32; ++d) {
-                u4 x = value_operand<TY, HD>(v, lane, m, d);
+                u4 x = value_operand<TY, HD, KG>(v, lane, m, d);
                 if (FINITE) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {   // (an exponent of ones carries into the sign's place)
@@ -320,12 +377,12 @@ __device__ __forceinline__ void add_values(Rows<TY, HD>& w, const f16v* s, const
     }
 }
 // What a row sees of a tile's infinities and NaNs
-template <int TY, int HD>
+template <int TY, int HD, int KG>
 __device__ __forceinline__ void add_others(Rows<TY, HD>& w, const uint8_t* v, int key0) {
-    typedef Lds<TY, HD> L;
+    typedef Lds<TY, HD, KG> L;
     const int half = lane_here() >> 5;
 #pragma unroll 1
-    for (int row = 0; row < L::N; ++row) {
+    for (int row = 0; row < L::NW; ++row) {
         if (!__any(key0 + row < w.lim)) break;
 #pragma unroll
         for (int d = 0; d < HD / 32; ++d)
@@ -350,18 +407,18 @@ __device__ __forceinline__ void add_others(Rows<TY, HD>& w, const uint8_t* v, in
     }
 }
 
-template <int TY, int HD>
+template <int TY, int HD, int KG>
 __device__ __forceinline__ void raw_scores(const Rows<TY, HD>& w, f16v* s, const uint8_t* k, int lane) {
-    typedef Lds<TY, HD> L;
+    typedef Lds<TY, HD, KG> L;
     const int half = lane >> 5;
 #pragma unroll
-    for (int b = 0; b < L::N / 32; ++b)
+    for (int b = 0; b < L::NW / 32; ++b)
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[b][r] = 0.0f;
 #pragma unroll
     for (int i = 0; i < Rows<TY, HD>::NQ; ++i)
 #pragma unroll
-        for (int b = 0; b < L::N / 32; ++b) {
+        for (int b = 0; b < L::NW / 32; ++b) {
             const int row = 32 * b + (lane & 31);
             const u4 x = *(const u4*)(k + (row * L::CH + (2 * i + half ^ L::key(row))) * 16);
             if constexpr (TY == FT_F32) {
@@ -375,28 +432,78 @@ __device__ __forceinline__ void raw_scores(const Rows<TY, HD>& w, f16v* s, const
         }
 }
 
-template <int TY, int HD>
+// Waves that have seen other keys for the same rows: sums and totals by the rows'
+// common maximum, in the order of the groups. A wave ends up with the elements
+// 32 d .. where d % KG is its group's number. parts: [PW], of a wave.
+template <int TY, int HD, int KG>
+__device__ __forceinline__ void join(Rows<TY, HD>& w, int wave, uint8_t* lds) {
+    constexpr int ND = HD / 32;
+    const int lane = threadIdx.x & 63, col = lane & 31, group = wave % KG, first = wave - group;
+    float2(*ml)[PR] = (float2(*)[PR])lds;                                   // [PW]
+    f4(*sums)[ND][4][64] = (f4(*)[ND][4][64])(lds + sizeof(float2) * PW * PR);   // [PW]
+    w.l += __shfl_xor(w.l, 32);
+    __syncthreads();
+    if (lane < PR) ml[wave][col] = float2{w.m, w.l};
+    __syncthreads();
+    float m = kNegInf;
+#pragma unroll
+    for (int j = 0; j < KG; ++j) m = fmaxf(m, ml[first + j][col].x);
+    const auto factor = [&](float x) { return x == kNegInf ? 0.0f : exp2_((x - m) * w.rk); };
+    const float f = factor(w.m);
+    w.l = 0.0f;
+#pragma unroll
+    for (int j = 0; j < KG; ++j) {
+        const float2 v = ml[first + j][col];
+        w.l += v.y * factor(v.x);
+    }
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+        w.o[d] *= f;
+        if (d % KG == group) continue;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sums[wave][d][i][lane] = f4{w.o[d][4 * i], w.o[d][4 * i + 1], w.o[d][4 * i + 2], w.o[d][4 * i + 3]};
+    }
+    __syncthreads();
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+        if (d % KG != group) continue;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f4 x = {0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < KG; ++j)
+                x += j == group ? f4{w.o[d][4 * i], w.o[d][4 * i + 1], w.o[d][4 * i + 2], w.o[d][4 * i + 3]} : sums[first + j][d][i][lane];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) w.o[d][4 * i + r] = x[r];
+        }
+    }
+}
+template <int HD> constexpr int kJoinLds = PW * PR * 8 + PW * HD * PR * 4;
+
+template <int TY, int HD, int KG>
 __global__ __launch_bounds__(PW * 64, HD <= 128 ? 2 : 1) void prompt_kernel(PromptAttention a, int G, int blocks) {
-    typedef Lds<TY, HD> L;
-    constexpr int ES = Type<TY>::size;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[2][2][L::tile];
-    // Heads first, so that a head's blocks stay on an XCD where heads are a multiple
-    // of 8; a sequence's last rows, which see most keys, begin first.
+    typedef Lds<TY, HD, KG> L;
+    constexpr int ES = Type<TY>::size, BM = kBlockRows<KG>, NB = L::NW / 32;
+    constexpr int bytes = KG > 1 && kJoinLds<HD> > 4 * L::tile ? kJoinLds<HD> : 4 * L::tile;
+    __shared__ __attribute__((aligned(16))) uint8_t lds_[bytes];
+    uint8_t(*lds)[2][L::tile] = (uint8_t(*)[2][L::tile])lds_;   // [2]: keys, values
+    // Heads first, so that a head's blocks stay on an XCD where heads are a multiple of 8.
     const int head = blockIdx.x % a.kv_heads;
     Job job;
-    if (!find_job(a, G, blocks - 1 - (int)(blockIdx.x / a.kv_heads), job)) return;
+    if (!find_job<BM>(a, G, (int)(blockIdx.x / a.kv_heads), blocks, job)) return;
     const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int part = wave % KG, row0 = job.row0 + wave / KG * PR;
     Rows<TY, HD> w;
-    const int row = min(job.row0 + wave * PR + col, job.nrows - 1);
+    const int row = min(row0 + col, job.nrows - 1);
     const int tok = row / G, hq = head * G + row - tok * G;
     w.lim = a.causal ? tok + 1 : job.len;
     // keys that some row of the block sees, that all of them do, that some row of the wave does
-    const int block_hi = a.causal ? (min(job.row0 + PW * PR, job.nrows) - 1) / G + 1 : job.len;
+    const int block_hi = a.causal ? (min(job.row0 + BM, job.nrows) - 1) / G + 1 : job.len;
     const int block_lo = a.causal ? job.row0 / G + 1 : job.len;
     const int hi = __builtin_amdgcn_readlane(w.lim, 31);
 
-    Loads<TY, HD> kl, vl;
+    Loads<TY, HD, KG> kl, vl;
     const uint32_t ks = (uint32_t)(a.ks * ES), vs = (uint32_t)(a.vs * ES);
     kl.set(ks, false);
     vl.set(vs, true);
@@ -428,32 +535,37 @@ __global__ __launch_bounds__(PW * 64, HD <= 128 ? 2 : 1) void prompt_kernel(Prom
         asm volatile("s_barrier" ::: "memory");
         if (key0 + L::N < block_hi) load(key0 + L::N, at ^ 1);
     };
-    f16v s[L::N / 32];
+    f16v s[NB];
     for (; key0 + L::N <= block_lo; key0 += L::N, at ^= 1) {
         next();
-        raw_scores<TY, HD>(w, s, lds[at][0], lane);
-        weigh<TY, HD, L::N / 32>(w, s, key0, false);
-        add_values<TY, HD, false>(w, s, lds[at][1], lane);
+        raw_scores<TY, HD, KG>(w, s, lds[at][0] + part * L::part, lane);
+        weigh<TY, HD, NB>(w, s, key0, false);
+        add_values<TY, HD, KG, false>(w, s, lds[at][1] + part * L::part, lane);
     }
     // the tiles that some of the block's rows see in part or not at all
     for (; key0 < block_hi; key0 += L::N, at ^= 1) {
         next();
-        if (key0 >= hi) continue;
-        raw_scores<TY, HD>(w, s, lds[at][0], lane_here());
-        weigh<TY, HD, L::N / 32>(w, s, key0, true);
-        if (__builtin_expect(any_bad<TY, HD>(lds[at][1]), 0)) {
+        const int first = key0 + part * L::NW;   // the wave's part of the tile
+        const uint8_t* v = lds[at][1] + part * L::part;
+        if (first >= hi) continue;
+        raw_scores<TY, HD, KG>(w, s, lds[at][0] + part * L::part, lane_here());
+        weigh<TY, HD, NB>(w, s, first, true);
+        if (__builtin_expect(any_bad<TY, HD, KG>(v), 0)) {
             stay_a_branch();
-            add_values<TY, HD, true>(w, s, lds[at][1], lane_here());
-            add_others<TY, HD>(w, lds[at][1], key0);
+            add_values<TY, HD, KG, true>(w, s, v, lane_here());
+            add_others<TY, HD, KG>(w, v, first);
         } else {
-            add_values<TY, HD, false>(w, s, lds[at][1], lane_here());
+            add_values<TY, HD, KG, false>(w, s, v, lane_here());
         }
     }
-    const float inv = 1.0f / (w.l + __shfl_xor(w.l, 32));
-    if (job.row0 + wave * PR + col >= job.nrows) return;
+    if constexpr (KG > 1) join<TY, HD, KG>(w, wave, lds_);
+    else w.l += __shfl_xor(w.l, 32);
+    const float inv = 1.0f / w.l;
+    if (row0 + col >= job.nrows) return;
     const long long y = ((job.s + (long long)tok) * a.q_heads + hq) * HD + 4 * half;
 #pragma unroll
-    for (int d = 0; d < HD / 32; ++d)
+    for (int d = 0; d < HD / 32; ++d) {
+        if (d % KG != part) continue;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             f4 x;
@@ -464,20 +576,43 @@ __global__ __launch_bounds__(PW * 64, HD <= 128 ? 2 : 1) void prompt_kernel(Prom
             else if constexpr (TY == FT_F16) *(h4*)((_Float16*)a.y + e) = h4{(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3]};
             else *(b4*)((__bf16*)a.y + e) = b4{(__bf16)x[0], (__bf16)x[1], (__bf16)x[2], (__bf16)x[3]};
         }
+    }
 }
 
+template <int TY, int HD, int KG>
+hipError_t start(const PromptAttention& a, hipStream_t s) {
+    const int G = a.q_heads / a.kv_heads, blocks = (int)((long long)a.tokens * G / kBlockRows<KG>) + a.seqs;
+    prompt_kernel<TY, HD, KG><<<(unsigned)blocks * a.kv_heads, PW * 64, 0, s>>>(a, G, blocks);
+    return hipGetLastError();
+}
+// Groups by how many blocks of 128 rows there would be. With two or four, blocks are
+// shorter and more, at more loads a row and a join: where the chip is not full, or
+// full for so short that its last blocks count. Up to these (fp16, us, one group and
+// two: heads of 64, 12 of 4096 tokens, 396 blocks 58.7, 45.7; 32 over 8 of 2048, 520
+// 34.8, 35.6. Heads of 128, 453 blocks 65, 53; 516 34, 38. Heads of 256, one block
+// a CU, 263 84, 73; 396 161, 183. fp32, bound by its products: heads of 64, 664 64.5,
+// 53.3; heads of 128, 520 387, 340; 664 90, 116. Four groups and two: heads of 64,
+// 129 16.9, 21.0; 204 22.5, 22.7; heads of 128, 63 15.7, 18.6; 83 14.2, 10.8.)
+template <int TY, int HD> constexpr int kTwoGroups = HD > 128 ? (TY == FT_F32 ? 0 : 272) : TY != FT_F32 ? 448 : HD == 64 ? 1024 : 512;
+template <int TY, int HD> constexpr int kFourGroups = HD == 64 ? 128 : TY != FT_F32 && HD <= 128 ? 64 : 0;
+template <int TY, int HD>
+hipError_t by_blocks(const PromptAttention& a, hipStream_t s) {
+    const long long blocks = (long long)a.tokens * a.q_heads / kBlockRows<1> + (long long)a.seqs * a.kv_heads;
+    if constexpr (kFourGroups<TY, HD> > 0)
+        if (blocks <= kFourGroups<TY, HD>) return start<TY, HD, 4>(a, s);
+    if constexpr (kTwoGroups<TY, HD> > 0)
+        if (blocks <= kTwoGroups<TY, HD>) return start<TY, HD, 2>(a, s);
+    return start<TY, HD, 1>(a, s);
+}
 template <int TY>
 hipError_t by_head(const PromptAttention& a, hipStream_t s) {
-    const int G = a.q_heads / a.kv_heads, blocks = (int)((long long)a.tokens * G / (PW * PR)) + a.seqs;
-    const unsigned grid = (unsigned)blocks * a.kv_heads;
     switch (a.hd) {
-    case 64: prompt_kernel<TY, 64><<<grid, PW * 64, 0, s>>>(a, G, blocks); break;
-    case 96: prompt_kernel<TY, 96><<<grid, PW * 64, 0, s>>>(a, G, blocks); break;
-    case 128: prompt_kernel<TY, 128><<<grid, PW * 64, 0, s>>>(a, G, blocks); break;
-    case 256: prompt_kernel<TY, 256><<<grid, PW * 64, 0, s>>>(a, G, blocks); break;
-    default: return hipErrorInvalidValue;
+    case 64: return by_blocks<TY, 64>(a, s);
+    case 96: return by_blocks<TY, 96>(a, s);
+    case 128: return by_blocks<TY, 128>(a, s);
+    case 256: return by_blocks<TY, 256>(a, s);
     }
-    return hipGetLastError();
+    return hipErrorInvalidValue;
 }
 
 }  // namespace
