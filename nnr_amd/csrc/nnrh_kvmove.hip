@@ -5,6 +5,7 @@
 #include "nnrh_decode.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace nnrh {
 namespace {
@@ -48,112 +49,173 @@ __device__ __forceinline__ TokenAt token_at(const KvCache& c, const KvMoves& m, 
     return r;
 }
 
-// One block a sequence, head, keys or values, layer; its waves take its tokens in
-// turn, four at a time in flight. All of them are read before any is written, so
-// that a call may permute them. Keys move in words of 8 elements; of values, where
-// neighbours in memory are a tile's tokens, a token's byte is stored by itself, and
-// its nibble turned into the new one by an exclusive-or with what is there: the
-// word's other nibbles stay as they are whoever else changes them, and whatever the
-// order.
-constexpr int MU = 4;
-template <int BITS>
+// One block a sequence, head, keys or values, layer; its waves take tokens in turn.
+// All are read before any is written, so that a call may permute them. Keys move in
+// words of 8 elements. Of values, a word (two, 8 bits) holds 8 tokens of an element:
+// tokens that go to the same word are a chain, whose first loads it, puts all of
+// them in and stores it, so that no two lanes change one word. Bound by latency: the
+// positions, the table, the tokens, the words that they go to, each a trip to memory
+// (4 tokens of 2 caches x 8 heads of 128, 8 bits, 4.7 us; 7 of 64 sequences, 8
+// caches, 4 bits, 24: a key is 16 lines of memory with 4 bytes of it each, so that this is 117 MB).
+constexpr int MU = 4;   // tokens in flight a wave
+
+// a token's place, which is the same for all lanes, in scalar registers: a lane adds
+// its own part of the address
+struct Place {
+    long long part;
+    int tile, slot, in;   // tile of the page; of its tokens: the word of 8 (0 .. 3), the token
+};
+__device__ __forceinline__ Place place_of(const TokenAt& t) {
+    const long long part = t.part;
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)part), hi = __builtin_amdgcn_readfirstlane((int)(part >> 32));
+    const int tok = __builtin_amdgcn_readfirstlane(t.tok);
+    return Place{(long long)((uint64_t)hi << 32 | lo), tok >> 5, tok >> 2 & 3, tok & 31};
+}
+
+template <int BITS, int HD>
 __global__ __launch_bounds__(256) void kv_move_tokens_kernel(KvCache c, KvLayers l, KvMoves m) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-    constexpr int BB = BITS == 8 ? 1024 : 512, KW = BITS == 8 ? 2 : 1;   // KW: words of 8 key codes
-    typedef uint32_t key_t __attribute__((ext_vector_type(KW)));
+    constexpr int BB = BITS == 8 ? 1024 : 512, KW = BITS == 8 ? 2 : 1;   // KW: words of 8 codes
+    constexpr int NC = HD / 32, groups = BITS == 8 ? 1 : NC, NE = (HD + 63) / 64, octs = HD / 8;
+    typedef uint32_t word_t __attribute__((ext_vector_type(KW)));
     const int head = blockIdx.y >> 1, values = blockIdx.y & 1, b = blockIdx.x;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-    const int NC = c.hd / 32, groups = BITS == 8 ? 1 : NC;
     uint8_t* data = l.data[blockIdx.z];
     TokenAt* from = (TokenAt*)lds;
     TokenAt* to = from + m.n;
-    uint16_t* scales = (uint16_t*)(to + m.n);                             // [n][groups]
-    uint8_t* codes = (uint8_t*)(scales + (m.n * groups + 3) / 4 * 4);     // keys: [n][hd / 8][KW] words; values: a byte each
+    int* chain = (int*)(to + m.n);                                        // the next token of a word, + 1 << 16 for a first one
+    uint16_t* scales = (uint16_t*)(chain + (m.n + 1) / 2 * 2);            // [n][groups]
+    uint8_t* codes = (uint8_t*)(scales + (m.n * groups + 3) / 4 * 4);     // keys: [n][octs] words; values: a byte each
     for (int i = threadIdx.x; i < m.n; i += blockDim.x) {
         const long long at = (long long)b * m.n + i;
         TokenAt x = token_at(c, m, b, head, m.src[at]), y = token_at(c, m, b, head, m.dst[at]);
+        if (x.part < 0) y.part = -1;
         if (y.part < 0) x.part = -1;
         from[i] = x;
         to[i] = y;
     }
     __syncthreads();
-    const long long cb = kv_codes_bytes(c.page_size, c.hd, BITS);
+    if (values) {
+        // 8 tokens share a word: 4 g .. of a tile and those 16 further
+        const auto same = [&](const TokenAt& x, const TokenAt& y) {
+            return x.part == y.part && (x.tok >> 5) == (y.tok >> 5) && (x.tok >> 2 & 3) == (y.tok >> 2 & 3);
+        };
+        for (int i = threadIdx.x; i < m.n; i += blockDim.x) {
+            const TokenAt t = to[i];
+            int next = i + 1, before = i - 1;
+            while (next < m.n && !same(to[next], t)) ++next;
+            while (before >= 0 && !same(to[before], t)) --before;
+            chain[i] = next | (before < 0) << 16;
+        }
+    }
+    const long long cb = kv_codes_bytes(c.page_size, HD, BITS);
     const long long codes0 = values ? cb : 0, scales0 = 2 * cb + (values ? 2LL * c.page_size * groups : 0);
-    const auto scale_place = [&](const TokenAt& t, int g) {
-        const int in = t.tok & 31;
-        return (uint16_t*)(data + t.part + scales0) + (long long)g * c.page_size + (t.tok & ~31) +
-               (BITS == 4 && !values ? kv_pair(in) : kv_slot(in));
+    const auto scale_place = [&](const Place& t) {   // of group `lane`
+        return (uint16_t*)(data + t.part + scales0) + (t.tile * 32 + (BITS == 4 && !values ? kv_pair(t.in) : kv_slot(t.in))) +
+               lane * c.page_size;
     };
-    // eight key elements of a token
-    const auto key_place = [&](const TokenAt& t, int oct) {
-        const int in = t.tok & 31;
-        return (key_t*)(data + t.part + ((long long)(t.tok >> 5) * NC + (oct >> 2)) * BB) + ((in & 15) + 16 * (oct & 3)) * 2 + (in >> 4);
+    // a key's elements 8 lane ..
+    const auto key_place = [&](const Place& t) {
+        return (word_t*)(data + t.part + t.tile * (NC * BB)) + ((t.in & 15) * 2 + (t.in >> 4)) + ((lane >> 2) * (BB / (KW * 4)) + 32 * (lane & 3));
     };
-    // the word that holds a token's value e, and which of its bytes or nibbles that is
-    const auto value_place = [&](const TokenAt& t, int e, int* which) {
-        const int slot = kv_slot(t.tok & 31), j = slot & 7;
-        uint32_t* w = (uint32_t*)(data + t.part + codes0 + ((long long)(t.tok >> 5) * NC + (e >> 5)) * BB) +
-                      ((e & 15) + 16 * (slot >> 3)) * 2 * KW + (e >> 4 & 1) * KW;
-        *which = BITS == 8 ? j & 3 : (j >> 1) + 4 * (j & 1);
-        return BITS == 8 ? w + (j >> 2) : w;
+    // the word with a token's value e = lane + 64 k; which of its codes that is
+    const auto value_place = [&](const Place& t, int k) {
+        return (word_t*)(data + t.part + codes0 + t.tile * (NC * BB)) + 32 * t.slot +
+               (((lane >> 5) + 2 * k) * (BB / (KW * 4)) + (lane & 15) * 2 + (lane >> 4 & 1));
     };
-    // fn(token, place of the lane's element) over the wave's tokens and the elements `width` of a token, `load` first
-    // for MU of them
-    const auto each = [&](int width, auto load, auto store) {
-        for (int e = lane; e < width; e += 64)
-            for (int t0 = wave; t0 < m.n; t0 += MU * waves) {
-                decltype(load(0, 0)) x[MU];
-                bool some[MU];
+    const auto code_at = [](const Place& t) { return kv_slot(t.in) & 7; };
+    const bool scale_lane = lane < groups, key_lane = lane < octs;
+    const auto value_lane = [&](int k) { return HD % 64 == 0 || lane + 64 * k < HD; };
+    for (int t0 = wave; t0 < m.n; t0 += MU * waves) {
+        word_t x[MU][NE];
+        uint16_t sc[MU];
+        Place at[MU];
 #pragma unroll
-                for (int u = 0; u < MU; ++u) {
-                    const int t = t0 + u * waves;
-                    some[u] = t < m.n && from[t].part >= 0;
-                    if (some[u]) x[u] = load(t, e);
-                }
+        for (int u = 0; u < MU; ++u) {
+            at[u].part = -1;
+            if (t0 + u * waves < m.n) at[u] = place_of(from[t0 + u * waves]);
+            if (at[u].part < 0) continue;
+            if (scale_lane) sc[u] = *scale_place(at[u]);
+            if (values) {
 #pragma unroll
-                for (int u = 0; u < MU; ++u)
-                    if (some[u]) store(t0 + u * waves, e, x[u]);
+                for (int k = 0; k < NE; ++k)
+                    if (value_lane(k)) x[u][k] = *value_place(at[u], k);
+            } else if (key_lane) {
+                x[u][0] = *key_place(at[u]);
             }
-    };
-    each(groups, [&](int t, int g) { return *scale_place(from[t], g); }, [&](int t, int g, uint16_t x) { scales[t * groups + g] = x; });
-    if (!values)
-        each(c.hd / 8, [&](int t, int o) { return *key_place(from[t], o); },
-             [&](int t, int o, key_t x) { ((key_t*)codes)[t * (c.hd / 8) + o] = x; });
-    else
-        each(c.hd,
-             [&](int t, int e) {
-                 int which;
-                 const uint32_t w = *value_place(from[t], e, &which);
-                 return BITS == 8 ? w >> (8 * which) & 255u : kv_unturn(w) >> (4 * which) & 15u;
-             },
-             [&](int t, int e, uint32_t x) { codes[t * c.hd + e] = (uint8_t)x; });
+        }
+#pragma unroll
+        for (int u = 0; u < MU; ++u) {
+            if (at[u].part < 0) continue;
+            const int t = t0 + u * waves, j = code_at(at[u]);
+            if (scale_lane) scales[t * groups + lane] = sc[u];
+            if (values) {
+#pragma unroll
+                for (int k = 0; k < NE; ++k)
+                    if (value_lane(k))
+                        codes[t * HD + lane + 64 * k] = (uint8_t)(BITS == 8 ? x[u][k][KW - 1 & j >> 2] >> (8 * (j & 3))
+                                                                            : kv_unturn(x[u][k][0]) >> (4 * ((j >> 1) + 4 * (j & 1))) & 15u);
+            } else if (key_lane) {
+                ((word_t*)codes)[t * octs + lane] = x[u][0];
+            }
+        }
+    }
     __syncthreads();
-    each(groups, [&](int t, int g) { return scales[t * groups + g]; }, [&](int t, int g, uint16_t x) { *scale_place(to[t], g) = x; });
-    if (!values)
-        each(c.hd / 8, [&](int t, int o) { return ((const key_t*)codes)[t * (c.hd / 8) + o]; },
-             [&](int t, int o, key_t x) { *key_place(to[t], o) = x; });
-    else
-        each(c.hd,
-             [&](int t, int e) {
-                 int which;
-                 const uint32_t* p = value_place(to[t], e, &which);
-                 const uint32_t code = codes[t * c.hd + e];
-                 if constexpr (BITS == 8) return code;
-                 // (what another thread does to the word meanwhile leaves this nibble)
-                 const uint32_t old = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                 return kv_turn((kv_unturn(old) >> (4 * which) & 15u ^ code) << (4 * which));
-             },
-             [&](int t, int e, uint32_t x) {
-                 int which;
-                 uint32_t* p = value_place(to[t], e, &which);
-                 if constexpr (BITS == 8) ((uint8_t*)p)[which] = (uint8_t)x;
-                 else if (x) __hip_atomic_fetch_xor(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-             });
+    for (int t0 = wave; t0 < m.n; t0 += MU * waves) {
+        word_t x[MU][NE];
+        Place at[MU];
+        int next[MU];
+#pragma unroll
+        for (int u = 0; u < MU; ++u) {
+            const int t = t0 + u * waves;
+            at[u].part = -1;
+            if (t < m.n) at[u] = place_of(to[t]);
+            if (at[u].part < 0) continue;
+            if (scale_lane) *scale_place(at[u]) = scales[t * groups + lane];
+            if (!values) {
+                if (key_lane) *key_place(at[u]) = ((const word_t*)codes)[t * octs + lane];
+                continue;
+            }
+            next[u] = __builtin_amdgcn_readfirstlane(chain[t]);
+            if (!(next[u] >> 16)) at[u].part = -1;   // (another token's)
+            else {
+#pragma unroll
+                for (int k = 0; k < NE; ++k)
+                    if (value_lane(k)) x[u][k] = *value_place(at[u], k);
+            }
+        }
+        if (!values) continue;
+#pragma unroll
+        for (int u = 0; u < MU; ++u) {
+            if (at[u].part < 0) continue;
+            for (int i = t0 + u * waves, n = next[u] & 0xffff; ; n = __builtin_amdgcn_readfirstlane(chain[i]) & 0xffff) {
+                const int in = __builtin_amdgcn_readfirstlane(to[i].tok) & 31, j = kv_slot(in) & 7;
+#pragma unroll
+                for (int k = 0; k < NE; ++k) {
+                    const uint32_t code = codes[min(i * HD + lane + 64 * k, m.n * HD - 1)];   // (of a lane past the head: any)
+                    word_t& w = x[u][k];
+                    if constexpr (BITS == 8) {
+                        const uint32_t mask = 255u << (8 * (j & 3)), bits = code << (8 * (j & 3));
+                        if (j >> 2) w[KW - 1] = (w[KW - 1] & ~mask) | bits;
+                        else w[0] = (w[0] & ~mask) | bits;
+                    } else {
+                        const int sh = 4 * ((j >> 1) + 4 * (j & 1));
+                        w[0] = (w[0] & ~kv_turn(15u << sh)) | kv_turn(code << sh);
+                    }
+                }
+                i = n;
+                if (i >= m.n) break;
+            }
+#pragma unroll
+            for (int k = 0; k < NE; ++k)
+                if (value_lane(k)) *value_place(at[u], k) = x[u][k];
+        }
+    }
 }
 
 size_t move_lds(const KvCache& c, int n) {
     const int groups = kv_groups(c.hd, c.bits);
-    return (size_t)n * 2 * sizeof(TokenAt) + (n * groups + 3) / 4 * 8 + (size_t)n * c.hd;
+    return (size_t)n * (2 * sizeof(TokenAt) + 4) + 8 + (n * groups + 3) / 4 * 8 + (size_t)n * c.hd;
 }
 
 }  // namespace
@@ -176,10 +238,22 @@ hipError_t launch_kv_copy_pages(const KvCache& c, const KvLayers& l, int layers,
 hipError_t launch_kv_move_tokens(const KvCache& c, const KvLayers& l, int layers, const KvMoves& m, hipStream_t s) {
     const dim3 grid((unsigned)m.batch, (unsigned)(2 * c.heads), (unsigned)layers);
     const size_t lds = move_lds(c, m.n);
-    const int threads = 64 * std::min(4, (m.n + 7) / 8);
-    if (c.bits == 8) kv_move_tokens_kernel<8><<<grid, threads, lds, s>>>(c, l, m);
-    else kv_move_tokens_kernel<4><<<grid, threads, lds, s>>>(c, l, m);
-    return hipGetLastError();
+    // waves: the chip's 8192, or as many as there are tokens
+    const long long blocks = (long long)grid.x * grid.y * grid.z;
+    const int threads = 64 * (int)std::max(1LL, std::min({4LL, (long long)m.n, 8192 / blocks}));
+    const auto go = [&](auto hd) {
+        constexpr int HD = decltype(hd)::value;
+        if (c.bits == 8) kv_move_tokens_kernel<8, HD><<<grid, threads, lds, s>>>(c, l, m);
+        else kv_move_tokens_kernel<4, HD><<<grid, threads, lds, s>>>(c, l, m);
+        return hipGetLastError();
+    };
+    switch (c.hd) {
+    case 64: return go(std::integral_constant<int, 64>{});
+    case 96: return go(std::integral_constant<int, 96>{});
+    case 128: return go(std::integral_constant<int, 128>{});
+    case 256: return go(std::integral_constant<int, 256>{});
+    }
+    return hipErrorInvalidValue;
 }
 
 }  // namespace nnrh
