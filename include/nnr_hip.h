@@ -692,8 +692,10 @@ int nnrh_kv_attention(const nnrh_kv_cache_desc* c, const void* cache_dev, const 
  * seq - 1, and of the drafts those j (at position seq_lens[b] - seq + j) with
  * tree[b * tree_batch_stride + s * seq + j] != 0: itself too only if so. One byte a
  * pair, in device memory, read when the kernels run, over nothing that the call
- * writes; a stride of 0: one tree for the batch. At most 4096 drafts. Workspace
- * and everything else as nnrh_kv_attention has it.                          */
+ * writes; a stride of 0: one tree for the batch. At most 4096 drafts. The workspace
+ * is of nnrh_kv_tree_attention_workspace's size; everything else as
+ * nnrh_kv_attention has it.                                                 */
+int nnrh_kv_tree_attention_workspace(const nnrh_kv_cache_desc* c, const nnrh_kv_attention_desc* a, size_t* bytes);
 int nnrh_kv_tree_attention(const nnrh_kv_cache_desc* c, const void* cache_dev, const nnrh_kv_attention_desc* a,
                            const uint8_t* tree_dev, long long tree_batch_stride, const void* q_dev, void* y_dev,
                            void* workspace_dev, void* stream);

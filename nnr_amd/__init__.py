@@ -771,16 +771,16 @@ class KVCache:
                 self._tokens(k, page_table, seq_lens), k.data_ptr(), v.data_ptr())
         return k, v
 
-    def attention_workspace(self, batch, seq, q_heads, max_pages, prefix_len=0, dtype=None):
+    def attention_workspace(self, batch, seq, q_heads, max_pages, prefix_len=0, dtype=None, tree=False):
         """Bytes of workspace that such an attention takes, whatever the lengths: of
         queries of type `dtype`, or enough for any type. (Keys are split by how
-        many rows a block holds, and that goes by the type.)"""
+        many rows a block holds, and that goes by the type.) tree: with a tree of drafts."""
         _int32(batch=batch, seq=seq, q_heads=q_heads, max_pages=max_pages, prefix_len=prefix_len)
         sizes = []
         for dt in (F32, F16, BF16) if dtype is None else (_float_dt(dtype),):
             d = KvAttentionDesc(dt, batch, seq, q_heads, 0, 0, 1.0, None, max_pages, None, None, int(prefix_len))
             n = ct.c_size_t()
-            check(lib().nnrh_kv_attention_workspace(self.desc, d, n))
+            check((lib().nnrh_kv_tree_attention_workspace if tree else lib().nnrh_kv_attention_workspace)(self.desc, d, n))
             sizes.append(n.value)
         return max(sizes)
 
@@ -831,7 +831,7 @@ class KVCache:
             if not tree.is_contiguous():
                 tree = tree.contiguous()
         n = ct.c_size_t()
-        rc = self._L.nnrh_kv_attention_workspace(self.desc, d, n)
+        rc = (self._L.nnrh_kv_attention_workspace if tree is None else self._L.nnrh_kv_tree_attention_workspace)(self.desc, d, n)
         if rc:
             check(rc)
         ws = None

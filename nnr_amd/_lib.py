@@ -50,6 +50,7 @@ EXPORTS = [
     "nnrh_matmul_nbits_create", "nnrh_matmul_nbits_run", "nnrh_matmul_nbits_destroy",
     "nnrh_kv_cache_bytes", "nnrh_kv_cache_write", "nnrh_kv_cache_read",
     "nnrh_kv_attention_workspace", "nnrh_kv_attention", "nnrh_kv_tree_attention",
+    "nnrh_kv_tree_attention_workspace",
     "nnrh_kv_copy_pages", "nnrh_kv_move_tokens", "nnrh_rotary", "nnrh_prompt_attention",
 ]
 
@@ -252,6 +253,7 @@ def lib():
         "nnrh_kv_cache_read": (i, [P(KvCacheDesc), vp, P(KvTokens), vp, vp, vp]),
         "nnrh_kv_attention_workspace": (i, [P(KvCacheDesc), P(KvAttentionDesc), P(sz)]),
         "nnrh_kv_attention": (i, [P(KvCacheDesc), vp, P(KvAttentionDesc), vp, vp, vp, vp]),
+        "nnrh_kv_tree_attention_workspace": (i, [P(KvCacheDesc), P(KvAttentionDesc), P(sz)]),
         "nnrh_kv_tree_attention": (i, [P(KvCacheDesc), vp, P(KvAttentionDesc), vp, ll, vp, vp, vp, vp]),
         "nnrh_kv_copy_pages": (i, [P(KvCacheDesc), P(vp), i, vp, vp, i, vp]),
         "nnrh_kv_move_tokens": (i, [P(KvCacheDesc), P(vp), i, P(KvMoves), vp]),

@@ -2518,16 +2518,31 @@ int kv_attention_args(const nnrh_kv_cache_desc* d, const void* cache, const nnrh
 
 }  // namespace
 
-extern "C" int nnrh_kv_attention_workspace(const nnrh_kv_cache_desc* d, const nnrh_kv_attention_desc* a, size_t* bytes) {
+namespace {
+
+int attention_workspace(const nnrh_kv_cache_desc* d, const nnrh_kv_attention_desc* a, const uint8_t* tree, size_t* bytes) {
     KvCache c;
     KvAttention r;
     if (!bytes) return set_err(NNRH_ERR_INVALID, "kv_attention_workspace: NULL");
     const int rc = kv_attention_args(d, nullptr, a, &c, &r);
     if (rc != NNRH_OK) return rc;
+    r.tree = tree;
     if (a->max_pages < 0 || (long long)a->max_pages * c.page_size > (1 << 30))
         return set_err(NNRH_ERR_INVALID, "kv_attention_workspace: %d pages", a->max_pages);
     *bytes = r.batch && r.seq ? kv_attention_workspace(c, r) : 0;
     return NNRH_OK;
+}
+
+}  // namespace
+
+extern "C" int nnrh_kv_attention_workspace(const nnrh_kv_cache_desc* d, const nnrh_kv_attention_desc* a, size_t* bytes) {
+    return attention_workspace(d, a, nullptr, bytes);
+}
+
+extern "C" int nnrh_kv_tree_attention_workspace(const nnrh_kv_cache_desc* d, const nnrh_kv_attention_desc* a, size_t* bytes) {
+    if (a && a->seq > 4096) return set_err(NNRH_ERR_UNSUPPORTED, "kv_tree_attention: %d drafts (at most 4096)", a->seq);
+    static const uint8_t some = 0;   // (that there is a tree is what counts)
+    return attention_workspace(d, a, &some, bytes);
 }
 
 namespace {
@@ -2555,6 +2570,8 @@ int kv_attention(const nnrh_kv_cache_desc* d, const void* cache, const nnrh_kv_a
     if (overlap(q, qsize, y, ysize) && !(q == y && dense)) return set_err(NNRH_ERR_INVALID, "kv_attention: y lies over q");
     const size_t all = (size_t)c.num_pages * kv_page_bytes(c);
     if (overlap(y, ysize, c.data, all)) return set_err(NNRH_ERR_INVALID, "kv_attention: y lies over the cache");
+    r.tree = tree;
+    r.tree_bstride = tree_bs;
     const size_t need = kv_attention_workspace(c, r);
     if (need && !workspace) return set_err(NNRH_ERR_INVALID, "kv_attention: this shape needs a workspace of %zu bytes", need);
     if ((uintptr_t)workspace & 255) return set_err(NNRH_ERR_INVALID, "kv_attention: the workspace must be 256-byte aligned");
@@ -2572,8 +2589,6 @@ int kv_attention(const nnrh_kv_cache_desc* d, const void* cache, const nnrh_kv_a
     }
     r.q = q;
     r.y = y;
-    r.tree = tree;
-    r.tree_bstride = tree_bs;
     ProfScope ps("kv_attention", S(stream));
     HIP_TRY(launch_kv_attention(c, r, workspace, S(stream)), "kv_attention");
     return NNRH_OK;

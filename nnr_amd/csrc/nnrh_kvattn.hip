@@ -655,7 +655,7 @@ template <int HD, int BITS> struct RawTile {
 __device__ __forceinline__ bool tree_sees(const AttnArgs& p, const Job& job, int row, int key) {
     const int line = job.pre ? 0 : (row / p.a.q_heads - job.b * p.a.seq) * p.a.seq;
     const int d = key - job.drafts;
-    const bool draft = key >= job.drafts && (unsigned)d < (unsigned)p.a.seq;
+    const bool draft = (unsigned)d < (unsigned)p.a.seq;
     const uint8_t* tree = p.a.tree + job.b * p.a.tree_bstride;
     const uint8_t sees = tree[(uint32_t)(line + (draft ? d : 0))];
     return (!draft) | (sees != 0);
@@ -749,19 +749,19 @@ __device__ __forceinline__ void put_rows(const AttnArgs& p, const Job& job, int 
 // elements, and holds elements 64 apart of the result, the mean so far. As near
 // to a sum in fp32 as that comes whatever the sizes of queries, keys and values,
 // and some 50 times as slow as the products.
-template <int HD, int BITS, int NP, bool TREE>
-__device__ __forceinline__ void slow_row(const AttnArgs& p, const Job& job, int row, int lim) {
-    constexpr int NC = HD / 32, BB = BITS == 8 ? 1024 : 512, NE = (HD + 63) / 64;
+template <int HD> struct SlowRow {
+    static constexpr int NE = (HD + 63) / 64;
+    float m = kNegInf, l = 0.0f, y[NE] = {};
+};
+template <int HD, int BITS, bool TREE>
+__device__ __forceinline__ void slow_range(const AttnArgs& p, const Job& job, int row, int lim, int lane, SlowRow<HD>& r) {
+    constexpr int NC = HD / 32, BB = BITS == 8 ? 1024 : 512, NE = SlowRow<HD>::NE;
     const KvAttention& a = p.a;
-    int lane = threadIdx.x & 63;
-    asm volatile("" : "+v"(lane));   // nothing of this path in registers before it
+    float &m = r.m, &l = r.l, *y = r.y;
     const int tok = lane & 31, half = lane >> 5;
     const int bt = row / a.q_heads, hq = row - bt * a.q_heads, bq = bt / a.seq;
     const long long q0 = (long long)bq * a.q_bstride + (long long)(bt - bq * a.seq) * a.q_tstride + (long long)hq * HD;
     const long long vcodes = kv_codes_bytes(p.c.page_size, HD, BITS), vscales = (long long)p.c.page_size * kv_groups(HD, BITS);
-    float m = kNegInf, l = 0.0f, y[NE];
-#pragma unroll
-    for (int i = 0; i < NE; ++i) y[i] = 0.0f;
     const int t1 = min(job.t1, (lim + 31) / 32);
     for (int tile = job.t0; tile < t1; ++tile) {
         const TilePtr t = tile_ptr<HD, BITS>(p, job.head, page_id(job, p, tile), tile);
@@ -822,29 +822,50 @@ __device__ __forceinline__ void slow_row(const AttnArgs& p, const Job& job, int 
             }
         }
     }
+}
+// part: its place among the partial results, or < 0: the result itself
+template <int HD, int NP>
+__device__ __forceinline__ void slow_put(const AttnArgs& p, int row, long long part, int lane, const SlowRow<HD>& r) {
+    const KvAttention& a = p.a;
     // as the products leave it: totals are of weights with their largest at 2^top
     constexpr float unit = NP == 1 ? kTop - kSlack : kTop;
-    const long long part = (long long)row * p.slots + job.slot;
-    if (p.slots > 1 && lane == 0) p.part_ml[part] = float2{m, ldexpf(l, (int)unit)};
+    if (part >= 0 && lane == 0) p.part_ml[part] = float2{r.m, ldexpf(r.l, (int)unit)};
 #pragma unroll
-    for (int i = 0; i < NE; ++i) {
+    for (int i = 0; i < SlowRow<HD>::NE; ++i) {
         const int e = lane + 64 * i;
         if (HD % 64 && e >= HD) break;
-        if (p.slots > 1) p.part_o[part * HD + e] = y[i];
-        else if (a.type == FT_F32) ((float*)a.y)[(long long)row * HD + e] = y[i];
-        else if (a.type == FT_F16) ((_Float16*)a.y)[(long long)row * HD + e] = (_Float16)y[i];
-        else ((__bf16*)a.y)[(long long)row * HD + e] = (__bf16)y[i];
+        if (part >= 0) p.part_o[part * HD + e] = r.y[i];
+        else if (a.type == FT_F32) ((float*)a.y)[(long long)row * HD + e] = r.y[i];
+        else if (a.type == FT_F16) ((_Float16*)a.y)[(long long)row * HD + e] = (_Float16)r.y[i];
+        else ((__bf16*)a.y)[(long long)row * HD + e] = (__bf16)r.y[i];
     }
+}
+// the lane, so that nothing of this path is in registers before it
+__device__ __forceinline__ int slow_lane() {
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
+    return lane;
+}
+template <int HD, int BITS, int NP, bool TREE>
+__device__ __forceinline__ void slow_row(const AttnArgs& p, const Job& job, int row, int lim) {
+    const int lane = slow_lane();
+    SlowRow<HD> r;
+    slow_range<HD, BITS, TREE>(p, job, row, lim, lane, r);
+    slow_put<HD, NP>(p, row, p.slots > 1 ? (long long)row * p.slots + job.slot : -1, lane, r);
+}
+// The kernel's arguments, its only ones, read anew, so that none of them stay in
+// registers for this path.
+__device__ __forceinline__ const AttnArgs& args_here() {
+    uintptr_t args = (uintptr_t)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(args));
+    return *(const AttnArgs*)args;
 }
 // of 16 rows (one a lane of the first group) those that are asked for, every `of`th from `first` on
 template <int HD, int BITS, int NP, bool TREE>
 __device__ __forceinline__ void slow_rows(const Job& job, int at, int lim, bool again, int first, int of) {
     const uint32_t todo = (uint32_t)__ballot(again) & 0xffffu;
     if (!todo) return;
-    // (read anew from the kernel's arguments, its only ones, so that none of them stay in registers for this path)
-    uintptr_t args = (uintptr_t)__builtin_amdgcn_kernarg_segment_ptr();
-    asm volatile("" : "+s"(args));
-    const AttnArgs& p = *(const AttnArgs*)args;
+    const AttnArgs& p = args_here();
 #pragma unroll 1
     for (int i = first; i < 16; i += of)
         if (todo >> i & 1) slow_row<HD, BITS, NP, TREE>(p, job, __builtin_amdgcn_readlane(at, i), __builtin_amdgcn_readlane(lim, i));
@@ -965,13 +986,13 @@ template <int HD, int BITS, bool TREE> constexpr int kManyTiles = (HD == 128 && 
 // A tile is turned into operands once, a part by each wave, and lies in LDS
 // for all of them; the next tile is written beside it meanwhile, and the codes
 // of the one after are on their way.
-template <int HD, int BITS> struct Parts {
-    static constexpr int NC = HD / 32, NU = (2 * NC + AW - 1) / AW;   // a wave's blocks (NC of keys, then NC of values)
+template <int HD, int BITS, int W = AW> struct Parts {   // W: the block's waves
+    static constexpr int NC = HD / 32, NU = (2 * NC + W - 1) / W;   // a wave's blocks (NC of keys, then NC of values)
     typedef uint32_t vec __attribute__((ext_vector_type(BITS == 8 ? 4 : 2)));
     // block of round u; is it one of keys (known at compile time where the waves divide them)
-    __device__ __forceinline__ static int block(int u, int wave) { return wave + u * AW; }
-    __device__ __forceinline__ static bool keys(int u, int b) { return NC % AW == 0 ? u < NC / AW : b < NC; }
-    __device__ __forceinline__ static bool none(int b) { return 2 * NC % AW != 0 && b >= 2 * NC; }
+    __device__ __forceinline__ static int block(int u, int wave) { return wave + u * W; }
+    __device__ __forceinline__ static bool keys(int u, int b) { return NC % W == 0 ? u < NC / W : b < NC; }
+    __device__ __forceinline__ static bool none(int b) { return 2 * NC % W != 0 && b >= 2 * NC; }
     vec code[NU];
     u4 sc[NU];                    // 4 bits: a value block's scales; a key block's pair in the first word
     u4 ks, vs;                    // 8 bits
@@ -1231,6 +1252,409 @@ __global__ __launch_bounds__(AW * 64, HD <= 128 ? (!PM && !OM && NP == 1 ? 3 : 2
     }
 }
 
+// ---- drafts of many rows (16-bit tensors) ---------------------------------------
+// A sequence's drafts, times the heads of a group, fill a block's rows by themselves,
+// so its prefix and its own keys are one run of tiles that a block takes a part of;
+// parts are of equal length whatever the lengths (a part of the longest sequence's
+// pages would leave most blocks of the others with nothing).
+// Four waves of 32 rows share tiles that are turned into operands once, two of them
+// between two barriers. 32x32 products leave a lane 16 scores of one row; tokens
+// 4 g .. and 16 + 4 g .. of a tile, which lie side by side in a value block, are eight
+// of them.
+// Bound by the vector units: a score takes a scale, a maximum, a product-sum, an exp,
+// a total, a value's scale, a maximum and half a conversion, 10 issue slots, 16 of
+// them for the 32 cycles that its products take. 24 sequences of up to 4096 tokens
+// after a prefix of 1000, 64 drafts, 32 heads over 8 of 128: 162 to 180 us with the
+// join's 18 (the kernel above, in its place: 250). One sequence of 1800, 15 drafts:
+// 17 us, most of it a block's start, its first tiles' way from memory, and the join.
+typedef float f16v __attribute__((ext_vector_type(16)));
+constexpr int kTreeWaves = 4, kTreeTiles = 2;   // waves of a block; tiles between two barriers
+template <int HD> struct TreeRows {
+    static constexpr int NK = HD / 16, ND = HD / 32;
+    h8 q[NK];           // elements 16 k + 8 half ..
+    f16v o[ND];         // sums of kTop p v in units of 2^eu: elements 32 d + 8 (r / 4) + 4 half + r % 4
+    float rf, rk;       // as in Rows
+    float m, l, x;      // x: 8 bits: the largest weight with its value's scale, this lane's
+    int ek, eu;
+    int at;             // its place among all rows
+};
+template <int HD, int BITS> struct TreeLds {
+    h8 frag[2][kTreeTiles][4 * (HD / 32)][64];   // a tile's keys (c, i), then its values
+    float scale[2][kTreeTiles][2][32];   // 8 bits: keys', and values' over the unit, in the order of a lane's scores
+    int unit[2];                     // 8 bits: the values'
+    int far[kTreeWaves];
+};
+
+template <int HD, int BITS>
+__device__ __forceinline__ void tree_rows(const AttnArgs& p, const Job& job, int row0, TreeRows<HD>& w) {
+    const KvAttention& a = p.a;
+    const int col = threadIdx.x & 31, half = (threadIdx.x & 63) >> 5;
+    const int r = min(row0 + col, job.nrows - 1), tok = r / p.G, hq = job.head * p.G + (r - tok * p.G);
+    w.at = (job.b * a.seq + tok) * a.q_heads + hq;
+    const bool neg = a.scale < 0.0f;
+    const long long at = (long long)job.b * a.q_bstride + (long long)tok * a.q_tstride + (long long)hq * HD + 8 * half;
+    u4 raw[HD / 16];
+#pragma unroll
+    for (int k = 0; k < HD / 16; ++k) raw[k] = *(const u4*)((const uint16_t*)a.q + at + 16 * k);
+    float v[HD / 16][8], top = 0.0f;
+#pragma unroll
+    for (int k = 0; k < HD / 16; ++k)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t h = raw[k][j >> 1] >> (16 * (j & 1));
+            v[k][j] = a.type == FT_F16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)h) : bf16_lo(h);
+            top = fmaxf(top, fabsf(v[k][j]));
+        }
+    top = swap_max(top, true);
+    int e = 0;
+    if (top > 0.0f && top < __builtin_inff()) e = 15 - __builtin_amdgcn_frexp_expf(top);
+    w.rf = ldexpf(fabsf(a.scale) * 1.44269504088896341f, -e);
+    w.rk = fmaxf(w.rf, kLeast);
+#pragma unroll
+    for (int k = 0; k < HD / 16; ++k)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w.q[k][j] = (_Float16)ldexpf(neg ? -v[k][j] : v[k][j], e);
+    w.m = kNegInf;
+    w.l = w.x = 0.0f;
+    w.eu = kNoUnit;
+    w.ek = BITS == 8 ? 0 : kNoUnit;
+#pragma unroll
+    for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) w.o[d][i] = 0.0f;
+}
+
+// Tiles in LDS against a wave's rows: raw scores, then weights and sums. hides: bit 16
+// z + r: the lane's score r of tile z is of a draft that its row does not see; held:
+// tokens in each; some: not all have 32.
+template <int HD, int BITS>
+__device__ __forceinline__ const h8* tree_operands(const TreeLds<HD, BITS>& lds, int at) {
+    const int col = threadIdx.x & 31, half = (threadIdx.x & 63) >> 5;
+    return &lds.frag[at][0][0][0] + ((col >> 4) * 64 + (col & 15) + 16 * half);
+}
+template <int HD, int BITS>
+__device__ __forceinline__ void tree_scores(const TreeRows<HD>& w, const TreeLds<HD, BITS>& lds, int at, f16v* s) {
+    constexpr int NC = HD / 32, KT = kTreeTiles;
+    const h8* f = tree_operands(lds, at);
+#pragma unroll
+    for (int z = 0; z < KT; ++z) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[z][r] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k)
+            s[z] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[z * 4 * NC * 64 + (k >> 1) * 128 + (k & 1) * 32], w.q[k], s[z], 0, 0, 0);
+    }
+}
+template <int HD, int BITS>
+__device__ __forceinline__ void tree_values(TreeRows<HD>& w, const TreeLds<HD, BITS>& lds, int at, f16v* s, const int* held, bool some,
+                                            uint32_t hides, int ek, int en) {
+    constexpr int NC = HD / 32, KT = kTreeTiles;
+    const int half = (threadIdx.x & 63) >> 5;
+    const h8* f = tree_operands(lds, at);
+    if constexpr (BITS == 8) {
+#pragma unroll
+        for (int z = 0; z < KT; ++z)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const f4 ks = *(const f4*)&lds.scale[at][z][0][16 * half + 4 * i];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[z][4 * i + r] *= ks[r];
+            }
+        en = __builtin_amdgcn_readfirstlane(lds.unit[at]);
+    } else if (ek != w.ek) {
+        stay_a_branch();
+        w.m = ldexpf(w.m, w.ek - ek);
+        w.rk = fmaxf(ldexpf(w.rf, ek), kLeast);
+        w.ek = ek;
+    }
+    if (__builtin_expect(some || __any(hides), 0)) {
+        stay_a_branch();
+#pragma unroll
+        for (int z = 0; z < KT; ++z) {
+            const int end = held[z] - 4 * half;
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if ((8 * (r >> 2) + (r & 3) >= end) | (hides >> (16 * z + r) & 1)) s[z][r] = kNegInf;
+        }
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int z = 0; z < KT; ++z)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[z][r]);
+    mx = swap_max(mx, true);
+    const bool up = mx * w.rk > __builtin_fmaf(w.m, w.rk, kSlack);
+    if (__builtin_expect(__any(up) || en != w.eu, 0)) {
+        stay_a_branch();
+        const float al = up ? exp2_((w.m - mx) * w.rk) : 1.0f;
+        w.m = up ? mx : w.m;
+        w.l *= al;
+        const float g = ldexpf(al, w.eu - en);
+        w.x *= g;
+#pragma unroll
+        for (int d = 0; d < NC; ++d) w.o[d] *= g;
+        w.eu = en;
+    }
+    const float off = kTop - kSlack - (w.m == kNegInf ? 0.0f : w.m * w.rk);
+    float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int z = 0; z < KT; ++z) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            s[z][r] = exp2_(__builtin_fmaf(s[z][r], w.rk, off));
+            sum[r & 1] += s[z][r];
+        }
+        if constexpr (BITS == 8) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const f4 vs = *(const f4*)&lds.scale[at][z][1][16 * half + 4 * i];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    s[z][4 * i + r] *= vs[r];
+                    w.x = fmaxf(w.x, s[z][4 * i + r]);
+                }
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            h8 pf;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) pf[j] = (_Float16)s[z][4 * m + (j & 3) + 8 * (j >> 2)];
+#pragma unroll
+            for (int d = 0; d < NC; ++d)
+                w.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[z * 4 * NC * 64 + (2 * NC + 2 * d) * 64 + m * 32], pf, w.o[d], 0, 0, 0);
+        }
+    }
+    w.l += sum[0] + sum[1];
+}
+
+struct TreeJob {
+    Job job;
+    int pre, t0, t1;   // tiles: the prefix's, then the sequence's; t0 .. t1 are the block's
+};
+// heads first (to XCDs in turn), a sequence's parts last
+__device__ __forceinline__ TreeJob tree_job(const AttnArgs& p, uint32_t block) {
+    const KvAttention& a = p.a;
+    TreeJob t;
+    const uint32_t xg = block / (uint32_t)p.c.heads, xb = xg / (uint32_t)p.own_groups, xs = xb / (uint32_t)a.batch;
+    const int group = (int)(xg - xb * p.own_groups);
+    t.job.pre = false;
+    t.job.head = (int)(block - xg * p.c.heads);
+    t.job.b = (int)(xb - xs * a.batch);
+    t.job.split = t.job.slot = (int)xs;
+    t.job.row0 = group * kTreeWaves * 32;
+    t.job.nrows = a.seq * p.G;
+    t.job.table = a.table + (long long)t.job.b * a.max_pages;
+    const int len = scalar_load(a.lens, t.job.b);
+    t.job.len = max(min((long long)len, (long long)a.max_pages * p.c.page_size), 0ll);
+    t.job.drafts = len - a.seq;
+    t.pre = (a.prefix_len + 31) / 32;
+    const int all = t.pre + (int)((t.job.len + 31) / 32), split = t.job.split;
+    const int each = (int)((unsigned)all / (unsigned)p.slots), more = all - each * p.slots;   // (the first ones have one more)
+    t.t0 = split * each + min(split, more);
+    t.t1 = t.t0 + each + (split < more ? 1 : 0);
+    return t;
+}
+
+template <int HD, int BITS>
+__global__ __launch_bounds__(kTreeWaves * 64, 2) void kv_tree_kernel(AttnArgs p) {
+    typedef Parts<HD, BITS, kTreeWaves> Raw;
+    constexpr int NC = HD / 32, W = kTreeWaves;
+    __shared__ __attribute__((aligned(16))) TreeLds<HD, BITS> lds;
+    const KvAttention& a = p.a;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 31, half = lane >> 5, g = lane >> 4;
+    const TreeJob part_of = tree_job(p, blockIdx.x);
+    const Job& job = part_of.job;
+    const int row0 = job.row0 + wave * 32, pre = part_of.pre, t0 = part_of.t0, t1 = part_of.t1;
+
+    constexpr int KT = kTreeTiles;
+    Raw raw[KT] = {};
+    uint32_t sc[KT] = {};            // 8 bits, the first wave: a scale of token `col`, its key's or (the other half) its value's
+    uint32_t seen_k = 0;             // of keys' the largest, as bits
+    Seen<BITS> scales;
+    int id[KT], held[KT], held_next[KT], ek = 0, en = 0, ek_next = kNoUnit, en_next = kNoUnit;
+    const auto pages = [&](int t) {
+#pragma unroll
+        for (int z = 0; z < KT; ++z, ++t)
+            id[z] = t >= t1 ? -1 : t < pre ? scalar_load(a.prefix_table, t >> p.page_shift) : scalar_load(job.table, (t - pre) >> p.page_shift);
+    };
+    const auto load = [&](int t) {
+#pragma unroll
+        for (int z = 0; z < KT; ++z, ++t) {
+            const int tile = t < pre ? t : t - pre;
+            raw[z].load(p, job.head, id[z], tile, wave);
+            if (BITS == 8 && wave == 0) {
+                const TilePtr at = tile_ptr<HD, BITS>(p, job.head, id[z], tile);
+                sc[z] = at.scales[(half ? p.c.page_size : 0) + kv_slot(col)];
+            }
+        }
+    };
+    // raw tiles -> operands; tokens that a tile does not hold have scale 0
+    const auto convert = [&](int t, int at) {
+        float fk = 1.0f, fv = 1.0f;
+#pragma unroll
+        for (int z = 0; z < KT; ++z) {
+            const long long left = t + z < pre ? a.prefix_len - 32LL * (t + z) : job.len - 32LL * (t + z - pre);
+            held_next[z] = raw[z].ok ? (int)max(min(left, 32ll), 0ll) : 0;
+        }
+        if constexpr (BITS == 4) {
+            uint32_t tk = 0, tv = 0;
+            u2 k[KT], v[KT];
+#pragma unroll
+            for (int z = 0; z < KT; ++z) {
+                k[z] = of_tokens(raw[z].all_k, held_next[z], true);
+                v[z] = of_tokens(raw[z].all_v, held_next[z], false);
+                tk = pair_max(tk, pair_max(k[z][0], k[z][1]));
+                tv = pair_max(tv, pair_max(v[z][0], v[z][1]));
+            }
+            ek_next = unit_of(tk, ek_next);
+            en_next = unit_of(tv, en_next);
+            if ((t / KT) % W == wave) {   // (one wave of the block is enough)
+                stay_a_branch();
+#pragma unroll
+                for (int z = 0; z < KT; ++z) scales.add(k[z], v[z]);
+            }
+            fk = ldexpf(1.0f, -ek_next);
+            fv = ldexpf(1.0f, -en_next);
+        } else if (wave == 0) {
+            uint32_t have[KT], top = 0;
+#pragma unroll
+            for (int z = 0; z < KT; ++z) {
+                have[z] = col < held_next[z] ? sc[z] : 0;
+                if (!half) seen_k = umax(seen_k, have[z]);
+                top = umax(top, half ? have[z] : 0);
+            }
+            en_next = max(en_next, ceil_exp(__builtin_amdgcn_readfirstlane(umax16_32(umax_16(top))), kNoUnit));
+#pragma unroll
+            for (int z = 0; z < KT; ++z) {
+                const float v = bf16_lo(have[z]);
+                lds.scale[at][z][half][16 * (col >> 2 & 1) + 4 * (col >> 3) + (col & 3)] = half ? ldexpf(v, -en_next) : v;
+            }
+            if (lane == 0) lds.unit[at] = en_next;
+        }
+#pragma unroll
+        for (int z = 0; z < KT; ++z)
+#pragma unroll
+            for (int u = 0; u < Raw::NU; ++u) {
+                const int b = Raw::block(u, wave);
+                if (Raw::none(b)) break;
+                h8* to = &lds.frag[at][z][2 * b][lane];
+                if constexpr (BITS == 8) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) to[64 * i] = codes8(raw[z].code[u][2 * i], raw[z].code[u][2 * i + 1]);
+                } else if (Raw::keys(u, b)) {
+                    const uint32_t s = held_pair(raw[z].sc[u][0], held_next[z]);
+                    to[0] = key4(raw[z].code[u][0], bf16_lo(s), fk);
+                    to[64] = key4(raw[z].code[u][1], bf16_hi(s), fk);
+                } else {
+                    Scale4 s[4];
+                    value_scales(held_scales(raw[z].sc[u], held_next[z]), fv, s);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) to[64 * i] = codes4(raw[z].code[u][i], s[0], s[1], s[2], s[3]);
+                }
+            }
+    };
+    TreeRows<HD> w;
+    pages(t0);
+    load(t0);
+    pages(t0 + KT);
+    tree_rows<HD, BITS>(p, job, row0, w);   // (a wave past the rows repeats the last one)
+    convert(t0, 0);
+    load(t0 + KT);
+    pages(t0 + 2 * KT);
+    __syncthreads();
+    int at = 0;
+    for (int t = t0; t < t1; t += KT, at ^= 1) {
+        bool some = false;
+#pragma unroll
+        for (int z = 0; z < KT; ++z) {
+            held[z] = held_next[z];
+            some |= held[z] < 32;
+        }
+        ek = ek_next;
+        en = en_next;
+        uint32_t hides = 0;
+        if (__builtin_expect(t + KT > pre && 32 * (t + KT - pre) > job.drafts, 0)) {
+            stay_a_branch();
+#pragma unroll 1   // (code that hardly ever runs a second time: the less of it, the sooner it is there)
+            for (int z = 0; z < KT; ++z) {
+                if (t + z < pre) continue;
+                uint32_t line = 0;
+#pragma unroll 4
+                for (int r = 0; r < 16; ++r)
+                    line |= (uint32_t)!tree_sees(p, job, w.at, 32 * (t + z - pre) + 8 * (r >> 2) + 4 * half + (r & 3)) << r;
+                hides |= line << (16 * z);
+            }
+        }
+        f16v s[KT];
+        tree_scores(w, lds, at, s);
+        // past the last tile for nothing: without a branch
+        convert(t + KT, at ^ 1);
+        load(t + 2 * KT);
+        pages(t + 3 * KT);
+        tree_values(w, lds, at, s, held, some, hides, ek, en);
+        __syncthreads();
+    }
+    const bool wave_far = BITS == 8 ? __any(seen_k >= kLargeScale) : __any(scales.far(w.ek, w.eu));
+    if (lane == 0) lds.far[wave] = wave_far;
+    __syncthreads();
+    bool again = false;
+#pragma unroll
+    for (int v = 0; v < W; ++v) again |= lds.far[v] != 0;
+    if (row0 >= job.nrows) return;
+    const float l = w.l + __shfl_xor(w.l, 32);
+    again |= BITS == 8 && swap_max(w.x, true) < kFarWeight && w.eu != kNoUnit && l > 0.0f;
+    const bool mine = row0 + col < job.nrows, none = w.m == kNegInf && l == 0.0f;
+    const float inv = none ? 0.0f : 1.0f / l;
+    const long long part = (long long)w.at * p.slots + job.slot;
+    // (fn(element, four of them): one loop a kind of result, of which one runs)
+    const auto each_four = [&](auto fn) {
+#pragma unroll
+        for (int d = 0; d < NC; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                f4 y;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) y[r] = ldexpf(w.o[d][4 * i + r] * inv, w.eu);
+                fn(32 * d + 8 * i + 4 * half, y);
+            }
+    };
+    if (mine && !again) {
+        if (p.slots > 1) {
+            if (!half) p.part_ml[part] = float2{w.m == kNegInf ? kNegInf : w.m * w.rk, l};
+            if (!none) each_four([&](int e, f4 y) { *(f4*)(p.part_o + part * HD + e) = y; });
+        } else {
+            each_four([&](int e, f4 y) { store_y4(a, (long long)w.at * HD + e, y); });
+        }
+    }
+    const uint32_t todo = (uint32_t)__ballot(again && mine);   // (both halves have the row's)
+    if (!todo) return;
+    // (all of it anew, so that no registers are held for this)
+    const AttnArgs& q = args_here();
+    uint32_t block = blockIdx.x;
+    asm volatile("" : "+s"(block));
+    const TreeJob again_of = tree_job(q, block);
+#pragma unroll 1
+    for (int i = 0; i < 32; ++i) {
+        if (!(todo >> i & 1)) continue;
+        const int row = __builtin_amdgcn_readlane(w.at, i), slow = slow_lane();
+        SlowRow<HD> r;
+        Job from = again_of.job;
+        const int len = (int)from.len;
+        const int* own_table = from.table;
+#pragma unroll 1
+        for (int own = 0; own < 2; ++own) {
+            from.pre = !own;
+            from.table = own ? own_table : q.a.prefix_table;
+            from.t0 = own ? max(again_of.t0 - again_of.pre, 0) : again_of.t0;
+            from.t1 = own ? again_of.t1 - again_of.pre : min(again_of.t1, again_of.pre);
+            slow_range<HD, BITS, true>(q, from, row, own ? len : q.a.prefix_len, slow, r);
+        }
+        slow_put<HD, 1>(q, row, q.slots > 1 ? (long long)row * q.slots + from.slot : -1, slow, r);
+    }
+}
+
 // One wave a row: the mean of its partial results, by their totals, in a fixed
 // order, several slots side by side where a row is shorter than the wave.
 template <int HD>
@@ -1280,6 +1704,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(AttnArgs p) {
 // How a call is cut up; of shapes alone, so that the workspace is known before
 struct Plan {
     bool pre_many, own_many;
+    bool tree;                     // kv_tree_kernel
     int pre_groups, own_groups, pre_slots, own_slots, pre_chunk, own_chunk;
 };
 int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
@@ -1289,6 +1714,22 @@ Plan plan(const KvCache& c, const KvAttention& a) {
     const long long own_rows = (long long)a.seq * G, pre_rows = own_rows * a.batch;
     const int np = a.type == FT_F32 ? 2 : 1, many = AW * 16 * (c.hd <= 128 && np == 1 ? 2 : 1);
     p.own_many = own_rows > 16;
+    p.tree = false;
+    if (a.tree && p.own_many && np == 1 && c.hd <= 128) {
+        p.tree = true;
+        p.own_groups = ceil_div(own_rows, kTreeWaves * 32);
+        const long long items = (long long)p.own_groups * c.heads * a.batch;
+        const long long tiles = (a.prefix_len + 31) / 32 + (long long)a.max_pages * c.page_size / 32;
+        // Parts of 8 tiles or more, to 768 blocks: of sequences of many lengths, one and
+        // a half times what runs at once. (24 sequences of 64 drafts, lengths to 4096:
+        // 512 blocks 206 us, 768 162, 1536 174; all of them 2080 long: 105, 105, 122.)
+        // Of 4 while that is no more than a block a CU. (One sequence of 1800, 15
+        // drafts: 17.7 us, of 8 tiles 22; 4096, 64 drafts, two blocks a CU: 29.6 and 24.4.)
+        p.own_slots = (int)std::max({1ll, std::min(256 / items, tiles / 4), std::min(768 / items, tiles / 8)});
+        p.pre_many = false;
+        p.pre_groups = p.pre_slots = p.pre_chunk = p.own_chunk = 0;
+        return p;
+    }
     p.pre_many = a.prefix_len && pre_rows > 16;
     p.own_groups = ceil_div(own_rows, p.own_many ? many : 16);
     p.pre_groups = a.prefix_len ? ceil_div(pre_rows, p.pre_many ? many : 16) : 0;
@@ -1324,6 +1765,12 @@ Plan plan(const KvCache& c, const KvAttention& a) {
 
 template <int HD, int BITS, int NP, bool TREE>
 void start(const AttnArgs& p, const Plan& pl, unsigned blocks, hipStream_t s) {
+    if constexpr (TREE && NP == 1 && HD <= 128) {
+        if (pl.tree) kv_tree_kernel<HD, BITS><<<blocks, kTreeWaves * 64, 0, s>>>(p);
+        else if (pl.pre_many) kv_attn_kernel<HD, BITS, NP, true, false, TREE><<<blocks, AW * 64, 0, s>>>(p);
+        else kv_attn_kernel<HD, BITS, NP, false, false, TREE><<<blocks, AW * 64, 0, s>>>(p);
+        return;
+    }
     if (pl.own_many) kv_attn_kernel<HD, BITS, NP, true, true, TREE><<<blocks, AW * 64, 0, s>>>(p);
     else if (pl.pre_many) kv_attn_kernel<HD, BITS, NP, true, false, TREE><<<blocks, AW * 64, 0, s>>>(p);
     else kv_attn_kernel<HD, BITS, NP, false, false, TREE><<<blocks, AW * 64, 0, s>>>(p);

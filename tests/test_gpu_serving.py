@@ -516,7 +516,7 @@ def test_tree_of_a_chain_is_causal(dev, bits, S):
     # a mask that is a view, another stream, a workspace of the call's
     wide = torch.zeros((S, 2 * S), dtype=torch.bool, device=dev)
     wide[:, ::2] = chain
-    ws = torch.empty(cache.attention_workspace(B, S, H * G, 5, dtype=torch.float16), dtype=torch.uint8, device=dev)
+    ws = torch.empty(cache.attention_workspace(B, S, H * G, 5, dtype=torch.float16, tree=True), dtype=torch.uint8, device=dev)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     got = cache.attention(q, td, ld, tree=wide[:, ::2], workspace=ws, stream=side.cuda_stream)

@@ -126,6 +126,30 @@ def tree(a, at=MEM[7], stride=9, cache=None, y=MEM[2], ws=MEM[6]):
     return _lib.lib().nnrh_kv_tree_attention(C.byref(c), MEM[0], C.byref(a), at, stride, MEM[1], y, ws, None)
 
 
+def tree_workspace(a, c=None):
+    n = C.c_size_t()
+    return _lib.lib().nnrh_kv_tree_attention_workspace(C.byref(c or cache_desc()), C.byref(a), C.byref(n)), n.value
+
+
+def test_tree_workspace():
+    """Partial results of rows x (elements + 2) floats, once a part; none where one block sees all of a sequence"""
+    L, c, n = _lib.lib(), cache_desc(), C.c_size_t()
+    for seq, pages in ((1, 2), (3, 2), (64, 2), (17, 512), (4096, 512), (64, 0)):
+        a = attention_desc(seq=seq, q_batch_stride=seq * 1024, q_token_stride=1024, max_pages=pages)
+        rc, size = tree_workspace(a)
+        rows = a.batch * seq * a.q_heads
+        assert rc == 0 and size % (rows * (c.head_dim * 4 + 8)) == 0
+        assert size == 0 or size >= 2 * rows * (c.head_dim * 4 + 8)
+    assert tree_workspace(attention_desc(seq=0)) == (0, 0) and tree_workspace(attention_desc(batch=0)) == (0, 0)
+    for kw, rc in ((dict(seq=4097), UNSUPPORTED), (dict(max_pages=-1), INVALID), (dict(max_pages=1 << 30), INVALID),
+                   (dict(dtype=_lib.S8), UNSUPPORTED), (dict(q_heads=7), INVALID)):
+        assert tree_workspace(attention_desc(**{**dict(seq=3), **kw}))[0] == rc, kw
+    a = attention_desc(seq=3)
+    assert L.nnrh_kv_tree_attention_workspace(C.byref(c), C.byref(a), None) == INVALID
+    assert L.nnrh_kv_tree_attention_workspace(None, C.byref(a), C.byref(n)) == INVALID
+    assert L.nnrh_kv_tree_attention_workspace(C.byref(c), None, C.byref(n)) == INVALID
+
+
 @pytest.mark.parametrize("kw,rc", [
     (dict(dtype=_lib.S8), UNSUPPORTED), (dict(q_heads=7), INVALID), (dict(prefix_len=-1), INVALID), (dict(batch=-1), INVALID),
     (dict(seq=-1), INVALID), (dict(page_table_dev=None), INVALID), (dict(seq=4097, q_token_stride=1024), UNSUPPORTED)])
@@ -136,6 +160,7 @@ def test_tree_refuses(kw, rc):
 @pytest.mark.parametrize("kw,rc", BAD_CACHES)
 def test_tree_refuses_caches(kw, rc):
     assert tree(attention_desc(seq=3, q_batch_stride=4096), cache=cache_desc(**kw)) == rc
+    assert tree_workspace(attention_desc(seq=3, q_batch_stride=4096), cache_desc(**kw))[0] == rc
 
 
 def test_tree_refuses_memory():
