@@ -234,9 +234,17 @@ template <int TY, int HD> struct Rows {
 // The sums of wide heads lie in the accumulator half of the register file, which
 // products read and write but no other instruction does. Left to itself the compiler
 // takes all of them to the other half and back at every tile for this one that hardly
-// ever runs. (The waits are for a product's result, and before the next one.)
+// ever runs. (The waits are for a product's result, and before the next one; all sums
+// are their operands, so that no product moves past them.)
+__device__ __forceinline__ void acc_wait(f16v* o) {
+    asm volatile("s_nop 15\n\ts_nop 15" : "+a"(o[0]), "+a"(o[1]), "+a"(o[2]), "+a"(o[3]), "+a"(o[4]), "+a"(o[5]), "+a"(o[6]), "+a"(o[7]));
+}
+__device__ __forceinline__ void acc_stay(f16v* o) {
+    asm volatile("" : "+a"(o[0]), "+a"(o[1]), "+a"(o[2]), "+a"(o[3]), "+a"(o[4]), "+a"(o[5]), "+a"(o[6]), "+a"(o[7]));
+}
 template <int HD> __device__ __forceinline__ void scale_acc(f16v* o, float al) {
-    asm volatile("s_nop 15\n\ts_nop 15");
+    static_assert(HD == 256);
+    acc_wait(o);
 #pragma unroll
     for (int d = 0; d < HD / 32; ++d)
 #pragma unroll
@@ -246,12 +254,18 @@ template <int HD> __device__ __forceinline__ void scale_acc(f16v* o, float al) {
                          : "+a"(x), "=&v"(y) : "v"(al));
             o[d][r] = x;
         }
-    asm volatile("s_nop 7");
+    acc_wait(o);
+}
+__device__ __forceinline__ float add_acc(float o, float x) {
+    float y;
+    asm volatile("v_accvgpr_read_b32 %1, %0\n\ts_nop 1\n\tv_add_f32 %1, %1, %2\n\ts_nop 1\n\tv_accvgpr_write_b32 %0, %1"
+                 : "+a"(o), "=&v"(y) : "v"(x));
+    return o;
 }
 
 // Scores of NB x 16 keys a lane, raw, to weights 2^top p. key0: of the tile;
 // masked: some row does not see all of it.
-template <int TY, int HD, int NB>
+template <int TY, int HD, int KG, int NB>
 __device__ __forceinline__ void weigh(Rows<TY, HD>& w, f16v* s, int key0, bool masked) {
     const int half = (threadIdx.x & 63) >> 5;
     if (masked) {
@@ -278,7 +292,7 @@ __device__ __forceinline__ void weigh(Rows<TY, HD>& w, f16v* s, int key0, bool m
         w.m = up ? mx : w.m;
         w.l *= al;
         if constexpr (HD > 128) {
-            scale_acc<HD>(w.o, al);
+            if (key0 >= NB * 32 * KG) scale_acc<HD>(w.o, al);   // (before a wave's first tile the sums are zeros)
         } else {
 #pragma unroll
             for (int d = 0; d < HD / 32; ++d) w.o[d] *= al;
@@ -320,13 +334,12 @@ __device__ __forceinline__ u4 value_operand(const uint8_t* v, int lane, int m, i
 template <int TY, int HD, int KG>
 __device__ __forceinline__ bool any_bad(const uint8_t* v) {
     typedef Lds<TY, HD, KG> L;
-    const int lane = lane_here();
+    const uint8_t* at = v + lane_here() * 16;
     us2 top = {0, 0};
     bool bad = false;
-#pragma unroll 4
-    for (int i = lane; i < L::NW * L::real; i += 64) {
-        const int row = i / L::real;
-        const u4 x = *(const u4*)(v + (row * L::CH + (i % L::real ^ L::value(row))) * 16);
+#pragma unroll 8
+    for (int i = 0; i < L::NW * L::CH / 64; ++i) {   // (in any order; what is held and not a row's is zeros)
+        const u4 x = *(const u4*)(at + i * 1024);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if constexpr (TY == FT_F32) bad |= (x[j] & 0x7fffffffu) >= 0x7f800000u;
@@ -381,29 +394,50 @@ template <int TY, int HD, int KG>
 __device__ __forceinline__ void add_others(Rows<TY, HD>& w, const uint8_t* v, int key0) {
     typedef Lds<TY, HD, KG> L;
     const int half = lane_here() >> 5;
-#pragma unroll 1
-    for (int row = 0; row < L::NW; ++row) {
-        if (!__any(key0 + row < w.lim)) break;
+    // (what is not finite of elements 32 d .. in a row that the lane's row sees)
+    const auto of_row = [&](int row, int d, auto add) {
 #pragma unroll
-        for (int d = 0; d < HD / 32; ++d)
+        for (int i = 0; i < 4; ++i) {
+            const int e = 32 * d + 8 * i + 4 * half, c = e * Type<TY>::size / 16;
+            const uint8_t* at = v + (row * L::CH + (c ^ L::value(row))) * 16 + e * Type<TY>::size % 16;
+            float x[4];
+            if constexpr (TY == FT_F32) {
+                const f4 y = *(const f4*)at;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int e = 32 * d + 8 * i + 4 * half, c = e * Type<TY>::size / 16;
-                const uint8_t* at = v + (row * L::CH + (c ^ L::value(row))) * 16 + e * Type<TY>::size % 16;
-                float x[4];
-                if constexpr (TY == FT_F32) {
-                    const f4 y = *(const f4*)at;
+                for (int r = 0; r < 4; ++r) x[r] = y[r];
+            } else {
+                const typename Type<TY>::v4 y = *(const typename Type<TY>::v4*)at;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) x[r] = y[r];
-                } else {
-                    const typename Type<TY>::v4 y = *(const typename Type<TY>::v4*)at;
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) x[r] = (float)y[r];
-                }
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (!(fabsf(x[r]) < __builtin_inff()) && key0 + row < w.lim) w.o[d][4 * i + r] += x[r];
+                for (int r = 0; r < 4; ++r) x[r] = (float)y[r];
             }
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (!(fabsf(x[r]) < __builtin_inff()) && key0 + row < w.lim) add(4 * i + r, x[r]);
+        }
+    };
+    if constexpr (HD > 128) {   // 32 elements at a time in registers that additions reach
+        acc_wait(w.o);
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d) {
+            float sum[16];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sum[r] = -0.0f;
+#pragma unroll 1
+            for (int row = 0; row < L::NW; ++row) {
+                if (!__any(key0 + row < w.lim)) break;
+                of_row(row, d, [&](int r, float x) { sum[r] += x; });
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) w.o[d][r] = add_acc(w.o[d][r], sum[r]);
+        }
+        acc_wait(w.o);
+    } else {
+#pragma unroll 1
+        for (int row = 0; row < L::NW; ++row) {
+            if (!__any(key0 + row < w.lim)) break;
+#pragma unroll
+            for (int d = 0; d < HD / 32; ++d) of_row(row, d, [&](int r, float x) { w.o[d][r] += x; });
+        }
     }
 }
 
@@ -430,6 +464,18 @@ __device__ __forceinline__ void raw_scores(const Rows<TY, HD>& w, f16v* s, const
                 s[b] = Type<TY>::mfma(x, w.q[i], s[b]);
             }
         }
+    if constexpr (TY != FT_F32 && HD > 64) {
+        // four reads on their way before the product that needs the first (of its own the
+        // compiler takes one; heads of 256, 32 over 8 of 4096 tokens: 342 us, so 324)
+        constexpr int ahead = 4, all = Rows<TY, HD>::NQ * (L::NW / 32);
+        __builtin_amdgcn_sched_group_barrier(0x100, ahead, 0);
+#pragma unroll
+        for (int i = 0; i < all - ahead; ++i) {
+            __builtin_amdgcn_sched_group_barrier(8, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(8, ahead, 0);
+    }
 }
 
 // Waves that have seen other keys for the same rows: sums and totals by the rows'
@@ -539,7 +585,7 @@ __global__ __launch_bounds__(PW * 64, HD <= 128 ? 2 : 1) void prompt_kernel(Prom
     for (; key0 + L::N <= block_lo; key0 += L::N, at ^= 1) {
         next();
         raw_scores<TY, HD, KG>(w, s, lds[at][0] + part * L::part, lane);
-        weigh<TY, HD, NB>(w, s, key0, false);
+        weigh<TY, HD, KG, NB>(w, s, key0, false);
         add_values<TY, HD, KG, false>(w, s, lds[at][1] + part * L::part, lane);
     }
     // the tiles that some of the block's rows see in part or not at all
@@ -549,7 +595,7 @@ __global__ __launch_bounds__(PW * 64, HD <= 128 ? 2 : 1) void prompt_kernel(Prom
         const uint8_t* v = lds[at][1] + part * L::part;
         if (first >= hi) continue;
         raw_scores<TY, HD, KG>(w, s, lds[at][0] + part * L::part, lane_here());
-        weigh<TY, HD, NB>(w, s, first, true);
+        weigh<TY, HD, KG, NB>(w, s, first, true);
         if (__builtin_expect(any_bad<TY, HD, KG>(v), 0)) {
             stay_a_branch();
             add_values<TY, HD, KG, true>(w, s, v, lane_here());
@@ -557,6 +603,7 @@ __global__ __launch_bounds__(PW * 64, HD <= 128 ? 2 : 1) void prompt_kernel(Prom
         } else {
             add_values<TY, HD, KG, false>(w, s, v, lane_here());
         }
+        if constexpr (HD > 128) acc_stay(w.o);
     }
     if constexpr (KG > 1) join<TY, HD, KG>(w, wave, lds_);
     else w.l += __shfl_xor(w.l, 32);
