@@ -18,7 +18,7 @@
 // weights p are rounded to the tensors' type (11 or 8 bits), which is as far off
 // as rounding the result is, and would cost a second product to avoid. They are
 // held as 2^top p: fp16 has no small numbers (p <= 2^15 there, and weights down to
-// 2^-35 of the largest keep a bit); in bf16 and fp32 a sum of largest numbers must
+// 2^-32 of the largest keep a bit); in bf16 and fp32 a sum of largest numbers must
 // not pass them (2^20 equal weights of such values still do not).
 #include "nnrh_decode.h"
 
@@ -43,20 +43,22 @@ constexpr int PW = 4, PR = 32;              // waves of a block, rows of a wave
 // tile for the same rows, and are joined at the end.
 template <int KG> constexpr int kBlockRows = PW / KG * PR;
 template <int TY, int KG> constexpr int kWaveKeys = TY != FT_F32 && KG == 1 ? 64 : 32;   // of a tile
-constexpr float kSlack = 4.0f;              // powers of two by which scores may outgrow the maximum that they refer to
 constexpr float kNegInf = -__builtin_inff();
 constexpr float kLeast = 1e-37f;            // a factor of 0 would make NaN of a masked score, -inf
 
+// slack: powers of two by which scores may outgrow the maximum that they refer to.
+// (3 sequences to 2001, heads of 256, scores of a deviation of 1.4: with 4 in place of
+// these 70 us, 64 so; others 1-2 %.)
 template <int TY> struct Type;
 template <> struct Type<FT_F32> {
     static constexpr int size = 4;
-    static constexpr float top = -24.0f;
+    static constexpr float top = -30.0f, slack = 10.0f;
 };
 template <> struct Type<FT_F16> {
     typedef h4 v4;
     typedef h8 v8;
     static constexpr int size = 2;
-    static constexpr float top = 11.0f;
+    static constexpr float top = 8.0f, slack = 7.0f;
     static constexpr uint32_t inf = 0x7c00;
     __device__ static __forceinline__ f16v mfma(u4 a, u4 b, f16v c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
@@ -66,7 +68,7 @@ template <> struct Type<FT_BF16> {
     typedef b4 v4;
     typedef b8 v8;
     static constexpr int size = 2;
-    static constexpr float top = -24.0f;
+    static constexpr float top = -30.0f, slack = 10.0f;
     static constexpr uint32_t inf = 0x7f80;
     __device__ static __forceinline__ f16v mfma(u4 a, u4 b, f16v c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
@@ -250,7 +252,7 @@ template <int HD> __device__ __forceinline__ void scale_acc(f16v* o, float al) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             float x = o[d][r], y;
-            asm volatile("v_accvgpr_read_b32 %1, %0\n\ts_nop 1\n\tv_mul_f32 %1, %1, %2\n\ts_nop 1\n\tv_accvgpr_write_b32 %0, %1"
+            asm volatile("v_accvgpr_read_b32 %1, %0\n\tv_mul_f32 %1, %1, %2\n\tv_accvgpr_write_b32 %0, %1"
                          : "+a"(x), "=&v"(y) : "v"(al));
             o[d][r] = x;
         }
@@ -258,7 +260,7 @@ template <int HD> __device__ __forceinline__ void scale_acc(f16v* o, float al) {
 }
 __device__ __forceinline__ float add_acc(float o, float x) {
     float y;
-    asm volatile("v_accvgpr_read_b32 %1, %0\n\ts_nop 1\n\tv_add_f32 %1, %1, %2\n\ts_nop 1\n\tv_accvgpr_write_b32 %0, %1"
+    asm volatile("v_accvgpr_read_b32 %1, %0\n\tv_add_f32 %1, %1, %2\n\tv_accvgpr_write_b32 %0, %1"
                  : "+a"(o), "=&v"(y) : "v"(x));
     return o;
 }
@@ -285,7 +287,7 @@ __device__ __forceinline__ void weigh(Rows<TY, HD>& w, f16v* s, int key0, bool m
     mx = max_halves(mx);
     // the maximum moves on only where a score outgrows it by more than the slack (a row's
     // by itself: what other rows see has no part in its rounding)
-    const bool up = mx * w.rk > __builtin_fmaf(w.m, w.rk, kSlack);
+    const bool up = mx * w.rk > __builtin_fmaf(w.m, w.rk, Type<TY>::slack);
     if (__builtin_expect(__any(up), 0)) {
         stay_a_branch();
         const float al = up ? exp2_((w.m - mx) * w.rk) : 1.0f;
