@@ -639,7 +639,7 @@ hipError_t start(const PromptAttention& a, hipStream_t s) {
 // full for so short that its last blocks count. Up to these (fp16, us, one group and
 // two: heads of 64, 12 of 4096 tokens, 396 blocks 58.7, 45.7; 32 over 8 of 2048, 520
 // 34.8, 35.6. Heads of 128, 453 blocks 65, 53; 516 34, 38. Heads of 256, one block
-// a CU, 263 84, 73; 396 161, 183. fp32, bound by its products: heads of 64, 664 64.5,
+// a CU, 83 20.1, 16.3; 263 76, 68; 317 45, 58; 396 141, 170. fp32, bound by its products: heads of 64, 664 64.5,
 // 53.3; heads of 128, 520 387, 340; 664 90, 116. Four groups and two: heads of 64,
 // 129 16.9, 21.0; 204 22.5, 22.7; heads of 128, 63 15.7, 18.6; 83 14.2, 10.8.)
 template <int TY, int HD> constexpr int kTwoGroups = HD > 128 ? (TY == FT_F32 ? 0 : 272) : TY != FT_F32 ? 448 : HD == 64 ? 1024 : 512;
