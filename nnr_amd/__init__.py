@@ -604,6 +604,11 @@ def _on_device(device, **tensors):
             raise ValueError(f"{name} is on {t.device}, not on {device}")
 
 
+def _on_gpu(name, device):
+    if device.type != "cuda":
+        raise ValueError(f"{name}: on {device}, not on a GPU")
+
+
 class MatMulNBits:
     """y = a W^T + bias with 4-bit weights, W[n][k] = (q - zp) * scale of block
     k // block_size (com.microsoft MatMulNBits with a constant B).
@@ -826,6 +831,7 @@ class KVCache:
                 raise ValueError(f"tree must be bool [{S}, {S}] or [{B}, {S}, {S}]")
             if tree.device != self.device:
                 _on_device(self.device, tree=tree)
+            _on_gpu("the cache", self.device)
             if tree.dim() == 3 and tree.stride(0) == 0:   # one that was expanded
                 tree = tree[0]
             if not tree.is_contiguous():
@@ -888,6 +894,7 @@ def copy_pages(caches, source, destination, stream=None):
         raise ValueError(f"{count} sources, {destination.shape[0]} destinations")
     if count > 0x7fffffff:
         _int32(pages=count)
+    _on_gpu("the caches", cache.device)
     _launch(cache._index, cache._L.nnrh_kv_copy_pages, cache.desc, data, n, source.data_ptr(), destination.data_ptr(), count)
 
 
@@ -909,6 +916,7 @@ def move_tokens(caches, page_table, source, destination, stream=None):
         raise ValueError(f"page_table, source and destination are of {rows}, {(B, count)} and {tuple(destination.shape)}")
     if max(B, count, pages) > 0x7fffffff:
         _int32(batch=B, count=count, pages=pages)
+    _on_gpu("the caches", cache.device)
     moves = KvMoves(B, count, page_table.data_ptr(), pages, source.data_ptr(), destination.data_ptr())
     _launch(cache._index, cache._L.nnrh_kv_move_tokens, cache.desc, data, n, moves)
 
@@ -939,7 +947,7 @@ class RotaryEmbedding:
         self.head_dim, self.max_positions, self.rotary_dim = int(head_dim), int(max_positions), int(r)
         self.interleaved = bool(interleaved)
         if frequencies is None:
-            if original_positions is None:
+            if original_positions is None and factor > 0:
                 original_positions = max_positions / factor
             frequencies, m = rotary_frequencies(r, base, scaling, factor, original_positions)
             magnitude = m if magnitude is None else magnitude
@@ -947,9 +955,12 @@ class RotaryEmbedding:
         if f.shape != (r // 2,):
             raise ValueError(f"{tuple(f.shape)} frequencies, {r // 2} expected")
         device = torch.device("cuda" if device is None else device)
+        if device.type != "cuda":
+            raise ValueError(f"a table on {device}, not on a GPU")
         angles = torch.arange(max_positions, dtype=torch.float64, device=device)[:, None] * f.to(device)
         m = 1.0 if magnitude is None else float(magnitude)
         self.table = torch.stack((angles.cos() * m, angles.sin() * m), -1).float()
+        torch.cuda.current_stream(self.table.device).synchronize()   # whatever stream the calls are on
         self.device, self._index = self.table.device, self.table.device.index
         self._torch, self._table, self._run = torch, self.table.data_ptr(), lib().nnrh_rotary
 
@@ -1042,6 +1053,7 @@ def prompt_attention(q, k, v, starts, scale=None, causal=True, y=None, stream=No
         raise ValueError("q, k and v must agree in type")
     if k.device != device or v.device != device:
         _on_device(device, k=k, v=v)
+    _on_gpu("q", device)
     starts = _int32_tensor("starts", starts, device, 1)
     seqs = starts.shape[0] - 1
     if seqs < 0:

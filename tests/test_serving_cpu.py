@@ -72,11 +72,27 @@ def test_frequencies(scaling, factor, r):
     assert np.abs(f / want - 1).max() < 1e-14 and abs(m - wm) < 1e-14
 
 
+def test_python_refuses_host_memory():
+    """Tensors that no kernel can read"""
+    t = torch.zeros((4, 2, 64))
+    starts, one = torch.tensor([0, 4], dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    cache = nnr_amd.KVCache(2, 2, 64, page_size=32, device="cpu")
+    calls = (lambda: nnr_amd.prompt_attention(t, t, t, starts),
+             lambda: nnr_amd.RotaryEmbedding(64, 10, device="cpu"),
+             lambda: nnr_amd.copy_pages(cache, one, one),
+             lambda: nnr_amd.move_tokens([cache], one[None], one[None], one[None]),
+             lambda: cache.attention(t[None], one[None], one, tree=torch.ones((4, 4), dtype=torch.bool)))
+    for call in calls:
+        with pytest.raises(ValueError, match="not on a GPU"):
+            call()
+
+
 def test_frequencies_refuse():
     for kw in (dict(scaling="cubic"), dict(factor=0.0), dict(base=-1.0), dict(scaling="yarn")):
         with pytest.raises(ValueError):
             nnr_amd.rotary_frequencies(64, **kw)
-    for kw in (dict(rotary_dim=63), dict(rotary_dim=66), dict(max_positions=0), dict(frequencies=[1.0])):
+    for kw in (dict(rotary_dim=63), dict(rotary_dim=66), dict(max_positions=0), dict(frequencies=[1.0]),
+               dict(scaling="linear", factor=0.0)):
         with pytest.raises(ValueError):
             nnr_amd.RotaryEmbedding(**{**dict(head_dim=64, max_positions=10, device="cpu"), **kw})
 
