@@ -18,7 +18,7 @@
 // weights p are rounded to the tensors' type (11 or 8 bits), which is as far off
 // as rounding the result is, and would cost a second product to avoid. They are
 // held as 2^top p: fp16 has no small numbers (p <= 2^15 there, and weights down to
-// 2^-32 of the largest keep a bit); in bf16 and fp32 a sum of largest numbers must
+// 2^-35 of the largest keep a bit); in bf16 and fp32 a sum of largest numbers must
 // not pass them (2^20 equal weights of such values still do not).
 #include "nnrh_decode.h"
 
@@ -47,8 +47,8 @@ constexpr float kNegInf = -__builtin_inff();
 constexpr float kLeast = 1e-37f;            // a factor of 0 would make NaN of a masked score, -inf
 
 // slack: powers of two by which scores may outgrow the maximum that they refer to.
-// (3 sequences to 2001, heads of 256, scores of a deviation of 1.4: with 4 in place of
-// these 70 us, 64 so; others 1-2 %.)
+// (3 sequences to 2001, heads of 256, bf16, scores of a deviation of 1.4: with 4 in
+// place of 10 70 us, 64 so; others 1-2 %. In fp16 it would be small weights' bits.)
 template <int TY> struct Type;
 template <> struct Type<FT_F32> {
     static constexpr int size = 4;
@@ -58,7 +58,7 @@ template <> struct Type<FT_F16> {
     typedef h4 v4;
     typedef h8 v8;
     static constexpr int size = 2;
-    static constexpr float top = 8.0f, slack = 7.0f;
+    static constexpr float top = 11.0f, slack = 4.0f;
     static constexpr uint32_t inf = 0x7c00;
     __device__ static __forceinline__ f16v mfma(u4 a, u4 b, f16v c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);

@@ -206,6 +206,21 @@ def test_prompt_scores_grow(dev, t, hd):
 
 
 @pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("hd,Hq,Hk,lens", [(256, 2, 1, [400, 33]), (256, 40, 40, [300, 300, 300]), (96, 2, 2, [400])])
+def test_prompt_scores_grow_by_little(dev, t, hd, Hq, Hk, lens):
+    """Scores that grow by 2^8 of a weight every 32 tokens (the maximum moves at some of the tiles, in some of the rows), over
+    random ones; few blocks and more than the chip holds at once"""
+    rows, starts = prompts(6, lens, Hq, Hk, hd, t)
+    q, k, v = parts(rows, Hq, Hk)
+    q[:, :, 0] = 1
+    for b, n in enumerate(lens):
+        k[starts[b]:starts[b + 1], :, 0] = (torch.arange(n) // 32).float()[:, None] * 5.5
+    q[1::3, :, 0] = 0
+    y = nnr_amd.prompt_attention(q.to(dev), k.to(dev), v.to(dev), ints(dev, starts), scale=1.0)
+    near(y, *R.prompt(q, k, v, starts, 1.0, True), t)
+
+
+@pytest.mark.parametrize("t", TYPES)
 def test_prompt_large_values(dev, t):
     """The largest numbers of a type as values, whose sums pass them where their means do not"""
     rows, starts = prompts(2, [300], 2, 1, 64, t)
@@ -488,6 +503,23 @@ def test_tree_scales_far_apart(dev, t, bits, S):
         x[:, n - S + 1] = 3e4 if t == torch.float16 else 1e6
         return x
     check_tree(dev, t, bits, 64, 1, 2, tree, [S, 90], 0, 32, seed=9, vscale=vscale)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("hd", [64, 96, 128])
+def test_tree_scales_far_apart_in_parts(dev, t, bits, hd):
+    """As before, behind a prefix, over several parts of prefix and sequence, with more rows than a block has"""
+    S = 40
+    tree = random_tree(np.random.default_rng(4), S)
+    tree[:, 1] = False
+    tree[1, 1] = tree[5, 1] = True
+
+    def vscale(B, n):
+        x = torch.full((B, n, 1, 1), 1e-3)
+        x[:, n - S + 1] = 3e4 if t == torch.float16 else 1e6
+        return x
+    check_tree(dev, t, bits, hd, 1, 4, tree, [S, 700, 230], 300, 64, seed=11, vscale=vscale)
 
 
 @pytest.mark.parametrize("bits", [8, 4])
