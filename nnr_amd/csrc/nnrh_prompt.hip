@@ -308,9 +308,10 @@ __device__ __forceinline__ void weigh(Rows<TY, HD>& w, f16v* s, int key0, bool m
     for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            // (the difference first in fp32: of large scores' products little would be left)
-            const float x = TY == FT_F32 ? __builtin_fmaf(s[b][r] - base, w.rk, top) : __builtin_fmaf(s[b][r], w.rk, off);
-            s[b][r] = exp2_(x);
+            // (the difference first in fp32: of large scores' products little would be left;
+            // nor of an exponent's last bits beside 2^top)
+            if constexpr (TY == FT_F32) s[b][r] = exp2_((s[b][r] - base) * w.rk) * ldexpf(1.0f, (int)top);
+            else s[b][r] = exp2_(__builtin_fmaf(s[b][r], w.rk, off));
             sum[r & 1] += s[b][r];
         }
     w.l += sum[0] + sum[1];
