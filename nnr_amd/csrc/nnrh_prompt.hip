@@ -200,25 +200,34 @@ template <int TY, int HD, int KG> struct Lds {
 };
 // A thread's loads of a tile: bytes from the tile's first row
 template <int TY, int HD, int KG> struct Loads {
-    uint32_t at[Lds<TY, HD, KG>::loads];
-    __device__ __forceinline__ void set(uint32_t stride, bool values) {
-        typedef Lds<TY, HD, KG> L;
-#pragma unroll
-        for (int i = 0; i < L::loads; ++i) {
-            const int id = i * PW * 64 + threadIdx.x, row = id / L::CH;
-            const int chunk = id % L::CH ^ (values ? L::value(row) : L::key(row));
-            at[i] = chunk < L::real ? row * stride + chunk * 16 : 0xfffffff0u;   // (none: nothing is read there)
-        }
+    typedef Lds<TY, HD, KG> L;
+    uint32_t at[L::loads];
+    static __device__ __forceinline__ uint32_t place(int i, int thread, uint32_t stride, bool values) {
+        const int id = i * PW * 64 + thread, row = id / L::CH;
+        const int chunk = id % L::CH ^ (values ? L::value(row) : L::key(row));
+        return chunk < L::real ? row * stride + chunk * 16 : 0xfffffff0u;   // (none: nothing is read there)
     }
-    // rows: those that are left from the tile's first on; what is past them reads as 0
-    __device__ __forceinline__ void load(const uint8_t* first, uint32_t stride, int rows, uint8_t* lds) const {
-        typedef Lds<TY, HD, KG> L;
+    __device__ __forceinline__ void set(uint32_t stride, bool values) {
+#pragma unroll
+        for (int i = 0; i < L::loads; ++i) at[i] = place(i, threadIdx.x, stride, values);
+    }
+    // rows: those that are left from the tile's first on; what is past them reads as 0.
+    // fn(i): the bytes of load i
+    template <class F> static __device__ __forceinline__ void start(const uint8_t* first, uint32_t stride, int rows, uint8_t* lds, F fn) {
         const uint32_t bytes = (uint32_t)(min(rows, L::N) - 1) * stride + HD * Type<TY>::size;
         const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)first, (short)0, (int)bytes, 0x00020000);
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
         for (int i = 0; i < L::loads; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (NNRH_LDS void*)(lds + (i * PW + wave) * 1024), 16, (int)at[i], 0, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (NNRH_LDS void*)(lds + (i * PW + wave) * 1024), 16, (int)fn(i), 0, 0, 0);
+    }
+    __device__ __forceinline__ void load(const uint8_t* first, uint32_t stride, int rows, uint8_t* lds) const {
+        start(first, stride, rows, lds, [&](int i) { return at[i]; });
+    }
+    // with places found anew, for want of registers
+    static __device__ __forceinline__ void load_anew(const uint8_t* first, uint32_t stride, int rows, uint8_t* lds, bool values) {
+        const int thread = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 64 + lane_here();
+        start(first, stride, rows, lds, [&](int i) { return place(i, thread, stride, values); });
     }
 };
 
@@ -529,11 +538,17 @@ __device__ __forceinline__ void join(Rows<TY, HD>& w, int wave, uint8_t* lds) {
 }
 template <int HD> constexpr int kJoinLds = PW * PR * 8 + PW * HD * PR * 4;
 
+// Two tiles of wide fp32 heads do not fit twice: there is a place for keys and one for
+// values, and each is loaded as soon as all waves have read it, while they work on the
+// other.
+template <int TY, int HD, int KG> constexpr bool kOnce = 4 * Lds<TY, HD, KG>::tile > 160 * 1024;
+
 template <int TY, int HD, int KG>
 __global__ __launch_bounds__(PW * 64, HD <= 128 ? 2 : 1) void prompt_kernel(PromptAttention a, int G, int blocks) {
     typedef Lds<TY, HD, KG> L;
     constexpr int ES = Type<TY>::size, BM = kBlockRows<KG>, NB = L::NW / 32;
-    constexpr int bytes = KG > 1 && kJoinLds<HD> > 4 * L::tile ? kJoinLds<HD> : 4 * L::tile;
+    constexpr bool once = kOnce<TY, HD, KG>;
+    constexpr int held = (once ? 2 : 4) * L::tile, bytes = KG > 1 && kJoinLds<HD> > held ? kJoinLds<HD> : held;
     __shared__ __attribute__((aligned(16))) uint8_t lds_[bytes];
     uint8_t(*lds)[2][L::tile] = (uint8_t(*)[2][L::tile])lds_;   // [2]: keys, values
     // Heads first, so that a head's blocks stay on an XCD where heads are a multiple of 8.
@@ -578,27 +593,9 @@ __global__ __launch_bounds__(PW * 64, HD <= 128 ? 2 : 1) void prompt_kernel(Prom
         for (int r = 0; r < 16; ++r) w.o[d][r] = 0.0f;
 
     int at = 0, key0 = 0;
-    const auto next = [&] {
-        // this tile is there, and the one before has been read by all
-        __builtin_amdgcn_s_waitcnt(0);
-        asm volatile("s_barrier" ::: "memory");
-        if (key0 + L::N < block_hi) load(key0 + L::N, at ^ 1);
-    };
     f16v s[NB];
-    for (; key0 + L::N <= block_lo; key0 += L::N, at ^= 1) {
-        next();
-        raw_scores<TY, HD, KG>(w, s, lds[at][0] + part * L::part, lane);
-        weigh<TY, HD, KG, NB>(w, s, key0, false);
-        add_values<TY, HD, KG, false>(w, s, lds[at][1] + part * L::part, lane);
-    }
-    // the tiles that some of the block's rows see in part or not at all
-    for (; key0 < block_hi; key0 += L::N, at ^= 1) {
-        next();
-        const int first = key0 + part * L::NW;   // the wave's part of the tile
-        const uint8_t* v = lds[at][1] + part * L::part;
-        if (first >= hi) continue;
-        raw_scores<TY, HD, KG>(w, s, lds[at][0] + part * L::part, lane_here());
-        weigh<TY, HD, KG, NB>(w, s, first, true);
+    // a wave's part of the tile, with some rows that do not see all of it
+    const auto add_masked = [&](const uint8_t* v, int first) {
         if (__builtin_expect(any_bad<TY, HD, KG>(v), 0)) {
             stay_a_branch();
             add_values<TY, HD, KG, true>(w, s, v, lane_here());
@@ -607,12 +604,58 @@ __global__ __launch_bounds__(PW * 64, HD <= 128 ? 2 : 1) void prompt_kernel(Prom
             add_values<TY, HD, KG, false>(w, s, v, lane_here());
         }
         if constexpr (HD > 128) acc_stay(w.o);
+    };
+    if constexpr (once) {
+        static_assert(L::loads == 16);   // what the waits count
+        for (; key0 < block_hi; key0 += L::N) {
+            const int first = key0 + part * L::NW;
+            const bool sees = first < hi, more = key0 + L::N < block_hi, masked = key0 + L::N > block_lo;
+            asm volatile("s_waitcnt vmcnt(16) lgkmcnt(0)\n\ts_barrier" ::: "memory");   // the keys; the values are on their way
+            if (sees) raw_scores<TY, HD, KG>(w, s, lds[0][0] + part * L::part, lane_here());
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            if (more) kl.load_anew(k + (long long)(key0 + L::N) * ks, ks, job.len - key0 - L::N, lds[0][0], false);
+            if (sees) weigh<TY, HD, KG, NB>(w, s, first, masked);
+            if (more) asm volatile("s_waitcnt vmcnt(16)\n\ts_barrier" ::: "memory");    // the values; the next keys are on their way
+            else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+            const uint8_t* v_ = lds[0][1] + part * L::part;
+            if (sees) {
+                if (masked) add_masked(v_, first);
+                else add_values<TY, HD, KG, false>(w, s, v_, lane_here());
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            if (more) vl.load_anew(v + (long long)(key0 + L::N) * vs, vs, job.len - key0 - L::N, lds[0][1], true);
+        }
+    } else {
+        const auto next = [&] {
+            // this tile is there, and the one before has been read by all
+            __builtin_amdgcn_s_waitcnt(0);
+            asm volatile("s_barrier" ::: "memory");
+            if (key0 + L::N < block_hi) load(key0 + L::N, at ^ 1);
+        };
+        for (; key0 + L::N <= block_lo; key0 += L::N, at ^= 1) {
+            next();
+            raw_scores<TY, HD, KG>(w, s, lds[at][0] + part * L::part, lane);
+            weigh<TY, HD, KG, NB>(w, s, key0, false);
+            add_values<TY, HD, KG, false>(w, s, lds[at][1] + part * L::part, lane);
+        }
+        // the tiles that some of the block's rows see in part or not at all
+        for (; key0 < block_hi; key0 += L::N, at ^= 1) {
+            next();
+            const int first = key0 + part * L::NW;   // the wave's part of the tile
+            if (first >= hi) continue;
+            raw_scores<TY, HD, KG>(w, s, lds[at][0] + part * L::part, lane_here());
+            weigh<TY, HD, KG, NB>(w, s, first, true);
+            add_masked(lds[at][1] + part * L::part, first);
+        }
     }
     if constexpr (KG > 1) join<TY, HD, KG>(w, wave, lds_);
     else w.l += __shfl_xor(w.l, 32);
     const float inv = 1.0f / w.l;
-    if (row0 + col >= job.nrows) return;
-    const long long y = ((job.s + (long long)tok) * a.q_heads + hq) * HD + 4 * half;
+    // (found anew where registers are short)
+    const int l_ = HD > 128 ? lane_here() : lane, mine = row0 + (l_ & 31);
+    if (mine >= job.nrows) return;
+    const int of = HD > 128 ? mine / G : tok, h = HD > 128 ? head * G + mine - of * G : hq;
+    const long long y = ((job.s + (long long)of) * a.q_heads + h) * HD + 4 * (l_ >> 5);
 #pragma unroll
     for (int d = 0; d < HD / 32; ++d) {
         if (d % KG != part) continue;
@@ -640,18 +683,18 @@ hipError_t start(const PromptAttention& a, hipStream_t s) {
 // full for so short that its last blocks count. Up to these (fp16, us, one group and
 // two: heads of 64, 12 of 4096 tokens, 396 blocks 58.7, 45.7; 32 over 8 of 2048, 520
 // 34.8, 35.6. Heads of 128, 453 blocks 65, 53; 516 34, 38. Heads of 256, one block
-// a CU, 83 20.1, 16.3; 263 76, 68; 317 45, 58; 396 141, 170. fp32, bound by its products: heads of 64, 664 64.5,
+// a CU, 83 20.1, 16.3; 263 76, 68; 317 45, 58; 396 141, 170; fp32 117 153, 97; 258 1048,
+// 701; 395 100, 131; 504 576, 723. fp32, bound by its products: heads of 64, 664 64.5,
 // 53.3; heads of 128, 520 387, 340; 664 90, 116. Four groups and two: heads of 64,
 // 129 16.9, 21.0; 204 22.5, 22.7; heads of 128, 63 15.7, 18.6; 83 14.2, 10.8.)
-template <int TY, int HD> constexpr int kTwoGroups = HD > 128 ? (TY == FT_F32 ? 0 : 272) : TY != FT_F32 ? 448 : HD == 64 ? 1024 : 512;
+template <int TY, int HD> constexpr int kTwoGroups = HD > 128 ? 272 : TY != FT_F32 ? 448 : HD == 64 ? 1024 : 512;
 template <int TY, int HD> constexpr int kFourGroups = HD == 64 ? 128 : TY != FT_F32 && HD <= 128 ? 64 : 0;
 template <int TY, int HD>
 hipError_t by_blocks(const PromptAttention& a, hipStream_t s) {
     const long long blocks = (long long)a.tokens * a.q_heads / kBlockRows<1> + (long long)a.seqs * a.kv_heads;
     if constexpr (kFourGroups<TY, HD> > 0)
         if (blocks <= kFourGroups<TY, HD>) return start<TY, HD, 4>(a, s);
-    if constexpr (kTwoGroups<TY, HD> > 0)
-        if (blocks <= kTwoGroups<TY, HD>) return start<TY, HD, 2>(a, s);
+    if (blocks <= kTwoGroups<TY, HD>) return start<TY, HD, 2>(a, s);
     return start<TY, HD, 1>(a, s);
 }
 template <int TY>

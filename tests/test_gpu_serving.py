@@ -254,6 +254,25 @@ def test_prompt_unseen_values(dev, t, hd, what):
 
 
 @pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_prompt_unseen_values_of_many(dev, t, hd):
+    """The same with more blocks than the chip holds at once (a block has more rows then)"""
+    lens, H, at = [300] * 3, 100, 437
+    rows, starts = prompts(7, lens, H, H, hd, t)
+    q, k, v = (x.to(dev) for x in parts(rows, H, H))
+    sd = ints(dev, starts)
+    clean = nnr_amd.prompt_attention(q, k, v, sd)
+    for what in (float("nan"), float("-inf")):
+        bad = v.clone()
+        bad[at, 60, 9] = what
+        y = nnr_amd.prompt_attention(q, k, bad, sd)
+        hit = torch.zeros(y.shape, dtype=torch.bool, device=dev)
+        hit[at:600, 60, 9] = True
+        assert torch.equal(y[~hit], clean[~hit])
+        assert (y[hit].isnan() if what != what else y[hit] == what).all()
+
+
+@pytest.mark.parametrize("t", TYPES)
 def test_prompt_unseen_kinds(dev, t):
     """Infinities of both signs and NaNs side by side, beside values of both signs."""
     n, hd = 100, 64
