@@ -264,7 +264,7 @@ struct Job {
     long long len;               // tokens that the source holds
     int t0, t1;                  // tiles
     const int32_t* table;
-    int drafts;                  // position of the first draft (may be negative); with a prefix's rows, or none: the largest
+    int drafts;                  // position of the first draft (may be negative); of the prefix nothing is one
 };
 
 // With drafts (TREE) a row's limit is its sequence's end, and of the tokens from
@@ -296,7 +296,7 @@ __device__ __forceinline__ void set_rows(const AttnArgs& p, const Job& job, int 
         w.hi = max(w.hi, __shfl_xor(w.hi, o));
     }
     w.lo = __builtin_amdgcn_readfirstlane(w.lo);
-    if (TREE) w.lo = min(w.lo, max(job.drafts, 0));
+    if (TREE && !job.pre) w.lo = min(w.lo, max(job.drafts, 0));
     w.hi = __builtin_amdgcn_readfirstlane(w.hi);
 }
 
@@ -651,11 +651,11 @@ template <int HD, int BITS> struct RawTile {
 // Does the row (its place among all) see the token at `key`, as far as the tree has
 // a say (key: of a tile that exists, maybe past the sequence's end). A byte is loaded
 // for any key, the first draft's where it is none, so that a tile's loads run side by
-// side; the prefix's rows, which see all, load the tree's first.
+// side; against the prefix, of which rows see all, the tree's first.
 __device__ __forceinline__ bool tree_sees(const AttnArgs& p, const Job& job, int row, int key) {
     const int line = job.pre ? 0 : (row / p.a.q_heads - job.b * p.a.seq) * p.a.seq;
     const int d = key - job.drafts;
-    const bool draft = (unsigned)d < (unsigned)p.a.seq;
+    const bool draft = !job.pre & ((unsigned)d < (unsigned)p.a.seq);
     const uint8_t* tree = p.a.tree + job.b * p.a.tree_bstride;
     const uint8_t sees = tree[(uint32_t)(line + (draft ? d : 0))];
     return (!draft) | (sees != 0);
@@ -1238,7 +1238,7 @@ __global__ __launch_bounds__(AW * 64, HD <= 128 ? (!PM && !OM && NP == 1 ? 3 : 2
         const long long cap = (long long)a.max_pages * p.c.page_size, len = scalar_load(a.lens, job.b);
         job.len = len < cap ? len : cap;
     }
-    job.drafts = 0x7fffffff;
+    job.drafts = 0;
     if (TREE && !job.pre) job.drafts = scalar_load(a.lens, job.b) - a.seq;
     const int chunk = job.pre ? p.pre_chunk : p.own_chunk;
     job.t0 = job.split * chunk;

@@ -1,0 +1,75 @@
+"""Operators around a decoder's cache where a part, a page, a length or a step has its end: against float64,
+like test_gpu_serving.py."""
+import numpy as np
+import pytest
+import torch
+
+import decode_ref as D
+import nnr_amd
+import serving_ref as R
+from test_gpu_serving import TYPES, cache_of, gen, ints, near, parts, prompts, random_tree, tables, tokens
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------------------
+# trees of drafts
+
+def tree_parts(cache, batch, S, Hq, per, prefix, t, length):
+    """Tiles [first, end) of a sequence's parts: the prefix's, then its own, in parts of equal length whose number the
+    workspace tells."""
+    size = cache.attention_workspace(batch, S, Hq, per, prefix, dtype=t, tree=True)
+    count = max(1, size // (batch * S * Hq * (cache.head_dim * 4 + 8)))
+    tiles = -(-prefix // 32) + -(-length // 32)
+    each, more = divmod(tiles, count)
+    ends = np.cumsum([each + (i < more) for i in range(count)]).tolist()
+    return list(zip([0] + ends[:-1], ends))
+
+
+@pytest.mark.parametrize("t", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("hd", [64, 96, 128])
+@pytest.mark.parametrize("prefix,lens,far_pre,far_own", [
+    (300, [40, 200], [20, 180], []), (64, [40, 60], [], [5]), (300, [300, 290], [], [10]), (33, [41], [32], [])])
+def test_tree_computed_again_behind_a_prefix(dev, t, bits, hd, prefix, lens, far_pre, far_own):
+    """A few large values that no row gives weight to, beside such of 1e-3: rows of the parts that hold them are computed
+    again in fp32. Those parts hold tokens of the prefix at the positions that drafts have in their sequence, and the
+    tree's first line hides all drafts but one."""
+    S, H, G, page = 40, 1, 4, 32
+    tree = random_tree(np.random.default_rng(4), S)
+    B, pre_pages, per = len(lens), -(-prefix // page), max(-(-n // page) for n in lens)
+    table, pages, spare = tables(np.random.default_rng(hd), B, per, pre_pages + 1)
+    cache = cache_of(dev, pages, H, hd, page_size=page, bits=bits)
+    for b, n in enumerate(lens):
+        found = False
+        for first, end in tree_parts(cache, B, S, H * G, per, prefix, t, n):
+            far = any(first <= p // 32 < end for p in far_pre) or any(first <= -(-prefix // 32) + p // 32 < end for p in far_own)
+            found |= far and any(first <= p // 32 < end for p in range(n - S + 1, min(n, prefix)))
+        assert found, "no part is computed again that the drafts' positions meet in the prefix"
+    most = max(lens)
+    k, v = tokens(1, B, most, H, hd, t)
+    pk, pv = tokens(2, 1, prefix, H, hd, t)
+    q = torch.randn((B, S, H * G, hd), generator=gen(3)).to(t)
+    big = 3e4 if t == torch.float16 else 1e6
+    q[..., 0] = 4
+    small_v = [x * 1e-3 for x in (v, pv)]
+    v[:], pv[:] = small_v
+    for x, y, at in ((pk, pv, [(0, p) for p in far_pre]), (k, v, [(b, most - n + p) for b, n in enumerate(lens) for p in far_own])):
+        for b, p in at:
+            x[b, p], x[b, p, :, 0] = 0, -8 * hd ** 0.5      # a score 32 less than one of 0
+            y[b, p] = big
+    cache.write(k.to(dev), v.to(dev), table.to(dev), ints(dev, lens))
+    pt = spare[:pre_pages].to(dev)
+    cache.write(pk.to(dev), pv.to(dev), pt[None], ints(dev, [prefix]))
+    y = cache.attention(q.to(dev), table.to(dev), ints(dev, lens), prefix_table=pt, prefix_len=prefix, tree=tree.to(dev)).cpu()
+    sc = np.float32(hd ** -0.5).item()
+    for b, n in enumerate(lens):
+        sees = torch.ones((S, prefix + n), dtype=torch.bool)
+        sees[:, prefix + n - S:] = tree
+        kx, vx = (torch.cat([D.quantize(x, bits)[0] for x in (p[0, :, 0], o[b, most - n:, 0])]) for p, o in ((pk, k), (pv, v)))
+        ref, w, tol = R.attend(q[b], kx, vx, sc, sees, 0.0)
+        # Parts without a large value are the products': weights of 2^-11 and steps of small ones in parts of what
+        # those hold at most, queries with a common power of two. (A part with one rounds no weight.)
+        low = 2.0 ** -39 * q[b].double().abs().amax((1, 2))[:, None, None] * kx.abs().sum(-1).amax() * sc
+        steps = len(vx) * R.CACHE_FLOOR[t] * max(x.double().abs().amax().item() for x in small_v)
+        near(y[b], ref, R.rounded(ref, w, tol + 2 * low * w + steps, t, R.CACHE_WEIGHTS[t]), t)
