@@ -1556,13 +1556,18 @@ __global__ __launch_bounds__(kTreeWaves * 64, 2) void kv_tree_kernel(AttnArgs p)
             }
     };
     TreeRows<HD> w;
-    pages(t0);
-    load(t0);
-    pages(t0 + KT);
+    // (a part without tiles may be of a cache without pages, which has no page 0 to read in place of those that do not exist)
+    if (t0 < t1) {
+        pages(t0);
+        load(t0);
+        pages(t0 + KT);
+    }
     tree_rows<HD, BITS>(p, job, row0, w);   // (a wave past the rows repeats the last one)
-    convert(t0, 0);
-    load(t0 + KT);
-    pages(t0 + 2 * KT);
+    if (t0 < t1) {
+        convert(t0, 0);
+        load(t0 + KT);
+        pages(t0 + 2 * KT);
+    }
     __syncthreads();
     int at = 0;
     for (int t = t0; t < t1; t += KT, at ^= 1) {

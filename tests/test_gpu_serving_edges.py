@@ -73,3 +73,21 @@ def test_tree_computed_again_behind_a_prefix(dev, t, bits, hd, prefix, lens, far
         low = 2.0 ** -39 * q[b].double().abs().amax((1, 2))[:, None, None] * kx.abs().sum(-1).amax() * sc
         steps = len(vx) * R.CACHE_FLOOR[t] * max(x.double().abs().amax().item() for x in small_v)
         near(y[b], ref, R.rounded(ref, w, tol + 2 * low * w + steps, t, R.CACHE_WEIGHTS[t]), t)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("hd", [64, 256])
+@pytest.mark.parametrize("S", [2, 40])
+def test_tree_over_a_cache_without_pages(dev, t, bits, hd, S):
+    """Nothing to see, and no memory behind the cache: zeros. So it is with lengths of 0 and tables without columns."""
+    q, tree = torch.randn((2, S, 4, hd), generator=gen(1)).to(t).to(dev), torch.ones((S, S), dtype=torch.bool, device=dev)
+    none = nnr_amd.KVCache(0, 2, hd, page_size=32, bits=bits, device=dev)
+    for per in (0, 1, 40):
+        for prefix in (0, 70):
+            y = none.attention(q, ints(dev, [[0] * per] * 2).view(2, per), ints(dev, [S, 1000]), prefix_table=ints(dev, [0, 0, 0]),
+                               prefix_len=prefix, tree=tree)
+            assert not y.any()
+    some = cache_of(dev, 3, 2, hd, page_size=32, bits=bits)
+    assert not some.attention(q, ints(dev, [[0], [1]]), ints(dev, [0, -5]), tree=tree).any()
+    assert not some.attention(q, ints(dev, [[], []]).view(2, 0), ints(dev, [S, 9]), tree=tree).any()
