@@ -90,6 +90,11 @@ __device__ __forceinline__ float max_halves(float m) {   // over lanes 32 apart
 }
 // keeps the compiler from computing both sides of a branch that is hardly ever taken
 __device__ __forceinline__ void stay_a_branch() { asm volatile(""); }
+// no load or store moves past it
+__device__ __forceinline__ void in_order() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
 // the lane, for what is rarely done: nothing that follows from it is kept in registers before
 __device__ __forceinline__ int lane_here() {
     int lane = threadIdx.x & 63;
@@ -582,6 +587,7 @@ __global__ __launch_bounds__(PW * 64, HD <= 128 ? 2 : 1) void prompt_kernel(Prom
     const uint8_t* v = (const uint8_t*)a.v + (job.s * a.vs + (long long)head * HD) * ES;
     const auto load = [&](int key0, int at) {
         kl.load(k + (long long)key0 * ks, ks, job.len - key0, lds[at][0]);
+        if constexpr (once) in_order();   // (the first wait there counts values behind keys)
         vl.load(v + (long long)key0 * vs, vs, job.len - key0, lds[at][1]);
     };
     load(0, 0);
