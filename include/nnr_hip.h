@@ -770,7 +770,7 @@ int nnrh_rotary(const nnrh_rotary_desc* d, const void* q_dev, const void* k_dev,
  * Scores, totals and sums are fp32; weights meet 16-bit values rounded to their
  * type. Values are such that 2^20 times the largest stays below 2^128 (fp16: any).
  * q [tokens][q_heads][head_dim], k and v [tokens][kv_heads][head_dim] with token
- * strides in elements (at most 2^22; heads are dense), y dense; addresses and strides
+ * strides in elements (at most 2^22; one token's say nothing; heads are dense), y dense; addresses and strides
  * in bytes are multiples of 16. y may be q itself where q is dense, and overlaps
  * nothing else. head_dim 64, 96, 128 or 256. No workspace.                  */
 typedef struct nnrh_prompt_attention_desc {

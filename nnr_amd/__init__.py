@@ -1075,10 +1075,11 @@ def prompt_attention(q, k, v, starts, scale=None, causal=True, y=None, stream=No
 
 
 def _dense_heads(t):
-    """[tokens, heads, head_dim] with dense heads and 16-byte steps, itself or a copy, and the tokens' step"""
+    """[tokens, heads, head_dim] with dense heads and 16-byte steps of 2^22 elements at most, itself or a copy, and the
+    tokens' step"""
     st, shape = t.stride(), t.shape
     if (st[2] != 1 or (st[1] != shape[2] and shape[1] > 1) or t.data_ptr() % 16 or
-            (st[0] * t.element_size() % 16 and shape[0] > 1)):
+            ((st[0] * t.element_size() % 16 or st[0] > 1 << 22) and shape[0] > 1)):
         t = t.contiguous()
         if t.data_ptr() % 16:
             t = t.clone()

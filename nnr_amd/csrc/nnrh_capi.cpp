@@ -2831,20 +2831,24 @@ extern "C" int nnrh_prompt_attention(const nnrh_prompt_attention_desc* d, const 
     if ((uintptr_t)d->starts_dev & 3) return set_err(NNRH_ERR_INVALID, "prompt_attention: alignment of the starts");
     const size_t es = float_type_size(type);
     const size_t qw = (size_t)d->q_heads * d->head_dim * es, kw = (size_t)d->kv_heads * d->head_dim * es, n = d->tokens;
-    for (const long long st : {d->q_stride, d->k_stride, d->v_stride}) {
-        if (st < 0 || (n > 1 && st * es % 16))
+    const bool steps = n > 1;   // (one token's are not taken and say nothing)
+    const long long qs = steps ? d->q_stride : (long long)(qw / es), ks = steps ? d->k_stride : (long long)(kw / es),
+                    vs = steps ? d->v_stride : (long long)(kw / es);
+    for (const long long st : {qs, ks, vs}) {
+        if (st < 0 || st * es % 16)
             return set_err(NNRH_ERR_INVALID, "prompt_attention: a stride of %lld (multiples of 16 bytes)", st);
         // (64 rows of a tile in 31 bits)
-        if (st > (1 << 22)) return set_err(NNRH_ERR_UNSUPPORTED, "prompt_attention: a stride of %lld (at most 2^22)", st);
+        if (steps && st > (1 << 22))
+            return set_err(NNRH_ERR_UNSUPPORTED, "prompt_attention: a stride of %lld (at most 2^22)", st);
     }
     const size_t ysize = n * qw;
     const auto extent = [&](long long st, size_t w) { return (n - 1) * st * es + w; };
-    const bool in_place = y == q && (n == 1 || (size_t)d->q_stride * es == qw);
-    if ((!in_place && overlap(y, ysize, q, extent(d->q_stride, qw))) || overlap(y, ysize, k, extent(d->k_stride, kw)) ||
-        overlap(y, ysize, v, extent(d->v_stride, kw)) || overlap(y, ysize, d->starts_dev, ((size_t)d->seqs + 1) * 4))
+    const bool in_place = y == q && (size_t)qs * es == qw;
+    if ((!in_place && overlap(y, ysize, q, extent(qs, qw))) || overlap(y, ysize, k, extent(ks, kw)) ||
+        overlap(y, ysize, v, extent(vs, kw)) || overlap(y, ysize, d->starts_dev, ((size_t)d->seqs + 1) * 4))
         return set_err(NNRH_ERR_INVALID, "prompt_attention: y lies over q, k, v or the starts");
-    const PromptAttention a{q, k, v, y, type, d->q_stride, d->k_stride, d->v_stride, d->tokens, d->seqs, d->q_heads,
-                            d->kv_heads, d->head_dim, d->scale, d->causal != 0, d->starts_dev};
+    const PromptAttention a{q, k, v, y, type, qs, ks, vs, d->tokens, d->seqs, d->q_heads, d->kv_heads, d->head_dim, d->scale,
+                            d->causal != 0, d->starts_dev};
     ProfScope ps("prompt_attention", S(stream));
     HIP_TRY(launch_prompt_attention(a, S(stream)), "prompt_attention");
     return NNRH_OK;

@@ -91,3 +91,32 @@ def test_tree_over_a_cache_without_pages(dev, t, bits, hd, S):
     some = cache_of(dev, 3, 2, hd, page_size=32, bits=bits)
     assert not some.attention(q, ints(dev, [[0], [1]]), ints(dev, [0, -5]), tree=tree).any()
     assert not some.attention(q, ints(dev, [[], []]).view(2, 0), ints(dev, [S, 9]), tree=tree).any()
+
+
+# ---------------------------------------------------------------------------
+# attention of prompts
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("n", [1, 3])
+def test_prompt_tokens_far_apart(dev, t, n):
+    """Tokens at steps past 2^22 elements: the last ones of long sequences. A single token's step says nothing."""
+    S, H, hd = 1060, 32, 128
+    x = torch.zeros((n, S, 3 * H, hd), dtype=t, device=dev)
+    x[:, -1] = torch.randn((n, 3 * H, hd), generator=gen(n)).to(t).to(dev)
+    q, k, v = (x[:, -1, i * H:(i + 1) * H] for i in range(3))
+    assert q.stride(0) > 1 << 22
+    starts = ints(dev, [0, n])
+    want = nnr_amd.prompt_attention(q.contiguous(), k.contiguous(), v.contiguous(), starts)
+    assert torch.equal(nnr_amd.prompt_attention(q, k, v, starts), want)
+    near(want, *R.prompt(q.cpu(), k.cpu(), v.cpu(), [0, n], np.float32(hd ** -0.5).item(), True), t)
+    if n == 1:
+        assert torch.equal(want, v)
+        y = q[0, :, :].unsqueeze(0)      # in place
+        assert nnr_amd.prompt_attention(y, k, v, starts, y=y) is y and torch.equal(y, want)
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_prompt_of_one_token_many_heads(dev, t):
+    """A row of more than 2^22 elements is no step either."""
+    q, k, v = torch.randn((3, 1, 17000, 256), device=dev).to(t).unbind(0)
+    assert torch.equal(nnr_amd.prompt_attention(q, k, v, ints(dev, [0, 1])), v)
