@@ -2716,17 +2716,20 @@ struct Lines {
     size_t width, bs, ts;
     int batch, seq;
     size_t extent() const { return (batch - 1) * bs + (seq - 1) * ts + width; }
-    // one step that leads through all lines
-    bool even() const { return batch == 1 || seq == 1 || bs == seq * ts; }
-    size_t step() const { return seq > 1 ? ts : batch > 1 ? bs : 0; }
+    // a step whose multiples all lines begin at, of a single line or where there is none 0
+    size_t step() const {
+        if (batch == 1 || seq == 1) return seq > 1 ? ts : batch > 1 ? bs : 0;
+        const size_t least = std::min(bs, ts);
+        return least && std::max(bs, ts) % least == 0 ? least : 0;
+    }
 };
-// Do lines of a and b share memory? Those of one wider tensor's rows (equal, even
-// steps) may lie between each other; of other patterns whose extents meet it is
-// taken for granted.
+// Do lines of a and b share memory? Those of one wider tensor's rows (equal steps, a
+// part of a longer one's tokens too) may lie between each other; of other patterns
+// whose extents meet it is taken for granted.
 bool share(const Lines& a, const Lines& b) {
     if (!overlap((void*)a.at, a.extent(), (void*)b.at, b.extent())) return false;
     const size_t step = a.step();
-    if (!a.even() || !b.even() || step != b.step() || step == 0) return true;
+    if (step != b.step() || step == 0) return true;
     const size_t d = a.at <= b.at ? (b.at - a.at) % step : (step - (a.at - b.at) % step) % step;
     return d < a.width || d + b.width > step;
 }

@@ -120,3 +120,50 @@ def test_prompt_of_one_token_many_heads(dev, t):
     """A row of more than 2^22 elements is no step either."""
     q, k, v = torch.randn((3, 1, 17000, 256), device=dev).to(t).unbind(0)
     assert torch.equal(nnr_amd.prompt_attention(q, k, v, ints(dev, [0, 1])), v)
+
+
+# ---------------------------------------------------------------------------
+# rotary positions
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("lay", ["part", "tokens first", "part of tokens first", "side by side"])
+def test_rotary_in_place_of_rows(dev, t, lay):
+    """Queries and keys of one projection's output turned in place: its first tokens of a longer buffer, or with tokens
+    before sequences in memory, or two such. What is not theirs stays."""
+    B, S, most, Hq, Hk, hd = 3, 5, 9, 4, 2, 64
+    rope = nnr_amd.RotaryEmbedding(hd, 100, device=dev)
+    width = (Hq + 2 * Hk) * hd
+    whole = torch.randn((2, B, most, width), generator=gen(1)).to(t).to(dev)
+    if lay == "part":
+        rows = whole[0, :, 2:2 + S]
+    elif lay == "side by side":      # sequences a token's step apart from each other
+        rows = whole[0].reshape(-1)[:S * B * width].view(S, B, width).transpose(0, 1)
+    else:
+        rows = whole[0].view(most, B, width).transpose(0, 1)[:, :S] if lay == "tokens first" else \
+            whole.view(-1)[:most * 2 * B * width].view(most, 2 * B, width).transpose(0, 1)[1:1 + B, 1:1 + S]
+    pos = torch.randint(0, 100, (B, S), generator=gen(2)).to(torch.int32).to(dev)
+    q, k = rows[..., :Hq * hd].unflatten(-1, (Hq, hd)), rows[..., Hq * hd:(Hq + Hk) * hd].unflatten(-1, (Hk, hd))
+    want, before = rope(q, k, pos), whole.clone()
+    f, m = R.frequencies(hd, 10000.0)
+    for x, y in zip((q, k), want):
+        near(y, *R.rotate(x.cpu(), pos.cpu(), f, m, False, 100), t)
+    out = rope(q, k, pos, out=(q, k))
+    assert out[0] is q and torch.equal(q, want[0]) and torch.equal(k, want[1])
+    q.zero_(), k.zero_()
+    after = whole.clone()
+    whole.copy_(before)
+    q.zero_(), k.zero_()
+    assert torch.equal(whole, after)      # but for theirs as before
+
+
+def test_rotary_refuses_rows_that_meet(dev):
+    """Of a longer buffer too: keys' rows that begin within queries', a step that is no multiple of the other."""
+    rope = nnr_amd.RotaryEmbedding(64, 100, device=dev)
+    buffer = torch.zeros(4000, device=dev)
+    pos = ints(dev, [[0, 1, 2]] * 2)
+    at = lambda first, heads, bs, ts: buffer.as_strided((2, 3, heads, 64), (bs, ts, 64, 1), first)
+    q, k = at(0, 2, 5 * 192, 192), at(128, 1, 5 * 192, 192)
+    assert rope(q, k, pos, out=(q, k))[0] is q
+    for k in (at(64, 1, 5 * 192, 192), at(127, 1, 5 * 192, 192), at(129, 1, 5 * 192, 192), at(128, 1, 5 * 192 + 64, 192)):
+        with pytest.raises(nnr_amd.NnrHipError):
+            rope(q, k, pos, out=(q, k))
