@@ -740,7 +740,7 @@ int nnrh_kv_move_tokens(const nnrh_kv_cache_desc* c, void* const* caches, int la
  * in fp32, which the caller makes (scaled for long contexts or not). positions:
  * int32 [batch][seq], read when the kernel runs. A token at a negative position
  * (padding) is copied as it is; one at max_positions or beyond gives NaN.
- * Strides in elements; heads are dense. Results go to qy and ky, which may be q and
+ * Strides in elements (rows within 2^54 of the first); heads are dense. Results go to qy and ky, which may be q and
  * k at the same strides, and whose rows otherwise share no memory with q, k and each
  * other (rows of q and k may lie side by side in one tensor). Addresses are aligned
  * to the element; of 16-byte multiples they are faster. 0 heads: no such tensor. Fewer than

@@ -2768,7 +2768,9 @@ extern "C" int nnrh_rotary(const nnrh_rotary_desc* d, const void* q, const void*
         const long long width = (long long)parts[i].heads * d->head_dim, bs = parts[i].bs, ts = parts[i].ts;
         if (!width) continue;
         if (bs < 0 || ts < 0) return set_err(NNRH_ERR_INVALID, "rotary: strides %lld, %lld", bs, ts);
-        if (bs > (1LL << 38) || ts > (1LL << 38)) return set_err(NNRH_ERR_UNSUPPORTED, "rotary: strides %lld, %lld", bs, ts);
+        // (beyond any memory; extents in bytes would pass 64 bits)
+        if (bs > (1LL << 38) || ts > (1LL << 38) || (double)(d->batch - 1) * bs + (double)(d->seq - 1) * ts > (double)(1LL << 54))
+            return set_err(NNRH_ERR_UNSUPPORTED, "rotary: strides %lld, %lld", bs, ts);
         const bool rows = d->seq <= 1 || ts >= width, seqs = d->batch <= 1 || bs >= (d->seq - 1) * ts + width;
         const bool inner = d->batch <= 1 || bs >= width, outer = d->seq <= 1 || ts >= (d->batch - 1) * bs + width;
         if (parts[i].out && !(rows && seqs) && !(inner && outer))
