@@ -930,7 +930,7 @@ class RotaryEmbedding:
     scaling, for contexts `factor` times as long as the `original_positions` (max_positions / factor
     unless given) that a model was trained at:
       "linear"  f_i / factor
-      "ntk"     the base times factor^(r / (r - 2)), r = rotary_dim: the lowest frequency is divided by factor
+      "ntk"     the base times factor^(r / (r - 2)), r = rotary_dim > 2: the lowest frequency is divided by factor
       "yarn"    f_i where a pair turns 32 times and more within original_positions, f_i / factor where
                 not even once, a linear ramp between; cosines and sines times 0.1 ln(factor) + 1
     frequencies: rotary_dim / 2 numbers in place of all that, with `magnitude` a
@@ -1020,6 +1020,8 @@ def rotary_frequencies(rotary_dim, base=10000.0, scaling=None, factor=1.0, origi
     if not (base > 0 and factor > 0):
         raise ValueError(f"base {base}, factor {factor}")
     r = rotary_dim
+    if scaling == "ntk" and r == 2 and factor != 1:
+        raise ValueError("ntk stretches the base, of which a single pair's frequency, 1, does not depend")
     if scaling == "ntk" and r > 2:
         base = base * factor ** (r / (r - 2))
     f = float(base) ** (-np.arange(0, r, 2, dtype=np.float64) / max(r, 1))

@@ -1,7 +1,8 @@
-"""Sizes of the operators around a decoder's cache at which a product of two of them passes 64 bits: refused before
-anything reaches a GPU (the addresses are no memory)."""
+"""The ends of ranges of the operators around a decoder's cache, refused before anything reaches a GPU (the addresses
+are no memory): sizes whose product passes 64 bits, a single rotary pair."""
 import pytest
 
+import nnr_amd
 from nnr_amd import _lib
 from test_decode_cpu import MEM
 from test_serving_cpu import rotary, rotary_desc
@@ -18,3 +19,15 @@ def test_rotary_extents(axis, which, n, step):
     used, kw = which[0], dict(dtype=_lib.F32, batch=1, seq=1, q_heads=0, k_heads=0, head_dim=64)
     kw.update({f"{used}_heads": 1, "batch" if axis == "batch" else "seq": n, f"{used}_{axis}_stride": 64, f"{used}y_{axis}_stride": 64})
     assert rotary(rotary_desc(**{**kw, f"{which}_{axis}_stride": step}), qy=MEM[2], ky=MEM[3]) == UNSUPPORTED
+
+
+def test_ntk_of_a_single_pair():
+    """Its frequency is 1 whatever the base: nothing could be stretched."""
+    with pytest.raises(ValueError, match="single pair"):
+        nnr_amd.rotary_frequencies(2, scaling="ntk", factor=4.0)
+    with pytest.raises(ValueError, match="single pair"):
+        nnr_amd.RotaryEmbedding(64, 100, rotary_dim=2, scaling="ntk", factor=4.0, device="cpu")
+    assert nnr_amd.rotary_frequencies(2, scaling="ntk", factor=1.0)[0].tolist() == [1.0]
+    assert nnr_amd.rotary_frequencies(0, scaling="ntk", factor=4.0)[0].size == 0
+    f, m = nnr_amd.rotary_frequencies(4, 10000.0, "ntk", 4.0)
+    assert m == 1 and f[0] == 1 and abs(f[1] * 4 * 100 - 1) < 1e-14
