@@ -1042,7 +1042,8 @@ def prompt_attention(q, k, v, starts, scale=None, causal=True, y=None, stream=No
     projection's output). Sequence b is tokens starts[b] .. starts[b + 1] - 1 (int32 [sequences +
     1] on q's device, ascending); a token sees its sequence's tokens up to itself, or all
     of them where causal is False. Tokens of no sequence are left as they are in
-    y, which is new memory unless it is given."""
+    y, which is new memory unless it is given. In float32 and bfloat16 values lie below 2^108, and what a key adds to
+    a result is held in steps of 2^-119: those of 2^-95 and more have all their bits."""
     if stream is not None:
         with _current(q.device, stream):
             return prompt_attention(q, k, v, starts, scale, causal, y)

@@ -19,7 +19,8 @@
 // as rounding the result is, and would cost a second product to avoid. They are
 // held as 2^top p: fp16 has no small numbers (p <= 2^15 there, and weights down to
 // 2^-35 of the largest keep a bit); in bf16 and fp32 a sum of largest numbers must
-// not pass them (2^20 equal weights of such values still do not).
+// not pass them (2^20 equal weights of such values still do not), for which sums of results
+// under 2^-96 are no normal fp32 numbers: their steps, 2^-149, are 2^-119 of a result.
 //
 // Bound by the order of a wave's own work (products, maximum, weights, products), which
 // two waves a SIMD hide in part, at heads of 256 one cannot: 8192 tokens, 32 heads over

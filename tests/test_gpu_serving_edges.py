@@ -167,3 +167,22 @@ def test_rotary_refuses_rows_that_meet(dev):
     for k in (at(64, 1, 5 * 192, 192), at(127, 1, 5 * 192, 192), at(129, 1, 5 * 192, 192), at(128, 1, 5 * 192 + 64, 192)):
         with pytest.raises(nnr_amd.NnrHipError):
             rope(q, k, pos, out=(q, k))
+
+
+@pytest.mark.parametrize("t,e", [(torch.float32, e) for e in (-95, -105, -126)] + [(torch.bfloat16, e) for e in (-95, -110, -126)] +
+                         [(torch.float16, e) for e in (-14, -23)])
+@pytest.mark.parametrize("hd,Hq,Hk,lens", [(64, 2, 1, [300, 20]), (128, 4, 2, [150]), (256, 2, 1, [70, 3]), (256, 40, 40, [90] * 4)])
+def test_prompt_small_values(dev, t, e, hd, Hq, Hk, lens):
+    """Values whose weighted sums are small. Sums are of 2^-30 p v in fp32 and bf16: steps of the smallest fp32 numbers,
+    2^-149, are 2^-119 of a result (its weights' total is 1 and more). A key rounds, or cuts, its product and a sum, a tile of
+    32 the sums once more, and joined groups of waves a few times."""
+    rows, starts = prompts(hd, lens, Hq, Hk, hd, t)
+    q, k, v = parts(rows, Hq, Hk)
+    v[:] = torch.ldexp(1 + torch.rand(v.shape, generator=gen(5), dtype=torch.float64), torch.tensor(e)).to(t)
+    y = nnr_amd.prompt_attention(q.to(dev), k.to(dev), v.to(dev), ints(dev, starts))
+    ref, tol = R.prompt(q, k, v, starts, np.float32(hd ** -0.5).item(), True)
+    if t != torch.float16:
+        tol = tol + (2.25 * max(lens) + 8) * 2.0 ** -119
+    near(y, ref, tol, t)
+    if e >= -95:      # hardly more than such results round anyway (fp16's of 2^-23 to half of its least step, 2^-25)
+        assert ((y.cpu().double() - ref).abs() <= ref * (D.HALF[t] + R.PROMPT_WEIGHTS[t] + 2.0 ** -17) + D.TINY[t]).all()
