@@ -832,7 +832,7 @@ class KVCache:
             if tree.device != self.device:
                 _on_device(self.device, tree=tree)
             _on_gpu("the cache", self.device)
-            if tree.dim() == 3 and tree.stride(0) == 0:   # one that was expanded
+            if tree.dim() == 3 and tree.stride(0) == 0 and B:   # one that was expanded
                 tree = tree[0]
             if not tree.is_contiguous():
                 tree = tree.contiguous()

@@ -186,3 +186,27 @@ def test_prompt_small_values(dev, t, e, hd, Hq, Hk, lens):
     near(y, ref, tol, t)
     if e >= -95:      # hardly more than such results round anyway (fp16's of 2^-23 to half of its least step, 2^-25)
         assert ((y.cpu().double() - ref).abs() <= ref * (D.HALF[t] + R.PROMPT_WEIGHTS[t] + 2.0 ** -17) + D.TINY[t]).all()
+
+
+# ---------------------------------------------------------------------------
+# nothing to do
+
+def test_empty_calls(dev):
+    """No sequences (with a tree that is expanded over them), no tokens, no heads of queries or keys"""
+    cache = nnr_amd.KVCache(2, 1, 64, page_size=32, device=dev)
+    tree = torch.ones((3, 3), dtype=torch.bool, device=dev)
+    q, td, ld = torch.zeros((2, 3, 2, 64), device=dev), ints(dev, [[0], [1]]), ints(dev, [5, 6])
+    for mask in (tree, tree.expand(0, 3, 3), tree.repeat(0, 1, 1)):
+        assert cache.attention(q[:0], td[:0], ld[:0], tree=mask).shape == (0, 3, 2, 64)
+    for mask in (tree[:0, :0], tree[:0, :0].expand(2, 0, 0)):
+        assert cache.attention(q[:, :0], td, ld, tree=mask).shape == (2, 0, 2, 64)
+    rope, pos = nnr_amd.RotaryEmbedding(64, 100, device=dev), ints(dev, [[1, 2, 3], [4, 5, 6]])
+    k = torch.randn((2, 3, 1, 64), device=dev)
+    want = rope(q, k, pos)[1]
+    for inplace in (False, True):
+        x = k.clone()
+        none, y = rope(q[:, :, :0], x, pos, out=(q[:, :, :0], x) if inplace else None)
+        assert none.shape == (2, 3, 0, 64) and torch.equal(y, want)
+        x = k.clone()
+        assert torch.equal(rope(x, q[:, :, :0], pos, out=(x, q[:, :, :0]) if inplace else None)[0], want)
+    assert rope(q[:0], k[:0], pos[:0])[0].shape == (0, 3, 2, 64) and rope(q[:, :0], k[:, :0], pos[:, :0])[1].shape == (2, 0, 1, 64)
