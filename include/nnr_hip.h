@@ -739,12 +739,12 @@ int nnrh_kv_move_tokens(const nnrh_kv_cache_desc* c, void* const* caches, int la
  * in fp32, rounded once. table: [max_positions][rotary_dim / 2] pairs (cosine, sine)
  * in fp32, which the caller makes (scaled for long contexts or not). positions:
  * int32 [batch][seq], read when the kernel runs. A token at a negative position
- * (padding) is copied as it is; one at max_positions or beyond gives NaN.
+ * (padding) is copied as it is; one at max_positions or beyond gives NaN in all that turns.
  * Strides in elements (rows within 2^54 of the first); heads are dense. Results go to qy and ky, which may be q and
  * k at the same strides, and whose rows otherwise share no memory with q, k and each
  * other (rows of q and k may lie side by side in one tensor). Addresses are aligned
  * to the element; of 16-byte multiples they are faster. 0 heads: no such tensor. Fewer than
- * 2^31 elements.                                                            */
+ * 2^31 elements; at most 2^20 heads, of 2^16 elements.                       */
 typedef struct nnrh_rotary_desc {
     int dtype;
     int batch, seq, q_heads, k_heads;
@@ -775,7 +775,8 @@ int nnrh_rotary(const nnrh_rotary_desc* d, const void* q_dev, const void* k_dev,
  * q [tokens][q_heads][head_dim], k and v [tokens][kv_heads][head_dim] with token
  * strides in elements (at most 2^22; one token's say nothing; heads are dense), y dense; addresses and strides
  * in bytes are multiples of 16. y may be q itself where q is dense, and overlaps
- * nothing else. head_dim 64, 96, 128 or 256. No workspace.                  */
+ * nothing else. head_dim 64, 96, 128 or 256; at most 32767 kv_heads; tokens q_heads / 128
+ * and seqs kv_heads at most 2^23 together. No workspace.                     */
 typedef struct nnrh_prompt_attention_desc {
     int dtype;
     int tokens, seqs, q_heads, kv_heads, head_dim;

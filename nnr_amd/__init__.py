@@ -932,7 +932,9 @@ class RotaryEmbedding:
       "linear"  f_i / factor
       "ntk"     the base times factor^(r / (r - 2)), r = rotary_dim > 2: the lowest frequency is divided by factor
       "yarn"    f_i where a pair turns 32 times and more within original_positions, f_i / factor where
-                not even once, a linear ramp between; cosines and sines times 0.1 ln(factor) + 1
+                not even once, between them a ramp that is linear in the turns, as the method's paper has
+                it; cosines and sines times 0.1 ln(factor) + 1. (Implementations whose ramp is linear in a pair's
+                number, between two rounded ones, differ in between: theirs go in as frequencies.)
     frequencies: rotary_dim / 2 numbers in place of all that, with `magnitude` a
     factor of cosines and sines (1 unless given). Tables are formed in 64 bits and held in 32, on
     `device` or the current one."""
@@ -976,7 +978,7 @@ class RotaryEmbedding:
     def __call__(self, q, k, positions, out=None, stream=None):
         """(q, k) turned: q [batch, seq, heads, head_dim], k with heads of its own,
         positions int32 [batch, seq] (negative: padding, left as it is; from
-        max_positions on: NaN). The first two axes may be strided. out: two tensors
+        max_positions on: NaN in all that turns). The first two axes may be strided. out: two tensors
         for the results, (q, k) themselves to work in place; new ones unless given."""
         if stream is not None:
             with _current(self.device, stream):

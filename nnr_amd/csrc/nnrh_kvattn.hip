@@ -1261,12 +1261,20 @@ __global__ __launch_bounds__(AW * 64, HD <= 128 ? (!PM && !OM && NP == 1 ? 3 : 2
 // between two barriers. 32x32 products leave a lane 16 scores of one row; tokens
 // 4 g .. and 16 + 4 g .. of a tile, which lie side by side in a value block, are eight
 // of them.
-// Bound by the vector units: a score takes a scale, a maximum, a product-sum, an exp,
-// a total, a value's scale, a maximum and half a conversion, 10 issue slots, 16 of
-// them for the 32 cycles that its products take. 24 sequences of up to 4096 tokens
-// after a prefix of 1000, 64 drafts, 32 heads over 8 of 128: 162 to 180 us with the
-// join's 18 (the kernel above, in its place: 250). One sequence of 1800, 15 drafts:
-// 17 us, most of it a block's start, its first tiles' way from memory, and the join.
+// A score takes a scale, a maximum, a product-sum, an exp, a total, a value's scale, a
+// maximum and half a conversion, 10 issue slots, 16 of them for the 32 cycles that its
+// products take. 24 sequences of up to 4096 tokens after a prefix of 1000, 64 drafts, 32
+// heads over 8 of 128: 162 to 180 us with the join's 18 (the kernel above, in its place:
+// 250). Vector units are 50 % busy there, matrix units 29, waves wait 26 % of their time:
+// no unit bounds it, but that a short sequence has as many parts as a long one, which
+// end sooner and are joined all the same (all of them 2080 long, as many tokens: 105).
+// One sequence of 1800, 15 drafts: 13 us for four tiles a block, of which 11.5 pass where
+// it has one or none (a launch, lengths and table, the first codes, the parts), the join 4.
+// fp32 tensors and heads of 256 go to the kernel above: of 256 registers two pieces of
+// queries and weights, or 128 of sums and 64 of queries, leave too few, so that no such
+// variant was built. (The same 24 sequences: fp32 307 us, heads of 256 499, both 633,
+// little more than without a tree, 300, 481, 612; one of 4096, 64 drafts, 27, 36, 43, in
+// bf16 with heads of 128 23.)
 typedef float f16v __attribute__((ext_vector_type(16)));
 constexpr int kTreeWaves = 4, kTreeTiles = 2;   // waves of a block; tiles between two barriers
 template <int HD> struct TreeRows {

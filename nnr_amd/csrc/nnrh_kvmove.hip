@@ -57,7 +57,8 @@ __device__ __forceinline__ TokenAt token_at(const KvCache& c, const KvMoves& m, 
 // them in and stores it, so that no two lanes change one word. Bound by latency: the
 // positions, the table, the tokens, the words that they go to, each a trip to memory
 // (4 tokens of 2 caches x 8 heads of 128, 8 bits, 4.7 us; 7 of 64 sequences, 8
-// caches, 4 bits, 24: a key is 16 lines of memory with 4 bytes of it each, so that this is 117 MB).
+// caches, 4 bits, 24: its 8192 blocks have one wave each, which makes the trips to tokens and
+// words twice. A key is 4 bytes of each of 16 lines: 117 MB asked of L2, 35 of memory, a copy's 7 us).
 constexpr int MU = 4;   // tokens in flight a wave
 
 // a token's place, which is the same for all lanes, in scalar registers: a lane adds

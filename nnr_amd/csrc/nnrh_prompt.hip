@@ -699,8 +699,10 @@ hipError_t start(const PromptAttention& a, hipStream_t s) {
 // 34.8, 35.6. Heads of 128, 453 blocks 65, 53; 516 34, 38. Heads of 256, one block
 // a CU, 83 20.1, 16.3; 263 76, 68; 317 45, 58; 396 141, 170; fp32 117 153, 97; 258 1048,
 // 701; 395 100, 131; 504 576, 723. fp32, bound by its products: heads of 64, 664 64.5,
-// 53.3; heads of 128, 520 387, 340; 664 90, 116. Four groups and two: heads of 64,
-// 129 16.9, 21.0; 204 22.5, 22.7; heads of 128, 63 15.7, 18.6; 83 14.2, 10.8.)
+// 53.3; heads of 128, 520 387, 340; 664 90, 116; heads of 96 as of 128: fp16 383 33.7, 32.9,
+// 396 77.8, 68.7; 491 26.2, 29.9; fp32 480 712, 596; 520 300, 274; 658 402, 446. Four groups
+// and two: heads of 64, 129 16.9, 21.0; 204 22.5, 22.7; heads of 128, 63 15.7, 18.6; 83 14.2, 10.8;
+// of 96, 63 21.3, 24.1; 77 16.3, 17.5; 133 23.4, 20.4.)
 template <int TY, int HD> constexpr int kTwoGroups = HD > 128 ? 272 : TY != FT_F32 ? 448 : HD == 64 ? 1024 : 512;
 template <int TY, int HD> constexpr int kFourGroups = HD == 64 ? 128 : TY != FT_F32 && HD <= 128 ? 64 : 0;
 template <int TY, int HD>
