@@ -26,21 +26,16 @@ def tree_parts(cache, batch, S, Hq, per, prefix, t, length):
     return list(zip([0] + ends[:-1], ends))
 
 
-@pytest.mark.parametrize("t", [torch.float16, torch.bfloat16])
-@pytest.mark.parametrize("bits", [8, 4])
-@pytest.mark.parametrize("hd", [64, 96, 128])
-@pytest.mark.parametrize("prefix,lens,far_pre,far_own", [
-    (300, [40, 200], [20, 180], []), (64, [40, 60], [], [5]), (300, [300, 290], [], [10]), (33, [41], [32], [])])
-def test_tree_computed_again_behind_a_prefix(dev, t, bits, hd, prefix, lens, far_pre, far_own):
+def check_computed_again(dev, t, bits, hd, S, G, prefix, lens, far_pre, far_own, in_parts):
     """A few large values that no row gives weight to, beside such of 1e-3: rows of the parts that hold them are computed
-    again in fp32. Those parts hold tokens of the prefix at the positions that drafts have in their sequence, and the
-    tree's first line hides all drafts but one."""
-    S, H, G, page = 40, 1, 4, 32
+    again in fp32. in_parts: those parts hold tokens of the prefix at the positions that drafts have in their sequence.
+    The tree's first line hides all drafts but one."""
+    H, page = 1, 32
     tree = random_tree(np.random.default_rng(4), S)
     B, pre_pages, per = len(lens), -(-prefix // page), max(-(-n // page) for n in lens)
     table, pages, spare = tables(np.random.default_rng(hd), B, per, pre_pages + 1)
     cache = cache_of(dev, pages, H, hd, page_size=page, bits=bits)
-    for b, n in enumerate(lens):
+    for b, n in enumerate(lens if in_parts else []):
         found = False
         for first, end in tree_parts(cache, B, S, H * G, per, prefix, t, n):
             far = any(first <= p // 32 < end for p in far_pre) or any(first <= -(-prefix // 32) + p // 32 < end for p in far_own)
@@ -73,6 +68,26 @@ def test_tree_computed_again_behind_a_prefix(dev, t, bits, hd, prefix, lens, far
         low = 2.0 ** -39 * q[b].double().abs().amax((1, 2))[:, None, None] * kx.abs().sum(-1).amax() * sc
         steps = len(vx) * R.CACHE_FLOOR[t] * max(x.double().abs().amax().item() for x in small_v)
         near(y[b], ref, R.rounded(ref, w, tol + 2 * low * w + steps, t, R.CACHE_WEIGHTS[t]), t)
+
+
+FAR = [(300, [40, 200], [20, 180], []), (64, [40, 60], [], [5]), (300, [300, 290], [], [10]), (33, [41], [32], [])]
+
+
+@pytest.mark.parametrize("t", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("hd", [64, 96, 128])
+@pytest.mark.parametrize("prefix,lens,far_pre,far_own", FAR)
+def test_tree_computed_again_behind_a_prefix(dev, t, bits, hd, prefix, lens, far_pre, far_own):
+    check_computed_again(dev, t, bits, hd, 40, 4, prefix, lens, far_pre, far_own, True)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("t,hd,S,G", [(torch.float32, 64, 40, 4), (torch.float32, 256, 40, 2), (torch.bfloat16, 256, 40, 2),
+                                      (torch.float16, 128, 3, 2), (torch.float32, 96, 3, 1), (torch.float16, 256, 5, 3)])
+@pytest.mark.parametrize("prefix,lens,far_pre,far_own", FAR)
+def test_tree_computed_again_elsewhere(dev, bits, t, hd, S, G, prefix, lens, far_pre, far_own):
+    """The same of other types, wide heads and few rows, whose prefix is a block's of its own"""
+    check_computed_again(dev, t, bits, hd, S, G, prefix, lens, far_pre, far_own, False)
 
 
 @pytest.mark.parametrize("t", TYPES)
@@ -210,3 +225,115 @@ def test_empty_calls(dev):
         x = k.clone()
         assert torch.equal(rope(x, q[:, :, :0], pos, out=(x, q[:, :, :0]) if inplace else None)[0], want)
     assert rope(q[:0], k[:0], pos[:0])[0].shape == (0, 3, 2, 64) and rope(q[:, :0], k[:, :0], pos[:, :0])[1].shape == (2, 0, 1, 64)
+
+
+# ---------------------------------------------------------------------------
+# large sizes, results in place
+
+@pytest.mark.parametrize("t", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("S", [3, 40])
+def test_tree_in_place(dev, t, bits, S):
+    """Rows that are computed again read their queries a second time, when others' results lie where queries were."""
+    B, H, G, hd, page = 2, 2, 4, 64, 32
+    table, pages, _ = tables(np.random.default_rng(S), B, 3, 1)
+    cache, td, ld = cache_of(dev, pages, H, hd, page_size=page, bits=bits), table.to(dev), ints(dev, [S, 90])
+    k, v = tokens(1, B, 96, H, hd, t)
+    v *= 1e-3
+    v[:, 96 - S + 1] = 1e4
+    cache.write(k.to(dev), v.to(dev), td, ld)
+    q = torch.randn((B, S, H * G, hd), generator=gen(2)).to(t).to(dev)
+    tree = random_tree(np.random.default_rng(3), S)
+    tree[2:, 1] = False
+    want = cache.attention(q, td, ld, tree=tree.to(dev))
+    assert cache.attention_workspace(B, S, H * G, 3, dtype=t, tree=True) == 0
+    assert cache.attention(q, td, ld, tree=tree.to(dev), y=q) is q and torch.equal(q, want)
+
+
+@pytest.mark.parametrize("t", [torch.float32, torch.float16])
+@pytest.mark.parametrize("S,n", [(4096, 4096), (1000, 1777)])
+def test_tree_of_many_drafts(dev, t, S, n):
+    """As many as a tree may have: a chain, against the causal call, both within a tolerance of the 64-bit result."""
+    H, G, hd, page, bits = 1, 2, 64, 128, 8
+    per = -(-n // page)
+    table, pages, _ = tables(np.random.default_rng(1), 1, per, 2)
+    cache, td, ld = cache_of(dev, pages, H, hd, page_size=page, bits=bits), table.to(dev), ints(dev, [n])
+    k, v = tokens(1, 1, n, H, hd, t)
+    cache.write(k.to(dev), v.to(dev), td, ld)
+    q = torch.randn((1, S, H * G, hd), generator=gen(2)).to(t)
+    chain = torch.ones((S, S), dtype=torch.bool).tril()
+    y = cache.attention(q.to(dev), td, ld, tree=chain.to(dev))
+    some = torch.tensor([0, 1, 31, 64, S // 2, S - 2, S - 1])
+    sees = torch.cat((torch.ones((len(some), n - S), dtype=torch.bool), chain[some]), -1)
+    kx, vx = (D.quantize(x[0, :, 0], bits)[0] for x in (k, v))
+    ref, w, tol = R.attend(q[0, some], kx, vx, np.float32(hd ** -0.5).item(), sees, R.CACHE_FLOOR[t])
+    low = 2.0 ** -39 * q.double().abs().amax() * kx.abs().sum(-1).amax() * hd ** -0.5
+    tol = R.rounded(ref, w, tol + 2 * low * w, t, R.CACHE_WEIGHTS[t])
+    near(y[0, some.to(dev)], ref, tol, t)
+    near(cache.attention(q.to(dev), td, ld)[0, some.to(dev)], ref, tol, t)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_cache_past_32_bits(dev, bits):
+    """Pages whose bytes begin past 2^32: written, copied, moved within and attended to as those at the front are."""
+    H, hd, page, t = 8, 128, 4096, torch.float16
+    size = 2 * H * page * (hd * bits // 8 + 2 * (1 if bits == 8 else hd // 32))
+    pages = (5 << 30) // size
+    far = nnr_amd.KVCache(pages, H, hd, page_size=page, bits=bits, device=dev)
+    near_ = nnr_amd.KVCache(4, H, hd, page_size=page, bits=bits, device=dev)
+    assert (pages - 2) * size > 1 << 32
+    k, v = (torch.randn((1, 5000, H, hd), generator=gen(i)).to(t).to(dev) for i in (1, 2))
+    ld, S = ints(dev, [5000]), 40
+    q, tree = torch.randn((1, S, 2 * H, hd), generator=gen(3)).to(t).to(dev), random_tree(np.random.default_rng(1), S).to(dev)
+    at = {}
+    for c, own, to in ((near_, [0, 1], [2, 3]), (far, [pages - 1, 2], [pages - 2, pages - 3])):
+        td = ints(dev, [own])
+        c.write(k, v, td, ld)
+        nnr_amd.copy_pages(c, ints(dev, own), ints(dev, to))
+        moved = ints(dev, [[4990, 7, 4100]]), ints(dev, [[4970, 4971, 8]])
+        nnr_amd.move_tokens(c, ints(dev, [to]), *moved)
+        at[c] = [c.attention(q, ints(dev, [x]), ld, tree=tree) for x in (own, to)] + \
+            [x for p in (own, to) for x in c.read(5000, ints(dev, [p]), ld, t)]
+    assert all(torch.equal(a, b) for a, b in zip(at[near_], at[far])) and not torch.equal(at[far][0], at[far][1])
+
+
+def test_prompts_past_32_bits(dev):
+    """Tokens whose elements begin past 2^32, of queries, keys and values and of results"""
+    T, H, hd, t = 1_200_000, 16, 256, torch.bfloat16
+    rows = torch.empty((T, 3 * H, hd), dtype=t, device=dev)
+    rows[-900:] = torch.randn((900, 3 * H, hd), generator=gen(1)).to(t).to(dev)
+    y = torch.empty((T, H, hd), dtype=t, device=dev)
+    y[-1000:] = 7
+    q, k, v = rows[:, :H], rows[:, H:2 * H], rows[:, 2 * H:]
+    nnr_amd.prompt_attention(q, k, v, ints(dev, [T - 900, T - 300, T - 299, T]), y=y)
+    want = nnr_amd.prompt_attention(q[-900:], k[-900:], v[-900:], ints(dev, [0, 600, 601, 900]))
+    assert (y[-1000:-900] == 7).all()
+    near(y[-300:, :2], *R.prompt(*(x[-300:, :2].cpu() for x in (q, k, v)), [0, 1, 300], 1 / 16, True), t)
+    # (other numbers of blocks, and so other groups of waves: twice the rounding of weights, of values at most, and of results)
+    assert ((y[-900:].float() - want.float()).abs() <= 2.0 ** -7 * (v[-900:].abs().max() + want.float().abs())).all()
+
+
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16])
+def test_prompt_of_a_long_document(dev, t):
+    n, hd = 70001, 64
+    q, k, v = (torch.randn((n, 1, hd), generator=gen(i)).to(t) for i in range(3))
+    y = nnr_amd.prompt_attention(*(x.to(dev) for x in (q, k, v)), ints(dev, [0, n]))
+    for i in (0, 1, 63, 4097, 65535, 65536, n - 1):
+        ref, w, tol = R.attend(q[i:i + 1], k[:i + 1, 0], v[:i + 1, 0], 0.125, torch.ones((1, i + 1), dtype=torch.bool), R.PROMPT_FLOOR[t])
+        near(y[i:i + 1], ref, R.rounded(ref, w, tol, t, R.PROMPT_WEIGHTS[t]), t)
+
+
+def test_rotary_past_32_bits(dev):
+    """Sequences 2^31 elements and more apart, in place"""
+    step = (1 << 31) + 64
+    rows = torch.empty(2 * step + 3 * 192, dtype=torch.float16, device=dev).as_strided((3, 2, 3, 64), (step, 192, 64, 1))
+    rows.copy_(torch.randn((3, 2, 3, 64), generator=gen(1)))
+    rope, pos = nnr_amd.RotaryEmbedding(64, 100, device=dev), ints(dev, [[1, 2], [50, 51], [98, 99]])
+    q, k = rows[:, :, :2], rows[:, :, 2:]
+    want = rope(q.contiguous(), k.contiguous(), pos)
+    out = rope(q, k, pos)
+    assert all(torch.equal(a, b) for a, b in zip(out, want))
+    f, m = R.frequencies(64, 10000.0)
+    near(out[0], *R.rotate(q.cpu(), pos.cpu(), f, m, False, 100), torch.float16)
+    alone = q.contiguous(), k.contiguous()
+    assert rope(q, alone[1], pos, out=(q, alone[1]))[0] is q and torch.equal(q, want[0]) and torch.equal(alone[1], want[1])
