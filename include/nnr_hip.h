@@ -771,7 +771,7 @@ int nnrh_rotary(const nnrh_rotary_desc* d, const void* q_dev, const void* k_dev,
  * type. Values are such that 2^20 times the largest stays below 2^128 (fp16: any). In
  * fp32 and bf16 what a key adds to a result is held in steps of 2^-119 (weights of 2^-30
  * leave the room above), so that results of 2^-95 and more have all their bits, and
- * those under 2^-120 are 0.
+ * those under 2^-120 may be 0.
  * q [tokens][q_heads][head_dim], k and v [tokens][kv_heads][head_dim] with token
  * strides in elements (at most 2^22; one token's say nothing; heads are dense), y dense; addresses and strides
  * in bytes are multiples of 16. y may be q itself where q is dense, and overlaps
